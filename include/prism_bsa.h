@@ -13,7 +13,9 @@
  * its host layer reaches these functions through the torch.ops.prism
  * operators (prism_amd/csrc/torch_ops.cpp) or through ctypes.
  *
- * dtype codes: PRISM_F32 = 0, PRISM_BF16 = 1.
+ * dtype codes: PRISM_F32 = 0, PRISM_BF16 = 1; the layer's operators (row norms,
+ * rotary positions, window attention) also take PRISM_F16 = 2, and the norms
+ * write PRISM_E4M3 = 3 (OCP float8 e4m3) and PRISM_I8 = 4.
  * Layouts: "THW order" = the reference's flattened (t, h, w) token order of a
  * padded grid T x Hg x Wg (all multiples of 8); "tile order" = the per-zone
  * anisotropic rearrangement of _build_rearrange_index
@@ -32,6 +34,9 @@ extern "C" {
 
 #define PRISM_F32 0
 #define PRISM_BF16 1
+#define PRISM_F16 2
+#define PRISM_E4M3 3
+#define PRISM_I8 4
 
 /* Message of the last failed call on this host thread ("" if none). */
 const char* prism_last_error(void);
@@ -99,6 +104,47 @@ int prism_a2v_norms(const void* res, int dtype, int64_t S, int C, void* out, int
  * below 4 GiB. */
 int prism_linear_rownorm(const void* x, const void* w, const void* bias, int64_t M, int N, int K, void* y,
                          void* norms, int norms_dtype, float* partial, hipStream_t stream);
+
+/* ------------------------------------------------------------------ row norms */
+
+/* Root-mean-square norm of rows (the norms of wan_video_dit.py:699-705) with
+ * the residual's addition: h = x + r, y = h / sqrt(mean(h^2) + eps) * w.
+ * x, r: M rows of N (<= 16384) of `dtype`, x_stride / r_stride elements apart; r NULL: h =
+ * x, else h [M, N] receives the sum rounded to dtype (y is of the unrounded
+ * sum); w: [N] of w_dtype (dtype or PRISM_F32) or NULL.  y: [M, N] of
+ * out_dtype: dtype, or PRISM_E4M3 / PRISM_I8 codes of y / scale[m] with
+ * scale[m] = max(max |y[m, :]| / qmax, 2^-126), qmax 448 / 127 (a row with a NaN or an
+ * infinity in y has a scale that is not finite).  inv: [M] = 1 / sqrt(..), or
+ * NULL.  h may be r or x itself (same rows, stride N). */
+int prism_rms_norm(const void* x, int64_t x_stride, const void* r, int64_t r_stride, const void* w, int w_dtype,
+                   int dtype, int64_t M, int N, float eps, void* h, void* y, int out_dtype, float* scale, float* inv,
+                   hipStream_t stream);
+
+/* Gradients of prism_rms_norm: dx [M, N] (r has the same one) = s (g - xh
+ * mean(g xh)) + dh with g = dy w, xh = h s, s = inv, and dw [N] (w_dtype; NULL
+ * to skip) = sum over rows of dy xh.  dh: gradient of h, or NULL.  partial:
+ * workspace of parts * N floats for dw (prism_rms_norm_parts), added in a fixed
+ * order. */
+int prism_rms_norm_parts(int64_t M, int N, int* parts);
+int prism_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh, int64_t dh_stride, const void* h,
+                       int64_t h_stride, const void* w, int w_dtype, int dtype, int64_t M, int N, const float* inv,
+                       void* dx, float* partial, int parts, void* dw, hipStream_t stream);
+
+/* ------------------------------------------------------------------ rotary positions */
+
+/* Rotary positions on q [B, Hq, S, D] and k [B, Hk, S, D] (Hk = 0: none; the
+ * rotation of wan_video_dit.py:699-705): pair p of the first R channels,
+ * (2p, 2p + 1) where interleaved, else (p, p + R/2), turns by pos * freqs[p]
+ * radians (back by as much where inverse) and is scaled by amplitude; other
+ * channels are copied.  D <= 256.  strides (host, elements): batch, head, token
+ * of q, out_q, k, out_k; channels are adjacent.  pos: int32, or int64 with
+ * pos64, read at batch / token / axis strides pos_strides (host); pairs below
+ * axis_end[a] (host, 1 to 4 axes, ascending to R/2) and not of an earlier axis turn with axis a.
+ * out_q / out_k may be q / k themselves. */
+int prism_rotary(const void* q, const void* k, int dtype, int B, int64_t S, int Hq, int Hk, int D, int R,
+                 const int64_t* strides, const double* freqs, const void* pos, int pos64,
+                 const int64_t* pos_strides, int axes, const int32_t* axis_end, int interleaved, float amplitude,
+                 int inverse, void* out_q, void* out_k, hipStream_t stream);
 
 /* ------------------------------------------------------------------ geometry */
 

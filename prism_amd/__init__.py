@@ -10,6 +10,9 @@ Public surface (reference names):
   flash_attn_bsa              bsa_interface.py:683 (_attention_bsa.apply)
   a2v_token_norms             wan_video_dit.py:742-752 (A2V residual norms)
   a2v_bridge_projection       interactionv2.py:348 o-projection with the norms fused
+and what the layer runs around it (wan_video_dit.py:699-705):
+  rms_norm, rms_norm_quant    residual addition + root-mean-square norm, 8-bit output
+  rotary_frequencies, apply_rotary, grid_positions  rotary positions on q and k
 All compute runs in libprism_bsa.so, reached through the torch.ops.prism
 operators of libprism_torch.so (build: python prism_amd/build.py).
 """
@@ -20,6 +23,8 @@ from .dynamic_block_shape import (  # noqa: F401
 )
 from .dynamic_block_attention import _TILE, flash_attn_bsa_3d_dynamic, plan_dynamic  # noqa: F401
 from .adapter import DynamicBlockSparseAttention, a2v_bridge_projection, a2v_token_norms, valid_mask_for  # noqa: F401
+from .rotary import apply_rotary, grid_positions, rotary_frequencies  # noqa: F401
+from .row_norm import rms_norm, rms_norm_quant  # noqa: F401
 from .uniform_block_attention import flash_attn_bsa, flash_attn_bsa_3d, flash_attn_bsa_cross  # noqa: F401
 
 __version__ = "0.1.0"

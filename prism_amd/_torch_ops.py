@@ -89,6 +89,23 @@ def _register_fakes():
     def _(x, weight, bias, norms_dtype):
         return _empty(x, (x.shape[0], weight.shape[0]), x.dtype), _empty(x, (x.shape[0],), f32 if norms_dtype == 0 else bf16)
 
+    f8, i8 = torch.float8_e4m3fn, torch.int8
+
+    @reg("prism::rms_norm")
+    def _(x, residual, weight, eps, out_code, want_inv):
+        m = x.shape[0]
+        return (_empty(x, x.shape, {3: f8, 4: i8}.get(out_code, x.dtype)),
+                _empty(x, x.shape, x.dtype) if residual is not None else _none(x),
+                _empty(x, (m,), f32) if out_code >= 3 else _none(x), _empty(x, (m,), f32) if want_inv else _none(x))
+
+    @reg("prism::rms_norm_bwd")
+    def _(dy, dh, h, weight, inv, want_dw):
+        return _empty(h, h.shape, h.dtype), _empty(h, weight.shape, weight.dtype) if want_dw else _none(h)
+
+    @reg("prism::rotary")
+    def _(q, k, freqs, positions, axis_pairs, interleaved, amplitude, inverse):
+        return torch.empty_like(q), torch.empty_like(k) if k is not None else _none(q)
+
     @reg("prism::zone_layout")
     def _(shape_ids):
         nz = shape_ids.numel()

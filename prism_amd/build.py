@@ -9,8 +9,8 @@
 
 Each csrc/*.hip file is compiled by hipcc for gfx950 only and linked into one
 shared library exporting the C-ABI declared in include/prism_bsa.h;
-csrc/torch_ops.cpp (host C++, no device code) is built on top of it into
-libprism_torch.so, the TORCH_LIBRARY(prism) operators.  Files
+csrc/torch_ops.cpp and torch_layer_ops.cpp (host C++, no device code) are built
+on top of it into libprism_torch.so, the TORCH_LIBRARY(prism) operators.  Files
 whose results are bit-exact parity targets are compiled with
 -ffp-contract=off (their fused operations are written out explicitly).
 """
@@ -27,11 +27,11 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD_DIR = os.path.join(HERE, "_build")
 LIB_NAME = "libprism_bsa.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
-TORCH_OPS_SRC = "torch_ops.cpp"
+TORCH_OPS_SRCS = ["torch_ops.cpp", "torch_layer_ops.cpp"]
 TORCH_OPS_PATH = os.path.join(HERE, "libprism_torch.so")
 
 SOURCES = ["errors.hip", "stats.hip", "layout.hip", "select.hip", "lists.hip", "attn_fwd.hip", "attn_bwd.hip",
-           "oproj.hip", "validate.hip", "peak.hip"]
+           "oproj.hip", "rownorm.hip", "rotary.hip", "validate.hip", "peak.hip"]
 CANONICAL = {"stats.hip", "layout.hip", "select.hip"}
 
 COMMON_FLAGS = [
@@ -76,7 +76,7 @@ def _compile(src: str, sanitize: bool = False) -> str:
 
 
 def _torch_ops_cmd(out: str):
-    """g++ line of the PyTorch operator library (csrc/torch_ops.cpp): torch's
+    """g++ line of the PyTorch operator library (csrc/torch_*ops.cpp): torch's
     headers and libraries, HIP's runtime headers, linked against
     libprism_bsa.so found next to it at load time."""
     import torch
@@ -86,7 +86,8 @@ def _torch_ops_cmd(out: str):
     libs = [f"-L{d}" for d in cpp_extension.library_paths()]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     return [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1",
-            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *inc, os.path.join(CSRC, TORCH_OPS_SRC), "-o", out, *libs,
+            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *inc, *[os.path.join(CSRC, f) for f in TORCH_OPS_SRCS], "-o", out,
+            *libs,
             f"-L{HERE}", "-lprism_bsa", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN"]
 
 

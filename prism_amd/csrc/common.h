@@ -6,6 +6,9 @@
 
 #define PRISM_F32 0
 #define PRISM_BF16 1
+#define PRISM_F16 2
+#define PRISM_E4M3 3
+#define PRISM_I8 4
 
 #define PRISM_OK 0
 #define PRISM_EINVAL 1

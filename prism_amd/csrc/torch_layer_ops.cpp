@@ -1,0 +1,167 @@
+// PyTorch operators of what runs around and beside the block-sparse attention
+// (TORCH_LIBRARY_FRAGMENT(prism)): row norms, rotary positions and window
+// attention.  As in torch_ops.cpp, each wraps one extern "C" entry point of
+// include/prism_bsa.h, checks what the kernels assume, allocates its outputs
+// and workspaces through the caching allocator and launches on the current HIP
+// stream of its tensors' device.
+#include "torch_common.h"
+
+#include <limits>
+
+namespace {
+
+int type_code(const Tensor& t, const char* name) {
+  if (t.scalar_type() == at::kFloat) return PRISM_F32;
+  if (t.scalar_type() == at::kBFloat16) return PRISM_BF16;
+  if (t.scalar_type() == at::kHalf) return PRISM_F16;
+  TORCH_CHECK_TYPE(false, "prism: ", name, ": unsupported dtype ", t.scalar_type(), " (float32, bfloat16 or float16)");
+  return -1;
+}
+void same_device(const Tensor& like, const OptT& t, const char* name) {
+  on_gpu(t, name);
+  if (t && t->defined())
+    TORCH_CHECK_VALUE(t->device() == like.device(), "prism: ", name, " is on ", t->device(), ", not on ", like.device());
+}
+Tensor unit_rows(const Tensor& t) { return t.numel() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+int32_t small(int64_t n, const char* name) {
+  TORCH_CHECK_VALUE(n >= 0 && n <= std::numeric_limits<int32_t>::max(), "prism: ", name, " out of range");
+  return (int32_t)n;
+}
+
+// ------------------------------------------------------------------ row norms
+// rows M x N: y, h (with a residual), scale (8-bit outputs), 1 / rms (on request)
+std::tuple<Tensor, Tensor, Tensor, Tensor> rms_norm(const Tensor& x_, const OptT& r_, const OptT& w_, double eps,
+                                                    int64_t out_code, bool want_inv) {
+  on_gpu(x_, "x");
+  same_device(x_, r_, "residual");
+  same_device(x_, w_, "weight");
+  TORCH_CHECK_VALUE(x_.dim() == 2, "rms_norm: x must be [M, N]");
+  const int dt = type_code(x_, "rms_norm");
+  const int64_t M = x_.size(0), N = x_.size(1);
+  check_dtype(r_, x_.scalar_type(), "residual");
+  if (r_) TORCH_CHECK_VALUE(r_->sizes() == x_.sizes(), "rms_norm: residual must have x's shape");
+  if (w_) TORCH_CHECK_VALUE(w_->dim() == 1 && w_->size(0) == N, "rms_norm: weight must be [N]");
+  const int wdt = w_ ? type_code(*w_, "rms_norm weight") : dt;
+  const c10::DeviceGuard guard(x_.device());
+  const Tensor x = unit_rows(x_);
+  const OptT r = r_ ? OptT(unit_rows(*r_)) : OptT(), w = cont(w_);
+  const at::ScalarType ot = out_code == PRISM_E4M3 ? at::kFloat8_e4m3fn : out_code == PRISM_I8 ? at::kChar : x.scalar_type();
+  const bool quant = out_code == PRISM_E4M3 || out_code == PRISM_I8;
+  Tensor y = at::empty({M, N}, opts(x, ot));
+  Tensor h = r ? at::empty({M, N}, x.options()) : none_like(x);
+  Tensor scale = quant ? at::empty({M}, opts(x, at::kFloat)) : none_like(x);
+  Tensor inv = want_inv ? at::empty({M}, opts(x, at::kFloat)) : none_like(x);
+  PRISM_TORCH_CALL(prism_rms_norm, x.data_ptr(), x.stride(0), p(r), r ? r->stride(0) : 0, p(w), wdt, dt, M,
+                   small(N, "N"), (float)eps, r ? h.data_ptr() : nullptr, y.data_ptr(),
+                   (int)(quant ? out_code : dt), quant ? scale.data_ptr<float>() : nullptr,
+                   want_inv ? inv.data_ptr<float>() : nullptr, stream_of(x));
+  return {y, h, scale, inv};
+}
+
+std::tuple<Tensor, Tensor> rms_norm_bwd(const Tensor& dy_, const OptT& dh_, const Tensor& h_, const OptT& w_,
+                                        const Tensor& inv_, bool want_dw) {
+  on_gpu(h_, "h");
+  same_device(h_, dy_, "dy");
+  same_device(h_, dh_, "dh");
+  same_device(h_, w_, "weight");
+  same_device(h_, inv_, "inv");
+  TORCH_CHECK_VALUE(h_.dim() == 2, "rms_norm_bwd: h must be [M, N]");
+  const int dt = type_code(h_, "rms_norm_bwd");
+  const int64_t M = h_.size(0), N = h_.size(1);
+  check_dtype(dy_, h_.scalar_type(), "dy");
+  check_dtype(dh_, h_.scalar_type(), "dh");
+  check_dtype(inv_, at::kFloat, "inv");
+  TORCH_CHECK_VALUE(dy_.sizes() == h_.sizes() && (!dh_ || dh_->sizes() == h_.sizes()),
+                    "rms_norm_bwd: gradients must have h's shape");
+  TORCH_CHECK_VALUE(inv_.numel() == M, "rms_norm_bwd: inv must be [M]");
+  if (w_) TORCH_CHECK_VALUE(w_->dim() == 1 && w_->size(0) == N, "rms_norm_bwd: weight must be [N]");
+  TORCH_CHECK_VALUE(!want_dw || w_, "rms_norm_bwd: a weight gradient needs the weight");
+  const int wdt = w_ ? type_code(*w_, "rms_norm weight") : dt;
+  const c10::DeviceGuard guard(h_.device());
+  const Tensor h = unit_rows(h_), dy = unit_rows(dy_), inv = inv_.contiguous();
+  const OptT dh = dh_ ? OptT(unit_rows(*dh_)) : OptT(), w = cont(w_);
+  Tensor dx = at::empty({M, N}, h.options());
+  if (M == 0) return {dx, want_dw ? at::zeros({N}, w->options()) : none_like(h)};
+  Tensor dw = want_dw ? at::empty({N}, w->options()) : none_like(h);
+  int parts = 0;
+  check_rc(prism_rms_norm_parts(M, small(N, "N"), &parts));
+  Tensor partial = want_dw ? at::empty({parts, N}, opts(h, at::kFloat)) : none_like(h);
+  PRISM_TORCH_CALL(prism_rms_norm_bwd, dy.data_ptr(), dy.stride(0), p(dh), dh ? dh->stride(0) : 0, h.data_ptr(),
+                   h.stride(0), p(w), wdt, dt, M, small(N, "N"), inv.data_ptr<float>(), dx.data_ptr(),
+                   want_dw ? partial.data_ptr<float>() : nullptr, parts, want_dw ? dw.data_ptr() : nullptr,
+                   stream_of(h));
+  return {dx, dw};
+}
+
+// ------------------------------------------------------------------ rotary positions
+Tensor like_layout(const Tensor& x) { return at::empty_like(x); }  // x's dense strides, else contiguous
+
+std::tuple<Tensor, Tensor> rotary(const Tensor& q_, const OptT& k_, const Tensor& freqs_, const Tensor& pos_,
+                                  c10::IntArrayRef axis_pairs, bool interleaved, double amplitude, bool inverse) {
+  on_gpu(q_, "q");
+  same_device(q_, k_, "k");
+  same_device(q_, freqs_, "freqs");
+  same_device(q_, pos_, "positions");
+  TORCH_CHECK_VALUE(q_.dim() == 4, "rotary: q must be [B, H, S, D]");
+  const int dt = type_code(q_, "rotary");
+  check_dtype(freqs_, at::kDouble, "freqs");
+  check_dtype(k_, q_.scalar_type(), "k");
+  const int64_t B = q_.size(0), S = q_.size(2), D = q_.size(3);
+  if (k_)
+    TORCH_CHECK_VALUE(k_->dim() == 4 && k_->size(0) == B && k_->size(2) == S && k_->size(3) == D,
+                      "rotary: k must be [B, Hk, S, D] with q's B, S and D");
+  TORCH_CHECK_VALUE(freqs_.dim() == 1, "rotary: freqs must be [pairs]");
+  TORCH_CHECK_TYPE(pos_.scalar_type() == at::kInt || pos_.scalar_type() == at::kLong,
+                   "prism: positions must be int32 or int64, got ", pos_.scalar_type());
+  // positions [S], [B, S], and with axes [S, A], [B, S, A]
+  const int64_t A = axis_pairs.empty() ? 1 : (int64_t)axis_pairs.size();
+  const bool has_axis = !axis_pairs.empty();
+  const int64_t rank = pos_.dim() - (has_axis ? 1 : 0);
+  TORCH_CHECK_VALUE((rank == 1 || rank == 2) && pos_.size(rank - 1) == S && (rank == 1 || pos_.size(0) == B || pos_.size(0) == 1) &&
+                        (!has_axis || pos_.size(-1) == A),
+                    "rotary: positions must be [S] or [B, S]", has_axis ? " with one entry per axis" : "", ", got ",
+                    pos_.sizes());
+  TORCH_CHECK_VALUE(A <= 4, "rotary: at most 4 axes");
+  const c10::DeviceGuard guard(q_.device());
+  const Tensor q = unit_rows(q_), freqs = freqs_.contiguous();
+  const OptT k = k_ ? OptT(unit_rows(*k_)) : OptT();
+  Tensor oq = like_layout(q), ok = k ? like_layout(*k) : none_like(q);
+  if (oq.numel() && oq.stride(3) != 1) oq = at::empty(q.sizes(), q.options());
+  if (k && ok.numel() && ok.stride(3) != 1) ok = at::empty(k->sizes(), k->options());
+  int64_t strides[12] = {q.stride(0), q.stride(1), q.stride(2), oq.stride(0), oq.stride(1), oq.stride(2)};
+  if (k) {
+    const int64_t s[6] = {k->stride(0), k->stride(1), k->stride(2), ok.stride(0), ok.stride(1), ok.stride(2)};
+    for (int i = 0; i < 6; ++i) strides[6 + i] = s[i];
+  }
+  const int64_t pos_strides[3] = {rank == 2 && pos_.size(0) > 1 ? pos_.stride(0) : 0, pos_.stride(rank - 1),
+                                  has_axis ? pos_.stride(-1) : 0};
+  int32_t axis_end[4] = {};
+  int64_t at = 0;
+  for (int64_t a = 0; a < A; ++a) {
+    at += has_axis ? axis_pairs[a] : freqs.numel();
+    TORCH_CHECK_VALUE(!has_axis || axis_pairs[a] >= 0, "rotary: negative axis size");
+    axis_end[a] = small(at, "pairs");
+  }
+  PRISM_TORCH_CALL(prism_rotary, q.data_ptr(), p(k), dt, small(B, "B"), S, small(q.size(1), "heads"),
+                   k ? small(k->size(1), "heads") : 0, small(D, "D"), small(2 * freqs.numel(), "rotary dim"), strides,
+                   freqs.data_ptr<double>(), pos_.data_ptr(), pos_.scalar_type() == at::kLong, pos_strides, (int)A,
+                   axis_end, interleaved, (float)amplitude, inverse, oq.data_ptr(), k ? ok.data_ptr() : nullptr,
+                   stream_of(q));
+  return {oq, ok};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(prism, m) {
+  m.def("rms_norm(Tensor x, Tensor? residual, Tensor? weight, float eps, int out_code, bool want_inv) "
+        "-> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("rms_norm_bwd(Tensor dy, Tensor? dh, Tensor h, Tensor? weight, Tensor inv, bool want_dw) -> (Tensor, Tensor)");
+  m.def("rotary(Tensor q, Tensor? k, Tensor freqs, Tensor positions, int[] axis_pairs, bool interleaved, "
+        "float amplitude, bool inverse) -> (Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(prism, CUDA, m) {
+  m.impl("rms_norm", &rms_norm);
+  m.impl("rms_norm_bwd", &rms_norm_bwd);
+  m.impl("rotary", &rotary);
+}

@@ -163,6 +163,51 @@ def linear_rownorm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
                code)
 
 
+# ------------------------------------------------------------------ layer operators
+F16, E4M3, I8 = 2, 3, 4
+_QUANT_CODES = {torch.float8_e4m3fn: E4M3, torch.int8: I8}
+
+
+def _layer_code(t: torch.Tensor, name: str) -> int:
+    code = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}.get(t.dtype)
+    if code is None:
+        raise TypeError(f"prism_amd: {name}: unsupported dtype {t.dtype} (float32, bfloat16 or float16)")
+    return code
+
+
+def rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float,
+             out_dtype: Optional[torch.dtype] = None, want_inv: bool = False):
+    """Rows [M, N]: (y, h, scale, inv) with h = x + residual (None without
+    one), y = h / sqrt(mean(h^2) + eps) * weight in x's dtype, or codes of
+    out_dtype (float8_e4m3fn, int8) with their scales [M]; inv [M] fp32 on
+    request, else None."""
+    _cuda(x, residual, weight)
+    code = _layer_code(x, "rms_norm") if out_dtype is None else _QUANT_CODES.get(out_dtype)
+    if code is None:
+        raise TypeError(f"prism_amd: rms_norm: unsupported output dtype {out_dtype} (float8_e4m3fn or int8)")
+    y, h, scale, inv = _op("rms_norm", x, residual, weight, float(eps), code, bool(want_inv))
+    return y, (h if residual is not None else None), (scale if out_dtype is not None else None), \
+        (inv if want_inv else None)
+
+
+def rms_norm_bwd(dy: torch.Tensor, dh: Optional[torch.Tensor], h: torch.Tensor, weight: Optional[torch.Tensor],
+                 inv: torch.Tensor, want_dw: bool):
+    """(dx, dw) of rms_norm's rows; dx is also the residual's gradient."""
+    _cuda(dy, dh, h, weight, inv)
+    dx, dw = _op("rms_norm_bwd", dy, dh, h, weight, inv, bool(want_dw))
+    return dx, (dw if want_dw else None)
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, positions: torch.Tensor, axis_pairs,
+           interleaved: bool, amplitude: float, inverse: bool = False):
+    """q [B,Hq,S,D] and k [B,Hk,S,D] (or None) turned by positions x freqs;
+    axis_pairs: pairs per axis ([]: one position per token).  Returns (q', k')."""
+    _cuda(q, k, freqs, positions)
+    oq, ok = _op("rotary", q, k, freqs, positions, list(axis_pairs), bool(interleaved), float(amplitude),
+                 bool(inverse))
+    return oq, (ok if k is not None else None)
+
+
 # ------------------------------------------------------------------ geometry
 class ZoneLayout:
     """Per-call block/tile bookkeeping for one set of shape ids.

@@ -1,0 +1,100 @@
+"""Argument checks of the layer's operators and the rotary frequencies, on the
+CPU (no kernel runs)."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import prism_amd
+from prism_amd import _lib
+
+
+def test_norm_refusals():
+    x = torch.randn(3, 8)
+    w = torch.ones(8)
+    with pytest.raises(ValueError, match="GPU"):
+        prism_amd.rms_norm(x, w)
+    with pytest.raises(ValueError, match="GPU"):
+        prism_amd.rms_norm_quant(x, w)
+    with pytest.raises(ValueError, match="weight"):
+        prism_amd.rms_norm(x, torch.ones(7))
+    with pytest.raises(TypeError, match="weight"):
+        prism_amd.rms_norm(x, w.double())
+    with pytest.raises(TypeError, match="residual"):
+        prism_amd.rms_norm(x, w, residual=x.half())
+    with pytest.raises(ValueError, match="residual"):
+        prism_amd.rms_norm(x, w, residual=x[:2])
+    with pytest.raises(ValueError, match="eps"):
+        prism_amd.rms_norm(x, w, eps=-1.0)
+    with pytest.raises(ValueError, match="last dimension"):
+        prism_amd.rms_norm(torch.randn(3, 0))
+    with pytest.raises(ValueError, match="gradient"):
+        prism_amd.rms_norm_quant(x.requires_grad_(True), w)
+
+
+def test_norm_capi_refusals():
+    lib = _lib.load()
+    one = ctypes.c_void_p(16)
+    for M, N, dtype, out in ((4, 0, 0, 0), (4, 16385, 0, 0), (-1, 8, 0, 0), (4, 8, 5, 5), (4, 8, 1, 0), (4, 8, 1, 3)):
+        # (the last: 8 bits without scales)
+        assert lib.prism_rms_norm(one, N, None, 0, None, dtype, dtype, M, N, 1e-6, None, one, out, None, None, None) == 1
+    assert lib.prism_rms_norm(one, 8, one, 8, None, 1, 1, 4, 8, 1e-6, None, one, 1, None, None, None) == 1  # h missing
+    assert lib.prism_rms_norm_bwd(one, 8, None, 0, one, 8, None, 1, 1, 4, 8, one, one, None, 1, one, None) == 1
+    parts = ctypes.c_int(0)
+    assert lib.prism_rms_norm_parts(75600, 5120, ctypes.byref(parts)) == 0 and 1 <= parts.value <= 1024
+    assert lib.prism_rms_norm_parts(0, 5120, ctypes.byref(parts)) == 1
+
+
+def test_rotary_refusals():
+    q = torch.randn(1, 2, 5, 16)
+    f, _ = prism_amd.rotary_frequencies(16, device="cpu")
+    at = torch.arange(5)
+    with pytest.raises(ValueError, match="GPU"):
+        prism_amd.apply_rotary(q, None, f, at)
+    with pytest.raises(TypeError, match="float64"):
+        prism_amd.apply_rotary(q, None, f.float(), at)
+    with pytest.raises(ValueError, match="fit"):
+        prism_amd.apply_rotary(q[..., :14], None, f, at)
+    with pytest.raises(ValueError, match="k "):
+        prism_amd.apply_rotary(q, q[:, :, :4], f, at)
+    with pytest.raises(ValueError, match="B, H, S, D"):
+        prism_amd.apply_rotary(q[0], None, f, at)
+    with pytest.raises(ValueError, match="sections"):
+        prism_amd.apply_rotary(q, None, f, at, sections=(8, 6))
+
+
+def test_rotary_capi_refusals():
+    lib = _lib.load()
+    one = ctypes.c_void_p(16)
+    strides, ps, ends = (ctypes.c_int64 * 12)(), (ctypes.c_int64 * 3)(), (ctypes.c_int32 * 4)(8)
+    call = lambda dtype=1, D=16, R=16, axes=1, q=one: lib.prism_rotary(  # noqa: E731
+        q, None, dtype, 1, 4, 2, 0, D, R, strides, one, one, 0, ps, axes, ends, 1, 1.0, 0, one, None, None)
+    assert [call(dtype=3), call(D=257), call(R=15), call(R=18), call(axes=5), call(axes=0), call(q=None), call(R=14)] == [1] * 8
+
+
+def test_frequencies():
+    f, a = prism_amd.rotary_frequencies(8, device="cpu")
+    assert a == 1.0 and torch.allclose(f, torch.tensor([1, 0.1, 0.01, 0.001], dtype=torch.float64))
+    f2, _ = prism_amd.rotary_frequencies(128, sections=(44, 42, 42), device="cpu")
+    one, _ = prism_amd.rotary_frequencies(42, device="cpu")
+    assert f2.shape == (64,) and torch.equal(f2[22:43], one) and torch.equal(f2[43:], one)
+    lin, _ = prism_amd.rotary_frequencies(8, scaling="linear", factor=4.0, device="cpu")
+    assert torch.allclose(lin, f / 4)
+    ntk, _ = prism_amd.rotary_frequencies(8, scaling="ntk", factor=4.0, device="cpu")
+    assert float(ntk[0]) == 1.0 and math.isclose(float(ntk[-1]), float(f[-1]) / 4, rel_tol=1e-12)
+    # yarn: the fastest pairs kept, the slowest divided, amplitude grown
+    plain, _ = prism_amd.rotary_frequencies(128, device="cpu")
+    yarn, a = prism_amd.rotary_frequencies(128, scaling="yarn", factor=8.0, original_length=8192, device="cpu")
+    turns = plain * 8192 / (2 * math.pi)
+    assert torch.equal(yarn[turns > 40], plain[turns > 40]) and torch.allclose(yarn[turns < 0.8], plain[turns < 0.8] / 8)
+    assert math.isclose(a, 0.1 * math.log(8) + 1) and (yarn <= plain).all() and (yarn >= plain / 8 * (1 - 1e-12)).all()
+    for bad in (dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=8, sections=(4, 2)), dict(rotary_dim=8, scaling="x"),
+                dict(rotary_dim=8, scaling="yarn", factor=2.0), dict(rotary_dim=8, base=0.5), dict(rotary_dim=8, factor=0.5),
+                dict(rotary_dim=4, sections=(2, 2), scaling="ntk", factor=2.0)):
+        with pytest.raises(ValueError):
+            prism_amd.rotary_frequencies(device="cpu", **bad)
+
+
+def test_grid_positions_cpu():
+    assert prism_amd.grid_positions((1, 2, 2), device="cpu").tolist() == [[0, 0, 0], [0, 0, 1], [0, 1, 0], [0, 1, 1]]
