@@ -146,6 +146,47 @@ int prism_rotary(const void* q, const void* k, int dtype, int B, int64_t S, int 
                  const int64_t* pos_strides, int axes, const int32_t* axis_end, int interleaved, float amplitude,
                  int inverse, void* out_q, void* out_k, hipStream_t stream);
 
+/* ------------------------------------------------------------------ window attention */
+
+/* Attention over a sliding window and the first tokens (sinks).  q: [B, Hq, Sq,
+ * D], k, v: [B, Hk, Sk, D] of dtype (PRISM_BF16 / PRISM_F16), D 64 or 128, Hq /
+ * Hk query heads in a row share a key head; channels adjacent, strides (host, elements: batch,
+ * head, token of q, k, v, o) multiples of 8, pointers 16-byte aligned.  With L =
+ * kv_lens[b] keys (Sk if NULL; cut to 0 .. Sk) and n = q_lens[b] queries (Sq if NULL) query i
+ * stands at p = i + L - n and sees key j < L where p - window < j <= p or j <
+ * sinks and j <= p (causal), else where |p - j| < window or j < sinks.  o: 0
+ * for queries that see nothing and rows i >= n; lse: [B, Hq, Sq] fp32 natural
+ * log-sum-exp of the scaled scores (-inf there), or NULL.  Rows of k and v that
+ * no query sees are not read.  No counterpart in the reference. */
+int prism_window_fwd(const void* q, const void* k, const void* v, int dtype, int B, int Hq, int Hk, int64_t Sq,
+                     int64_t Sk, int D, const int64_t* strides, int64_t window, int64_t sinks, int causal,
+                     const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, float* lse,
+                     hipStream_t stream);
+
+/* prism_window_fwd for few query rows over many keys (single tokens over a
+ * cache): the keys are cut over `splits` workgroups per 32 rows, whose partial
+ * results part_o (floats * D floats) and part_ml (2 * floats) a second kernel
+ * joins in order; prism_window_token_plan gives splits and floats (0 for one
+ * split: no workspace). */
+int prism_window_token_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int64_t window, int64_t sinks, int causal,
+                            int* splits, int64_t* floats);
+int prism_window_token(const void* q, const void* k, const void* v, int dtype, int B, int Hq, int Hk, int64_t Sq,
+                       int64_t Sk, int D, const int64_t* strides, int64_t window, int64_t sinks, int causal,
+                       const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, float* lse, int splits,
+                       float* part_o, float* part_ml, hipStream_t stream);
+
+/* Gradients of prism_window_fwd from do [B, Hq, Sq, D], its o and lse: dq, dk,
+ * dv (rows that nothing reaches are 0).  strides (host): batch, head, token of
+ * q, k, v, o, do, dq, dk, dv, as above.  rows: workspace of 2 * B * Hq * Sq
+ * floats; acc: of as many floats as prism_window_bwd_plan says (NULL for 0).
+ * Deterministic (no atomics). */
+int prism_window_bwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal,
+                          int64_t* floats);
+int prism_window_bwd(const void* do_, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                     int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, const int64_t* strides,
+                     int64_t window, int64_t sinks, int causal, const int32_t* q_lens, const int32_t* kv_lens,
+                     float sm_scale, void* dq, void* dk, void* dv, float* rows, float* acc, hipStream_t stream);
+
 /* ------------------------------------------------------------------ geometry */
 
 /* _build_block_tile_maps (dynamic_block_attention.py:138-170) in CSR form.

@@ -10,6 +10,7 @@ Public surface (reference names):
   flash_attn_bsa              bsa_interface.py:683 (_attention_bsa.apply)
   a2v_token_norms             wan_video_dit.py:742-752 (A2V residual norms)
   a2v_bridge_projection       interactionv2.py:348 o-projection with the norms fused
+  flash_attn_window           attention over a sliding window and the first tokens
 and what the layer runs around it (wan_video_dit.py:699-705):
   rms_norm, rms_norm_quant    residual addition + root-mean-square norm, 8-bit output
   rotary_frequencies, apply_rotary, grid_positions  rotary positions on q and k
@@ -26,5 +27,6 @@ from .adapter import DynamicBlockSparseAttention, a2v_bridge_projection, a2v_tok
 from .rotary import apply_rotary, grid_positions, rotary_frequencies  # noqa: F401
 from .row_norm import rms_norm, rms_norm_quant  # noqa: F401
 from .uniform_block_attention import flash_attn_bsa, flash_attn_bsa_3d, flash_attn_bsa_cross  # noqa: F401
+from .window_attention import flash_attn_window  # noqa: F401
 
 __version__ = "0.1.0"

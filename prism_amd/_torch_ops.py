@@ -106,6 +106,14 @@ def _register_fakes():
     def _(q, k, freqs, positions, axis_pairs, interleaved, amplitude, inverse):
         return torch.empty_like(q), torch.empty_like(k) if k is not None else _none(q)
 
+    @reg("prism::window_fwd")
+    def _(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse):
+        return torch.empty_like(q), _empty(q, q.shape[:3], f32) if want_lse else _none(q)
+
+    @reg("prism::window_bwd")
+    def _(do, q, k, v, o, lse, window, sinks, causal, q_lens, kv_lens, sm_scale):
+        return torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+
     @reg("prism::zone_layout")
     def _(shape_ids):
         nz = shape_ids.numel()

@@ -31,7 +31,8 @@ TORCH_OPS_SRCS = ["torch_ops.cpp", "torch_layer_ops.cpp"]
 TORCH_OPS_PATH = os.path.join(HERE, "libprism_torch.so")
 
 SOURCES = ["errors.hip", "stats.hip", "layout.hip", "select.hip", "lists.hip", "attn_fwd.hip", "attn_bwd.hip",
-           "oproj.hip", "rownorm.hip", "rotary.hip", "validate.hip", "peak.hip"]
+           "oproj.hip", "rownorm.hip", "rotary.hip", "window_fwd.hip", "window_token.hip", "window_bwd.hip",
+           "validate.hip", "peak.hip"]
 CANONICAL = {"stats.hip", "layout.hip", "select.hip"}
 
 COMMON_FLAGS = [

@@ -150,6 +150,119 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& q_, const OptT& k_, const Tensor
   return {oq, ok};
 }
 
+// ------------------------------------------------------------------ window attention
+// t as the window kernels take it: adjacent channels, 16-byte aligned rows at
+// strides of whole 16-byte pieces; else a contiguous copy
+Tensor win_rows(const Tensor& t) {
+  bool ok = t.numel() == 0 || (t.stride(3) == 1 && (uintptr_t)t.data_ptr() % 16 == 0);
+  for (int d = 0; d < 3 && ok; ++d) ok = t.size(d) <= 1 || t.stride(d) % 8 == 0;
+  if (ok && t.size(2) > 1) ok = t.stride(2) < (1 << 24);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+void win_strides(const Tensor& t, int64_t* s) {
+  for (int d = 0; d < 3; ++d) s[d] = t.size(d) > 1 ? t.stride(d) : 0;
+}
+Tensor win_like(const Tensor& t) {
+  Tensor o = at::empty_like(t);  // t's layout where that is dense
+  return o.numel() == 0 || o.stride(3) == 1 ? o : at::empty(t.sizes(), t.options());
+}
+
+// query rows (tokens x heads of a group) up to which a call goes to the kernel
+// for single tokens
+constexpr int64_t kTokenRows = 64;
+
+struct WinShape {
+  int dt;
+  int64_t B, Hq, Hk, Sq, Sk, D;
+};
+WinShape check_window(const Tensor& q, const Tensor& k, const Tensor& v, const OptT& q_lens, const OptT& kv_lens) {
+  on_gpu(q, "q");
+  same_device(q, k, "k");
+  same_device(q, v, "v");
+  same_device(q, q_lens, "q_lens");
+  same_device(q, kv_lens, "kv_lens");
+  TORCH_CHECK_TYPE(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf,
+                   "prism: window attention takes bfloat16 or float16, got ", q.scalar_type());
+  check_dtype(k, q.scalar_type(), "k");
+  check_dtype(v, q.scalar_type(), "v");
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == q.size(0) &&
+                        k.size(3) == q.size(3),
+                    "window attention: q must be [B, Hq, Sq, D], k and v [B, Hk, Sk, D], got ", q.sizes(), ", ",
+                    k.sizes(), ", ", v.sizes());
+  WinShape s{q.scalar_type() == at::kBFloat16 ? PRISM_BF16 : PRISM_F16, q.size(0), q.size(1), k.size(1), q.size(2),
+             k.size(2), q.size(3)};
+  for (const OptT* l : {&q_lens, &kv_lens}) {
+    check_dtype(*l, at::kInt, "lengths");
+    if (*l) TORCH_CHECK_VALUE((*l)->dim() == 1 && (*l)->size(0) == s.B, "window attention: lengths must be [B]");
+  }
+  return s;
+}
+
+std::tuple<Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window,
+                                      int64_t sinks, bool causal, const OptT& q_lens_, const OptT& kv_lens_,
+                                      double sm_scale, bool want_lse) {
+  const WinShape s = check_window(q_, k_, v_, q_lens_, kv_lens_);
+  const c10::DeviceGuard guard(q_.device());
+  const Tensor q = win_rows(q_), k = win_rows(k_), v = win_rows(v_);
+  const OptT q_lens = cont(q_lens_), kv_lens = cont(kv_lens_);
+  Tensor o = win_like(q);
+  Tensor lse = want_lse ? at::empty({s.B, s.Hq, s.Sq}, opts(q, at::kFloat)) : none_like(q);
+  int64_t st[12];
+  win_strides(q, st);
+  win_strides(k, st + 3);
+  win_strides(v, st + 6);
+  win_strides(o, st + 9);
+  float* lp = want_lse ? lse.data_ptr<float>() : nullptr;
+  const int B = small(s.B, "B"), Hq = small(s.Hq, "heads"), Hk = small(s.Hk, "heads"), D = small(s.D, "D");
+  if (s.Hk > 0 && s.Sq * (s.Hq / s.Hk) <= kTokenRows) {
+    int splits = 1;
+    int64_t floats = 0;
+    check_rc(prism_window_token_plan(B, Hq, Hk, s.Sq, s.Sk, window, sinks, causal, &splits, &floats));
+    Tensor part = splits > 1 ? at::empty({floats * (s.D + 2)}, opts(q, at::kFloat)) : none_like(q);
+    float* po = splits > 1 ? part.data_ptr<float>() : nullptr;
+    PRISM_TORCH_CALL(prism_window_token, q.data_ptr(), k.data_ptr(), v.data_ptr(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st,
+                     window, sinks, causal, (const int32_t*)p(q_lens), (const int32_t*)p(kv_lens), (float)sm_scale,
+                     o.data_ptr(), lp, splits, po, po ? po + floats * s.D : nullptr, stream_of(q));
+    return {o, lse};
+  }
+  PRISM_TORCH_CALL(prism_window_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st,
+                   window, sinks, causal, (const int32_t*)p(q_lens), (const int32_t*)p(kv_lens), (float)sm_scale,
+                   o.data_ptr(), lp, stream_of(q));
+  return {o, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor> window_bwd(const Tensor& do_, const Tensor& q_, const Tensor& k_, const Tensor& v_,
+                                              const Tensor& o_, const Tensor& lse_, int64_t window, int64_t sinks,
+                                              bool causal, const OptT& q_lens_, const OptT& kv_lens_,
+                                              double sm_scale) {
+  const WinShape s = check_window(q_, k_, v_, q_lens_, kv_lens_);
+  for (const auto& t : {std::make_pair(&do_, "do"), std::make_pair(&o_, "o")}) {
+    same_device(q_, *t.first, t.second);
+    check_dtype(*t.first, q_.scalar_type(), t.second);
+    TORCH_CHECK_VALUE(t.first->sizes() == q_.sizes(), "window_bwd: ", t.second, " must have q's shape");
+  }
+  same_device(q_, lse_, "lse");
+  check_dtype(lse_, at::kFloat, "lse");
+  TORCH_CHECK_VALUE(lse_.numel() == s.B * s.Hq * s.Sq, "window_bwd: lse must be [B, Hq, Sq]");
+  const c10::DeviceGuard guard(q_.device());
+  const Tensor q = win_rows(q_), k = win_rows(k_), v = win_rows(v_), o = win_rows(o_), d = win_rows(do_);
+  const Tensor lse = lse_.contiguous();
+  const OptT q_lens = cont(q_lens_), kv_lens = cont(kv_lens_);
+  Tensor dq = win_like(q), dk = win_like(k), dv = win_like(v);
+  int64_t st[24], floats = 0;
+  const Tensor* all[8] = {&q, &k, &v, &o, &d, &dq, &dk, &dv};
+  for (int i = 0; i < 8; ++i) win_strides(*all[i], st + 3 * i);
+  const int B = small(s.B, "B"), Hq = small(s.Hq, "heads"), Hk = small(s.Hk, "heads"), D = small(s.D, "D");
+  check_rc(prism_window_bwd_plan(B, Hq, Hk, s.Sq, s.Sk, D, window, sinks, causal, &floats));
+  Tensor rows = at::empty({2 * s.B * s.Hq * s.Sq}, opts(q, at::kFloat));
+  Tensor acc = floats ? at::empty({floats}, opts(q, at::kFloat)) : none_like(q);
+  PRISM_TORCH_CALL(prism_window_bwd, d.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                   lse.data_ptr<float>(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st, window, sinks, causal,
+                   (const int32_t*)p(q_lens), (const int32_t*)p(kv_lens), (float)sm_scale, dq.data_ptr(), dk.data_ptr(),
+                   dv.data_ptr(), rows.data_ptr<float>(), floats ? acc.data_ptr<float>() : nullptr, stream_of(q));
+  return {dq, dk, dv};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(prism, m) {
@@ -158,10 +271,16 @@ TORCH_LIBRARY_FRAGMENT(prism, m) {
   m.def("rms_norm_bwd(Tensor dy, Tensor? dh, Tensor h, Tensor? weight, Tensor inv, bool want_dw) -> (Tensor, Tensor)");
   m.def("rotary(Tensor q, Tensor? k, Tensor freqs, Tensor positions, int[] axis_pairs, bool interleaved, "
         "float amplitude, bool inverse) -> (Tensor, Tensor)");
+  m.def("window_fwd(Tensor q, Tensor k, Tensor v, int window, int sinks, bool causal, Tensor? q_lens, "
+        "Tensor? kv_lens, float sm_scale, bool want_lse) -> (Tensor, Tensor)");
+  m.def("window_bwd(Tensor do, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, int window, int sinks, bool causal, "
+        "Tensor? q_lens, Tensor? kv_lens, float sm_scale) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(prism, CUDA, m) {
   m.impl("rms_norm", &rms_norm);
   m.impl("rms_norm_bwd", &rms_norm_bwd);
   m.impl("rotary", &rotary);
+  m.impl("window_fwd", &window_fwd);
+  m.impl("window_bwd", &window_bwd);
 }

@@ -1,0 +1,252 @@
+// What the window attention kernels share (gfx950): which keys a run of query
+// rows sees, the copies of their K and V rows into LDS, element types.
+//
+// Rows.  The G query heads that share a key head are one set of rows: row r of
+// a (sequence, key head) is token r / G of query head hk G + r % G, so a tile of
+// rows covers few tokens and each staged K / V tile serves all heads of the
+// group.
+//
+// Keys.  Token i of a sequence with L keys and n queries stands at p = i + L -
+// n.  A run of tokens sees the sinks [0, nsink) and the keys [ws, hi] of its
+// windows: a virtual list u = 0 .. n - 1 with key(u) = u for u < nsink, u + shift
+// beyond.  Tiles of 64 (or 32) entries of that list are staged, so a few sinks
+// cost no tile of their own, and rows of memory that no query of the run sees
+// are never read (an entry past the end re-reads the last one): what stands in
+// unused cache rows, NaN included, cannot reach a result.  Entry u is visible to
+// the token at p where a <= u <= b or u < c (TokenSpan).
+#pragma once
+#include <initializer_list>
+
+#include "common.h"
+#include "mfma.h"
+#include "tile_dma.h"
+
+// ------------------------------------------------------------ element types
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+struct WinBf16 {
+  static __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16(a, b); }
+  static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+};
+// (operands travel as bf16x8: eight 16-bit values whatever their type)
+struct WinF16 {
+  static __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+  }
+  static __device__ __forceinline__ float lo(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[0]; }
+  static __device__ __forceinline__ float hi(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[1]; }
+};
+
+// B operand of k-step tt from an accumulator of 32-row blocks (b_from_acc for either type)
+template <class E>
+__device__ __forceinline__ bf16x8 win_b_from_acc(const f32x16* acc, int tt) {
+  const int h = tt >> 1, j0 = 2 * (tt & 1);
+  uint4 pb;
+  pb.x = E::pack(acc[h][4 * j0 + 0], acc[h][4 * j0 + 1]);
+  pb.y = E::pack(acc[h][4 * j0 + 2], acc[h][4 * j0 + 3]);
+  pb.z = E::pack(acc[h][4 * j0 + 4], acc[h][4 * j0 + 5]);
+  pb.w = E::pack(acc[h][4 * j0 + 6], acc[h][4 * j0 + 7]);
+  return as_bf16x8(pb);
+}
+
+// ------------------------------------------------------------ arguments
+struct WinTensor {  // [B, H, S, D], channels adjacent; strides in elements
+  uint16_t* p;
+  int64_t b, h, s;
+};
+struct WinArgs {
+  WinTensor q, k, v, o;
+  const int32_t *q_lens, *kv_lens;  // [B] or null
+  int B, Hk, G, Sq, Sk;
+  int window, sinks, causal;
+  float scale, scale_log2;
+  float* lse;                       // [B, Hk G, Sq] natural log, -inf for rows that see nothing; or null
+  int tiles;                        // row tiles of a (sequence, key head)
+  int total;                        // work items of the launch
+  // single tokens: key splits, their partial results (o [splits, B Hk, tiles, 32, D], m and l [.., 32] each)
+  int splits;
+  float *part_o, *part_ml;
+};
+
+// ------------------------------------------------------------ spans
+struct SeqSpan {
+  int L, n, off;  // keys, queries, position of token 0
+};
+__device__ __forceinline__ SeqSpan seq_span(const WinArgs& a, int b) {
+  SeqSpan s;
+  s.L = a.Sk;
+  s.n = a.Sq;
+  if (a.kv_lens) {  // (lengths outside the tensors are cut to them)
+    const int x = a.kv_lens[b];
+    s.L = x < 0 ? 0 : x < a.Sk ? x : a.Sk;
+  }
+  if (a.q_lens) {
+    const int x = a.q_lens[b];
+    s.n = x < 0 ? 0 : x < a.Sq ? x : a.Sq;
+  }
+  s.off = s.L - s.n;
+  return s;
+}
+
+// the virtual key list of tokens i0 .. i1 (i0 > i1: none)
+struct KeyList {
+  int nsink, shift, n;
+  __device__ __forceinline__ int key(int u) const { return u < nsink ? u : u + shift; }
+};
+__device__ __forceinline__ KeyList key_list(const WinArgs& a, const SeqSpan& s, int i0, int i1) {
+  KeyList k;
+  const int pmin = i0 + s.off, pmax = i1 + s.off;
+  const int top = a.causal ? pmax : pmax + a.window - 1;
+  const int hi = top < s.L - 1 ? top : s.L - 1;
+  int ns = a.causal ? (a.sinks < pmax + 1 ? a.sinks : pmax + 1) : a.sinks;
+  ns = ns < s.L ? ns : s.L;
+  ns = ns > 0 ? ns : 0;
+  const int lo = pmin - a.window + 1;
+  const int ws = lo > ns ? lo : ns;
+  k.nsink = ns;
+  k.shift = ws - ns;
+  k.n = ns + (hi >= ws ? hi - ws + 1 : 0);
+  if (i0 > i1) k.n = k.nsink = 0;
+  return k;
+}
+
+// entries of the list that the token at p sees: a <= u <= b or u < c
+struct TokenSpan {
+  int a, b, c;
+};
+__device__ __forceinline__ TokenSpan token_span(const WinArgs& a, const KeyList& k, int p) {
+  TokenSpan t;
+  const int lo = p - a.window + 1 - k.shift, hi = (a.causal ? p : p + a.window - 1) - k.shift;
+  t.a = lo > k.nsink ? lo : k.nsink;
+  t.b = hi < k.n - 1 ? hi : k.n - 1;
+  t.c = a.causal && p + 1 < k.nsink ? p + 1 : k.nsink;
+  return t;
+}
+// bit j of the result: entry u0 + j is visible, j < 64
+__device__ __forceinline__ uint64_t span_bits(const TokenSpan& t, int u0) {
+  const int lo = t.a - u0 > 0 ? t.a - u0 : 0, hi = t.b - u0 < 63 ? t.b - u0 : 63;
+  uint64_t m = hi >= lo ? (~0ull << lo) & (~0ull >> (63 - hi)) : 0ull;
+  const int c = t.c - u0;
+  m |= c >= 64 ? ~0ull : c > 0 ? (1ull << c) - 1 : 0ull;
+  return m;
+}
+
+// Which entries the tokens p0 .. p1 of a wave see: some of [u0, u1], all of it.
+// (token_span's bounds grow with p, so the ends of the run give them.)
+struct WaveSpan {
+  int a_any, b_any, c_any, a_all, b_all, c_all;
+  __device__ __forceinline__ void init(const WinArgs& w, const KeyList& k, int p0, int p1) {
+    const TokenSpan f = token_span(w, k, p0), l = token_span(w, k, p1);
+    a_any = f.a; b_any = l.b; c_any = l.c;
+    a_all = l.a; b_all = f.b; c_all = f.c;
+  }
+  __device__ __forceinline__ bool any(int u0, int u1) const { return (u1 >= a_any && u0 <= b_any) || u0 < c_any; }
+  __device__ __forceinline__ bool all(int u0, int u1) const { return (u0 >= a_all && u1 <= b_all) || u1 < c_all; }
+};
+
+// ------------------------------------------------------------ copies
+// 16 bytes per lane from a 64-bit address of its own: LDS[m0 + 16 lane] <- *src
+__device__ __forceinline__ void dma_b128_from(const void* src, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0) : "m0");
+}
+
+// Row and byte of the row that lane `lane` of KB-instruction i of a row tile
+// fetches (RowTile::src_offset for rows that are not adjacent in memory).
+// Instruction i + 4m is 4096 m / W rows further on, at the same byte.
+template <int D>
+struct RowSource {
+  using RT = RowTile<D>;
+  static constexpr int ROWS4 = 4096 / RT::W;
+  static __device__ __forceinline__ int row(int i, int lane) {
+    const int pos = 1024 * i + 16 * lane;
+    return 4 * (pos / RT::Q) + (((pos % RT::Q) >> 6) & 3);
+  }
+  static __device__ __forceinline__ int byte(int i, int lane) {
+    const int pos = 1024 * i + 16 * lane, rq = pos / RT::Q, rem = pos - rq * RT::Q;
+    return 16 * (4 * (rem >> 8) + (((rem >> 4) & 3) ^ (rq & 3)));
+  }
+};
+
+template <int D>
+struct WinTiles {
+  using RT = RowTile<D>;
+  static constexpr int STAGE = 2 * RT::BYTES, STAGE_KB = 2 * RT::KB;
+};
+
+// the tile copies of a 64-entry stage (K then V) by two waves (wid 0, 1)
+template <int D>
+struct StageCopy {
+  using RT = RowTile<D>;
+  using RS = RowSource<D>;
+  static constexpr int COUNT = RT::KB;  // instructions per wave and stage
+  const uint8_t *kb, *vb;               // K and V of the (sequence, key head)
+  int64_t kstep, vstep;                 // bytes per row
+  uint32_t koff[2], voff[2];            // lane offsets of instructions wid, wid + 2
+  int wid, lane;
+  __device__ __forceinline__ void init(const WinArgs& a, int b, int hk, int wid_, int lane_) {
+    wid = wid_;
+    lane = lane_;
+    kb = (const uint8_t*)uniform_ptr(a.k.p + b * a.k.b + hk * a.k.h);
+    vb = (const uint8_t*)uniform_ptr(a.v.p + b * a.v.b + hk * a.v.h);
+    kstep = 2 * a.k.s;
+    vstep = 2 * a.v.s;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = RS::row(wid + 2 * x, lane), c = RS::byte(wid + 2 * x, lane);
+      koff[x] = (uint32_t)r * (uint32_t)kstep + (uint32_t)c;
+      voff[x] = (uint32_t)r * (uint32_t)vstep + (uint32_t)c;
+    }
+  }
+  __device__ __forceinline__ void issue(const KeyList& k, int u0, uint32_t lds) const {
+    if ((u0 >= k.nsink || u0 + 63 < k.nsink) && u0 + 63 < k.n) {  // 64 adjacent keys
+      const int key0 = k.key(u0);
+      const uint8_t* kt = (const uint8_t*)uniform_ptr(kb + key0 * kstep);
+      const uint8_t* vt = (const uint8_t*)uniform_ptr(vb + key0 * vstep);
+#pragma unroll
+      for (int s = 0; s < COUNT; ++s) {
+        const int i = wid + 2 * s;
+        const bool isk = 2 * s < RT::KB;
+        const int m = ((2 * s) % RT::KB) >> 2;  // (instruction wid + 2 (s & 1) + 4 m of its tile)
+        const uint8_t* base = isk ? kt + m * RS::ROWS4 * kstep : vt + m * RS::ROWS4 * vstep;
+        dma_b128(isk ? koff[s & 1] : voff[s & 1], base, lds + (uint32_t)i * 1024u);
+      }
+      return;
+    }
+#pragma unroll 1
+    for (int s = 0; s < COUNT; ++s) {
+      const int i = wid + 2 * s, t = i < RT::KB ? i : i - RT::KB;
+      const int u = u0 + RS::row(t, lane), key = k.key(u < k.n ? u : k.n - 1);
+      const uint8_t* src = (i < RT::KB ? kb + key * kstep : vb + key * vstep) + RS::byte(t, lane);
+      dma_b128_from(src, uniform_u32(lds + (uint32_t)i * 1024u));
+    }
+  }
+};
+
+// work item -> (sequence, key head, row tile): row tiles of one key head are
+// neighbours (their windows overlap in an XCD's L2), the last ones, whose causal
+// lists are longest, first
+__device__ __forceinline__ void win_item(const WinArgs& a, int id, int& b, int& hk, int& tile) {
+  const int bh = id / a.tiles;
+  tile = a.tiles - 1 - (id - bh * a.tiles);
+  b = bh / a.Hk;
+  hk = bh - b * a.Hk;
+}
+
+// ------------------------------------------------------------ host side (window_fwd.hip)
+// PRISM_OK if the sizes, strides (3 per tensor) and pointers are what the kernels assume
+int win_check(const char* name, int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window,
+              int64_t sinks, float sm_scale, const int64_t* strides, int tensors,
+              std::initializer_list<const void*> pointers);
+// the arguments that all launches share (strides: q, k, v, o)
+WinArgs win_args(const void* q, const void* k, const void* v, void* o, int B, int Hq, int Hk, int64_t Sq, int64_t Sk,
+                 const int64_t* strides, int64_t window, int64_t sinks, int causal, const int32_t* q_lens,
+                 const int32_t* kv_lens, float sm_scale);

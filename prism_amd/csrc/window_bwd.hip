@@ -1,0 +1,680 @@
+// Window attention backward (gfx950, v_mfma_f32_32x32x16), of window_fwd.hip:
+//
+//   P = exp(scale q k - lse),  delta = rowsum(o do),  dS = P (do v - delta)
+//   dv = P^T do,  dk = scale dS^T q,  dq = scale dS k
+//
+// window_dq_kernel, by 128 rows, over the key list of the forward: S^T and dP^T
+// keep one query per lane column, dQ^T += K^T dS^T.  It also forms delta from
+// the rows of o and do that it holds, and leaves (m2, delta) = (lse log2 e, delta) of
+// every row for the second kernel.
+// window_dkdv_kernel, by 128 keys, over the tokens that see them, one query head
+// of the group after the other: eight waves, the two halves of each 64-row query
+// tile on different waves (partial sums added through LDS in a fixed order), the
+// two waves of a SIMD half an entry apart, as the block-sparse dK/dV
+// (attn_bwd.hip).  The sinks' key tiles are seen by every later token: long
+// lists, and all lists of a launch of few key tiles, are cut over several
+// workgroups, whose fp32 sums window_merge_kernel adds in order.  No atomics: the
+// same bits every time; sums over the heads that share a key head are fp32.
+//
+// Numbers: P and dS are rounded to the inputs' type for the products (float16: a
+// dS beyond 65,504 becomes infinite, which a loss scaler sees), the rest is fp32.
+#include <type_traits>
+
+#include "window.h"
+
+namespace {
+
+struct WinBwdArgs {
+  WinArgs w;                 // (w.o: the forward's output; w.lse: its lse)
+  WinTensor do_, dq, dk, dv;
+  float* m2;                 // [B Hq, Sq]
+  float* delta;              // [B Hq, Sq]
+  // dK/dV items: per (sequence, key head) the sink tiles, then the rest, each in
+  // its number of pieces; pieces of a cut tile leave their sums in acc
+  int sink_tiles, key_tiles, sink_splits, rest_splits, items;
+  float4* acc;
+};
+
+template <class E>
+__device__ __forceinline__ float dot8(bf16x8 a, bf16x8 b, float s) {
+  const uint4 x = __builtin_bit_cast(uint4, a), y = __builtin_bit_cast(uint4, b);
+  const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s = __builtin_fmaf(E::lo(xs[i]), E::lo(ys[i]), s);
+    s = __builtin_fmaf(E::hi(xs[i]), E::hi(ys[i]), s);
+  }
+  return s;
+}
+__device__ __forceinline__ float keep_or_zero(float x, uint32_t bits, int b) {
+  return __uint_as_float(__float_as_uint(x) & (uint32_t)__builtin_amdgcn_sbfe((int)bits, (uint32_t)b, 1u));
+}
+
+template <class E, int D>
+__global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs ba) {
+  const WinArgs& a = ba.w;
+  using T = WinTiles<D>;
+  using RT = typename T::RT;
+  constexpr int NS = D / 16, NDT = D / 32;
+  __shared__ __align__(1024) uint8_t smem[2 * T::STAGE];
+  const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+  const int w = (int)uniform_u32(threadIdx.x >> 6);
+  int b, hk, tile;
+  win_item(a, xcd_group_remap<32>((int)blockIdx.x, a.total), b, hk, tile);
+  const SeqSpan sq = seq_span(a, b);
+  const int rows = a.Sq * a.G, r0 = tile * 128, wr0 = r0 + 32 * w;
+  const int last = sq.n - 1;
+  auto token = [&](int r) { const int i = r / a.G; return i < last ? i : last; };
+  const KeyList kl = r0 / a.G > last ? KeyList{0, 0, 0} : key_list(a, sq, r0 / a.G, token(r0 + 127));
+  const int nt = (kl.n + 63) >> 6;
+
+  StageCopy<D> copy;
+  copy.init(a, b, hk, w & 1, lane);
+  const uint32_t lds0 = lds_addr(smem);
+  if (w < 2 && nt > 0) copy.issue(kl, 0, lds0);
+
+  RowOperand rop;  // K / V rows l32 (+ 32 kh as an immediate)
+  rop.init<RT>(0, l32, g);
+  TrOperand top;   // K^T over key rows 0 .. 63
+  top.init<RT>(0, lane);
+
+  const int r = wr0 + l32, rc = r < rows ? r : rows - 1;
+  const int i = rc / a.G, head = hk * a.G + (rc - i * a.G);
+  const int64_t lrow = ((int64_t)b * a.Hk * a.G + head) * a.Sq + i;
+  const bool live = i <= last;
+  bf16x8 qf[NS], df[NS];
+  float dlt = 0.0f;
+  {
+    const uint16_t* qp = a.q.p + b * a.q.b + head * a.q.h + i * a.q.s + 8 * g;
+    const uint16_t* dp = ba.do_.p + b * ba.do_.b + head * ba.do_.h + i * ba.do_.s + 8 * g;
+    const uint16_t* op = a.o.p + b * a.o.b + head * a.o.h + i * a.o.s + 8 * g;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      qf[s] = ld_bf16x8(qp + 16 * s);
+      df[s] = ld_bf16x8(dp + 16 * s);
+      dlt = dot8<E>(ld_bf16x8(op + 16 * s), df[s], dlt);
+    }
+  }
+  dlt = xor32_add(dlt);
+  const float lse = a.lse[lrow];
+  // rows that see nothing: P = 2^(s - inf) = 0
+  const float mq = lse == -__builtin_inff() ? __builtin_inff() : lse * 1.4426950408889634f;
+  if (r < rows && g == 0) {
+    ba.m2[lrow] = mq;
+    ba.delta[lrow] = dlt;
+  }
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    consume_regs(qf[s]);
+    consume_regs(df[s]);
+  }
+  consume_regs(mq);
+  consume_regs(dlt);
+  TokenSpan span = token_span(a, kl, i + sq.off);
+  if (!live) span = TokenSpan{1, 0, 0};
+  const int wi0 = (int)uniform_u32((uint32_t)(wr0 / a.G)), wi1 = (int)uniform_u32((uint32_t)token(wr0 + 31));
+  const bool some = wi0 <= last && wr0 < rows;
+  const bool whole = (wr0 + 31) / a.G <= last;
+  WaveSpan ws;
+  ws.init(a, kl, wi0 + sq.off, wi1 + sq.off);
+
+  f32x16 ndl;  // the dP^T chains start from -delta
+#pragma unroll
+  for (int x = 0; x < 16; ++x) ndl[x] = -dlt;
+  f32x16 dq[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) dq[dt] = f32x16_zero();
+
+  for (int t = 0; t < nt; ++t) {
+    dma_wait_all();
+    __syncthreads();
+    if (w < 2 && t + 1 < nt) copy.issue(kl, 64 * (t + 1), lds0 + (uint32_t)(((t + 1) & 1) * T::STAGE));
+    const int u0 = 64 * t;
+    if (!some || !ws.any(u0, u0 + 63)) continue;
+    const uint8_t* sK = smem + (t & 1) * T::STAGE;
+    const uint8_t* sV = sK + RT::BYTES;
+    f32x16 sacc[2] = {f32x16_zero(), f32x16_zero()}, pacc[2] = {ndl, ndl};
+    {
+      constexpr int NO = 4 * NS, RING = 4;
+      bf16x8 op[RING];
+      auto rd = [&](int x) { return rop.load(((x & 1) ? sV : sK) + RT::rows(32 * ((x >> 1) & 1)), x >> 2); };
+#pragma unroll
+      for (int x = 0; x + 1 < RING; ++x) op[x] = rd(x);
+#pragma unroll
+      for (int x = 0; x < NO; ++x) {
+        if (x + RING - 1 < NO) op[(x + RING - 1) % RING] = rd(x + RING - 1);
+        const int kh = (x >> 1) & 1;
+        if (x & 1) pacc[kh] = E::mfma(op[x % RING], df[x >> 2], pacc[kh]);
+        else sacc[kh] = E::mfma(op[x % RING], qf[x >> 2], sacc[kh]);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, RING - 1, 0);
+#pragma unroll
+      for (int x = 0; x + RING - 1 < NO; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, RING - 1, 0);
+    }
+    constexpr int NQ = 4 * NDT, RQ = 4;
+    bf16x8 kt[RQ];
+    auto rdk = [&](int x) { return top.load<RT>(sK, x / NDT, x % NDT); };
+#pragma unroll
+    for (int x = 0; x + 1 < RQ; ++x) kt[x] = rdk(x);
+    __builtin_amdgcn_s_setprio(1);
+    if (!whole || !ws.all(u0, u0 + 63)) {
+      const uint64_t mm = span_bits(span, u0) >> (4 * g);
+      const uint32_t bits[2] = {(uint32_t)mm, (uint32_t)(mm >> 32)};
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const int bit = 8 * (x >> 2) + (x & 3);
+          sacc[kh][x] = keep_or_ninf(sacc[kh][x], bits[kh], bit);
+          pacc[kh][x] = keep_or_zero(pacc[kh][x], bits[kh], bit);  // (what is not finite there stays out)
+        }
+    }
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const float p = fast_exp2(__builtin_fmaf(sacc[kh][x], a.scale_log2, -mq));
+        pacc[kh][x] = p * pacc[kh][x];
+      }
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
+      const bf16x8 sb = win_b_from_acc<E>(pacc, tt);
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) {
+        const int x = tt * NDT + dt;
+        if (x + RQ - 1 < NQ) kt[(x + RQ - 1) % RQ] = rdk(x + RQ - 1);
+        dq[dt] = E::mfma(kt[x % RQ], sb, dq[dt]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (x + RQ - 1 < NQ) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  }
+  if (r >= rows) return;
+  uint16_t* dqr = ba.dq.p + b * ba.dq.b + head * ba.dq.h + i * ba.dq.s;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+      uint2 o;
+      o.x = E::pack(dq[dt][4 * jj + 0] * a.scale, dq[dt][4 * jj + 1] * a.scale);
+      o.y = E::pack(dq[dt][4 * jj + 2] * a.scale, dq[dt][4 * jj + 3] * a.scale);
+      *reinterpret_cast<uint2*>(dqr + 32 * dt + 8 * jj + 4 * g) = o;
+    }
+}
+
+// ------------------------------------------------------------ dK / dV
+// Tokens that see key j: i0 <= i <= i1
+struct TokenRange {
+  int i0, i1;
+};
+__device__ __forceinline__ TokenRange tokens_of(const WinArgs& a, const SeqSpan& s, int j) {
+  if (j >= s.L) return {1, 0};
+  const bool sink = j < a.sinks;
+  const int p0 = a.causal ? j : sink ? s.off : j - a.window + 1;
+  const int i0 = p0 - s.off, i1 = j + a.window - 1 - s.off, end = s.n - 1;
+  return {i0 > 0 ? i0 : 0, sink || i1 > end ? end : i1};
+}
+
+struct DkdvItem {
+  int b, hk, tile, split, splits, slot;  // slot: first workspace piece of a cut tile plus split, -1: whole
+};
+__device__ __forceinline__ DkdvItem dkdv_item(const WinBwdArgs& a, int id) {
+  const int rest = a.key_tiles - a.sink_tiles;
+  const int per = a.sink_tiles * a.sink_splits + rest * a.rest_splits;
+  const int cut = (a.sink_splits > 1 ? a.sink_tiles * a.sink_splits : 0) + (a.rest_splits > 1 ? rest * a.rest_splits : 0);
+  const int bh = id / per, x = id - bh * per, sinks = a.sink_tiles * a.sink_splits;
+  DkdvItem d;
+  d.b = bh / a.w.Hk;
+  d.hk = bh - d.b * a.w.Hk;
+  const bool sink = x < sinks;
+  d.splits = sink ? a.sink_splits : a.rest_splits;
+  const int y = sink ? x : x - sinks;
+  d.tile = (sink ? 0 : a.sink_tiles) + y / d.splits;
+  d.split = y % d.splits;
+  d.slot = d.splits == 1 ? -1 : bh * cut + (sink ? x : (a.sink_splits > 1 ? sinks : 0) + y);
+  return d;
+}
+
+constexpr int kStages = 4, kAhead = 2;  // entry j + 2 is copied while j is multiplied (waves behind still read j - 1)
+
+template <int D>
+struct DkdvTiles {
+  using RT = RowTile<D>;
+  static constexpr int STAGE = 2 * RT::BYTES + 512;  // Q, dO, m2 and delta
+  static constexpr int NDT = D / 32;
+  static constexpr int RED = 4 * 64 * 2 * NDT * 16 * 4;
+  static constexpr int LDS = kStages * STAGE > RED ? kStages * STAGE : RED;
+};
+
+template <class E, int D>
+__global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
+  const WinArgs& a = ba.w;
+  using T = DkdvTiles<D>;
+  using RT = RowTile<D>;
+  using RS = RowSource<D>;
+  constexpr int NS = D / 16, NDT = D / 32, SB = T::STAGE, COUNT = 2 * RT::KB / 4;
+  __shared__ __align__(1024) uint8_t smem[T::LDS];
+  const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+  const int w = (int)uniform_u32(threadIdx.x >> 6);
+  const int kh = w & 1, qh = (w >> 1) & 1, tk = w >> 2;
+  const DkdvItem it = dkdv_item(ba, xcd_group_remap<32>((int)blockIdx.x, ba.items));
+  const SeqSpan sq = seq_span(a, it.b);
+  const int j0 = it.tile * 128;
+
+  // tokens that see some key of the tile (the first and the last key's, and the
+  // sinks' when it has some), as 64-token tiles of each head from lo on
+  int lo, hi;
+  {
+    const int jl = j0 + 127 < sq.L - 1 ? j0 + 127 : sq.L - 1;
+    const TokenRange f = tokens_of(a, sq, j0), l = tokens_of(a, sq, jl < j0 ? j0 : jl);
+    lo = f.i0 < l.i0 ? f.i0 : l.i0;
+    hi = f.i1 > l.i1 ? f.i1 : l.i1;
+    if (j0 >= sq.L || sq.n == 0) { lo = 0; hi = -1; }
+  }
+  const int nti = hi >= lo ? (hi - lo + 64) >> 6 : 0, all = nti * a.G;
+  const int e0 = (int)((int64_t)all * it.split / it.splits), e1 = (int)((int64_t)all * (it.split + 1) / it.splits);
+  const int n = e1 - e0;
+
+  // copies: waves 0-3 issue KB-instructions w, w + 4, ... (Q then dO), wave 3
+  // also the m2 row and wave 2 the delta row
+  const uint32_t lds0 = lds_addr(smem);
+  const int64_t qstep = 2 * a.q.s, dstep = 2 * ba.do_.s;
+  const int crow = RS::row(w & 3, lane), cbyte = RS::byte(w & 3, lane);
+  const uint32_t qoff = (uint32_t)crow * (uint32_t)qstep + (uint32_t)cbyte;
+  const uint32_t doff = (uint32_t)crow * (uint32_t)dstep + (uint32_t)cbyte;
+  auto issue = [&](int e, int st) {
+    if (w >= 4) return;
+    const int gh = e / nti, t0 = lo + 64 * (e - gh * nti), head = it.hk * a.G + gh;
+    const uint32_t base = lds0 + (uint32_t)(st * SB);
+    const uint8_t* qb = (const uint8_t*)uniform_ptr(a.q.p + it.b * a.q.b + head * a.q.h + t0 * a.q.s);
+    const uint8_t* db = (const uint8_t*)uniform_ptr(ba.do_.p + it.b * ba.do_.b + head * ba.do_.h + t0 * ba.do_.s);
+    const int left = hi - t0;  // rows past hi re-read it
+    if (left >= 63) {
+#pragma unroll
+      for (int s = 0; s < COUNT; ++s) {
+        const int m = s % (RT::KB / 4);
+        const bool isq = s < RT::KB / 4;
+        dma_b128(isq ? qoff : doff, isq ? qb + m * RS::ROWS4 * qstep : db + m * RS::ROWS4 * dstep,
+                 base + (uint32_t)(w + 4 * s) * 1024u);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < COUNT; ++s) {
+        const int m = s % (RT::KB / 4), row = crow + m * RS::ROWS4, rr = row < left ? row : left;
+        const bool isq = s < RT::KB / 4;
+        const uint32_t off = (uint32_t)rr * (uint32_t)(isq ? qstep : dstep) + (uint32_t)cbyte;
+        dma_b128(off, isq ? qb : db, base + (uint32_t)(w + 4 * s) * 1024u);
+      }
+    }
+    if (w >= 2) {
+      const float* rowsrc = (w == 3 ? ba.m2 : ba.delta) + ((int64_t)it.b * a.Hk * a.G + head) * a.Sq + t0;
+      dma_b32(4u * (uint32_t)(lane < left ? lane : left), uniform_ptr(rowsrc), base + 2u * RT::BYTES + (w == 3 ? 0u : 256u));
+    }
+  };
+  RowOperand rop;                // Q / dO rows 32 qh + l32
+  rop.init<RT>(32 * qh, l32, g);
+  TrOperand top;                 // Q^T / dO^T over query rows 32 qh .. 32 qh + 31
+  top.init<RT>(32 * qh, lane);
+#pragma unroll
+  for (int x = 0; x < kAhead; ++x)
+    if (x < n) issue(e0 + x, x);
+
+  const int jw = j0 + 64 * tk + 32 * kh, key = jw + l32;
+  bf16x8 kf[NS], vf[NS];
+  {
+    const int kc = key < a.Sk ? key : a.Sk - 1;
+    const uint16_t* kp = a.k.p + it.b * a.k.b + it.hk * a.k.h + kc * a.k.s + 8 * g;
+    const uint16_t* vp = a.v.p + it.b * a.v.b + it.hk * a.v.h + kc * a.v.s + 8 * g;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      kf[s] = ld_bf16x8(kp + 16 * s);
+      vf[s] = ld_bf16x8(vp + 16 * s);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    consume_regs(kf[s]);
+    consume_regs(vf[s]);
+  }
+  const TokenRange mine = tokens_of(a, sq, key);
+  // of the wave's 32 keys: tokens that see some, and all of them
+  int any0, any1, all0, all1;
+  {
+    const int jl = jw + 31 < sq.L - 1 ? jw + 31 : sq.L - 1;
+    const TokenRange f = tokens_of(a, sq, jw), l = tokens_of(a, sq, jl < jw ? jw : jl);
+    any0 = f.i0 < l.i0 ? f.i0 : l.i0;
+    any1 = f.i1 > l.i1 ? f.i1 : l.i1;
+    all0 = f.i0 > l.i0 ? f.i0 : l.i0;
+    all1 = f.i1 < l.i1 ? f.i1 : l.i1;
+    if (jw + 31 >= sq.L) all1 = -1;  // (lanes past the keys)
+    if (jw >= sq.L) any1 = -1;
+    if (jw < a.sinks && jw + 31 >= a.sinks) {  // the first key past the sinks sees the earliest end
+      const TokenRange x = tokens_of(a, sq, a.sinks);
+      all0 = all0 > x.i0 ? all0 : x.i0;
+      all1 = all1 < x.i1 ? all1 : x.i1;
+    }
+  }
+  f32x16 dk[NDT], dv[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) { dk[dt] = f32x16_zero(); dv[dt] = f32x16_zero(); }
+
+  // S = Q K^T and dP = dO V^T of one entry, then P and dS (B operands of the dV /
+  // dK products: query rows 32 qh + 8 j + 4 g + i in register 4 j + i, column =
+  // this lane's key); t0: the entry's first token of this wave's half
+  auto sdp = [&](const uint8_t* sQ, int t0, bf16x8* pb, bf16x8* sb) {
+    const uint8_t* sDO = sQ + RT::BYTES;
+    const float* sM = reinterpret_cast<const float*>(sQ + 2 * RT::BYTES);
+    const float* sDl = sM + 64;
+    f32x16 sacc = f32x16_zero(), pacc = f32x16_zero();
+    constexpr int NO = 2 * NS;
+    bf16x8 op[3];
+    auto rd = [&](int x) { return rop.load((x & 1) ? sDO : sQ, x >> 1); };
+    op[0] = rd(0);
+    op[1] = rd(1);
+#pragma unroll
+    for (int x = 0; x < NO; ++x) {
+      if (x + 2 < NO) op[(x + 2) % 3] = rd(x + 2);
+      if (x & 1) pacc = E::mfma(op[x % 3], vf[x >> 1], pacc);
+      else sacc = E::mfma(op[x % 3], kf[x >> 1], sacc);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+    for (int x = 0; x + 3 < NO; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+    const bool masked = t0 < all0 || t0 + 31 > all1;
+    uint32_t bits = ~0u;
+    if (masked) {  // rows of this half that see the lane's key
+      const int b0 = mine.i0 - t0 > 0 ? mine.i0 - t0 : 0, b1 = mine.i1 - t0 < 31 ? mine.i1 - t0 : 31;
+      bits = b1 >= b0 ? (~0u << b0) & (~0u >> (31 - b1)) : 0u;
+      bits >>= 4 * g;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int bit = 8 * (x >> 2) + (x & 3);
+        sacc[x] = keep_or_ninf(sacc[x], bits, bit);
+      }
+    }
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+      const float4 m4 = *reinterpret_cast<const float4*>(sM + 32 * qh + 8 * jj + 4 * g);
+      const float4 d4 = *reinterpret_cast<const float4*>(sDl + 32 * qh + 8 * jj + 4 * g);
+      const float mv[4] = {m4.x, m4.y, m4.z, m4.w}, dl4[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int rg = 4 * jj + x;
+        const float p = fast_exp2(__builtin_fmaf(sacc[rg], a.scale_log2, -mv[x]));
+        sacc[rg] = p;
+        pacc[rg] = p * (pacc[rg] - dl4[x]);
+      }
+    }
+    if (masked) {  // what is not finite in a row that does not see the key stays out
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int bit = 8 * (x >> 2) + (x & 3);
+        sacc[x] = keep_or_zero(sacc[x], bits, bit);
+        pacc[x] = keep_or_zero(pacc[x], bits, bit);
+      }
+    }
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2) {
+      pb[t2] = win_b_from_acc<E>(&sacc, t2);
+      sb[t2] = win_b_from_acc<E>(&pacc, t2);
+    }
+  };
+  // dV^T += dO^T P and dK^T += Q^T dS of one entry
+  auto dvdk = [&](const uint8_t* sQ, const bf16x8* pb, const bf16x8* sb) {
+    const uint8_t* sDO = sQ + RT::BYTES;
+    constexpr int NO = 4 * NDT, RING = 4;
+    bf16x8 op[RING];
+    auto rd = [&](int x) { return top.load<RT>((x & 1) ? sQ : sDO, x / (2 * NDT), (x >> 1) % NDT); };
+#pragma unroll
+    for (int x = 0; x + 1 < RING; ++x) op[x] = rd(x);
+#pragma unroll
+    for (int x = 0; x < NO; ++x) {
+      if (x + RING - 1 < NO) op[(x + RING - 1) % RING] = rd(x + RING - 1);
+      const int t2 = x / (2 * NDT), dt = (x >> 1) % NDT;
+      if (x & 1) dk[dt] = E::mfma(op[x % RING], sb[t2], dk[dt]);
+      else dv[dt] = E::mfma(op[x % RING], pb[t2], dv[dt]);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * (RING - 1), 0);
+#pragma unroll
+    for (int x = 0; x + RING - 1 < NO; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, RING - 1, 0);
+  };
+
+  // token tile of entry e, as it advances by one (no division in the loop)
+  int tile_i = n > 0 ? e0 % nti : 0;
+  auto half_of = [&] { return lo + 64 * tile_i + 32 * qh; };
+  auto next_tile = [&] { tile_i = tile_i + 1 == nti ? 0 : tile_i + 1; };
+  auto sees = [&](int t0) { return t0 + 31 >= any0 && t0 <= any1; };
+  if (tk == 0) {
+    int st = 0;
+    for (int x = 0; x < n; ++x) {
+      if (w >= 2) stage_wait<kAhead + 1, COUNT + 1>(n - 1 - x);
+      else stage_wait<kAhead + 1, COUNT>(n - 1 - x);
+      __syncthreads();
+      if (x + kAhead < n) issue(e0 + x + kAhead, (st + kAhead) % kStages);
+      const uint8_t* sQ = smem + st * SB;
+      st = st + 1 == kStages ? 0 : st + 1;
+      const int t0 = half_of();
+      next_tile();
+      if (!sees(t0)) continue;
+      bf16x8 pb[2], sb[2];
+      sdp(sQ, t0, pb, sb);
+      __builtin_amdgcn_s_setprio(1);
+      dvdk(sQ, pb, sb);
+      __builtin_amdgcn_s_setprio(0);
+    }
+  } else {
+    int st = 0;
+    bool pend = false;
+    const uint8_t* sPrev = smem;
+    bf16x8 pb[2], sb[2];
+    for (int x = 0; x < n; ++x) {
+      __syncthreads();
+      const uint8_t* sQ = smem + st * SB;
+      st = st + 1 == kStages ? 0 : st + 1;
+      const int t0 = half_of();
+      next_tile();
+      if (pend) dvdk(sPrev, pb, sb);
+      pend = sees(t0);
+      if (pend) {
+        sdp(sQ, t0, pb, sb);
+        sPrev = sQ;
+      }
+    }
+    if (pend) dvdk(sPrev, pb, sb);
+  }
+
+  // add the two query-half partials in a fixed order (qh = 0 + qh = 1)
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(smem);
+  const int slot = kh | tk << 1;
+  if (qh == 1) {
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        red[((slot * 2 * NDT + dt) * 16 + x) * 64 + lane] = dk[dt][x];
+        red[((slot * 2 * NDT + NDT + dt) * 16 + x) * 64 + lane] = dv[dt][x];
+      }
+  }
+  __syncthreads();
+  if (qh == 1) return;
+  uint16_t* dkr = ba.dk.p + it.b * ba.dk.b + it.hk * ba.dk.h + key * ba.dk.s;
+  uint16_t* dvr = ba.dv.p + it.b * ba.dv.b + it.hk * ba.dv.h + key * ba.dv.s;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) {
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      dk[dt][x] += red[((slot * 2 * NDT + dt) * 16 + x) * 64 + lane];
+      dv[dt][x] += red[((slot * 2 * NDT + NDT + dt) * 16 + x) * 64 + lane];
+    }
+    if (it.slot >= 0) {
+      float4* pa = ba.acc + ((int64_t)it.slot * 4 + slot) * 2 * NDT * 256 + lane;
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj) {
+        pa[(dt * 4 + jj) * 64] = make_float4(dk[dt][4 * jj], dk[dt][4 * jj + 1], dk[dt][4 * jj + 2], dk[dt][4 * jj + 3]);
+        pa[((NDT + dt) * 4 + jj) * 64] =
+            make_float4(dv[dt][4 * jj], dv[dt][4 * jj + 1], dv[dt][4 * jj + 2], dv[dt][4 * jj + 3]);
+      }
+      continue;
+    }
+    if (key >= a.Sk) continue;
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+      uint2 o;
+      o.x = E::pack(dk[dt][4 * jj + 0] * a.scale, dk[dt][4 * jj + 1] * a.scale);
+      o.y = E::pack(dk[dt][4 * jj + 2] * a.scale, dk[dt][4 * jj + 3] * a.scale);
+      *reinterpret_cast<uint2*>(dkr + 32 * dt + 8 * jj + 4 * g) = o;
+      o.x = E::pack(dv[dt][4 * jj + 0], dv[dt][4 * jj + 1]);
+      o.y = E::pack(dv[dt][4 * jj + 2], dv[dt][4 * jj + 3]);
+      *reinterpret_cast<uint2*>(dvr + 32 * dt + 8 * jj + 4 * g) = o;
+    }
+  }
+}
+
+// the pieces' sums of the cut tiles, in order: one workgroup per tile and
+// 32-column block of dK (blocks 0 .. NDT - 1) or dV; wave = 32 keys
+template <class E, int D>
+__global__ __launch_bounds__(256) void window_merge_kernel(WinBwdArgs a, int cut_sinks, int cut_rest) {
+  constexpr int NDT = D / 32, NB = 2 * NDT;
+  const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, w = threadIdx.x >> 6, blk = (int)blockIdx.y;
+  const int per = cut_sinks + cut_rest;  // cut tiles per (sequence, key head)
+  const int bh = (int)blockIdx.x / per, x = (int)blockIdx.x - bh * per;
+  const bool sink = x < cut_sinks;
+  const int S = sink ? a.sink_splits : a.rest_splits;
+  const int tile = sink ? x : a.sink_tiles + x - cut_sinks;
+  const int64_t first = (int64_t)bh * (cut_sinks * a.sink_splits + cut_rest * a.rest_splits) +
+                        (sink ? x * S : cut_sinks * a.sink_splits + (x - cut_sinks) * S);
+  const int b = bh / a.w.Hk, hk = bh - b * a.w.Hk, key = tile * 128 + 32 * w + l32;
+  if (key >= a.w.Sk) return;
+  const float4* pa = a.acc + ((first * 4 + w) * NB + blk) * 256 + lane;
+  float4 acc[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc[j] = pa[j * 64];
+  for (int s = 1; s < S; ++s)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 v = pa[(int64_t)s * 4 * NB * 256 + j * 64];
+      acc[j].x += v.x;
+      acc[j].y += v.y;
+      acc[j].z += v.z;
+      acc[j].w += v.w;
+    }
+  const bool isk = blk < NDT;
+  const WinTensor& t = isk ? a.dk : a.dv;
+  const float f = isk ? a.w.scale : 1.0f;
+  uint16_t* out = t.p + b * t.b + hk * t.h + key * t.s + 32 * (isk ? blk : blk - NDT) + 4 * g;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint2 u;
+    u.x = E::pack(acc[j].x * f, acc[j].y * f);
+    u.y = E::pack(acc[j].z * f, acc[j].w * f);
+    *reinterpret_cast<uint2*>(out + 8 * j) = u;
+  }
+}
+
+// pieces of the dK/dV lists: none longer than a third of a CU's share of the
+// launch (so the chip ends evenly), nor shorter than 8 entries
+struct DkdvPlan {
+  int64_t sink_tiles, key_tiles, sink_splits, rest_splits, pieces;
+};
+DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int64_t window, int64_t sinks, int causal) {
+  DkdvPlan p{};
+  p.key_tiles = (Sk + 127) / 128;
+  p.sink_tiles = ((sinks < Sk ? sinks : Sk) + 127) / 128;
+  const int64_t whole = (Sq + 63) / 64;
+  const int64_t span = window < Sq ? (causal ? window : 2 * window) + 127 : Sq;
+  const int64_t rest = G * (span < Sq ? (span + 63) / 64 : whole), sink = G * whole;
+  const int64_t nrest = p.key_tiles - p.sink_tiles;
+  const int64_t total = (int64_t)B * Hk * (p.sink_tiles * sink + nrest * rest);
+  int64_t target = (total + 767) / 768;
+  target = target > 8 ? target : 8;
+  auto cut = [&](int64_t n) { return n > target + target / 2 ? (n + target - 1) / target : 1; };
+  p.sink_splits = cut(sink);
+  p.rest_splits = cut(rest);
+  p.pieces = (int64_t)B * Hk * ((p.sink_splits > 1 ? p.sink_tiles * p.sink_splits : 0) +
+                                (p.rest_splits > 1 ? nrest * p.rest_splits : 0));
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int prism_window_bwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal,
+                          int64_t* floats) {
+  PRISM_REQUIRE(B >= 0 && Hk >= 1 && Hq >= Hk && Hq % Hk == 0 && Sq >= 0 && Sk >= 0 && D >= 1 && window >= 1 &&
+                    sinks >= 0 && floats,
+                "prism_window_bwd_plan: bad argument");
+  *floats = dkdv_plan(B, Hk, Hq / Hk, Sq, Sk, window, sinks, causal).pieces * 256 * D;
+  return PRISM_OK;
+}
+
+int prism_window_bwd(const void* do_, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                     int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, const int64_t* strides,
+                     int64_t window, int64_t sinks, int causal, const int32_t* q_lens, const int32_t* kv_lens,
+                     float sm_scale, void* dq, void* dk, void* dv, float* rows, float* acc, hipStream_t stream) {
+  if (const int rc = win_check("prism_window_bwd", dtype, B, Hq, Hk, Sq, Sk, D, window, sinks, sm_scale, strides, 8,
+                               {q, k, v, o, do_, dq, dk, dv}))
+    return rc;
+  if (B == 0) return PRISM_OK;
+  PRISM_REQUIRE(Sq == 0 || (q && o && do_ && lse && dq && rows), "prism_window_bwd: null pointer");
+  PRISM_REQUIRE(Sk == 0 || (k && v && dk && dv), "prism_window_bwd: null pointer");
+  const DkdvPlan p = dkdv_plan(B, Hk, Hq / Hk, Sq, Sk, window, sinks, causal);
+  PRISM_REQUIRE(p.pieces == 0 || acc, "prism_window_bwd: null workspace");
+  WinBwdArgs a{};
+  a.w = win_args(q, k, v, (void*)o, B, Hq, Hk, Sq, Sk, strides, window, sinks, causal, q_lens, kv_lens, sm_scale);
+  a.w.lse = (float*)lse;
+  const int64_t* s = strides + 12;
+  a.do_ = {(uint16_t*)do_, s[0], s[1], s[2]};
+  a.dq = {(uint16_t*)dq, s[3], s[4], s[5]};
+  a.dk = {(uint16_t*)dk, s[6], s[7], s[8]};
+  a.dv = {(uint16_t*)dv, s[9], s[10], s[11]};
+  a.m2 = rows;
+  a.delta = rows + (int64_t)B * Hq * Sq;
+  a.sink_tiles = (int)p.sink_tiles; a.key_tiles = (int)p.key_tiles;
+  a.sink_splits = (int)p.sink_splits; a.rest_splits = (int)p.rest_splits;
+  a.acc = (float4*)acc;
+  a.w.tiles = (int)((Sq * a.w.G + 127) / 128);
+  const int64_t total = (int64_t)B * Hk * a.w.tiles;
+  const int64_t rest = p.key_tiles - p.sink_tiles;
+  const int64_t items = (int64_t)B * Hk * (p.sink_tiles * p.sink_splits + rest * p.rest_splits);
+  PRISM_REQUIRE(total < (1ll << 31) && items < (1ll << 31), "prism_window_bwd: too many tiles");
+  a.w.total = (int)total;
+  a.items = (int)items;
+  const int cs = p.sink_splits > 1 ? a.sink_tiles : 0, cr = p.rest_splits > 1 ? (int)rest : 0;
+  auto run = [&](auto e, auto d) {
+    using E = decltype(e);
+    constexpr int DD = decltype(d)::value;
+    if (total) window_dq_kernel<E, DD><<<(unsigned)total, 256, 0, stream>>>(a);
+    if (items) window_dkdv_kernel<E, DD><<<(unsigned)items, 512, 0, stream>>>(a);
+    if (items && cs + cr)
+      window_merge_kernel<E, DD><<<dim3((unsigned)(B * Hk * (cs + cr)), DD / 16), 256, 0, stream>>>(a, cs, cr);
+  };
+  if (dtype == PRISM_BF16) {
+    if (D == 64) run(WinBf16{}, std::integral_constant<int, 64>{});
+    else run(WinBf16{}, std::integral_constant<int, 128>{});
+  } else {
+    if (D == 64) run(WinF16{}, std::integral_constant<int, 64>{});
+    else run(WinF16{}, std::integral_constant<int, 128>{});
+  }
+  PRISM_LAUNCH_CHECK("prism_window_bwd");
+  return PRISM_OK;
+}
+
+}  // extern "C"

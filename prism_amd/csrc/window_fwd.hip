@@ -1,0 +1,245 @@
+// Window attention forward (gfx950, v_mfma_f32_32x32x16): query token at
+// position p sees the keys p - W < j <= p (causal) or |p - j| < W, and the first
+// `sinks` keys (causal: those at or before p), of its sequence's length.
+//
+//   o = sum_j softmax_j(scale q k_j) v_j over the seen keys; 0, and lse -inf, where there are none
+//
+// Prompts and training (window_fwd_kernel): one workgroup of four waves per 128
+// rows, a wave per 32, two workgroups per CU, as the block-sparse forward over
+// pairs (attn_fwd.hip): K and V tiles of 64 entries of the key list (window.h)
+// are copied HBM -> LDS by global_load_lds_dwordx4 into two stages, S^T = K Q^T
+// keeps one query per lane column, softmax in base 2 with a lazy running
+// maximum, O^T += V^T P^T from the S^T accumulators.  Only tiles at the ends of a
+// window (and the one where the sinks end) are masked, by a 64-bit word per lane
+// made from three bounds; a wave skips tiles that none of its tokens sees.
+//
+// Numbers: scores, maximum, sum and output are fp32; P is rounded to the inputs'
+// type for the product with V (its error averages out over the keys), o once.
+#include "window.h"
+
+namespace {
+
+template <class E, int D>
+__global__ __launch_bounds__(256, 2) void window_fwd_kernel(WinArgs a) {
+  using T = WinTiles<D>;
+  using RT = typename T::RT;
+  constexpr int NS = D / 16, NDT = D / 32;
+  __shared__ __align__(1024) uint8_t smem[2 * T::STAGE];
+  const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+  const int w = (int)uniform_u32(threadIdx.x >> 6);
+  int b, hk, tile;
+  win_item(a, xcd_group_remap<32>((int)blockIdx.x, a.total), b, hk, tile);
+  const SeqSpan sq = seq_span(a, b);
+  const int rows = a.Sq * a.G, r0 = tile * 128, wr0 = r0 + 32 * w;
+  const int last = sq.n - 1;
+  auto token = [&](int r) { const int i = r / a.G; return i < last ? i : last; };
+  const KeyList kl = r0 / a.G > last ? KeyList{0, 0, 0} : key_list(a, sq, r0 / a.G, token(r0 + 127));
+  const int nt = (kl.n + 63) >> 6;
+
+  const float NINF = -__builtin_inff();
+  StageCopy<D> copy;
+  copy.init(a, b, hk, w & 1, lane);
+  const uint32_t lds0 = lds_addr(smem);
+  if (w < 2 && nt > 0) copy.issue(kl, 0, lds0);
+
+  RowOperand kop;
+  kop.init<RT>(0, l32, g);
+  TrOperand vop;
+  vop.init<RT>(0, lane);
+
+  // this lane's row (rows past the end re-read the last one and are not stored)
+  const int r = wr0 + l32, rc = r < rows ? r : rows - 1;
+  const int i = rc / a.G, head = hk * a.G + (rc - i * a.G);
+  const uint16_t* qp = a.q.p + b * a.q.b + head * a.q.h + i * a.q.s;
+  bf16x8 qf[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) qf[s] = ld_bf16x8(qp + 16 * s + 8 * g);
+#pragma unroll
+  for (int s = 0; s < NS; ++s) consume_regs(qf[s]);
+
+  const bool live = i <= last;  // rows past the sequence's queries see nothing
+  TokenSpan span = token_span(a, kl, i + sq.off);
+  if (!live) span = TokenSpan{1, 0, 0};
+  const int wi0 = (int)uniform_u32((uint32_t)(wr0 / a.G)), wi1 = (int)uniform_u32((uint32_t)token(wr0 + 31));
+  const bool some = wi0 <= last && wr0 < rows;
+  const bool whole = (wr0 + 31) / a.G <= last;  // every row of the wave is a query
+  WaveSpan ws;
+  ws.init(a, kl, wi0 + sq.off, wi1 + sq.off);
+
+  f32x16 acc_o[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) acc_o[dt] = f32x16_zero();
+  float m = NINF, l = 1.0f;
+
+  for (int t = 0; t < nt; ++t) {
+    dma_wait_all();
+    __syncthreads();
+    if (w < 2 && t + 1 < nt) copy.issue(kl, 64 * (t + 1), lds0 + (uint32_t)(((t + 1) & 1) * T::STAGE));
+    const int u0 = 64 * t;
+    if (!some || !ws.any(u0, u0 + 63)) continue;
+    const uint8_t* sK = smem + (t & 1) * T::STAGE;
+    const uint8_t* sV = sK + RT::BYTES;
+    // S^T[key][q] = K Q^T, two 32-key halves as interleaved MFMA chains, the K
+    // operands through a ring of four registers
+    f32x16 sacc[2] = {f32x16_zero(), f32x16_zero()};
+    {
+      constexpr int NO = 2 * NS, RING = 4;
+      bf16x8 kfr[RING];
+      auto rd = [&](int x) { return kop.load(sK + RT::rows(32 * (x & 1)), x >> 1); };
+#pragma unroll
+      for (int x = 0; x + 1 < RING; ++x) kfr[x] = rd(x);
+#pragma unroll
+      for (int x = 0; x < NO; ++x) {
+        if (x + RING - 1 < NO) kfr[(x + RING - 1) % RING] = rd(x + RING - 1);
+        sacc[x & 1] = E::mfma(kfr[x % RING], qf[x >> 1], sacc[x & 1]);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, RING - 1, 0);
+#pragma unroll
+      for (int x = 0; x + RING - 1 < NO; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, RING - 1, 0);
+    }
+    // V^T operands of the P V product, in flight while the softmax runs
+    bf16x8 vfr[4][NDT];
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) vfr[tt][dt] = vop.load<RT>(sV, tt, dt);
+    if (!whole || !ws.all(u0, u0 + 63)) {
+      // this lane's entries are 32 kh + 8 j + 4 g + x: bit (32 kh + 8 j + x) of the word >> 4 g
+      const uint64_t mm = span_bits(span, u0) >> (4 * g);
+      const uint32_t lo = (uint32_t)mm, hi = (uint32_t)(mm >> 32);
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int bit = 8 * (x >> 2) + (x & 3);
+        sacc[0][x] = keep_or_ninf(sacc[0][x], lo, bit);
+        sacc[1][x] = keep_or_ninf(sacc[1][x], hi, bit);
+      }
+    }
+    __builtin_amdgcn_s_setprio(2);
+    float mx = fmax_nn(sacc[0][0], sacc[1][0]);
+#pragma unroll
+    for (int x = 1; x < 16; ++x) mx = fmax_nn(fmax_nn(mx, sacc[0][x]), sacc[1][x]);
+    mx = xor32_max(mx) * a.scale_log2;
+    // the running reference moves only when the tile's maximum is more than 8
+    // above it (p <= 2^8): o = acc / l and lse = m + log2 l do not depend on it
+    const bool move = mx > m + 8.0f || (m == NINF && mx != NINF);
+    const float m_new = move ? mx : m;
+    const float alpha = move ? fast_exp2(m - m_new) : 1.0f;
+    const float mb = m_new == NINF ? 0.0f : m_new;
+    if (__builtin_amdgcn_ballot_w64(move)) {
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) acc_o[dt][x] *= alpha;
+    }
+    __builtin_amdgcn_s_setprio(1);
+    float ls = 0.0f;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
+      const int h = tt >> 1, x0 = 8 * (tt & 1);
+#pragma unroll
+      for (int x = x0; x < x0 + 8; ++x) {
+        const float p = fast_exp2(__builtin_fmaf(sacc[h][x], a.scale_log2, -mb));
+        sacc[h][x] = p;
+        ls += p;
+      }
+      const bf16x8 pb = win_b_from_acc<E>(sacc, tt);
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) acc_o[dt] = E::mfma(vfr[tt][dt], pb, acc_o[dt]);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x002, 28, 0);
+#pragma unroll
+    for (int x = 0; x < 3 * NDT; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 28 / NDT, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, NDT, 0);
+    ls = xor32_add(ls);
+    l = __builtin_fmaf(l, alpha, ls);
+    m = m_new;
+    __builtin_amdgcn_s_setprio(0);
+  }
+
+  if (r >= rows) return;
+  const float inv = 1.0f / l;
+  uint16_t* op = a.o.p + b * a.o.b + head * a.o.h + i * a.o.s;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint2 u;
+      u.x = E::pack(acc_o[dt][4 * j + 0] * inv, acc_o[dt][4 * j + 1] * inv);
+      u.y = E::pack(acc_o[dt][4 * j + 2] * inv, acc_o[dt][4 * j + 3] * inv);
+      *reinterpret_cast<uint2*>(op + 32 * dt + 8 * j + 4 * g) = u;
+    }
+  if (a.lse && g == 0)
+    a.lse[((int64_t)b * a.Hk * a.G + head) * a.Sq + i] = (m + __log2f(l)) * 0.6931471805599453f;
+}
+
+}  // namespace
+
+int win_check(const char* name, int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window,
+              int64_t sinks, float sm_scale, const int64_t* strides, int tensors,
+              std::initializer_list<const void*> pointers) {
+  PRISM_REQUIRE(dtype == PRISM_BF16 || dtype == PRISM_F16, "%s: dtype code %d (bfloat16 or float16)", name, dtype);
+  PRISM_REQUIRE(D == 64 || D == 128, "%s: head_dim %d unsupported (64, 128)", name, D);
+  PRISM_REQUIRE(B >= 0 && Hk >= 1 && Hq >= Hk && Hq % Hk == 0, "%s: %d query heads do not share %d key heads evenly", name,
+                Hq, Hk);
+  PRISM_REQUIRE(Sq >= 0 && Sk >= 0 && Sq < (1 << 29) && Sk < (1 << 29), "%s: lengths out of range", name);
+  PRISM_REQUIRE(Sq * (Hq / Hk) < (1ll << 30), "%s: too many query rows", name);
+  PRISM_REQUIRE(window >= 1 && sinks >= 0, "%s: window must be at least 1 and sinks at least 0", name);
+  PRISM_REQUIRE(sm_scale > 0.0f && sm_scale < __builtin_inff(), "%s: sm_scale must be positive and finite", name);
+  PRISM_REQUIRE(strides, "%s: null pointer", name);
+  // rows are copied 16 bytes at a time at 32-bit offsets inside a tile
+  for (int i = 0; i < tensors; ++i)
+    PRISM_REQUIRE(strides[3 * i] % 8 == 0 && strides[3 * i + 1] % 8 == 0 && strides[3 * i + 2] % 8 == 0 &&
+                      strides[3 * i + 2] >= 0 && strides[3 * i + 2] < (1 << 24),
+                  "%s: strides must be multiples of 8 elements, a row's below 2^24", name);
+  for (const void* p : pointers)
+    PRISM_REQUIRE(((uintptr_t)p & 15) == 0, "%s: pointers must be 16-byte aligned", name);
+  return PRISM_OK;
+}
+
+WinArgs win_args(const void* q, const void* k, const void* v, void* o, int B, int Hq, int Hk, int64_t Sq, int64_t Sk,
+                 const int64_t* s, int64_t window, int64_t sinks, int causal, const int32_t* q_lens,
+                 const int32_t* kv_lens, float sm_scale) {
+  WinArgs a{};
+  a.q = {(uint16_t*)q, s[0], s[1], s[2]};
+  a.k = {(uint16_t*)k, s[3], s[4], s[5]};
+  a.v = {(uint16_t*)v, s[6], s[7], s[8]};
+  a.o = {(uint16_t*)o, s[9], s[10], s[11]};
+  a.q_lens = q_lens; a.kv_lens = kv_lens;
+  a.B = B; a.Hk = Hk; a.G = Hq / Hk; a.Sq = (int)Sq; a.Sk = (int)Sk;
+  a.window = (int)(window < (1 << 29) ? window : 1 << 29);
+  a.sinks = (int)(sinks < Sk ? sinks : Sk);
+  a.causal = causal != 0;
+  a.scale = sm_scale; a.scale_log2 = sm_scale * 1.4426950408889634f;
+  return a;
+}
+
+extern "C" int prism_window_fwd(const void* q, const void* k, const void* v, int dtype, int B, int Hq, int Hk,
+                                int64_t Sq, int64_t Sk, int D, const int64_t* strides, int64_t window, int64_t sinks,
+                                int causal, const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o,
+                                float* lse, hipStream_t stream) {
+  if (const int rc = win_check("prism_window_fwd", dtype, B, Hq, Hk, Sq, Sk, D, window, sinks, sm_scale, strides, 4, {q, k, v, o})) return rc;
+  if (B == 0 || Sq == 0) return PRISM_OK;
+  PRISM_REQUIRE(q && o && (Sk == 0 || (k && v)), "prism_window_fwd: null pointer");
+  WinArgs a = win_args(q, k, v, o, B, Hq, Hk, Sq, Sk, strides, window, sinks, causal, q_lens, kv_lens, sm_scale);
+  a.lse = lse;
+  a.tiles = (int)((Sq * a.G + 127) / 128);
+  const int64_t total = (int64_t)B * Hk * a.tiles;
+  PRISM_REQUIRE(total < (1ll << 31), "prism_window_fwd: too many row tiles");
+  a.total = (int)total;
+  if (dtype == PRISM_BF16) {
+    if (D == 64) window_fwd_kernel<WinBf16, 64><<<a.total, 256, 0, stream>>>(a);
+    else window_fwd_kernel<WinBf16, 128><<<a.total, 256, 0, stream>>>(a);
+  } else {
+    if (D == 64) window_fwd_kernel<WinF16, 64><<<a.total, 256, 0, stream>>>(a);
+    else window_fwd_kernel<WinF16, 128><<<a.total, 256, 0, stream>>>(a);
+  }
+  PRISM_LAUNCH_CHECK("prism_window_fwd");
+  return PRISM_OK;
+}

@@ -208,6 +208,23 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, posi
     return oq, (ok if k is not None else None)
 
 
+def window_fwd(q, k, v, window: int, sinks: int, causal: bool, q_lens: Optional[torch.Tensor],
+               kv_lens: Optional[torch.Tensor], sm_scale: float, want_lse: bool):
+    """(o [B,Hq,Sq,D], lse [B,Hq,Sq] fp32 or None) of attention over a window and sinks."""
+    _cuda(q, k, v, q_lens, kv_lens)
+    o, lse = _op("window_fwd", q, k, v, int(window), int(sinks), bool(causal), q_lens, kv_lens, float(sm_scale),
+                 bool(want_lse))
+    return o, (lse if want_lse else None)
+
+
+def window_bwd(do, q, k, v, o, lse, window: int, sinks: int, causal: bool, q_lens: Optional[torch.Tensor],
+               kv_lens: Optional[torch.Tensor], sm_scale: float):
+    """(dq, dk, dv) of window_fwd."""
+    _cuda(do, q, k, v, o, lse, q_lens, kv_lens)
+    return _op("window_bwd", do, q, k, v, o, lse, int(window), int(sinks), bool(causal), q_lens, kv_lens,
+               float(sm_scale))
+
+
 # ------------------------------------------------------------------ geometry
 class ZoneLayout:
     """Per-call block/tile bookkeeping for one set of shape ids.

@@ -1,0 +1,99 @@
+"""Attention over a sliding window and the first tokens (sinks), MI355X
+implementation (csrc/window_*.hip): prompts and training steps, and single
+tokens of a stream over its cache.
+
+Beside the block-sparse attention, whose kept blocks follow the content, this
+one's follow the position: the form for token streams (an audio tower, frames
+generated one after the other), where each token sees the last `window` tokens
+and the stream's first `sinks`.  The reference has no counterpart.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+_NO_LIMIT = 1 << 29  # a window that no sequence reaches
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, causal, sm_scale, q_lens, kv_lens):
+        ctx.set_materialize_grads(False)
+        o, lse = ops.window_fwd(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, True)
+        ctx.how = (window, sinks, causal, sm_scale)
+        ctx.save_for_backward(q, k, v, o, lse, q_lens, kv_lens)
+        ctx.mark_non_differentiable(lse)
+        return o, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do, _):
+        if do is None:
+            return (None,) * 9
+        q, k, v, o, lse, q_lens, kv_lens = ctx.saved_tensors
+        window, sinks, causal, sm_scale = ctx.how
+        dq, dk, dv = ops.window_bwd(do, q, k, v, o, lse, window, sinks, causal, q_lens, kv_lens, sm_scale)
+        return dq, dk, dv, None, None, None, None, None, None
+
+
+def flash_attn_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Optional[int], *, sinks: int = 0,
+                      causal: bool = True, sm_scale: Optional[float] = None, q_lens: Optional[torch.Tensor] = None,
+                      kv_lens: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """softmax(sm_scale q k^T) v over the keys that each query sees.
+
+    q: [B, Hq, Sq, D], k, v: [B, Hk, Sk, D], bfloat16 or float16, D 64 or 128;
+    Hq a multiple of Hk (query heads h * Hq / Hk .. share key head h).  Any
+    strides; adjacent channels, 16-byte aligned rows and strides of whole 16
+    bytes are read in place (a cache or a projection laid out [B, S, H, D],
+    transposed), others are copied first.
+
+    The queries are the last of their sequence: with L keys and n queries,
+    query i stands at position p = i + L - n.  It sees key j < L where
+      causal:      p - window < j <= p, or j < sinks and j <= p
+      otherwise:   |p - j| < window, or j < sinks
+    window None: no limit.  kv_lens, q_lens: int32 [B] on the GPU, L and n per
+    sequence (default Sk and Sq; cut to them): a cache with room beyond its
+    tokens, a batch padded on the right (both the same lengths).  Keys beyond L,
+    and others that no query of the call sees, are not read and may hold
+    anything.  Queries that see no key, and rows i >= n, give 0 (and take no
+    gradient).  sm_scale (positive)
+    defaults to D^-1/2.
+
+    Returns o, of q's shape (and layout, where q is dense), with return_lse (o,
+    lse): lse [B, Hq, Sq] float32, the natural log of the sum of exponentials
+    of the scaled scores, -inf where nothing is seen (no gradient through it).
+    Differentiable in q, k, v; sums over shared heads are fp32."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("q, k, v must be [B, H, S, D]")
+    B, Hq, _, D = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if D not in (64, 128):
+        raise ValueError(f"head_dim {D} unsupported by the MI355X kernels (64, 128)")
+    if k.shape[1] < 1 or Hq < k.shape[1] or Hq % k.shape[1]:
+        raise ValueError(f"{Hq} query heads do not share {k.shape[1]} key heads evenly")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k, v must be all bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if window is not None and int(window) < 1:
+        raise ValueError(f"window must be at least 1 (or None), got {window}")
+    if int(sinks) < 0:
+        raise ValueError(f"sinks must not be negative, got {sinks}")
+    for t, name in ((q_lens, "q_lens"), (kv_lens, "kv_lens")):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (B,)):
+            raise ValueError(f"{name} must be int32 [{B}], got {t.dtype} {tuple(t.shape)}")
+    window = _NO_LIMIT if window is None else min(int(window), _NO_LIMIT)
+    sm_scale = D ** -0.5 if sm_scale is None else float(sm_scale)
+    if not 0 < sm_scale < float("inf"):
+        raise ValueError(f"sm_scale must be positive and finite, got {sm_scale}")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        o, lse = _WindowAttention.apply(q, k, v, window, int(sinks), bool(causal), sm_scale, q_lens, kv_lens)
+    else:
+        o, lse = ops.window_fwd(q, k, v, window, int(sinks), bool(causal), q_lens, kv_lens, sm_scale, return_lse)
+    return (o, lse) if return_lse else o
+
+
+__all__ = ["flash_attn_window"]

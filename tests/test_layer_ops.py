@@ -98,3 +98,75 @@ def test_frequencies():
 
 def test_grid_positions_cpu():
     assert prism_amd.grid_positions((1, 2, 2), device="cpu").tolist() == [[0, 0, 0], [0, 0, 1], [0, 1, 0], [0, 1, 1]]
+
+
+def test_window_refusals():
+    q, k = torch.randn(2, 4, 5, 64).bfloat16(), torch.randn(2, 2, 9, 64).bfloat16()
+    call = prism_amd.flash_attn_window
+    with pytest.raises(ValueError, match="GPU"):
+        call(q, k, k, 3)
+    with pytest.raises(ValueError, match="B, H, S, D"):
+        call(q[0], k, k, 3)
+    with pytest.raises(ValueError, match="mismatch"):
+        call(q, k, k[:, :, :8], 3)
+    with pytest.raises(ValueError, match="mismatch"):
+        call(q, k[:1], k[:1], 3)
+    with pytest.raises(ValueError, match="head_dim"):
+        call(q[..., :32], k[..., :32], k[..., :32], 3)
+    with pytest.raises(ValueError, match="evenly"):
+        call(q[:, :3], k, k, 3)
+    with pytest.raises(ValueError, match="evenly"):
+        call(q, k[:, :0], k[:, :0], 3)
+    with pytest.raises(TypeError, match="bfloat16"):
+        call(q.float(), k.float(), k.float(), 3)
+    with pytest.raises(TypeError, match="bfloat16"):
+        call(q, k, k.half(), 3)
+    with pytest.raises(ValueError, match="window"):
+        call(q, k, k, 0)
+    with pytest.raises(ValueError, match="sinks"):
+        call(q, k, k, 3, sinks=-1)
+    for lens in (torch.ones(2), torch.ones(3, dtype=torch.int32), torch.ones(2, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="kv_lens"):
+            call(q, k, k, 3, kv_lens=lens)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(ValueError, match="sm_scale"):
+            call(q, k, k, 3, sm_scale=scale)
+
+
+def test_window_capi_refusals():
+    lib = _lib.load()
+    one = ctypes.c_void_p(16)
+
+    def fwd(dtype=1, B=1, Hq=4, Hk=2, Sq=5, Sk=9, D=64, window=3, sinks=0, scale=0.1, stride=64, p=one):
+        st = (ctypes.c_int64 * 12)(*[stride] * 12)
+        return lib.prism_window_fwd(p, one, one, dtype, B, Hq, Hk, Sq, Sk, D, st, window, sinks, 1, None, None, scale, one,
+                                    None, None)
+
+    for bad in (dict(dtype=0), dict(Hk=3), dict(Hk=0), dict(D=32), dict(window=0), dict(sinks=-1), dict(scale=0.0),
+                dict(stride=65), dict(stride=1 << 24), dict(stride=-64), dict(p=None), dict(p=ctypes.c_void_p(8)),
+                dict(Sq=1 << 30), dict(Sk=1 << 30), dict(B=-1)):
+        assert fwd(**bad) == 1, bad
+    assert fwd(B=0) == 0
+    st = (ctypes.c_int64 * 24)(*[64] * 24)
+    token = lambda splits, ws: lib.prism_window_token(  # noqa: E731
+        one, one, one, 1, 1, 4, 2, 1, 9, 64, st, 3, 0, 1, None, None, 0.1, one, None, splits, ws, ws, None)
+    assert [token(0, one), token(257, one), token(2, None)] == [1, 1, 1]
+    bwd = lambda lse, rows: lib.prism_window_bwd(  # noqa: E731
+        one, one, one, one, one, lse, 1, 1, 4, 2, 5, 9, 64, st, 3, 0, 1, None, None, 0.1, one, one, one, rows, None, None)
+    assert [bwd(None, one), bwd(one, None)] == [1, 1]
+
+
+def test_window_plans():
+    """Workspaces stay small against the tensors: a bounded number of pieces."""
+    lib = _lib.load()
+    splits, floats = ctypes.c_int(0), ctypes.c_int64(0)
+    for B, Hq, Hk, Sq, Sk, W, sinks in ((8, 32, 8, 1, 32768, 4096, 4), (1, 1, 1, 1, 1 << 28, 1 << 28, 0), (1, 8, 8, 1, 1, 1, 0),
+                                        (1, 64, 1, 1, 100000, 100000, 0), (0, 4, 4, 1, 5, 5, 0), (64, 32, 8, 2, 9, 5, 2)):
+        assert lib.prism_window_token_plan(B, Hq, Hk, Sq, Sk, W, sinks, 1, ctypes.byref(splits), ctypes.byref(floats)) == 0
+        assert 1 <= splits.value <= 256
+        assert splits.value == 1 or splits.value * 256 <= Sk + 512
+        assert floats.value == (0 if splits.value == 1 else splits.value * 32 * B * Hk * -(-Sq * Hq // Hk // 32))
+    for B, Hq, Hk, Sq, Sk, W, sinks in ((1, 5, 5, 14040, 14040, 4680, 1560), (1, 1, 1, 200000, 200000, 64, 4), (1, 1, 1, 1, 1, 1, 0),
+                                        (4, 32, 8, 16384, 16384, 1 << 29, 0)):
+        assert lib.prism_window_bwd_plan(B, Hq, Hk, Sq, Sk, 128, W, sinks, 1, ctypes.byref(floats)) == 0
+        assert 0 <= floats.value <= 3000 * 256 * 128
