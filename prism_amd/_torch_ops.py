@@ -93,10 +93,10 @@ def _register_fakes():
 
     @reg("prism::rms_norm")
     def _(x, residual, weight, eps, out_code, want_inv):
-        m = x.shape[0]
         return (_empty(x, x.shape, {3: f8, 4: i8}.get(out_code, x.dtype)),
                 _empty(x, x.shape, x.dtype) if residual is not None else _none(x),
-                _empty(x, (m,), f32) if out_code >= 3 else _none(x), _empty(x, (m,), f32) if want_inv else _none(x))
+                _empty(x, x.shape[:-1], f32) if out_code >= 3 else _none(x),
+                _empty(x, (x.numel() // x.shape[-1],), f32) if want_inv else _none(x))
 
     @reg("prism::rms_norm_bwd")
     def _(dy, dh, h, weight, inv, want_dw):

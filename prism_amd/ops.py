@@ -34,7 +34,8 @@ _timings: Optional[Dict[str, List[Tuple[torch.cuda.Event, torch.cuda.Event]]]] =
 
 @contextlib.contextmanager
 def kernel_timing():
-    """Record HIP events around every C-ABI launch made inside the block.
+    """Record HIP events around every C-ABI launch made inside the block (but
+    the backward launches of the layer operators, whose autograd nodes are C++).
     Yields a dict name -> list of (start, end) events; after a synchronize,
     ``summarize(d)`` gives per-entry-point call counts and average ms."""
     global _timings
@@ -177,10 +178,10 @@ def _layer_code(t: torch.Tensor, name: str) -> int:
 
 def rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float,
              out_dtype: Optional[torch.dtype] = None, want_inv: bool = False):
-    """Rows [M, N]: (y, h, scale, inv) with h = x + residual (None without
+    """x [.., N]: (y, h, scale, inv) with h = x + residual (None without
     one), y = h / sqrt(mean(h^2) + eps) * weight in x's dtype, or codes of
-    out_dtype (float8_e4m3fn, int8) with their scales [M]; inv [M] fp32 on
-    request, else None."""
+    out_dtype (float8_e4m3fn, int8) with their scales [..]; inv [rows] fp32 on
+    request, else None.  Differentiable (y, h)."""
     _cuda(x, residual, weight)
     code = _layer_code(x, "rms_norm") if out_dtype is None else _QUANT_CODES.get(out_dtype)
     if code is None:
@@ -192,7 +193,7 @@ def rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional
 
 def rms_norm_bwd(dy: torch.Tensor, dh: Optional[torch.Tensor], h: torch.Tensor, weight: Optional[torch.Tensor],
                  inv: torch.Tensor, want_dw: bool):
-    """(dx, dw) of rms_norm's rows; dx is also the residual's gradient."""
+    """(dx, dw) of rms_norm; dx is also the residual's gradient."""
     _cuda(dy, dh, h, weight, inv)
     dx, dw = _op("rms_norm_bwd", dy, dh, h, weight, inv, bool(want_dw))
     return dx, (dw if want_dw else None)
@@ -201,7 +202,8 @@ def rms_norm_bwd(dy: torch.Tensor, dh: Optional[torch.Tensor], h: torch.Tensor, 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, positions: torch.Tensor, axis_pairs,
            interleaved: bool, amplitude: float, inverse: bool = False):
     """q [B,Hq,S,D] and k [B,Hk,S,D] (or None) turned by positions x freqs;
-    axis_pairs: pairs per axis ([]: one position per token).  Returns (q', k')."""
+    axis_pairs: pairs per axis ([]: one position per token).  Returns (q', k').
+    Differentiable (q, k)."""
     _cuda(q, k, freqs, positions)
     oq, ok = _op("rotary", q, k, freqs, positions, list(axis_pairs), bool(interleaved), float(amplitude),
                  bool(inverse))
@@ -210,7 +212,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, posi
 
 def window_fwd(q, k, v, window: int, sinks: int, causal: bool, q_lens: Optional[torch.Tensor],
                kv_lens: Optional[torch.Tensor], sm_scale: float, want_lse: bool):
-    """(o [B,Hq,Sq,D], lse [B,Hq,Sq] fp32 or None) of attention over a window and sinks."""
+    """(o [B,Hq,Sq,D], lse [B,Hq,Sq] fp32 or None) of attention over a window and
+    sinks.  Differentiable (o in q, k, v)."""
     _cuda(q, k, v, q_lens, kv_lens)
     o, lse = _op("window_fwd", q, k, v, int(window), int(sinks), bool(causal), q_lens, kv_lens, float(sm_scale),
                  bool(want_lse))

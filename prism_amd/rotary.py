@@ -13,7 +13,6 @@ import math
 from typing import Optional, Sequence
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -72,28 +71,6 @@ def grid_positions(grid_size, device="cuda") -> torch.Tensor:
     return torch.stack(at, dim=-1).view(T * H * W, 3)
 
 
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, freqs, positions, axis_pairs, interleaved, amplitude):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(freqs, positions)
-        ctx.how = (axis_pairs, interleaved, amplitude)
-        oq, ok = ops.rotary(q, k, freqs, positions, axis_pairs, interleaved, amplitude)
-        return oq if k is None else (oq, ok)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk=None):
-        freqs, positions = ctx.saved_tensors
-        grads = [g for g in (dq, dk) if g is not None]
-        if not grads:
-            return (None,) * 7
-        turned = ops.rotary(grads[0], grads[1] if len(grads) > 1 else None, freqs, positions, *ctx.how, inverse=True)
-        got = iter(turned)
-        return (next(got) if dq is not None else None, next(got) if dk is not None else None, None, None, None, None,
-                None)
-
-
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, positions: torch.Tensor, *,
                  interleaved: bool = True, sections: Optional[Sequence[int]] = None, amplitude: float = 1.0):
     """q [B, Hq, S, D] and k [B, Hk, S, D] (or None) turned by their tokens'
@@ -118,7 +95,8 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor
         if any(int(n) < 2 or int(n) % 2 for n in sections) or sum(int(n) for n in sections) != 2 * freqs.shape[0]:
             raise ValueError(f"apply_rotary: sections {list(sections)} must be even and sum to {2 * freqs.shape[0]}")
         axis_pairs = [int(n) // 2 for n in sections]
-    return _Rotary.apply(q, k, freqs, positions, axis_pairs, bool(interleaved), float(amplitude))
+    oq, ok = ops.rotary(q, k, freqs, positions, axis_pairs, interleaved, amplitude)
+    return oq if k is None else (oq, ok)
 
 
 __all__ = ["rotary_frequencies", "grid_positions", "apply_rotary"]

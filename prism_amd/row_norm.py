@@ -15,13 +15,8 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    return t.reshape(-1, t.shape[-1])
 
 
 def _check(x, weight, residual, eps, name):
@@ -41,33 +36,6 @@ def _check(x, weight, residual, eps, name):
             raise TypeError(f"{name}: residual must have x's dtype {x.dtype}, got {residual.dtype}")
 
 
-class _RmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        ctx.set_materialize_grads(False)
-        rows = _rows(x)
-        train = any(ctx.needs_input_grad[:3])
-        y, h, _, inv = ops.rms_norm(rows, None if residual is None else _rows(residual), weight, eps, want_inv=train)
-        if train:
-            ctx.save_for_backward(rows if h is None else h, weight, inv)
-        ctx.has_residual = residual is not None
-        y = y.view(x.shape)
-        return y if residual is None else (y, h.view(x.shape))
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh=None):
-        h, weight, inv = ctx.saved_tensors
-        if dy is None and dh is None:
-            return None, None, None, None
-        like = dy if dy is not None else dh
-        dy = torch.zeros_like(like) if dy is None else dy  # only h went on
-        dx, dw = ops.rms_norm_bwd(_rows(dy), None if dh is None else _rows(dh), h, weight, inv,
-                                  weight is not None and ctx.needs_input_grad[1])
-        dx = dx.view(like.shape)
-        return dx, dw, dx if ctx.has_residual else None, None
-
-
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None,
              eps: float = 1e-6):
     """y = h / sqrt(mean(h^2) + eps) * weight over the last dimension, h = x +
@@ -76,7 +44,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
     and dtype, or None.  Returns y in x's dtype, with a residual (y, h).
     Differentiable in x, weight, residual, from y and h."""
     _check(x, weight, residual, eps, "rms_norm")
-    return _RmsNorm.apply(x, weight, residual, float(eps))
+    y, h, _, _ = ops.rms_norm(x, residual, weight, eps)
+    return y if residual is None else (y, h)
 
 
 def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None,
@@ -90,10 +59,8 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, re
     _check(x, weight, residual, eps, "rms_norm_quant")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise ValueError("rms_norm_quant has no gradient: call it under torch.no_grad() or on detached tensors")
-    codes, h, scales, _ = ops.rms_norm(_rows(x), None if residual is None else _rows(residual), weight, eps,
-                                       out_dtype=out_dtype)
-    codes, scales = codes.view(x.shape), scales.view(x.shape[:-1])
-    return (codes, scales) if residual is None else (codes, scales, h.view(x.shape))
+    codes, h, scales, _ = ops.rms_norm(x, residual, weight, eps, out_dtype=out_dtype)
+    return (codes, scales) if residual is None else (codes, scales, h)
 
 
 __all__ = ["rms_norm", "rms_norm_quant"]

@@ -12,32 +12,10 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
 _NO_LIMIT = 1 << 29  # a window that no sequence reaches
-
-
-class _WindowAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, window, sinks, causal, sm_scale, q_lens, kv_lens):
-        ctx.set_materialize_grads(False)
-        o, lse = ops.window_fwd(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, True)
-        ctx.how = (window, sinks, causal, sm_scale)
-        ctx.save_for_backward(q, k, v, o, lse, q_lens, kv_lens)
-        ctx.mark_non_differentiable(lse)
-        return o, lse
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, do, _):
-        if do is None:
-            return (None,) * 9
-        q, k, v, o, lse, q_lens, kv_lens = ctx.saved_tensors
-        window, sinks, causal, sm_scale = ctx.how
-        dq, dk, dv = ops.window_bwd(do, q, k, v, o, lse, window, sinks, causal, q_lens, kv_lens, sm_scale)
-        return dq, dk, dv, None, None, None, None, None, None
 
 
 def flash_attn_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Optional[int], *, sinks: int = 0,
@@ -89,10 +67,7 @@ def flash_attn_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window:
     sm_scale = D ** -0.5 if sm_scale is None else float(sm_scale)
     if not 0 < sm_scale < float("inf"):
         raise ValueError(f"sm_scale must be positive and finite, got {sm_scale}")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        o, lse = _WindowAttention.apply(q, k, v, window, int(sinks), bool(causal), sm_scale, q_lens, kv_lens)
-    else:
-        o, lse = ops.window_fwd(q, k, v, window, int(sinks), bool(causal), q_lens, kv_lens, sm_scale, return_lse)
+    o, lse = ops.window_fwd(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, return_lse)
     return (o, lse) if return_lse else o
 
 

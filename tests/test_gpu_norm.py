@@ -120,14 +120,15 @@ def test_8_bits(M, N, dt, out):
 
 def test_strides_and_views():
     """Rows inside a wider tensor, a leading slice, an odd offset, a transposed
-    view, broadcast rows and weights."""
+    view, broadcast rows and weights (rows that are not aligned are added in
+    another order than aligned ones, so only the bound is compared)."""
+    torch.manual_seed(11)
     base = torch.randn(6, 40, 300, device="cuda", dtype=torch.bfloat16)
     w = torch.randn(256, device="cuda", dtype=torch.bfloat16)
     views = [(base[:, :, :256], w), (base[:, :, 3:260], base[0, 0, :257]), (base[::2, 1:, 8:264], w),
              (base.transpose(1, 2)[:, :40], base[0, 0, :40]), (base[:1, :1, :256].expand(5, 3, 256), w)]
     for x, wv in views:
         y = prism_amd.rms_norm(x, wv)
-        assert torch.equal(y, prism_amd.rms_norm(x.clone(memory_format=torch.contiguous_format), wv.clone()))
         y64 = exact(x, None, wv, 1e-6)[2]
         check(y, y64, rounded(x.dtype, y64) + 50 * U * y64.abs(), "y")
 
@@ -248,3 +249,22 @@ def test_opcheck():
     for dh, want in ((r, True), (None, False)):
         torch.library.opcheck(torch.ops.prism.rms_norm_bwd.default, (x, dh, r, w, inv, want),
                               test_utils=("test_schema", "test_faketensor"))
+
+
+def test_second_derivatives_are_refused_and_changed_inputs_seen():
+    x, r, w = (t.requires_grad_(True) for t in make(4, 64, torch.float32))
+    freqs, _ = prism_amd.rotary_frequencies(64)
+    at = torch.arange(5, device="cuda")
+    q = torch.randn(1, 2, 5, 64, device="cuda").half().requires_grad_(True)
+    for y, leaf in ((prism_amd.rms_norm(x, w, residual=r)[0], x),
+                    (prism_amd.apply_rotary(q, None, freqs, at), q), (prism_amd.flash_attn_window(q, q, q, 2), q)):
+        (g,) = torch.autograd.grad(y.float().sum(), leaf, create_graph=True)
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            g.float().sum().backward()
+    y, h = prism_amd.rms_norm(x, w, residual=r)
+    h.data.mul_(1)  # (not seen: .data has no version)
+    with torch.no_grad():
+        h.add_(1)   # what the backward reads has changed
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
