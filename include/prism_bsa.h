@@ -157,10 +157,15 @@ int prism_rotary(const void* q, const void* k, int dtype, int B, int64_t S, int 
  * sinks and j <= p (causal), else where |p - j| < window or j < sinks.  o: 0
  * for queries that see nothing and rows i >= n; lse: [B, Hq, Sq] fp32 natural
  * log-sum-exp of the scaled scores (-inf there), or NULL.  Rows of k and v that
- * no query sees are not read.  No counterpart in the reference. */
+ * no query sees are not read.  part: workspace of as many floats as prism_window_fwd_plan says
+ * (NULL for 0): row tiles of the launch's last round may be cut over several
+ * workgroups, whose sums a second kernel joins in order.  No counterpart in the
+ * reference. */
+int prism_window_fwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal,
+                          int64_t* floats);
 int prism_window_fwd(const void* q, const void* k, const void* v, int dtype, int B, int Hq, int Hk, int64_t Sq,
                      int64_t Sk, int D, const int64_t* strides, int64_t window, int64_t sinks, int causal,
-                     const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, float* lse,
+                     const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, float* lse, float* part,
                      hipStream_t stream);
 
 /* prism_window_fwd for few query rows over many keys (single tokens over a

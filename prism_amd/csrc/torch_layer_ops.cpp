@@ -237,9 +237,12 @@ std::tuple<Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_, const 
                      o.data_ptr(), lp, splits, po, po ? po + floats * s.D : nullptr, stream_of(q));
     return {o, lse};
   }
+  int64_t floats = 0;
+  check_rc(prism_window_fwd_plan(B, Hq, Hk, s.Sq, s.Sk, D, window, sinks, causal, &floats));
+  Tensor part = floats ? at::empty({floats}, opts(q, at::kFloat)) : none_like(q);
   PRISM_TORCH_CALL(prism_window_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st,
                    window, sinks, causal, (const int32_t*)p(q_lens), (const int32_t*)p(kv_lens), (float)sm_scale,
-                   o.data_ptr(), lp, stream_of(q));
+                   o.data_ptr(), lp, floats ? part.data_ptr<float>() : nullptr, stream_of(q));
   return {o, lse};
 }
 

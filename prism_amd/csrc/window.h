@@ -71,10 +71,12 @@ struct WinArgs {
   float scale, scale_log2;
   float* lse;                       // [B, Hk G, Sq] natural log, -inf for rows that see nothing; or null
   int tiles;                        // row tiles of a (sequence, key head)
-  int total;                        // work items of the launch
-  // single tokens: key splits, their partial results (o [splits, B Hk, tiles, 32, D], m and l [.., 32] each)
-  int splits;
-  float *part_o, *part_ml;
+  int total;                        // row tiles of the launch
+  // Work items: the first `whole` row tiles one each, every later one `splits`,
+  // item i of which takes the i-th part of its key list (single tokens: whole =
+  // 0) and leaves its sums in part (and m and l in part_ml)
+  int whole, splits, items;
+  float *part, *part_ml;
 };
 
 // ------------------------------------------------------------ spans
@@ -231,14 +233,25 @@ struct StageCopy {
   }
 };
 
-// work item -> (sequence, key head, row tile): row tiles of one key head are
-// neighbours (their windows overlap in an XCD's L2), the last ones, whose causal
-// lists are longest, first
-__device__ __forceinline__ void win_item(const WinArgs& a, int id, int& b, int& hk, int& tile) {
-  const int bh = id / a.tiles;
-  tile = a.tiles - 1 - (id - bh * a.tiles);
-  b = bh / a.Hk;
-  hk = bh - b * a.Hk;
+// Work item -> (sequence, key head, row tile), part of its list and workspace
+// slot (-1: whole).  Row tiles of one key head are neighbours (their windows
+// overlap in an XCD's L2), the last ones, whose causal lists are longest, first.
+struct WinItem {
+  int b, hk, tile, split, slot;
+};
+__device__ __forceinline__ WinItem win_tile(const WinArgs& a, int index, int split, int slot) {
+  WinItem it;
+  const int bh = index / a.tiles;
+  it.tile = a.tiles - 1 - (index - bh * a.tiles);
+  it.b = bh / a.Hk;
+  it.hk = bh - it.b * a.Hk;
+  it.split = split;
+  it.slot = slot;
+  return it;
+}
+__device__ __forceinline__ WinItem win_item(const WinArgs& a, int id) {
+  const int y = id - a.whole, q = y / a.splits;
+  return id < a.whole ? win_tile(a, id, 0, -1) : win_tile(a, a.whole + q, y - q * a.splits, a.splits == 1 ? -1 : y);
 }
 
 // ------------------------------------------------------------ host side (window_fwd.hip)
@@ -250,3 +263,28 @@ int win_check(const char* name, int dtype, int B, int Hq, int Hk, int64_t Sq, in
 WinArgs win_args(const void* q, const void* k, const void* v, void* o, int B, int Hq, int Hk, int64_t Sq, int64_t Sk,
                  const int64_t* strides, int64_t window, int64_t sinks, int causal, const int32_t* q_lens,
                  const int32_t* kv_lens, float sm_scale);
+
+// How a launch of `total` tiles (of about `units` list entries each) is cut so
+// that it ends evenly on `slots` workgroups at a time: whole rounds as they are,
+// and the tiles of the last round in the number of parts that takes least time,
+// a part costing its entries and 3 more, the second kernel 5.
+struct WinCut {
+  int64_t whole, splits;
+};
+inline WinCut win_cut(int64_t total, int64_t slots, int64_t units) {
+  WinCut c{total / slots * slots, 1};
+  const int64_t rest = total - c.whole;
+  double best = 0;
+  for (int64_t s = 1; s <= 32 && (s == 1 || units >= 4 * s); ++s) {
+    const double cost = (double)((rest * s + slots - 1) / slots) * ((double)units / (double)s + 3) + (s > 1 ? 5 : 0);
+    if (s == 1 || cost < best) {
+      best = cost;
+      c.splits = s;
+    }
+  }
+  if (c.splits == 1) c.whole = total;
+  return c;
+}
+// the cut of a launch over row tiles of 128 (forward, dQ)
+WinCut win_row_cut(int64_t slots, int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int64_t window, int64_t sinks,
+                   int causal);

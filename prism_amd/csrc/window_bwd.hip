@@ -29,9 +29,10 @@ struct WinBwdArgs {
   WinTensor do_, dq, dk, dv;
   float* m2;                 // [B Hq, Sq]
   float* delta;              // [B Hq, Sq]
-  // dK/dV items: per (sequence, key head) the sink tiles, then the rest, each in
-  // its number of pieces; pieces of a cut tile leave their sums in acc
-  int sink_tiles, key_tiles, sink_splits, rest_splits, items;
+  // dK/dV items: the sink tiles of all heads, sink_splits pieces each, then the
+  // other tiles, rest_whole whole and the others in rest_splits pieces; pieces of
+  // a cut tile leave their sums in acc
+  int sink_tiles, key_tiles, sink_splits, sink_items, rest_whole, rest_splits, items;
   float4* acc;
 };
 
@@ -59,19 +60,21 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs ba) {
   __shared__ __align__(1024) uint8_t smem[2 * T::STAGE];
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
   const int w = (int)uniform_u32(threadIdx.x >> 6);
-  int b, hk, tile;
-  win_item(a, xcd_group_remap<32>((int)blockIdx.x, a.total), b, hk, tile);
+  const WinItem it = win_item(a, xcd_group_remap<32>((int)blockIdx.x, a.items));
+  const int b = it.b, hk = it.hk, tile = it.tile;
   const SeqSpan sq = seq_span(a, b);
   const int rows = a.Sq * a.G, r0 = tile * 128, wr0 = r0 + 32 * w;
   const int last = sq.n - 1;
   auto token = [&](int r) { const int i = r / a.G; return i < last ? i : last; };
   const KeyList kl = r0 / a.G > last ? KeyList{0, 0, 0} : key_list(a, sq, r0 / a.G, token(r0 + 127));
-  const int nt = (kl.n + 63) >> 6;
+  const int every = (kl.n + 63) >> 6;
+  const int t0 = it.slot < 0 ? 0 : every * it.split / a.splits;
+  const int t1 = it.slot < 0 ? every : every * (it.split + 1) / a.splits;
 
   StageCopy<D> copy;
   copy.init(a, b, hk, w & 1, lane);
   const uint32_t lds0 = lds_addr(smem);
-  if (w < 2 && nt > 0) copy.issue(kl, 0, lds0);
+  if (w < 2 && t1 > t0) copy.issue(kl, 64 * t0, lds0 + (uint32_t)((t0 & 1) * T::STAGE));
 
   RowOperand rop;  // K / V rows l32 (+ 32 kh as an immediate)
   rop.init<RT>(0, l32, g);
@@ -99,7 +102,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs ba) {
   const float lse = a.lse[lrow];
   // rows that see nothing: P = 2^(s - inf) = 0
   const float mq = lse == -__builtin_inff() ? __builtin_inff() : lse * 1.4426950408889634f;
-  if (r < rows && g == 0) {
+  if (r < rows && g == 0 && it.split == 0) {
     ba.m2[lrow] = mq;
     ba.delta[lrow] = dlt;
   }
@@ -125,10 +128,10 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs ba) {
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) dq[dt] = f32x16_zero();
 
-  for (int t = 0; t < nt; ++t) {
+  for (int t = t0; t < t1; ++t) {
     dma_wait_all();
     __syncthreads();
-    if (w < 2 && t + 1 < nt) copy.issue(kl, 64 * (t + 1), lds0 + (uint32_t)(((t + 1) & 1) * T::STAGE));
+    if (w < 2 && t + 1 < t1) copy.issue(kl, 64 * (t + 1), lds0 + (uint32_t)(((t + 1) & 1) * T::STAGE));
     const int u0 = 64 * t;
     if (!some || !ws.any(u0, u0 + 63)) continue;
     const uint8_t* sK = smem + (t & 1) * T::STAGE;
@@ -197,6 +200,15 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs ba) {
     }
     __builtin_amdgcn_s_setprio(0);
   }
+  if (it.slot >= 0) {
+    float4* pa = reinterpret_cast<float4*>(a.part) + ((int64_t)it.slot * 4 + w) * NDT * 256 + lane;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj)
+        pa[(dt * 4 + jj) * 64] = make_float4(dq[dt][4 * jj], dq[dt][4 * jj + 1], dq[dt][4 * jj + 2], dq[dt][4 * jj + 3]);
+    return;
+  }
   if (r >= rows) return;
   uint16_t* dqr = ba.dq.p + b * ba.dq.b + head * ba.dq.h + i * ba.dq.s;
 #pragma unroll
@@ -224,25 +236,34 @@ __device__ __forceinline__ TokenRange tokens_of(const WinArgs& a, const SeqSpan&
 }
 
 struct DkdvItem {
-  int b, hk, tile, split, splits, slot;  // slot: first workspace piece of a cut tile plus split, -1: whole
+  int b, hk, tile, split, splits, slot;  // slot: workspace piece, -1: the whole list
 };
 __device__ __forceinline__ DkdvItem dkdv_item(const WinBwdArgs& a, int id) {
-  const int rest = a.key_tiles - a.sink_tiles;
-  const int per = a.sink_tiles * a.sink_splits + rest * a.rest_splits;
-  const int cut = (a.sink_splits > 1 ? a.sink_tiles * a.sink_splits : 0) + (a.rest_splits > 1 ? rest * a.rest_splits : 0);
-  const int bh = id / per, x = id - bh * per, sinks = a.sink_tiles * a.sink_splits;
+  const int nrest = a.key_tiles - a.sink_tiles;
   DkdvItem d;
+  int bh;
+  if (id < a.sink_items) {
+    const int t = id / a.sink_splits;
+    bh = t / a.sink_tiles;
+    d.tile = t - bh * a.sink_tiles;
+    d.splits = a.sink_splits;
+    d.split = id - t * a.sink_splits;
+    d.slot = a.sink_splits > 1 ? id : -1;
+  } else {
+    const int y = id - a.sink_items, z = y - a.rest_whole;
+    const int t = z < 0 ? y : a.rest_whole + z / a.rest_splits;  // tile of the rest, all heads in a row
+    bh = t / nrest;
+    d.tile = a.sink_tiles + t - bh * nrest;
+    d.splits = z < 0 ? 1 : a.rest_splits;
+    d.split = z < 0 ? 0 : z % a.rest_splits;
+    d.slot = z < 0 || a.rest_splits == 1 ? -1 : (a.sink_splits > 1 ? a.sink_items : 0) + z;
+  }
   d.b = bh / a.w.Hk;
   d.hk = bh - d.b * a.w.Hk;
-  const bool sink = x < sinks;
-  d.splits = sink ? a.sink_splits : a.rest_splits;
-  const int y = sink ? x : x - sinks;
-  d.tile = (sink ? 0 : a.sink_tiles) + y / d.splits;
-  d.split = y % d.splits;
-  d.slot = d.splits == 1 ? -1 : bh * cut + (sink ? x : (a.sink_splits > 1 ? sinks : 0) + y);
   return d;
 }
 
+constexpr int kDqSlots = 512;  // workgroups of window_dq_kernel that the chip holds: two a CU
 constexpr int kStages = 4, kAhead = 2;  // entry j + 2 is copied while j is multiplied (waves behind still read j - 1)
 
 template <int D>
@@ -547,25 +568,61 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
   }
 }
 
-// the pieces' sums of the cut tiles, in order: one workgroup per tile and
-// 32-column block of dK (blocks 0 .. NDT - 1) or dV; wave = 32 keys
+// the parts of the row tiles of dQ that were cut, in order: one workgroup per
+// tile and 32 channels, the lanes of window_dq_kernel
 template <class E, int D>
-__global__ __launch_bounds__(256) void window_merge_kernel(WinBwdArgs a, int cut_sinks, int cut_rest) {
+__global__ __launch_bounds__(256) void window_dq_merge_kernel(WinBwdArgs ba) {
+  constexpr int NDT = D / 32;
+  const WinArgs& a = ba.w;
+  const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, w = threadIdx.x >> 6, dt = (int)blockIdx.y;
+  const WinItem it = win_tile(a, a.whole + (int)blockIdx.x, 0, 0);
+  const int r = it.tile * 128 + 32 * w + l32;
+  if (r >= a.Sq * a.G) return;
+  const float4* pa = reinterpret_cast<const float4*>(a.part) + (((int64_t)blockIdx.x * a.splits * 4 + w) * NDT + dt) * 256 + lane;
+  float4 acc[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc[j] = pa[j * 64];
+#pragma unroll 4
+  for (int s = 1; s < a.splits; ++s)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 v = pa[(int64_t)s * 4 * NDT * 256 + j * 64];
+      acc[j].x += v.x;
+      acc[j].y += v.y;
+      acc[j].z += v.z;
+      acc[j].w += v.w;
+    }
+  const int i = r / a.G, head = it.hk * a.G + (r - i * a.G);
+  uint16_t* out = ba.dq.p + it.b * ba.dq.b + head * ba.dq.h + i * ba.dq.s + 32 * dt + 4 * g;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint2 u;
+    u.x = E::pack(acc[j].x * a.scale, acc[j].y * a.scale);
+    u.y = E::pack(acc[j].z * a.scale, acc[j].w * a.scale);
+    *reinterpret_cast<uint2*>(out + 8 * j) = u;
+  }
+}
+
+// the pieces' sums of the cut key tiles (cut_sinks sink tiles, then the rest's),
+// in order: one workgroup per tile and 32-column block of dK (blocks 0 .. NDT - 1)
+// or dV; wave = 32 keys
+template <class E, int D>
+__global__ __launch_bounds__(256) void window_merge_kernel(WinBwdArgs a, int cut_sinks) {
   constexpr int NDT = D / 32, NB = 2 * NDT;
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, w = threadIdx.x >> 6, blk = (int)blockIdx.y;
-  const int per = cut_sinks + cut_rest;  // cut tiles per (sequence, key head)
-  const int bh = (int)blockIdx.x / per, x = (int)blockIdx.x - bh * per;
-  const bool sink = x < cut_sinks;
-  const int S = sink ? a.sink_splits : a.rest_splits;
-  const int tile = sink ? x : a.sink_tiles + x - cut_sinks;
-  const int64_t first = (int64_t)bh * (cut_sinks * a.sink_splits + cut_rest * a.rest_splits) +
-                        (sink ? x * S : cut_sinks * a.sink_splits + (x - cut_sinks) * S);
+  const int x = (int)blockIdx.x, z = x - cut_sinks;
+  const bool sink = z < 0;
+  const int S = sink ? a.sink_splits : a.rest_splits, nrest = a.key_tiles - a.sink_tiles;
+  const int64_t first = sink ? (int64_t)x * S : (int64_t)cut_sinks * a.sink_splits + (int64_t)z * S;
+  const int bh = sink ? x / a.sink_tiles : (a.rest_whole + z) / nrest;
+  const int tile = sink ? x - bh * a.sink_tiles : a.sink_tiles + a.rest_whole + z - bh * nrest;
   const int b = bh / a.w.Hk, hk = bh - b * a.w.Hk, key = tile * 128 + 32 * w + l32;
   if (key >= a.w.Sk) return;
   const float4* pa = a.acc + ((first * 4 + w) * NB + blk) * 256 + lane;
   float4 acc[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) acc[j] = pa[j * 64];
+#pragma unroll 4
   for (int s = 1; s < S; ++s)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -588,28 +645,45 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinBwdArgs a, int cut
   }
 }
 
-// pieces of the dK/dV lists: none longer than a third of a CU's share of the
-// launch (so the chip ends evenly), nor shorter than 8 entries
+// How the dK/dV lists are cut, for one workgroup a CU: the sinks' lists into
+// pieces no longer than the others, then the last round of tiles (win_cut).
 struct DkdvPlan {
-  int64_t sink_tiles, key_tiles, sink_splits, rest_splits, pieces;
+  int64_t sink_tiles, key_tiles, sink_splits, sink_items, rest_whole, rest_splits, rest_tiles, items, pieces;
 };
 DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int64_t window, int64_t sinks, int causal) {
   DkdvPlan p{};
+  const int64_t BH = (int64_t)B * Hk, whole = G * ((Sq + 63) / 64);
+  const int64_t span = window < Sq ? (causal ? window : 2 * window) + 127 : Sq;
   p.key_tiles = (Sk + 127) / 128;
   p.sink_tiles = ((sinks < Sk ? sinks : Sk) + 127) / 128;
-  const int64_t whole = (Sq + 63) / 64;
-  const int64_t span = window < Sq ? (causal ? window : 2 * window) + 127 : Sq;
-  const int64_t rest = G * (span < Sq ? (span + 63) / 64 : whole), sink = G * whole;
-  const int64_t nrest = p.key_tiles - p.sink_tiles;
-  const int64_t total = (int64_t)B * Hk * (p.sink_tiles * sink + nrest * rest);
-  int64_t target = (total + 767) / 768;
-  target = target > 8 ? target : 8;
-  auto cut = [&](int64_t n) { return n > target + target / 2 ? (n + target - 1) / target : 1; };
-  p.sink_splits = cut(sink);
-  p.rest_splits = cut(rest);
-  p.pieces = (int64_t)B * Hk * ((p.sink_splits > 1 ? p.sink_tiles * p.sink_splits : 0) +
-                                (p.rest_splits > 1 ? nrest * p.rest_splits : 0));
+  int64_t rest = span < Sq ? G * ((span + 63) / 64) : whole;
+  if (rest >= whole || p.sink_tiles == p.key_tiles) {  // all lists alike
+    p.sink_tiles = 0;
+    rest = whole;
+  }
+  const int64_t n = (rest > 8 ? rest : 8);
+  p.rest_tiles = BH * (p.key_tiles - p.sink_tiles);
+  p.sink_splits = p.sink_tiles ? (whole + n - 1) / n : 1;
+  int64_t head = BH * p.sink_tiles * p.sink_splits;  // pieces before the rest's tiles
+  const int64_t slots = 256, total = head + p.rest_tiles;
+  const WinCut c = win_cut(total, slots, rest);
+  p.rest_splits = c.splits;
+  p.rest_whole = c.whole > head ? c.whole - head : 0;
+  if (p.rest_whole > p.rest_tiles) p.rest_whole = p.rest_tiles;
+  if (c.splits == 1) p.rest_whole = p.rest_tiles;
+  if (c.whole == 0 && c.splits > 1 && p.sink_tiles) {  // less than a round: the sinks' pieces as short as the others
+    const int64_t m = rest / c.splits > 8 ? rest / c.splits : 8;
+    p.sink_splits = (whole + m - 1) / m < 256 ? (whole + m - 1) / m : 256;
+    head = BH * p.sink_tiles * p.sink_splits;
+  }
+  p.sink_items = head;
+  p.items = head + p.rest_whole + (p.rest_tiles - p.rest_whole) * p.rest_splits;
+  p.pieces = (p.sink_splits > 1 ? head : 0) + (p.rest_splits > 1 ? (p.rest_tiles - p.rest_whole) * p.rest_splits : 0);
   return p;
+}
+// float4-aligned workspace: dK/dV pieces, then dQ parts
+int64_t bwd_floats(const DkdvPlan& p, const WinCut& c, int64_t row_tiles, int64_t D) {
+  return p.pieces * 256 * D + (row_tiles - c.whole) * c.splits * 128 * D;
 }
 
 }  // namespace
@@ -621,7 +695,9 @@ int prism_window_bwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, 
   PRISM_REQUIRE(B >= 0 && Hk >= 1 && Hq >= Hk && Hq % Hk == 0 && Sq >= 0 && Sk >= 0 && D >= 1 && window >= 1 &&
                     sinks >= 0 && floats,
                 "prism_window_bwd_plan: bad argument");
-  *floats = dkdv_plan(B, Hk, Hq / Hk, Sq, Sk, window, sinks, causal).pieces * 256 * D;
+  const int64_t G = Hq / Hk;
+  *floats = bwd_floats(dkdv_plan(B, Hk, G, Sq, Sk, window, sinks, causal),
+                       win_row_cut(kDqSlots, B, Hk, G, Sq, Sk, window, sinks, causal), (int64_t)B * Hk * ((Sq * G + 127) / 128), D);
   return PRISM_OK;
 }
 
@@ -630,13 +706,11 @@ int prism_window_bwd(const void* do_, const void* q, const void* k, const void* 
                      int64_t window, int64_t sinks, int causal, const int32_t* q_lens, const int32_t* kv_lens,
                      float sm_scale, void* dq, void* dk, void* dv, float* rows, float* acc, hipStream_t stream) {
   if (const int rc = win_check("prism_window_bwd", dtype, B, Hq, Hk, Sq, Sk, D, window, sinks, sm_scale, strides, 8,
-                               {q, k, v, o, do_, dq, dk, dv}))
+                               {q, k, v, o, do_, dq, dk, dv, acc}))
     return rc;
   if (B == 0) return PRISM_OK;
   PRISM_REQUIRE(Sq == 0 || (q && o && do_ && lse && dq && rows), "prism_window_bwd: null pointer");
   PRISM_REQUIRE(Sk == 0 || (k && v && dk && dv), "prism_window_bwd: null pointer");
-  const DkdvPlan p = dkdv_plan(B, Hk, Hq / Hk, Sq, Sk, window, sinks, causal);
-  PRISM_REQUIRE(p.pieces == 0 || acc, "prism_window_bwd: null workspace");
   WinBwdArgs a{};
   a.w = win_args(q, k, v, (void*)o, B, Hq, Hk, Sq, Sk, strides, window, sinks, causal, q_lens, kv_lens, sm_scale);
   a.w.lse = (float*)lse;
@@ -647,24 +721,29 @@ int prism_window_bwd(const void* do_, const void* q, const void* k, const void* 
   a.dv = {(uint16_t*)dv, s[9], s[10], s[11]};
   a.m2 = rows;
   a.delta = rows + (int64_t)B * Hq * Sq;
-  a.sink_tiles = (int)p.sink_tiles; a.key_tiles = (int)p.key_tiles;
-  a.sink_splits = (int)p.sink_splits; a.rest_splits = (int)p.rest_splits;
-  a.acc = (float4*)acc;
   a.w.tiles = (int)((Sq * a.w.G + 127) / 128);
   const int64_t total = (int64_t)B * Hk * a.w.tiles;
-  const int64_t rest = p.key_tiles - p.sink_tiles;
-  const int64_t items = (int64_t)B * Hk * (p.sink_tiles * p.sink_splits + rest * p.rest_splits);
-  PRISM_REQUIRE(total < (1ll << 31) && items < (1ll << 31), "prism_window_bwd: too many tiles");
+  const WinCut c = win_row_cut(kDqSlots, B, Hk, a.w.G, Sq, Sk, window, sinks, causal);
+  const DkdvPlan p = dkdv_plan(B, Hk, a.w.G, Sq, Sk, window, sinks, causal);
+  const int64_t cut = total - c.whole, items = c.whole + cut * c.splits;
+  PRISM_REQUIRE(items < (1ll << 31) && p.items < (1ll << 31), "prism_window_bwd: too many tiles");
+  PRISM_REQUIRE(p.pieces + cut == 0 || acc, "prism_window_bwd: null workspace");
   a.w.total = (int)total;
-  a.items = (int)items;
-  const int cs = p.sink_splits > 1 ? a.sink_tiles : 0, cr = p.rest_splits > 1 ? (int)rest : 0;
+  a.w.whole = (int)c.whole; a.w.splits = (int)c.splits; a.w.items = (int)items;
+  a.w.part = acc + p.pieces * 256 * D;
+  a.sink_tiles = (int)p.sink_tiles; a.key_tiles = (int)p.key_tiles;
+  a.sink_splits = (int)p.sink_splits; a.sink_items = (int)p.sink_items;
+  a.rest_whole = (int)p.rest_whole; a.rest_splits = (int)p.rest_splits; a.items = (int)p.items;
+  a.acc = (float4*)acc;
+  const int cut_sinks = p.sink_splits > 1 ? B * Hk * a.sink_tiles : 0;
+  const int64_t cut_keys = cut_sinks + (p.rest_splits > 1 ? p.rest_tiles - p.rest_whole : 0);
   auto run = [&](auto e, auto d) {
     using E = decltype(e);
     constexpr int DD = decltype(d)::value;
-    if (total) window_dq_kernel<E, DD><<<(unsigned)total, 256, 0, stream>>>(a);
-    if (items) window_dkdv_kernel<E, DD><<<(unsigned)items, 512, 0, stream>>>(a);
-    if (items && cs + cr)
-      window_merge_kernel<E, DD><<<dim3((unsigned)(B * Hk * (cs + cr)), DD / 16), 256, 0, stream>>>(a, cs, cr);
+    if (items) window_dq_kernel<E, DD><<<(unsigned)items, 256, 0, stream>>>(a);
+    if (cut) window_dq_merge_kernel<E, DD><<<dim3((unsigned)cut, DD / 32), 256, 0, stream>>>(a);
+    if (p.items) window_dkdv_kernel<E, DD><<<(unsigned)p.items, 512, 0, stream>>>(a);
+    if (cut_keys) window_merge_kernel<E, DD><<<dim3((unsigned)cut_keys, DD / 16), 256, 0, stream>>>(a, cut_sinks);
   };
   if (dtype == PRISM_BF16) {
     if (D == 64) run(WinBf16{}, std::integral_constant<int, 64>{});

@@ -27,20 +27,21 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WinArgs a) {
   __shared__ __align__(1024) uint8_t smem[2 * T::STAGE];
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
   const int w = (int)uniform_u32(threadIdx.x >> 6);
-  int b, hk, tile;
-  win_item(a, xcd_group_remap<32>((int)blockIdx.x, a.total), b, hk, tile);
+  const WinItem it = win_item(a, xcd_group_remap<32>((int)blockIdx.x, a.items));
+  const int b = it.b, hk = it.hk, tile = it.tile;
   const SeqSpan sq = seq_span(a, b);
   const int rows = a.Sq * a.G, r0 = tile * 128, wr0 = r0 + 32 * w;
   const int last = sq.n - 1;
   auto token = [&](int r) { const int i = r / a.G; return i < last ? i : last; };
   const KeyList kl = r0 / a.G > last ? KeyList{0, 0, 0} : key_list(a, sq, r0 / a.G, token(r0 + 127));
-  const int nt = (kl.n + 63) >> 6;
+  const int all = (kl.n + 63) >> 6;
+  const int t0 = it.slot < 0 ? 0 : all * it.split / a.splits, t1 = it.slot < 0 ? all : all * (it.split + 1) / a.splits;
 
   const float NINF = -__builtin_inff();
   StageCopy<D> copy;
   copy.init(a, b, hk, w & 1, lane);
   const uint32_t lds0 = lds_addr(smem);
-  if (w < 2 && nt > 0) copy.issue(kl, 0, lds0);
+  if (w < 2 && t1 > t0) copy.issue(kl, 64 * t0, lds0 + (uint32_t)((t0 & 1) * T::STAGE));
 
   RowOperand kop;
   kop.init<RT>(0, l32, g);
@@ -71,10 +72,10 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WinArgs a) {
   for (int dt = 0; dt < NDT; ++dt) acc_o[dt] = f32x16_zero();
   float m = NINF, l = 1.0f;
 
-  for (int t = 0; t < nt; ++t) {
+  for (int t = t0; t < t1; ++t) {
     dma_wait_all();
     __syncthreads();
-    if (w < 2 && t + 1 < nt) copy.issue(kl, 64 * (t + 1), lds0 + (uint32_t)(((t + 1) & 1) * T::STAGE));
+    if (w < 2 && t + 1 < t1) copy.issue(kl, 64 * (t + 1), lds0 + (uint32_t)(((t + 1) & 1) * T::STAGE));
     const int u0 = 64 * t;
     if (!some || !ws.any(u0, u0 + 63)) continue;
     const uint8_t* sK = smem + (t & 1) * T::STAGE;
@@ -163,6 +164,17 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WinArgs a) {
     __builtin_amdgcn_s_setprio(0);
   }
 
+  if (it.slot >= 0) {  // a part: unnormalised sums in register order, reference and sum
+    float4* pa = reinterpret_cast<float4*>(a.part) + ((int64_t)it.slot * 4 + w) * NDT * 256 + lane;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        pa[(dt * 4 + j) * 64] =
+            make_float4(acc_o[dt][4 * j], acc_o[dt][4 * j + 1], acc_o[dt][4 * j + 2], acc_o[dt][4 * j + 3]);
+    if (g == 0) reinterpret_cast<float2*>(a.part_ml)[((int64_t)it.slot * 4 + w) * 32 + l32] = make_float2(m, l);
+    return;
+  }
   if (r >= rows) return;
   const float inv = 1.0f / l;
   uint16_t* op = a.o.p + b * a.o.b + head * a.o.h + i * a.o.s;
@@ -179,7 +191,63 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WinArgs a) {
     a.lse[((int64_t)b * a.Hk * a.G + head) * a.Sq + i] = (m + __log2f(l)) * 0.6931471805599453f;
 }
 
+// the parts of a cut row tile, in order: one workgroup per tile and 32 channels,
+// the lanes of window_fwd_kernel
+template <class E, int D>
+__global__ __launch_bounds__(256) void window_fwd_join_kernel(WinArgs a) {
+  constexpr int NDT = D / 32;
+  const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, w = threadIdx.x >> 6, dt = (int)blockIdx.y;
+  const WinItem it = win_tile(a, a.whole + (int)blockIdx.x, 0, 0);
+  const int r = it.tile * 128 + 32 * w + l32;
+  if (r >= a.Sq * a.G) return;
+  const float NINF = -__builtin_inff();
+  const int64_t first = (int64_t)blockIdx.x * a.splits * 4 + w;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first * 32 + l32;
+  const float4* pa = reinterpret_cast<const float4*>(a.part) + (first * NDT + dt) * 256 + lane;
+  float top = NINF;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[(int64_t)s * 128].x);
+  float4 o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float l = 0.0f;
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 x = ml[(int64_t)s * 128];
+    const float f = x.x == NINF ? 0.0f : fast_exp2(x.x - top);  // (a part that sees nothing has sums of 0)
+    l = __builtin_fmaf(x.y, f, l);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 v = pa[(int64_t)s * 4 * NDT * 256 + j * 64];
+      o[j].x = __builtin_fmaf(v.x, f, o[j].x);
+      o[j].y = __builtin_fmaf(v.y, f, o[j].y);
+      o[j].z = __builtin_fmaf(v.z, f, o[j].z);
+      o[j].w = __builtin_fmaf(v.w, f, o[j].w);
+    }
+  }
+  const bool none = top == NINF;
+  const float inv = none ? 0.0f : 1.0f / l;
+  const int i = r / a.G, head = it.hk * a.G + (r - i * a.G);
+  uint16_t* op = a.o.p + it.b * a.o.b + head * a.o.h + i * a.o.s + 32 * dt + 4 * g;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint2 u;
+    u.x = E::pack(o[j].x * inv, o[j].y * inv);
+    u.y = E::pack(o[j].z * inv, o[j].w * inv);
+    *reinterpret_cast<uint2*>(op + 8 * j) = u;
+  }
+  if (a.lse && g == 0 && dt == 0)
+    a.lse[((int64_t)it.b * a.Hk * a.G + head) * a.Sq + i] = none ? NINF : (top + __log2f(l)) * 0.6931471805599453f;
+}
+
 }  // namespace
+
+WinCut win_row_cut(int64_t slots, int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int64_t window, int64_t sinks,
+                   int causal) {
+  const int64_t tokens = 128 / G + 1 < Sq ? 128 / G + 1 : Sq;
+  const int64_t side = window < Sk ? (causal ? window : 2 * window) : Sk;
+  const int64_t seen = side + tokens + sinks < Sk ? side + tokens + sinks : Sk;
+  return win_cut((int64_t)B * Hk * ((Sq * G + 127) / 128), slots, (seen + 63) / 64);
+}
 
 int win_check(const char* name, int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window,
               int64_t sinks, float sm_scale, const int64_t* strides, int tensors,
@@ -220,26 +288,57 @@ WinArgs win_args(const void* q, const void* k, const void* v, void* o, int B, in
   return a;
 }
 
-extern "C" int prism_window_fwd(const void* q, const void* k, const void* v, int dtype, int B, int Hq, int Hk,
-                                int64_t Sq, int64_t Sk, int D, const int64_t* strides, int64_t window, int64_t sinks,
-                                int causal, const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o,
-                                float* lse, hipStream_t stream) {
-  if (const int rc = win_check("prism_window_fwd", dtype, B, Hq, Hk, Sq, Sk, D, window, sinks, sm_scale, strides, 4, {q, k, v, o})) return rc;
+// workgroups of window_fwd_kernel that the chip holds: two a CU at D = 128, three
+// at 64 (registers)
+static int64_t fwd_slots(int D) { return D == 128 ? 512 : 768; }
+
+extern "C" {
+
+int prism_window_fwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal,
+                          int64_t* floats) {
+  PRISM_REQUIRE(B >= 0 && Hk >= 1 && Hq >= Hk && Hq % Hk == 0 && Sq >= 0 && Sk >= 0 && D >= 1 && window >= 1 &&
+                    sinks >= 0 && floats,
+                "prism_window_fwd_plan: bad argument");
+  const int64_t G = Hq / Hk;
+  const WinCut c = win_row_cut(fwd_slots(D), B, Hk, G, Sq, Sk, window, sinks, causal);
+  *floats = ((int64_t)B * Hk * ((Sq * G + 127) / 128) - c.whole) * c.splits * 128 * (D + 2);
+  return PRISM_OK;
+}
+
+int prism_window_fwd(const void* q, const void* k, const void* v, int dtype, int B, int Hq, int Hk, int64_t Sq,
+                     int64_t Sk, int D, const int64_t* strides, int64_t window, int64_t sinks, int causal,
+                     const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, float* lse, float* part,
+                     hipStream_t stream) {
+  if (const int rc = win_check("prism_window_fwd", dtype, B, Hq, Hk, Sq, Sk, D, window, sinks, sm_scale, strides, 4,
+                               {q, k, v, o, part}))
+    return rc;
   if (B == 0 || Sq == 0) return PRISM_OK;
   PRISM_REQUIRE(q && o && (Sk == 0 || (k && v)), "prism_window_fwd: null pointer");
   WinArgs a = win_args(q, k, v, o, B, Hq, Hk, Sq, Sk, strides, window, sinks, causal, q_lens, kv_lens, sm_scale);
   a.lse = lse;
   a.tiles = (int)((Sq * a.G + 127) / 128);
   const int64_t total = (int64_t)B * Hk * a.tiles;
-  PRISM_REQUIRE(total < (1ll << 31), "prism_window_fwd: too many row tiles");
+  const WinCut c = win_row_cut(fwd_slots(D), B, Hk, a.G, Sq, Sk, window, sinks, causal);
+  const int64_t cut = total - c.whole, items = c.whole + cut * c.splits;
+  PRISM_REQUIRE(items < (1ll << 31), "prism_window_fwd: too many row tiles");
+  PRISM_REQUIRE(cut == 0 || part, "prism_window_fwd: null workspace");
   a.total = (int)total;
+  a.whole = (int)c.whole; a.splits = (int)c.splits; a.items = (int)items;
+  a.part = part;
+  a.part_ml = part + cut * c.splits * 128 * D;
+  auto run = [&](auto kernel, auto join) {
+    kernel<<<(unsigned)items, 256, 0, stream>>>(a);
+    if (cut) join<<<dim3((unsigned)cut, (unsigned)(D / 32)), 256, 0, stream>>>(a);
+  };
   if (dtype == PRISM_BF16) {
-    if (D == 64) window_fwd_kernel<WinBf16, 64><<<a.total, 256, 0, stream>>>(a);
-    else window_fwd_kernel<WinBf16, 128><<<a.total, 256, 0, stream>>>(a);
+    if (D == 64) run(window_fwd_kernel<WinBf16, 64>, window_fwd_join_kernel<WinBf16, 64>);
+    else run(window_fwd_kernel<WinBf16, 128>, window_fwd_join_kernel<WinBf16, 128>);
   } else {
-    if (D == 64) window_fwd_kernel<WinF16, 64><<<a.total, 256, 0, stream>>>(a);
-    else window_fwd_kernel<WinF16, 128><<<a.total, 256, 0, stream>>>(a);
+    if (D == 64) run(window_fwd_kernel<WinF16, 64>, window_fwd_join_kernel<WinF16, 64>);
+    else run(window_fwd_kernel<WinF16, 128>, window_fwd_join_kernel<WinF16, 128>);
   }
   PRISM_LAUNCH_CHECK("prism_window_fwd");
   return PRISM_OK;
 }
+
+}  // extern "C"

@@ -10,6 +10,8 @@
 // vmcnt: no barrier until the end), so the CU keeps four waves' copies in flight.
 // The four waves' sums are joined in LDS, the workgroups' in a second kernel, both
 // in a fixed order.
+#include <type_traits>
+
 #include "window.h"
 
 namespace {
@@ -224,7 +226,7 @@ __global__ __launch_bounds__(256, 1) void window_token_kernel(WinArgs a) {
       *reinterpret_cast<uint2*>(a.o.p + b * a.o.b + head * a.o.h + i * a.o.s + d) = u;
     } else {
       const int64_t at = ((int64_t)split * a.total + id) * 32 + l32;
-      *reinterpret_cast<float4*>(a.part_o + at * D + d) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+      *reinterpret_cast<float4*>(a.part + at * D + d) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
     }
   }
   if (w == 0 && g == 0) {
@@ -253,19 +255,24 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinArgs a) {
   for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, a.part_ml[2 * (row + s * step)]);
   const float top = wave_max_xor(m);
   constexpr int C = D / 64;  // channels per lane
-  float o[C] = {}, l = 0.0f;
+  typedef typename std::conditional<C == 2, float2, float>::type V;
+  float o[2] = {0.0f, 0.0f}, l = 0.0f;
+#pragma unroll 8
   for (int s = 0; s < a.splits; ++s) {
-    const float ms = a.part_ml[2 * (row + s * step)], ls = a.part_ml[2 * (row + s * step) + 1];
-    if (ms == NINF && ls == 0.0f) continue;  // saw no key
-    const float f = fast_exp2(ms - top);
-    l = __builtin_fmaf(ls, f, l);
-    const float* p = a.part_o + (row + s * step) * D + C * lane;
-#pragma unroll
-    for (int c = 0; c < C; ++c) o[c] = __builtin_fmaf(p[c], f, o[c]);
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (row + s * step));
+    const V p = *reinterpret_cast<const V*>(a.part + (row + s * step) * D + C * lane);
+    const float f = ml.x == NINF ? 0.0f : fast_exp2(ml.x - top);  // (a part that sees nothing has sums of 0)
+    l = __builtin_fmaf(ml.y, f, l);
+    if constexpr (C == 2) {
+      o[0] = __builtin_fmaf(p.x, f, o[0]);
+      o[1] = __builtin_fmaf(p.y, f, o[1]);
+    } else {
+      o[0] = __builtin_fmaf(p, f, o[0]);
+    }
   }
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
   uint16_t* op = a.o.p + b * a.o.b + head * a.o.h + i * a.o.s + C * lane;
-  const uint32_t u = E::pack(o[0] * inv, C > 1 ? o[C - 1] * inv : 0.0f);
+  const uint32_t u = E::pack(o[0] * inv, o[1] * inv);
   if constexpr (C > 1) *reinterpret_cast<uint32_t*>(op) = u;
   else *op = (uint16_t)u;
   if (a.lse && lane == 0)
@@ -311,7 +318,7 @@ int prism_window_token(const void* q, const void* k, const void* v, int dtype, i
   const int64_t items = (int64_t)B * Hk * a.tiles;
   PRISM_REQUIRE(items * splits < (1ll << 31) && items < (1ll << 28), "prism_window_token: too many row tiles");
   a.total = (int)items;
-  a.splits = splits; a.part_o = part_o; a.part_ml = part_ml;
+  a.splits = splits; a.part = part_o; a.part_ml = part_ml;
   const unsigned grid = (unsigned)(items * splits), join = (unsigned)(items * 8);
   auto run = [&](auto kernel, auto joiner) {
     kernel<<<grid, 256, 0, stream>>>(a);

@@ -86,7 +86,8 @@ PROMPTS = [  # B, Sq, Sk, Hq, Hk, D, window, sinks, causal
     (1, 300, 40, 2, 2, 64, 16, 2, True), (1, 129, 700, 3, 3, 128, 65, 130, True), (2, 70, 70, 5, 5, 64, 5, 300, True),
     (1, 257, 257, 2, 2, 128, 30, 0, False), (2, 200, 300, 4, 4, 64, 64, 5, False), (1, 100, 600, 2, 2, 64, 3, 129, False),
     (1, 400, 400, 8, 1, 128, 128, 64, False), (1, 333, 100, 1, 1, 64, 9, 1, False), (2, 66, 66, 7, 1, 64, None, 0, False),
-    (1, 1100, 1100, 1, 1, 64, 257, 4, True),
+    (1, 1100, 1100, 1, 1, 64, 257, 4, True), (1, 1280, 1280, 53, 53, 128, 300, 4, True),
+    (1, 1100, 1100, 90, 90, 64, 200, 140, False), (2, 100, 3000, 2, 2, 128, 2500, 9, True),
 ]
 
 

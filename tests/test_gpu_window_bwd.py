@@ -74,6 +74,8 @@ CASES = [  # B, Sq, Sk, Hq, Hk, D, window, sinks, causal
     (2, 200, 300, 4, 4, 64, 64, 5, False), (1, 100, 600, 2, 2, 64, 3, 129, False), (1, 400, 400, 8, 1, 128, 128, 64, False),
     (1, 333, 100, 1, 1, 64, 9, 1, False), (2, 66, 66, 7, 1, 64, None, 0, False), (1, 1500, 1500, 8, 1, 64, 40, 4, True),
     (1, 1300, 1300, 2, 1, 128, 700, 150, False), (1, 2000, 2000, 4, 2, 128, None, 0, True),
+    # more tiles than the chip holds at once, and a few over: the last round is cut
+    (1, 1280, 1280, 53, 53, 128, 300, 4, True), (1, 1100, 1100, 90, 90, 64, 200, 140, False),
 ]
 
 

@@ -140,7 +140,7 @@ def test_window_capi_refusals():
     def fwd(dtype=1, B=1, Hq=4, Hk=2, Sq=5, Sk=9, D=64, window=3, sinks=0, scale=0.1, stride=64, p=one):
         st = (ctypes.c_int64 * 12)(*[stride] * 12)
         return lib.prism_window_fwd(p, one, one, dtype, B, Hq, Hk, Sq, Sk, D, st, window, sinks, 1, None, None, scale, one,
-                                    None, None)
+                                    None, one, None)
 
     for bad in (dict(dtype=0), dict(Hk=3), dict(Hk=0), dict(D=32), dict(window=0), dict(sinks=-1), dict(scale=0.0),
                 dict(stride=65), dict(stride=1 << 24), dict(stride=-64), dict(p=None), dict(p=ctypes.c_void_p(8)),
@@ -168,5 +168,7 @@ def test_window_plans():
         assert floats.value == (0 if splits.value == 1 else splits.value * 32 * B * Hk * -(-Sq * Hq // Hk // 32))
     for B, Hq, Hk, Sq, Sk, W, sinks in ((1, 5, 5, 14040, 14040, 4680, 1560), (1, 1, 1, 200000, 200000, 64, 4), (1, 1, 1, 1, 1, 1, 0),
                                         (4, 32, 8, 16384, 16384, 1 << 29, 0)):
+        assert lib.prism_window_fwd_plan(B, Hq, Hk, Sq, Sk, 128, W, sinks, 1, ctypes.byref(floats)) == 0
+        assert 0 <= floats.value <= 2 * 512 * 128 * 130
         assert lib.prism_window_bwd_plan(B, Hq, Hk, Sq, Sk, 128, W, sinks, 1, ctypes.byref(floats)) == 0
         assert 0 <= floats.value <= 3000 * 256 * 128
