@@ -164,18 +164,6 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs ba) {
 #pragma unroll
     for (int x = 0; x + 1 < RQ; ++x) kt[x] = rdk(x);
     __builtin_amdgcn_s_setprio(1);
-    if (!whole || !ws.all(u0, u0 + 63)) {
-      const uint64_t mm = span_bits(span, u0) >> (4 * g);
-      const uint32_t bits[2] = {(uint32_t)mm, (uint32_t)(mm >> 32)};
-#pragma unroll
-      for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int bit = 8 * (x >> 2) + (x & 3);
-          sacc[kh][x] = keep_or_ninf(sacc[kh][x], bits[kh], bit);
-          pacc[kh][x] = keep_or_zero(pacc[kh][x], bits[kh], bit);  // (what is not finite there stays out)
-        }
-    }
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
@@ -183,6 +171,17 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs ba) {
         const float p = fast_exp2(__builtin_fmaf(sacc[kh][x], a.scale_log2, -mq));
         pacc[kh][x] = p * pacc[kh][x];
       }
+    if (!whole || !ws.all(u0, u0 + 63)) {
+      // dS is 0 where the query does not see the key, whatever the unmasked
+      // values were (after the exponentials, which so stay in one block with the
+      // products before them)
+      const uint64_t mm = span_bits(span, u0) >> (4 * g);
+      const uint32_t bits[2] = {(uint32_t)mm, (uint32_t)(mm >> 32)};
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) pacc[kh][x] = keep_or_zero(pacc[kh][x], bits[kh], 8 * (x >> 2) + (x & 3));
+    }
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
       const bf16x8 sb = win_b_from_acc<E>(pacc, tt);
@@ -308,17 +307,23 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
   // also the m2 row and wave 2 the delta row
   const uint32_t lds0 = lds_addr(smem);
   const int64_t qstep = 2 * a.q.s, dstep = 2 * ba.do_.s;
-  const int crow = RS::row(w & 3, lane), cbyte = RS::byte(w & 3, lane);
-  const uint32_t qoff = (uint32_t)crow * (uint32_t)qstep + (uint32_t)cbyte;
-  const uint32_t doff = (uint32_t)crow * (uint32_t)dstep + (uint32_t)cbyte;
-  auto issue = [&](int e, int st) {
+  int copy_head = n > 0 ? e0 / nti : 0, copy_tile = n > 0 ? e0 - copy_head * nti : 0;  // the next entry to copy
+  auto issue = [&](int st) {
     if (w >= 4) return;
-    const int gh = e / nti, t0 = lo + 64 * (e - gh * nti), head = it.hk * a.G + gh;
+    const int t0 = lo + 64 * copy_tile, head = it.hk * a.G + copy_head;
+    if (++copy_tile == nti) {
+      copy_tile = 0;
+      ++copy_head;
+    }
     const uint32_t base = lds0 + (uint32_t)(st * SB);
     const uint8_t* qb = (const uint8_t*)uniform_ptr(a.q.p + it.b * a.q.b + head * a.q.h + t0 * a.q.s);
     const uint8_t* db = (const uint8_t*)uniform_ptr(ba.do_.p + it.b * ba.do_.b + head * ba.do_.h + t0 * ba.do_.s);
     const int left = hi - t0;  // rows past hi re-read it
+    // (lane offsets are formed anew for every entry: the products need every register)
+    const int ln = opaque_thread_id() & 63, crow = RS::row(w & 3, ln), cbyte = RS::byte(w & 3, ln);
     if (left >= 63) {
+      const uint32_t qoff = (uint32_t)crow * (uint32_t)qstep + (uint32_t)cbyte;
+      const uint32_t doff = (uint32_t)crow * (uint32_t)dstep + (uint32_t)cbyte;
 #pragma unroll
       for (int s = 0; s < COUNT; ++s) {
         const int m = s % (RT::KB / 4);
@@ -337,7 +342,7 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
     }
     if (w >= 2) {
       const float* rowsrc = (w == 3 ? ba.m2 : ba.delta) + ((int64_t)it.b * a.Hk * a.G + head) * a.Sq + t0;
-      dma_b32(4u * (uint32_t)(lane < left ? lane : left), uniform_ptr(rowsrc), base + 2u * RT::BYTES + (w == 3 ? 0u : 256u));
+      dma_b32(4u * (uint32_t)(ln < left ? ln : left), uniform_ptr(rowsrc), base + 2u * RT::BYTES + (w == 3 ? 0u : 256u));
     }
   };
   RowOperand rop;                // Q / dO rows 32 qh + l32
@@ -346,12 +351,12 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
   top.init<RT>(32 * qh, lane);
 #pragma unroll
   for (int x = 0; x < kAhead; ++x)
-    if (x < n) issue(e0 + x, x);
+    if (x < n) issue(x);
 
-  const int jw = j0 + 64 * tk + 32 * kh, key = jw + l32;
+  const int jw = j0 + 64 * tk + 32 * kh;
   bf16x8 kf[NS], vf[NS];
   {
-    const int kc = key < a.Sk ? key : a.Sk - 1;
+    const int kc = jw + l32 < a.Sk ? jw + l32 : a.Sk - 1;
     const uint16_t* kp = a.k.p + it.b * a.k.b + it.hk * a.k.h + kc * a.k.s + 8 * g;
     const uint16_t* vp = a.v.p + it.b * a.v.b + it.hk * a.v.h + kc * a.v.s + 8 * g;
 #pragma unroll
@@ -365,7 +370,6 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
     consume_regs(kf[s]);
     consume_regs(vf[s]);
   }
-  const TokenRange mine = tokens_of(a, sq, key);
   // of the wave's 32 keys: tokens that see some, and all of them
   int any0, any1, all0, all1;
   {
@@ -413,18 +417,6 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
-    const bool masked = t0 < all0 || t0 + 31 > all1;
-    uint32_t bits = ~0u;
-    if (masked) {  // rows of this half that see the lane's key
-      const int b0 = mine.i0 - t0 > 0 ? mine.i0 - t0 : 0, b1 = mine.i1 - t0 < 31 ? mine.i1 - t0 : 31;
-      bits = b1 >= b0 ? (~0u << b0) & (~0u >> (31 - b1)) : 0u;
-      bits >>= 4 * g;
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        const int bit = 8 * (x >> 2) + (x & 3);
-        sacc[x] = keep_or_ninf(sacc[x], bits, bit);
-      }
-    }
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
       const float4 m4 = *reinterpret_cast<const float4*>(sM + 32 * qh + 8 * jj + 4 * g);
@@ -438,7 +430,15 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
         pacc[rg] = p * (pacc[rg] - dl4[x]);
       }
     }
-    if (masked) {  // what is not finite in a row that does not see the key stays out
+    if (t0 < all0 || t0 + 31 > all1) {
+      // rows that do not see the lane's key: P and dS are 0 there, whatever the
+      // unmasked values were (the branch stands after the exponentials, which so
+      // stay in one block with the products before them)
+      const int ln = opaque_thread_id() & 63;
+      const TokenRange mine = tokens_of(a, sq, jw + (ln & 31));
+      const int b0 = mine.i0 - t0 > 0 ? mine.i0 - t0 : 0, b1 = mine.i1 - t0 < 31 ? mine.i1 - t0 : 31;
+      uint32_t bits = b1 >= b0 ? (~0u << b0) & (~0u >> (31 - b1)) : 0u;
+      bits >>= 4 * (ln >> 5);
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
         const int bit = 8 * (x >> 2) + (x & 3);
@@ -487,7 +487,7 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
       if (w >= 2) stage_wait<kAhead + 1, COUNT + 1>(n - 1 - x);
       else stage_wait<kAhead + 1, COUNT>(n - 1 - x);
       __syncthreads();
-      if (x + kAhead < n) issue(e0 + x + kAhead, (st + kAhead) % kStages);
+      if (x + kAhead < n) issue((st + kAhead) % kStages);
       const uint8_t* sQ = smem + st * SB;
       st = st + 1 == kStages ? 0 : st + 1;
       const int t0 = half_of();
@@ -535,6 +535,7 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
   }
   __syncthreads();
   if (qh == 1) return;
+  const int key = jw + (opaque_thread_id() & 31);
   uint16_t* dkr = ba.dk.p + it.b * ba.dk.b + it.hk * ba.dk.h + key * ba.dk.s;
   uint16_t* dvr = ba.dv.p + it.b * ba.dv.b + it.hk * ba.dv.h + key * ba.dv.s;
 #pragma unroll

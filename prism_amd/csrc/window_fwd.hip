@@ -205,6 +205,7 @@ __global__ __launch_bounds__(256) void window_fwd_join_kernel(WinArgs a) {
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first * 32 + l32;
   const float4* pa = reinterpret_cast<const float4*>(a.part) + (first * NDT + dt) * 256 + lane;
   float top = NINF;
+#pragma unroll 8
   for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[(int64_t)s * 128].x);
   float4 o[4];
 #pragma unroll
