@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs ba) {
   __shared__ __align__(1024) uint8_t smem[2 * T::STAGE];
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
   const int w = (int)uniform_u32(threadIdx.x >> 6);
-  const WinItem it = win_item(a, xcd_group_remap<32>((int)blockIdx.x, a.items));
+  const WinItem it = win_item(a, xcd_group_remap<8>((int)blockIdx.x, a.items));
   const int b = it.b, hk = it.hk, tile = it.tile;
   const SeqSpan sq = seq_span(a, b);
   const int rows = a.Sq * a.G, r0 = tile * 128, wr0 = r0 + 32 * w;
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
   const int w = (int)uniform_u32(threadIdx.x >> 6);
   const int kh = w & 1, qh = (w >> 1) & 1, tk = w >> 2;
-  const DkdvItem it = dkdv_item(ba, xcd_group_remap<32>((int)blockIdx.x, ba.items));
+  const DkdvItem it = dkdv_item(ba, xcd_group_remap<8>((int)blockIdx.x, ba.items));
   const SeqSpan sq = seq_span(a, it.b);
   const int j0 = it.tile * 128;
 
