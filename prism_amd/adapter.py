@@ -20,6 +20,7 @@ import torch
 from . import ops
 from .dynamic_block_attention import flash_attn_bsa_3d_dynamic
 from .dynamic_block_shape import ZONE_SIZE
+from .rotary import apply_rotary, grid_positions
 from .uniform_block_attention import bsa_chunked
 
 # default bsa_params keys and values read by the reference (wan_video_dit.py:415-421)
@@ -80,9 +81,15 @@ class DynamicBlockSparseAttention:
     (wan_video_dit.py:22-33, :401-427).  One key beyond the reference's:
     bsa_params["compact_lists"] (default True) keeps the work lists of a long
     launch in compact CSR form until the backward (O(nnz) memory; identical
-    results; False: dense buffers, as a short launch's always are)."""
+    results; False: dense buffers, as a short launch's always are).
 
-    def __init__(self, method: str = "ivpq", bsa_params: Optional[dict] = None):
+    rotary_freqs (with rotary_sections, the channels of a head per grid axis):
+    q and k arrive without positions and are turned here by their tokens' (t,
+    h, w) before the attention, as the layer does before it calls the reference
+    (wan_video_dit.py:699-705); see rotary_frequencies and apply_rotary."""
+
+    def __init__(self, method: str = "ivpq", bsa_params: Optional[dict] = None,
+                 rotary_freqs: Optional[torch.Tensor] = None, rotary_sections=None):
         if method not in ("ivpq", "penalty"):
             raise ValueError(f"unknown dynamic-block method: {method!r}")
         self.method = method
@@ -92,6 +99,16 @@ class DynamicBlockSparseAttention:
         self.training = False
         self.pass_id = 0
         self._dyn_shape_cache = None
+        if rotary_freqs is not None and (rotary_sections is None or len(rotary_sections) != 3):
+            raise ValueError("rotary_freqs needs rotary_sections, the channels per axis (t, h, w)")
+        self.rotary_freqs, self.rotary_sections = rotary_freqs, rotary_sections
+        self._positions = None  # ((grid, device), [S, 3]) of the last grid
+
+    def _rotate(self, q, k, grid):
+        key = (tuple(int(n) for n in grid), q.device)
+        if self._positions is None or self._positions[0] != key:
+            self._positions = (key, grid_positions(grid, q.device))
+        return apply_rotary(q, k, self.rotary_freqs, self._positions[1], sections=self.rotary_sections)
 
     def advance_pass(self) -> int:
         """Call once per real outer forward (advance_dynamic_block_pass_id)."""
@@ -106,6 +123,8 @@ class DynamicBlockSparseAttention:
         B, n_heads, S, D = q_bhsd.shape
         if S != T * H * W:
             raise ValueError(f"sequence length {S} != T*H*W of grid {tuple(grid_size)}")
+        if self.rotary_freqs is not None:
+            q_bhsd, k_bhsd = self._rotate(q_bhsd, k_bhsd, grid_size)
         (Tp, Hp, Wp), _ = padded_grid(grid_size)
         grid_padded = (Tp, Hp, Wp)
         cached = None
