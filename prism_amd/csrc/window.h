@@ -184,7 +184,10 @@ struct WinTiles {
   static constexpr int STAGE = 2 * RT::BYTES, STAGE_KB = 2 * RT::KB;
 };
 
-// the tile copies of a 64-entry stage (K then V) by two waves (wid 0, 1)
+// The tile copies of a 64-entry stage (K then V) by two waves (wid 0, 1).  At D =
+// 64 the lane offsets are formed anew for every tile, since registers decide how
+// many workgroups share a CU there; at D = 128 they are kept (dQ 423 -> 411 us,
+// forward 348 -> 336 us of a 480p step).
 template <int D>
 struct StageCopy {
   using RT = RowTile<D>;
@@ -192,34 +195,43 @@ struct StageCopy {
   static constexpr int COUNT = RT::KB;  // instructions per wave and stage
   const uint8_t *kb, *vb;               // K and V of the (sequence, key head)
   int64_t kstep, vstep;                 // bytes per row
-  uint32_t koff[2], voff[2];            // lane offsets of instructions wid, wid + 2
-  int wid, lane;
-  __device__ __forceinline__ void init(const WinArgs& a, int b, int hk, int wid_, int lane_) {
+  int wid;
+  uint32_t koff[2], voff[2];            // lane offsets of instructions wid, wid + 2 (D = 128)
+  __device__ __forceinline__ void offsets(int lane, uint32_t* ko, uint32_t* vo) const {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = RS::row(wid + 2 * x, lane), c = RS::byte(wid + 2 * x, lane);
+      ko[x] = (uint32_t)r * (uint32_t)kstep + (uint32_t)c;
+      vo[x] = (uint32_t)r * (uint32_t)vstep + (uint32_t)c;
+    }
+  }
+  __device__ __forceinline__ void init(const WinArgs& a, int b, int hk, int wid_, int lane) {
     wid = wid_;
-    lane = lane_;
     kb = (const uint8_t*)uniform_ptr(a.k.p + b * a.k.b + hk * a.k.h);
     vb = (const uint8_t*)uniform_ptr(a.v.p + b * a.v.b + hk * a.v.h);
     kstep = 2 * a.k.s;
     vstep = 2 * a.v.s;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int r = RS::row(wid + 2 * x, lane), c = RS::byte(wid + 2 * x, lane);
-      koff[x] = (uint32_t)r * (uint32_t)kstep + (uint32_t)c;
-      voff[x] = (uint32_t)r * (uint32_t)vstep + (uint32_t)c;
-    }
+    if constexpr (D == 128) offsets(lane, koff, voff);
   }
   __device__ __forceinline__ void issue(const KeyList& k, int u0, uint32_t lds) const {
+    const int lane = opaque_thread_id() & 63;
     if ((u0 >= k.nsink || u0 + 63 < k.nsink) && u0 + 63 < k.n) {  // 64 adjacent keys
       const int key0 = k.key(u0);
       const uint8_t* kt = (const uint8_t*)uniform_ptr(kb + key0 * kstep);
       const uint8_t* vt = (const uint8_t*)uniform_ptr(vb + key0 * vstep);
+      uint32_t ko[2], vo[2];
+      if constexpr (D == 128) {
+        ko[0] = koff[0]; ko[1] = koff[1]; vo[0] = voff[0]; vo[1] = voff[1];
+      } else {
+        offsets(lane, ko, vo);
+      }
 #pragma unroll
       for (int s = 0; s < COUNT; ++s) {
         const int i = wid + 2 * s;
         const bool isk = 2 * s < RT::KB;
         const int m = ((2 * s) % RT::KB) >> 2;  // (instruction wid + 2 (s & 1) + 4 m of its tile)
         const uint8_t* base = isk ? kt + m * RS::ROWS4 * kstep : vt + m * RS::ROWS4 * vstep;
-        dma_b128(isk ? koff[s & 1] : voff[s & 1], base, lds + (uint32_t)i * 1024u);
+        dma_b128(isk ? ko[s & 1] : vo[s & 1], base, lds + (uint32_t)i * 1024u);
       }
       return;
     }
@@ -266,17 +278,25 @@ WinArgs win_args(const void* q, const void* k, const void* v, void* o, int B, in
 
 // How a launch of `total` tiles (of about `units` list entries each) is cut so
 // that it ends evenly on `slots` workgroups at a time: whole rounds as they are,
-// and the tiles of the last round in the number of parts that takes least time,
-// a part costing its entries and 3 more, the second kernel 5.
+// and the tiles of the last round in the number of parts that takes least time
+// by this model, in entries of a full round: a part takes its entries and 3 more;
+// a round that fills a share x of the slots 0.5 + 0.5 x of a full one (fewer
+// workgroups on a CU each run faster); the second kernel 2, and 0.015 (D = 64:
+// 0.005) for each part's sums, written and read.  Measured, both kernels: 550
+// tiles of 133 entries over 512 slots at D = 128, uncut / 38 of them in 13 parts:
+// forward 428 / 357 us; 1,024 tiles of 17 entries over 768 slots at D = 64, uncut
+// / 256 of them in 3 parts: dQ 59 / 66 us.
 struct WinCut {
   int64_t whole, splits;
 };
-inline WinCut win_cut(int64_t total, int64_t slots, int64_t units) {
+inline WinCut win_cut(int64_t total, int64_t slots, int64_t units, int D) {
   WinCut c{total / slots * slots, 1};
   const int64_t rest = total - c.whole;
   double best = 0;
   for (int64_t s = 1; s <= 32 && (s == 1 || units >= 4 * s); ++s) {
-    const double cost = (double)((rest * s + slots - 1) / slots) * ((double)units / (double)s + 3) + (s > 1 ? 5 : 0);
+    const double full = (double)(rest * s / slots), x = (double)(rest * s % slots) / (double)slots;
+    const double rounds = full + (x > 0 ? 0.5 + 0.5 * x : 0);
+    const double cost = rounds * ((double)units / (double)s + 3) + (s > 1 ? 2 + (D == 64 ? 0.005 : 0.015) * (double)(rest * s) : 0);
     if (s == 1 || cost < best) {
       best = cost;
       c.splits = s;
@@ -286,5 +306,5 @@ inline WinCut win_cut(int64_t total, int64_t slots, int64_t units) {
   return c;
 }
 // the cut of a launch over row tiles of 128 (forward, dQ)
-WinCut win_row_cut(int64_t slots, int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int64_t window, int64_t sinks,
+WinCut win_row_cut(int64_t slots, int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks,
                    int causal);

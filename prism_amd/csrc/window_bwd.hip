@@ -7,11 +7,11 @@
 // keep one query per lane column, dQ^T += K^T dS^T.  It also forms delta from
 // the rows of o and do that it holds, and leaves (m2, delta) = (lse log2 e, delta) of
 // every row for the second kernel.
-// window_dkdv_kernel, by 128 keys, over the tokens that see them, one query head
-// of the group after the other: eight waves, the two halves of each 64-row query
-// tile on different waves (partial sums added through LDS in a fixed order), the
-// two waves of a SIMD half an entry apart, as the block-sparse dK/dV
-// (attn_bwd.hip).  The sinks' key tiles are seen by every later token: long
+// window_dkdv_kernel, by 128 keys (64 at D = 64), over the tokens that see them,
+// one query head of the group after the other: the two halves of each 64-row
+// query tile on different waves (partial sums added through LDS in a fixed
+// order); of the eight waves at D = 128 the two of a SIMD run half an entry apart,
+// as the block-sparse dK/dV (attn_bwd.hip).  The sinks' key tiles are seen by every later token: long
 // lists, and all lists of a launch of few key tiles, are cut over several
 // workgroups, whose fp32 sums window_merge_kernel adds in order.  No atomics: the
 // same bits every time; sums over the heads that share a key head are fp32.
@@ -52,7 +52,7 @@ __device__ __forceinline__ float keep_or_zero(float x, uint32_t bits, int b) {
 }
 
 template <class E, int D>
-__global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs ba) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_dq_kernel(WinBwdArgs ba) {
   const WinArgs& a = ba.w;
   using T = WinTiles<D>;
   using RT = typename T::RT;
@@ -121,9 +121,12 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs ba) {
   WaveSpan ws;
   ws.init(a, kl, wi0 + sq.off, wi1 + sq.off);
 
-  f32x16 ndl;  // the dP^T chains start from -delta
+  // the dP^T chains start from -delta (at D = 64 from 0, and delta is subtracted
+  // after them: 168 registers let three workgroups share a CU)
+  constexpr bool FROM = D != 64;
+  f32x16 ndl;
 #pragma unroll
-  for (int x = 0; x < 16; ++x) ndl[x] = -dlt;
+  for (int x = 0; x < 16; ++x) ndl[x] = FROM ? -dlt : 0.0f;
   f32x16 dq[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) dq[dt] = f32x16_zero();
@@ -169,7 +172,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs ba) {
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
         const float p = fast_exp2(__builtin_fmaf(sacc[kh][x], a.scale_log2, -mq));
-        pacc[kh][x] = p * pacc[kh][x];
+        pacc[kh][x] = FROM ? p * pacc[kh][x] : p * (pacc[kh][x] - dlt);
       }
     if (!whole || !ws.all(u0, u0 + 63)) {
       // dS is 0 where the query does not see the key, whatever the unmasked
@@ -262,38 +265,43 @@ __device__ __forceinline__ DkdvItem dkdv_item(const WinBwdArgs& a, int id) {
   return d;
 }
 
-constexpr int kDqSlots = 512;  // workgroups of window_dq_kernel that the chip holds: two a CU
-constexpr int kStages = 4, kAhead = 2;  // entry j + 2 is copied while j is multiplied (waves behind still read j - 1)
+// Keys of a workgroup.  D = 128: two tiles of 64, eight waves, all of a CU's
+// registers.  D = 64: one tile, four waves, and three workgroups share a CU, whose
+// phases drift apart by themselves.
+constexpr int key_tiles_of(int D) { return D == 64 ? 1 : 2; }
+constexpr int kAhead = 2;  // entry j + 2 is copied while j is multiplied
 
 template <int D>
 struct DkdvTiles {
   using RT = RowTile<D>;
+  static constexpr int KT = key_tiles_of(D), KEYS = 64 * KT, THREADS = 256 * KT;
+  static constexpr int STAGES = kAhead + KT;         // (the second tile's waves still read entry j - 1)
   static constexpr int STAGE = 2 * RT::BYTES + 512;  // Q, dO, m2 and delta
   static constexpr int NDT = D / 32;
-  static constexpr int RED = 4 * 64 * 2 * NDT * 16 * 4;
-  static constexpr int LDS = kStages * STAGE > RED ? kStages * STAGE : RED;
+  static constexpr int RED = 2 * KT * 64 * 2 * NDT * 16 * 4;
+  static constexpr int LDS = STAGES * STAGE > RED ? STAGES * STAGE : RED;
 };
 
 template <class E, int D>
-__global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
+__global__ __launch_bounds__(DkdvTiles<D>::THREADS, D == 64 ? 3 : 1) void window_dkdv_kernel(WinBwdArgs ba) {
   const WinArgs& a = ba.w;
   using T = DkdvTiles<D>;
   using RT = RowTile<D>;
   using RS = RowSource<D>;
-  constexpr int NS = D / 16, NDT = D / 32, SB = T::STAGE, COUNT = 2 * RT::KB / 4;
+  constexpr int NS = D / 16, NDT = D / 32, SB = T::STAGE, COUNT = 2 * RT::KB / 4, KEYS = T::KEYS, STAGES = T::STAGES;
   __shared__ __align__(1024) uint8_t smem[T::LDS];
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
   const int w = (int)uniform_u32(threadIdx.x >> 6);
   const int kh = w & 1, qh = (w >> 1) & 1, tk = w >> 2;
   const DkdvItem it = dkdv_item(ba, xcd_group_remap<8>((int)blockIdx.x, ba.items));
   const SeqSpan sq = seq_span(a, it.b);
-  const int j0 = it.tile * 128;
+  const int j0 = it.tile * KEYS;
 
   // tokens that see some key of the tile (the first and the last key's, and the
   // sinks' when it has some), as 64-token tiles of each head from lo on
   int lo, hi;
   {
-    const int jl = j0 + 127 < sq.L - 1 ? j0 + 127 : sq.L - 1;
+    const int jl = j0 + KEYS - 1 < sq.L - 1 ? j0 + KEYS - 1 : sq.L - 1;
     const TokenRange f = tokens_of(a, sq, j0), l = tokens_of(a, sq, jl < j0 ? j0 : jl);
     lo = f.i0 < l.i0 ? f.i0 : l.i0;
     hi = f.i1 > l.i1 ? f.i1 : l.i1;
@@ -481,15 +489,15 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
   auto half_of = [&] { return lo + 64 * tile_i + 32 * qh; };
   auto next_tile = [&] { tile_i = tile_i + 1 == nti ? 0 : tile_i + 1; };
   auto sees = [&](int t0) { return t0 + 31 >= any0 && t0 <= any1; };
-  if (tk == 0) {
+  if (T::KT == 1 || tk == 0) {
     int st = 0;
     for (int x = 0; x < n; ++x) {
       if (w >= 2) stage_wait<kAhead + 1, COUNT + 1>(n - 1 - x);
       else stage_wait<kAhead + 1, COUNT>(n - 1 - x);
       __syncthreads();
-      if (x + kAhead < n) issue((st + kAhead) % kStages);
+      if (x + kAhead < n) issue((st + kAhead) % STAGES);
       const uint8_t* sQ = smem + st * SB;
-      st = st + 1 == kStages ? 0 : st + 1;
+      st = st + 1 == STAGES ? 0 : st + 1;
       const int t0 = half_of();
       next_tile();
       if (!sees(t0)) continue;
@@ -507,7 +515,7 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
     for (int x = 0; x < n; ++x) {
       __syncthreads();
       const uint8_t* sQ = smem + st * SB;
-      st = st + 1 == kStages ? 0 : st + 1;
+      st = st + 1 == STAGES ? 0 : st + 1;
       const int t0 = half_of();
       next_tile();
       if (pend) dvdk(sPrev, pb, sb);
@@ -546,7 +554,7 @@ __global__ __launch_bounds__(512, 1) void window_dkdv_kernel(WinBwdArgs ba) {
       dv[dt][x] += red[((slot * 2 * NDT + NDT + dt) * 16 + x) * 64 + lane];
     }
     if (it.slot >= 0) {
-      float4* pa = ba.acc + ((int64_t)it.slot * 4 + slot) * 2 * NDT * 256 + lane;
+      float4* pa = ba.acc + ((int64_t)it.slot * 2 * T::KT + slot) * 2 * NDT * 256 + lane;
 #pragma unroll
       for (int jj = 0; jj < 4; ++jj) {
         pa[(dt * 4 + jj) * 64] = make_float4(dk[dt][4 * jj], dk[dt][4 * jj + 1], dk[dt][4 * jj + 2], dk[dt][4 * jj + 3]);
@@ -608,8 +616,8 @@ __global__ __launch_bounds__(256) void window_dq_merge_kernel(WinBwdArgs ba) {
 // in order: one workgroup per tile and 32-column block of dK (blocks 0 .. NDT - 1)
 // or dV; wave = 32 keys
 template <class E, int D>
-__global__ __launch_bounds__(256) void window_merge_kernel(WinBwdArgs a, int cut_sinks) {
-  constexpr int NDT = D / 32, NB = 2 * NDT;
+__global__ __launch_bounds__(128 * key_tiles_of(D)) void window_merge_kernel(WinBwdArgs a, int cut_sinks) {
+  constexpr int NDT = D / 32, NB = 2 * NDT, KW = 2 * key_tiles_of(D);
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, w = threadIdx.x >> 6, blk = (int)blockIdx.y;
   const int x = (int)blockIdx.x, z = x - cut_sinks;
   const bool sink = z < 0;
@@ -617,9 +625,9 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinBwdArgs a, int cut
   const int64_t first = sink ? (int64_t)x * S : (int64_t)cut_sinks * a.sink_splits + (int64_t)z * S;
   const int bh = sink ? x / a.sink_tiles : (a.rest_whole + z) / nrest;
   const int tile = sink ? x - bh * a.sink_tiles : a.sink_tiles + a.rest_whole + z - bh * nrest;
-  const int b = bh / a.w.Hk, hk = bh - b * a.w.Hk, key = tile * 128 + 32 * w + l32;
+  const int b = bh / a.w.Hk, hk = bh - b * a.w.Hk, key = tile * 32 * KW + 32 * w + l32;
   if (key >= a.w.Sk) return;
-  const float4* pa = a.acc + ((first * 4 + w) * NB + blk) * 256 + lane;
+  const float4* pa = a.acc + ((first * KW + w) * NB + blk) * 256 + lane;
   float4 acc[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) acc[j] = pa[j * 64];
@@ -627,7 +635,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinBwdArgs a, int cut
   for (int s = 1; s < S; ++s)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float4 v = pa[(int64_t)s * 4 * NB * 256 + j * 64];
+      const float4 v = pa[(int64_t)s * KW * NB * 256 + j * 64];
       acc[j].x += v.x;
       acc[j].y += v.y;
       acc[j].z += v.z;
@@ -646,17 +654,22 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinBwdArgs a, int cut
   }
 }
 
-// How the dK/dV lists are cut, for one workgroup a CU: the sinks' lists into
+// workgroups of window_dq_kernel that the chip holds: two a CU at D = 128, three
+// at 64 (registers)
+int64_t dq_slots(int D) { return D == 128 ? 512 : 768; }
+
+// How the dK/dV lists are cut, for one workgroup a CU (three at D = 64): the sinks' lists into
 // pieces no longer than the others, then the last round of tiles (win_cut).
 struct DkdvPlan {
   int64_t sink_tiles, key_tiles, sink_splits, sink_items, rest_whole, rest_splits, rest_tiles, items, pieces;
 };
-DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int64_t window, int64_t sinks, int causal) {
+DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal) {
   DkdvPlan p{};
+  const int64_t keys = 64 * key_tiles_of(D);
   const int64_t BH = (int64_t)B * Hk, whole = G * ((Sq + 63) / 64);
-  const int64_t span = window < Sq ? (causal ? window : 2 * window) + 127 : Sq;
-  p.key_tiles = (Sk + 127) / 128;
-  p.sink_tiles = ((sinks < Sk ? sinks : Sk) + 127) / 128;
+  const int64_t span = window < Sq ? (causal ? window : 2 * window) + keys - 1 : Sq;
+  p.key_tiles = (Sk + keys - 1) / keys;
+  p.sink_tiles = ((sinks < Sk ? sinks : Sk) + keys - 1) / keys;
   int64_t rest = span < Sq ? G * ((span + 63) / 64) : whole;
   if (rest >= whole || p.sink_tiles == p.key_tiles) {  // all lists alike
     p.sink_tiles = 0;
@@ -666,8 +679,8 @@ DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int64_t win
   p.rest_tiles = BH * (p.key_tiles - p.sink_tiles);
   p.sink_splits = p.sink_tiles ? (whole + n - 1) / n : 1;
   int64_t head = BH * p.sink_tiles * p.sink_splits;  // pieces before the rest's tiles
-  const int64_t slots = 256, total = head + p.rest_tiles;
-  const WinCut c = win_cut(total, slots, rest);
+  const int64_t slots = D == 64 ? 768 : 256, total = head + p.rest_tiles;
+  const WinCut c = win_cut(total, slots, rest, D);
   p.rest_splits = c.splits;
   p.rest_whole = c.whole > head ? c.whole - head : 0;
   if (p.rest_whole > p.rest_tiles) p.rest_whole = p.rest_tiles;
@@ -684,7 +697,7 @@ DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int64_t win
 }
 // float4-aligned workspace: dK/dV pieces, then dQ parts
 int64_t bwd_floats(const DkdvPlan& p, const WinCut& c, int64_t row_tiles, int64_t D) {
-  return p.pieces * 256 * D + (row_tiles - c.whole) * c.splits * 128 * D;
+  return p.pieces * 128 * key_tiles_of((int)D) * D + (row_tiles - c.whole) * c.splits * 128 * D;
 }
 
 }  // namespace
@@ -697,8 +710,8 @@ int prism_window_bwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, 
                     sinks >= 0 && floats,
                 "prism_window_bwd_plan: bad argument");
   const int64_t G = Hq / Hk;
-  *floats = bwd_floats(dkdv_plan(B, Hk, G, Sq, Sk, window, sinks, causal),
-                       win_row_cut(kDqSlots, B, Hk, G, Sq, Sk, window, sinks, causal), (int64_t)B * Hk * ((Sq * G + 127) / 128), D);
+  *floats = bwd_floats(dkdv_plan(B, Hk, G, Sq, Sk, D, window, sinks, causal),
+                       win_row_cut(dq_slots(D), B, Hk, G, Sq, Sk, D, window, sinks, causal), (int64_t)B * Hk * ((Sq * G + 127) / 128), D);
   return PRISM_OK;
 }
 
@@ -724,14 +737,14 @@ int prism_window_bwd(const void* do_, const void* q, const void* k, const void* 
   a.delta = rows + (int64_t)B * Hq * Sq;
   a.w.tiles = (int)((Sq * a.w.G + 127) / 128);
   const int64_t total = (int64_t)B * Hk * a.w.tiles;
-  const WinCut c = win_row_cut(kDqSlots, B, Hk, a.w.G, Sq, Sk, window, sinks, causal);
-  const DkdvPlan p = dkdv_plan(B, Hk, a.w.G, Sq, Sk, window, sinks, causal);
+  const WinCut c = win_row_cut(dq_slots(D), B, Hk, a.w.G, Sq, Sk, D, window, sinks, causal);
+  const DkdvPlan p = dkdv_plan(B, Hk, a.w.G, Sq, Sk, D, window, sinks, causal);
   const int64_t cut = total - c.whole, items = c.whole + cut * c.splits;
   PRISM_REQUIRE(items < (1ll << 31) && p.items < (1ll << 31), "prism_window_bwd: too many tiles");
   PRISM_REQUIRE(p.pieces + cut == 0 || acc, "prism_window_bwd: null workspace");
   a.w.total = (int)total;
   a.w.whole = (int)c.whole; a.w.splits = (int)c.splits; a.w.items = (int)items;
-  a.w.part = acc + p.pieces * 256 * D;
+  a.w.part = acc + p.pieces * 128 * key_tiles_of(D) * D;
   a.sink_tiles = (int)p.sink_tiles; a.key_tiles = (int)p.key_tiles;
   a.sink_splits = (int)p.sink_splits; a.sink_items = (int)p.sink_items;
   a.rest_whole = (int)p.rest_whole; a.rest_splits = (int)p.rest_splits; a.items = (int)p.items;
@@ -743,8 +756,8 @@ int prism_window_bwd(const void* do_, const void* q, const void* k, const void* 
     constexpr int DD = decltype(d)::value;
     if (items) window_dq_kernel<E, DD><<<(unsigned)items, 256, 0, stream>>>(a);
     if (cut) window_dq_merge_kernel<E, DD><<<dim3((unsigned)cut, DD / 32), 256, 0, stream>>>(a);
-    if (p.items) window_dkdv_kernel<E, DD><<<(unsigned)p.items, 512, 0, stream>>>(a);
-    if (cut_keys) window_merge_kernel<E, DD><<<dim3((unsigned)cut_keys, DD / 16), 256, 0, stream>>>(a, cut_sinks);
+    if (p.items) window_dkdv_kernel<E, DD><<<(unsigned)p.items, DkdvTiles<DD>::THREADS, 0, stream>>>(a);
+    if (cut_keys) window_merge_kernel<E, DD><<<dim3((unsigned)cut_keys, DD / 16), 128 * key_tiles_of(DD), 0, stream>>>(a, cut_sinks);
   };
   if (dtype == PRISM_BF16) {
     if (D == 64) run(WinBf16{}, std::integral_constant<int, 64>{});

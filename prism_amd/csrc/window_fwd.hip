@@ -20,7 +20,7 @@
 namespace {
 
 template <class E, int D>
-__global__ __launch_bounds__(256, 2) void window_fwd_kernel(WinArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void window_fwd_kernel(WinArgs a) {
   using T = WinTiles<D>;
   using RT = typename T::RT;
   constexpr int NS = D / 16, NDT = D / 32;
@@ -102,10 +102,12 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WinArgs a) {
       }
       __builtin_amdgcn_sched_group_barrier(0x008, RING - 1, 0);
     }
-    // V^T operands of the P V product, in flight while the softmax runs
-    bf16x8 vfr[4][NDT];
+    // V^T operands of the P V product, in flight while the softmax runs (at D = 64
+    // those of two steps at a time: 128 registers let four workgroups share a CU)
+    constexpr int VR = D == 64 ? 2 : 4;
+    bf16x8 vfr[VR][NDT];
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
+    for (int tt = 0; tt < VR; ++tt)
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) vfr[tt][dt] = vop.load<RT>(sV, tt, dt);
     if (!whole || !ws.all(u0, u0 + 63)) {
@@ -149,15 +151,20 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WinArgs a) {
       }
       const bf16x8 pb = win_b_from_acc<E>(sacc, tt);
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) acc_o[dt] = E::mfma(vfr[tt][dt], pb, acc_o[dt]);
+      for (int dt = 0; dt < NDT; ++dt) {
+        acc_o[dt] = E::mfma(vfr[tt % VR][dt], pb, acc_o[dt]);
+        if (tt + VR < 4) vfr[tt % VR][dt] = vop.load<RT>(sV, tt + VR, dt);
+      }
     }
-    __builtin_amdgcn_sched_group_barrier(0x002, 28, 0);
+    if constexpr (VR == 4) {
+      __builtin_amdgcn_sched_group_barrier(0x002, 28, 0);
 #pragma unroll
-    for (int x = 0; x < 3 * NDT; ++x) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 28 / NDT, 0);
+      for (int x = 0; x < 3 * NDT; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 28 / NDT, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, NDT, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, NDT, 0);
     ls = xor32_add(ls);
     l = __builtin_fmaf(l, alpha, ls);
     m = m_new;
@@ -242,12 +249,12 @@ __global__ __launch_bounds__(256) void window_fwd_join_kernel(WinArgs a) {
 
 }  // namespace
 
-WinCut win_row_cut(int64_t slots, int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int64_t window, int64_t sinks,
+WinCut win_row_cut(int64_t slots, int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks,
                    int causal) {
   const int64_t tokens = 128 / G + 1 < Sq ? 128 / G + 1 : Sq;
   const int64_t side = window < Sk ? (causal ? window : 2 * window) : Sk;
   const int64_t seen = side + tokens + sinks < Sk ? side + tokens + sinks : Sk;
-  return win_cut((int64_t)B * Hk * ((Sq * G + 127) / 128), slots, (seen + 63) / 64);
+  return win_cut((int64_t)B * Hk * ((Sq * G + 127) / 128), slots, (seen + 63) / 64, D);
 }
 
 int win_check(const char* name, int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window,
@@ -289,9 +296,9 @@ WinArgs win_args(const void* q, const void* k, const void* v, void* o, int B, in
   return a;
 }
 
-// workgroups of window_fwd_kernel that the chip holds: two a CU at D = 128, three
+// workgroups of window_fwd_kernel that the chip holds: two a CU at D = 128, four
 // at 64 (registers)
-static int64_t fwd_slots(int D) { return D == 128 ? 512 : 768; }
+static int64_t fwd_slots(int D) { return D == 128 ? 512 : 1024; }
 
 extern "C" {
 
@@ -301,7 +308,7 @@ int prism_window_fwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, 
                     sinks >= 0 && floats,
                 "prism_window_fwd_plan: bad argument");
   const int64_t G = Hq / Hk;
-  const WinCut c = win_row_cut(fwd_slots(D), B, Hk, G, Sq, Sk, window, sinks, causal);
+  const WinCut c = win_row_cut(fwd_slots(D), B, Hk, G, Sq, Sk, D, window, sinks, causal);
   *floats = ((int64_t)B * Hk * ((Sq * G + 127) / 128) - c.whole) * c.splits * 128 * (D + 2);
   return PRISM_OK;
 }
@@ -319,7 +326,7 @@ int prism_window_fwd(const void* q, const void* k, const void* v, int dtype, int
   a.lse = lse;
   a.tiles = (int)((Sq * a.G + 127) / 128);
   const int64_t total = (int64_t)B * Hk * a.tiles;
-  const WinCut c = win_row_cut(fwd_slots(D), B, Hk, a.G, Sq, Sk, window, sinks, causal);
+  const WinCut c = win_row_cut(fwd_slots(D), B, Hk, a.G, Sq, Sk, D, window, sinks, causal);
   const int64_t cut = total - c.whole, items = c.whole + cut * c.splits;
   PRISM_REQUIRE(items < (1ll << 31), "prism_window_fwd: too many row tiles");
   PRISM_REQUIRE(cut == 0 || part, "prism_window_fwd: null workspace");
