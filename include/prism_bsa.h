@@ -172,7 +172,7 @@ int prism_window_fwd(const void* q, const void* k, const void* v, int dtype, int
  * cache): the keys are cut over `splits` workgroups per 32 rows, whose partial
  * results part_o (floats * D floats) and part_ml (2 * floats) a second kernel
  * joins in order; prism_window_token_plan gives splits and floats (0 for one
- * split: no workspace). */
+ * split: no workspace), and splits = 0 where prism_window_fwd is the faster. */
 int prism_window_token_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int64_t window, int64_t sinks, int causal,
                             int* splits, int64_t* floats);
 int prism_window_token(const void* q, const void* k, const void* v, int dtype, int B, int Hq, int Hk, int64_t Sq,

@@ -179,10 +179,6 @@ Tensor win_like(const Tensor& t) {
   return o.numel() == 0 || o.stride(3) == 1 ? o : at::empty(t.sizes(), t.options());
 }
 
-// query rows (tokens x heads of a group) up to which a call goes to the kernel
-// for single tokens
-constexpr int64_t kTokenRows = 64;
-
 struct WinShape {
   int dt;
   int64_t B, Hq, Hk, Sq, Sk, D;
@@ -226,10 +222,10 @@ std::tuple<Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_, const 
   win_strides(o, st + 9);
   float* lp = want_lse ? lse.data_ptr<float>() : nullptr;
   const int B = small(s.B, "B"), Hq = small(s.Hq, "heads"), Hk = small(s.Hk, "heads"), D = small(s.D, "D");
-  if (s.Hk > 0 && s.Sq * (s.Hq / s.Hk) <= kTokenRows) {
-    int splits = 1;
-    int64_t floats = 0;
-    check_rc(prism_window_token_plan(B, Hq, Hk, s.Sq, s.Sk, window, sinks, causal, &splits, &floats));
+  int splits = 0;
+  int64_t floats = 0;
+  check_rc(prism_window_token_plan(B, Hq, Hk, s.Sq, s.Sk, window, sinks, causal, &splits, &floats));
+  if (splits) {
     Tensor part = splits > 1 ? at::empty({floats * (s.D + 2)}, opts(q, at::kFloat)) : none_like(q);
     float* po = splits > 1 ? part.data_ptr<float>() : nullptr;
     PRISM_TORCH_CALL(prism_window_token, q.data_ptr(), k.data_ptr(), v.data_ptr(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st,
@@ -237,7 +233,6 @@ std::tuple<Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_, const 
                      o.data_ptr(), lp, splits, po, po ? po + floats * s.D : nullptr, stream_of(q));
     return {o, lse};
   }
-  int64_t floats = 0;
   check_rc(prism_window_fwd_plan(B, Hq, Hk, s.Sq, s.Sk, D, window, sinks, causal, &floats));
   Tensor part = floats ? at::empty({floats}, opts(q, at::kFloat)) : none_like(q);
   PRISM_TORCH_CALL(prism_window_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st,

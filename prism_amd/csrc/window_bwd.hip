@@ -315,42 +315,52 @@ __global__ __launch_bounds__(DkdvTiles<D>::THREADS, D == 64 ? 3 : 1) void window
   // also the m2 row and wave 2 the delta row
   const uint32_t lds0 = lds_addr(smem);
   const int64_t qstep = 2 * a.q.s, dstep = 2 * ba.do_.s;
-  int copy_head = n > 0 ? e0 / nti : 0, copy_tile = n > 0 ? e0 - copy_head * nti : 0;  // the next entry to copy
+  // the next entry to copy: its head, token tile, and where its rows begin (one
+  // tile on at every entry: the scalar unit stands between the barrier and the
+  // first products)
+  int copy_head = n > 0 ? e0 / nti : 0, copy_tile = n > 0 ? e0 - copy_head * nti : 0;
+  const uint8_t *qcur, *dcur;
+  const float* rcur;
+  auto seek = [&] {
+    const int t0 = lo + 64 * copy_tile, head = it.hk * a.G + copy_head;
+    qcur = (const uint8_t*)uniform_ptr(a.q.p + it.b * a.q.b + head * a.q.h + t0 * a.q.s);
+    dcur = (const uint8_t*)uniform_ptr(ba.do_.p + it.b * ba.do_.b + head * ba.do_.h + t0 * ba.do_.s);
+    rcur = (const float*)uniform_ptr((w == 3 ? ba.m2 : ba.delta) + ((int64_t)it.b * a.Hk * a.G + head) * a.Sq + t0);
+  };
+  if (n > 0) seek();
   auto issue = [&](int st) {
     if (w >= 4) return;
-    const int t0 = lo + 64 * copy_tile, head = it.hk * a.G + copy_head;
-    if (++copy_tile == nti) {
-      copy_tile = 0;
-      ++copy_head;
-    }
-    const uint32_t base = lds0 + (uint32_t)(st * SB);
-    const uint8_t* qb = (const uint8_t*)uniform_ptr(a.q.p + it.b * a.q.b + head * a.q.h + t0 * a.q.s);
-    const uint8_t* db = (const uint8_t*)uniform_ptr(ba.do_.p + it.b * ba.do_.b + head * ba.do_.h + t0 * ba.do_.s);
-    const int left = hi - t0;  // rows past hi re-read it
+    const int left = hi - (lo + 64 * copy_tile);  // rows past hi re-read it
+    const uint32_t base = lds0 + (uint32_t)(st * SB) + 1024u * (uint32_t)w;
     // (lane offsets are formed anew for every entry: the products need every register)
     const int ln = opaque_thread_id() & 63, crow = RS::row(w & 3, ln), cbyte = RS::byte(w & 3, ln);
     if (left >= 63) {
       const uint32_t qoff = (uint32_t)crow * (uint32_t)qstep + (uint32_t)cbyte;
       const uint32_t doff = (uint32_t)crow * (uint32_t)dstep + (uint32_t)cbyte;
+      const uint8_t *qb = qcur, *db = dcur;
 #pragma unroll
-      for (int s = 0; s < COUNT; ++s) {
-        const int m = s % (RT::KB / 4);
-        const bool isq = s < RT::KB / 4;
-        dma_b128(isq ? qoff : doff, isq ? qb + m * RS::ROWS4 * qstep : db + m * RS::ROWS4 * dstep,
-                 base + (uint32_t)(w + 4 * s) * 1024u);
-      }
+      for (int m = 0; m < RT::KB / 4; ++m, qb += RS::ROWS4 * qstep) dma_b128(qoff, qb, base + 4096u * (uint32_t)m);
+#pragma unroll
+      for (int m = 0; m < RT::KB / 4; ++m, db += RS::ROWS4 * dstep)
+        dma_b128(doff, db, base + RT::BYTES + 4096u * (uint32_t)m);
     } else {
 #pragma unroll
       for (int s = 0; s < COUNT; ++s) {
         const int m = s % (RT::KB / 4), row = crow + m * RS::ROWS4, rr = row < left ? row : left;
         const bool isq = s < RT::KB / 4;
         const uint32_t off = (uint32_t)rr * (uint32_t)(isq ? qstep : dstep) + (uint32_t)cbyte;
-        dma_b128(off, isq ? qb : db, base + (uint32_t)(w + 4 * s) * 1024u);
+        dma_b128(off, isq ? qcur : dcur, base + 4096u * (uint32_t)s);
       }
     }
-    if (w >= 2) {
-      const float* rowsrc = (w == 3 ? ba.m2 : ba.delta) + ((int64_t)it.b * a.Hk * a.G + head) * a.Sq + t0;
-      dma_b32(4u * (uint32_t)(ln < left ? ln : left), uniform_ptr(rowsrc), base + 2u * RT::BYTES + (w == 3 ? 0u : 256u));
+    if (w >= 2)
+      dma_b32(4u * (uint32_t)(ln < left ? ln : left), rcur, lds0 + (uint32_t)(st * SB) + 2u * RT::BYTES + (w == 3 ? 0u : 256u));
+    if (++copy_tile == nti) {
+      copy_tile = 0;
+      if (++copy_head < a.G) seek();
+    } else {
+      qcur += 64 * qstep;
+      dcur += 64 * dstep;
+      rcur += 64;
     }
   };
   RowOperand rop;                // Q / dO rows 32 qh + l32

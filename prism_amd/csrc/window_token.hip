@@ -284,8 +284,24 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinArgs a) {
 
 extern "C" {
 
-// Workgroups per row tile: as many as give the chip one workgroup a CU, each
-// with two tiles of 32 keys or more per wave of the longest list that can occur
+// Whether a call goes to these kernels, and over how many workgroups (splits) the
+// keys of a row tile are cut.
+//
+// These kernels read the keys once per 32 rows, window_fwd_kernel once per 128:
+// it wins where many row tiles see many keys.  Measured at D = 128, these /
+// window_fwd_kernel (us), by row tiles of the launch and keys seen: 8 x 4,100: 13.6
+// / 24; 64 x 4,100: 20.6 / 25; 128 x 4,100: 28 / 28 (sharing one sequence) and 48 /
+// 35; 256 x 4,100: 82 / 39; 16 x 8,000: 16 / 37; 128 x 500: 15 / 19; 256 x 500: 17 /
+// 19; 512 x 500: 30 / 20; 256 x 300: 11 / 14; 512 x 300: 19 / 14.
+//
+// Splits: a second kernel costs 2 us, and each part 0.05 of its work, so up to 512
+// keys one workgroup, beyond that about sqrt(keys) / 2.5, and no more than give
+// each CU one workgroup.  Measured, D = 128, 1 row tile of 300 keys: 8.3 us in one
+// part, 10.2 in two; of 1,000: 13.3 in one, 9.6 in 8, 11.6 in 32; of 4,000: 37 in
+// one, 11.5 in 16, 12.4 in 64; of 32,000: 41 in 8, 16.3 in 64, 25 in 256.  Caches
+// read for the first time: 64 tiles of 4,100 keys 32.4 us in 3 parts, 33.4 in 4, 39
+// in 6; 16 tiles of 131,000 185 in 12, 189 in 16, 217 in 20 (rows 2 KB apart: 202 in
+// 12, 191 in 16); 128 tiles of 4,100 58.8 in one, 56.1 in two.
 int prism_window_token_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int64_t window, int64_t sinks, int causal,
                             int* splits, int64_t* floats) {
   PRISM_REQUIRE(B >= 0 && Hk >= 1 && Hq >= Hk && Hq % Hk == 0 && Sq >= 0 && Sk >= 0 && window >= 1 && sinks >= 0 &&
@@ -295,11 +311,15 @@ int prism_window_token_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int64
   const int64_t tokens = (32 + G - 1) / G < Sq ? (32 + G - 1) / G : Sq;
   const int64_t side = window < Sk ? (causal ? window : 2 * window) : Sk;
   const int64_t seen = side + tokens + sinks < Sk ? side + tokens + sinks : Sk;
-  const int64_t by_keys = (seen + 255) / 256, by_chip = items ? (256 + items - 1) / items : 1;
-  int64_t n = by_keys < by_chip ? by_keys : by_chip;
+  *floats = 0;
+  *splits = 0;
+  if (tiles > 1 && items > 64 && (items > 256 || seen > 1024)) return PRISM_OK;  // window_fwd_kernel's
+  const int64_t by_chip = items ? 256 / items : 1;
+  int64_t n = seen <= 512 ? 1 : (int64_t)(__builtin_sqrt((double)seen) / 2.5);
+  n = n < by_chip ? n : by_chip;
   n = n < 1 ? 1 : n < kMaxSplits ? n : kMaxSplits;
   *splits = (int)n;
-  *floats = n == 1 ? 0 : n * items * 32;
+  if (n > 1) *floats = n * items * 32;
   return PRISM_OK;
 }
 

@@ -164,8 +164,11 @@ def test_window_plans():
                                         (1, 64, 1, 1, 100000, 100000, 0), (0, 4, 4, 1, 5, 5, 0), (64, 32, 8, 2, 9, 5, 2)):
         assert lib.prism_window_token_plan(B, Hq, Hk, Sq, Sk, W, sinks, 1, ctypes.byref(splits), ctypes.byref(floats)) == 0
         assert 1 <= splits.value <= 256
-        assert splits.value == 1 or splits.value * 256 <= Sk + 512
+        assert splits.value == 1 or splits.value * 16 <= Sk
         assert floats.value == (0 if splits.value == 1 else splits.value * 32 * B * Hk * -(-Sq * Hq // Hk // 32))
+    # many rows over many keys are the other kernel's
+    assert lib.prism_window_token_plan(8, 32, 8, 16, 32768, 4096, 4, 1, ctypes.byref(splits), ctypes.byref(floats)) == 0
+    assert splits.value == 0 and floats.value == 0
     for B, Hq, Hk, Sq, Sk, W, sinks in ((1, 5, 5, 14040, 14040, 4680, 1560), (1, 1, 1, 200000, 200000, 64, 4), (1, 1, 1, 1, 1, 1, 0),
                                         (4, 32, 8, 16384, 16384, 1 << 29, 0)):
         assert lib.prism_window_fwd_plan(B, Hq, Hk, Sq, Sk, 128, W, sinks, 1, ctypes.byref(floats)) == 0
