@@ -266,6 +266,66 @@ __device__ __forceinline__ WinItem win_item(const WinArgs& a, int id) {
   return id < a.whole ? win_tile(a, id, 0, -1) : win_tile(a, a.whole + q, y - q * a.splits, a.splits == 1 ? -1 : y);
 }
 
+// ------------------------------------------------------------ values that are not finite
+// A product over a tile multiplies the values that a row does not see by 0, and 0
+// times a NaN or an infinity is a NaN.  The kernels therefore look at their sums
+// once, at the end: where one of a wave's 32 rows is not finite, the wave computes
+// its rows again key by key, adding only what each row sees.  (Rows that do see
+// such a value keep it; the others get what they would have without it.)  Slow,
+// about 4 ms for 4,000 keys, and free otherwise.
+template <int NDT>
+__device__ __forceinline__ bool win_not_finite(const f32x16* acc, float l, bool live) {
+  float t = 0.0f * l;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) t = __builtin_fmaf(acc[dt][x], 0.0f, t);
+  return __builtin_amdgcn_ballot_w64(live && t != t) != 0;
+}
+// acc, m, l of the lane's row (channels 32 dt + 8 j + 4 g + x in acc[dt][4 j + x]) over entries u0 .. u1 - 1
+template <class E, int D>
+__device__ __forceinline__ void win_careful(const WinArgs& a, const KeyList& kl, const TokenSpan& span, int u0, int u1,
+                                            const uint16_t* q, const uint8_t* kb, const uint8_t* vb, int64_t kstep,
+                                            int64_t vstep, int g, f32x16* acc, float& m, float& l) {
+  constexpr int NDT = D / 32;
+  const float NINF = -__builtin_inff();
+  m = NINF;
+  l = 0.0f;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) acc[dt] = f32x16_zero();
+#pragma unroll 1
+  for (int u = u0; u < u1; ++u) {
+    const int key = kl.key(u);
+    const uint16_t* k = (const uint16_t*)(kb + key * kstep) + 4 * g;
+    const uint16_t* v = (const uint16_t*)(vb + key * vstep) + 4 * g;
+    float s = 0.0f;
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      const uint2 x = *reinterpret_cast<const uint2*>(q + 4 * g + 8 * c), y = *reinterpret_cast<const uint2*>(k + 8 * c);
+      s = __builtin_fmaf(E::lo(x.x), E::lo(y.x), s);
+      s = __builtin_fmaf(E::hi(x.x), E::hi(y.x), s);
+      s = __builtin_fmaf(E::lo(x.y), E::lo(y.y), s);
+      s = __builtin_fmaf(E::hi(x.y), E::hi(y.y), s);
+    }
+    s = xor32_add(s) * a.scale_log2;
+    const bool sees = (u >= span.a && u <= span.b) || u < span.c;
+    const float top = sees ? fmaxf(m, s) : m;
+    const float alpha = m == top ? 1.0f : fast_exp2(m - top), p = fast_exp2(s - (top == NINF ? 0.0f : top));
+    m = top;
+    if (sees) l = __builtin_fmaf(l, alpha, p);
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint2 y = *reinterpret_cast<const uint2*>(v + 32 * dt + 8 * j);
+        const float w[4] = {E::lo(y.x), E::hi(y.x), E::lo(y.y), E::hi(y.y)};
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          acc[dt][4 * j + x] = sees ? __builtin_fmaf(p, w[x], acc[dt][4 * j + x] * alpha) : acc[dt][4 * j + x];
+      }
+  }
+}
+
 // ------------------------------------------------------------ host side (window_fwd.hip)
 // PRISM_OK if the sizes, strides (3 per tensor) and pointers are what the kernels assume
 int win_check(const char* name, int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window,

@@ -171,6 +171,11 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void window_fwd_kernel(WinArg
     __builtin_amdgcn_s_setprio(0);
   }
 
+  if (some && win_not_finite<NDT>(acc_o, l, live)) {
+    win_careful<E, D>(a, kl, span, 64 * t0, 64 * t1 < kl.n ? 64 * t1 : kl.n, qp, copy.kb, copy.vb, copy.kstep, copy.vstep, g,
+                      acc_o, m, l);
+    if (m == NINF && l == 0.0f) l = 1.0f;  // saw nothing
+  }
   if (it.slot >= 0) {  // a part: unnormalised sums in register order, reference and sum
     float4* pa = reinterpret_cast<float4*>(a.part) + ((int64_t)it.slot * 4 + w) * NDT * 256 + lane;
 #pragma unroll
@@ -232,7 +237,7 @@ __global__ __launch_bounds__(256) void window_fwd_join_kernel(WinArgs a) {
       o[j].w = __builtin_fmaf(v.w, f, o[j].w);
     }
   }
-  const bool none = top == NINF;
+  const bool none = top == NINF && l == 0.0f;
   const float inv = none ? 0.0f : 1.0f / l;
   const int i = r / a.G, head = it.hk * a.G + (r - i * a.G);
   uint16_t* op = a.o.p + it.b * a.o.b + head * a.o.h + i * a.o.s + 32 * dt + 4 * g;

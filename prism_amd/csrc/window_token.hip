@@ -182,6 +182,32 @@ __global__ __launch_bounds__(256, 1) void window_token_kernel(WinArgs a) {
     m = m_new;
   }
 
+  if (win_not_finite<NDT>(acc_o, l, i <= last)) {
+    // (the wave's tiles one after the other; a tile's partial sums join as the
+    // waves' do)
+    float mw = NINF, lw = 0.0f;
+    f32x16 ow[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) ow[dt] = f32x16_zero();
+#pragma unroll 1
+    for (int t = t0 + w; t < t1; t += 4) {
+      win_careful<E, D>(a, kl, span, 32 * t, 32 * t + 32 < kl.n ? 32 * t + 32 : kl.n, qp, kb, vb, kstep, vstep, g, acc_o, m, l);
+      const float top = fmaxf(mw, m);
+      const float f0 = mw == top ? 1.0f : fast_exp2(mw - top), f1 = m == NINF ? 0.0f : fast_exp2(m - top);
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          ow[dt][x] = m == NINF && l == 0.0f ? ow[dt][x] : __builtin_fmaf(acc_o[dt][x], f1, ow[dt][x] * f0);
+      lw = m == NINF && l == 0.0f ? lw : __builtin_fmaf(l, f1, lw * f0);
+      mw = top;
+    }
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) acc_o[dt] = ow[dt];
+    m = mw;
+    l = lw;
+  }
+
   // join the four waves: every wave's sums on the largest reference, then wave w
   // adds a quarter of the channels (registers 4 NDT w ...) in wave order
   __shared__ float ml[4][2][32];

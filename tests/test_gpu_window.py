@@ -133,6 +133,47 @@ def test_lengths(Sq):
                 check(q2, k2, v2, window, sinks=sinks, causal=causal, q_lens=ql, kv_lens=kv)
 
 
+@pytest.mark.parametrize("case", [
+    (1, 300, 300, 4, 2, 64, 40, 3, True), (1, 333, 400, 2, 2, 128, 65, 0, False), (2, 100, 3000, 2, 2, 128, 2500, 9, True),
+    (2, 1, 900, 8, 2, 64, 100, 4, True), (1, 6, 5000, 3, 1, 128, 2000, 0, True), (1, 7, 300, 8, 2, 128, 33, 2, False),
+], ids=lambda c: "-".join(str(x) for x in c))
+@pytest.mark.parametrize("dt", list(DT))
+def test_not_finite_values_stay_with_the_rows_that_see_them(case, dt):
+    """NaN and infinities in K, V and Q reach the rows that see them, and no other."""
+    B, Sq, Sk, Hq, Hk, D, window, sinks, causal = case
+    q, k, v = make(B, Sq, Sk, Hq, Hk, D, DT[dt], seed=Sk)
+    seen = seen_mask(B, Sq, Sk, window, sinks, causal, None, None)[0]
+    first = int(seen[0].nonzero()[-1])   # the first query's last key, the last query's first past the sinks
+    last = int(seen[-1].nonzero()[sinks if causal and Sk > window else 0])
+    for at, into, value in ((first, v, math.nan), (last, v, math.inf), (first, k, math.nan), (last, v, -math.inf)):
+        x = into.clone()
+        x[0, 0, at, 5] = value
+        k2, v2 = (x, v) if into is k else (k, x)
+        # what the other rows give without that key
+        heads = torch.arange(Hq, device="cuda") // (Hq // Hk) == 0
+        hit = torch.zeros((B, Hq, Sq), dtype=torch.bool, device="cuda")
+        hit[0] = heads[:, None] & seen[:, at][None]
+        want = prism_amd.flash_attn_window(q, k, v, window, sinks=sinks, causal=causal).float()
+        o, lse = prism_amd.flash_attn_window(q, k2, v2, window, sinks=sinks, causal=causal, return_lse=True)
+        assert o[~hit].isfinite().all() and lse[~hit].isfinite().all()
+        # both roundings of P and o, each at most a step of the largest |v|
+        tol = 4 * torch.finfo(q.dtype).eps * v.abs().max().float()
+        assert ((o.float() - want).abs()[~hit] <= tol).all()
+        got = o[hit]
+        if into is k:
+            assert got.isnan().all() and lse[hit].isnan().all()
+        else:
+            others = [c for c in range(D) if c != 5]
+            assert not got[:, 5].isfinite().any()
+            assert ((o.float() - want).abs()[hit][:, others] <= tol).all() and lse.isfinite().all()
+    x = q.clone()
+    x[0, 0, Sq // 2, 7] = math.nan
+    o = prism_amd.flash_attn_window(x, k, v, window, sinks=sinks, causal=causal)
+    assert o[0, 0, Sq // 2].isnan().all()
+    o[0, 0, Sq // 2] = 0
+    assert o.isfinite().all()
+
+
 def test_scale_and_large_scores():
     q, k, v = make(1, 150, 150, 2, 2, 64, torch.bfloat16, seed=1)
     for refused in (0.0, -0.3, math.nan):  # (a masked score times the scale has to stay -inf)
