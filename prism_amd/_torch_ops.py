@@ -91,6 +91,11 @@ def _register_fakes():
 
     f8, i8 = torch.float8_e4m3fn, torch.int8
 
+    def like(t, far=None):  # t's layout where that is dense with adjacent channels (and near rows), else contiguous
+        o = torch.empty_like(t)
+        near = far is None or o.shape[2] <= 1 or o.stride(2) < far
+        return o if o.numel() == 0 or (o.stride(3) == 1 and near) else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
     @reg("prism::rms_norm")
     def _(x, residual, weight, eps, out_code, want_inv):
         return (_empty(x, x.shape, {3: f8, 4: i8}.get(out_code, x.dtype)),
@@ -104,15 +109,15 @@ def _register_fakes():
 
     @reg("prism::rotary")
     def _(q, k, freqs, positions, axis_pairs, interleaved, amplitude, inverse):
-        return torch.empty_like(q), torch.empty_like(k) if k is not None else _none(q)
+        return like(q), like(k) if k is not None else _none(q)
 
     @reg("prism::window_fwd")
     def _(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse):
-        return torch.empty_like(q), _empty(q, q.shape[:3], f32) if want_lse else _none(q)
+        return like(q, 1 << 24), _empty(q, q.shape[:3], f32) if want_lse else _none(q)
 
     @reg("prism::window_bwd")
     def _(do, q, k, v, o, lse, window, sinks, causal, q_lens, kv_lens, sm_scale):
-        return torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        return like(q, 1 << 24), like(k, 1 << 24), like(v, 1 << 24)
 
     @reg("prism::zone_layout")
     def _(shape_ids):

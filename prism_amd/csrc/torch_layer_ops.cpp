@@ -106,7 +106,11 @@ std::tuple<Tensor, Tensor> rms_norm_bwd(const Tensor& dy_, const OptT& dh_, cons
 }
 
 // ------------------------------------------------------------------ rotary positions
-Tensor like_layout(const Tensor& x) { return at::empty_like(x); }  // x's dense strides, else contiguous
+// x's strides where they are dense with adjacent channels, else contiguous
+Tensor like_layout(const Tensor& x) {
+  Tensor o = at::empty_like(x);
+  return o.numel() == 0 || o.stride(3) == 1 ? o : at::empty(x.sizes(), x.options());
+}
 
 std::tuple<Tensor, Tensor> rotary(const Tensor& q_, const OptT& k_, const Tensor& freqs_, const Tensor& pos_,
                                   c10::IntArrayRef axis_pairs, bool interleaved, double amplitude, bool inverse) {
@@ -137,9 +141,7 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& q_, const OptT& k_, const Tensor
   const c10::DeviceGuard guard(q_.device());
   const Tensor q = unit_rows(q_), freqs = freqs_.contiguous();
   const OptT k = k_ ? OptT(unit_rows(*k_)) : OptT();
-  Tensor oq = like_layout(q), ok = k ? like_layout(*k) : none_like(q);
-  if (oq.numel() && oq.stride(3) != 1) oq = at::empty(q.sizes(), q.options());
-  if (k && ok.numel() && ok.stride(3) != 1) ok = at::empty(k->sizes(), k->options());
+  Tensor oq = like_layout(q_), ok = k_ ? like_layout(*k_) : none_like(q);
   int64_t strides[12] = {q.stride(0), q.stride(1), q.stride(2), oq.stride(0), oq.stride(1), oq.stride(2)};
   if (k) {
     const int64_t s[6] = {k->stride(0), k->stride(1), k->stride(2), ok.stride(0), ok.stride(1), ok.stride(2)};
@@ -174,9 +176,11 @@ Tensor win_rows(const Tensor& t) {
 void win_strides(const Tensor& t, int64_t* s) {
   for (int d = 0; d < 3; ++d) s[d] = t.size(d) > 1 ? t.stride(d) : 0;
 }
+// t's layout where that is dense, has adjacent channels and rows as near as the kernels take them
 Tensor win_like(const Tensor& t) {
-  Tensor o = at::empty_like(t);  // t's layout where that is dense
-  return o.numel() == 0 || o.stride(3) == 1 ? o : at::empty(t.sizes(), t.options());
+  Tensor o = at::empty_like(t);
+  const bool ok = o.numel() == 0 || (o.stride(3) == 1 && (o.size(2) <= 1 || o.stride(2) < (1 << 24)));
+  return ok ? o : at::empty(t.sizes(), t.options());
 }
 
 struct WinShape {
@@ -213,7 +217,7 @@ std::tuple<Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_, const 
   const c10::DeviceGuard guard(q_.device());
   const Tensor q = win_rows(q_), k = win_rows(k_), v = win_rows(v_);
   const OptT q_lens = cont(q_lens_), kv_lens = cont(kv_lens_);
-  Tensor o = win_like(q);
+  Tensor o = win_like(q_);
   Tensor lse = want_lse ? at::empty({s.B, s.Hq, s.Sq}, opts(q, at::kFloat)) : none_like(q);
   int64_t st[12];
   win_strides(q, st);
@@ -258,7 +262,7 @@ std::tuple<Tensor, Tensor, Tensor> window_bwd(const Tensor& do_, const Tensor& q
   const Tensor q = win_rows(q_), k = win_rows(k_), v = win_rows(v_), o = win_rows(o_), d = win_rows(do_);
   const Tensor lse = lse_.contiguous();
   const OptT q_lens = cont(q_lens_), kv_lens = cont(kv_lens_);
-  Tensor dq = win_like(q), dk = win_like(k), dv = win_like(v);
+  Tensor dq = win_like(q_), dk = win_like(k_), dv = win_like(v_);
   int64_t st[24], floats = 0;
   const Tensor* all[8] = {&q, &k, &v, &o, &d, &dq, &dk, &dv};
   for (int i = 0; i < 8; ++i) win_strides(*all[i], st + 3 * i);
@@ -278,11 +282,40 @@ using torch::autograd::AutogradContext;
 using torch::autograd::Variable;
 using torch::autograd::variable_list;
 
+// The nodes reach the kernels through the dispatcher, so that fake tensors (a
+// traced or compiled program) get the operators' fake implementations.
+template <class F>
+auto prism_op(const char* name, F*) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+#define PRISM_OP(f) ([]() -> const auto& { static const auto op = prism_op("prism::" #f, &f); return op; }())
+
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const OptT& t) { return t && t->defined() && t->requires_grad(); }
+// A leaf's gradient is added on the stream on which a graph first took the leaf,
+// as long as that graph lives.  If that was the default stream, a backward pass
+// captured into a graph would call on a stream that may not take part in a
+// capture, which ends the process: refused here, before anything is captured.
+void check_captured(const OptT& t) {
+  if (!wants_grad(t) || !t->is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+  if (!node) return;
+  const auto s = node->stream();
+  TORCH_CHECK(!s || s->id() != 0,
+              "prism: an input that requires gradients is still held by a graph of eager calls on the default stream; "
+              "free that graph (its outputs and losses), or pass a new leaf, before capturing");
+}
 template <class... T>
-bool grads_wanted(const T&... t) {
-  return at::GradMode::is_enabled() && (wants_grad(t) || ...);
+bool grads_wanted(const Tensor& first, const T&... t) {
+  if (!at::GradMode::is_enabled() || !(wants_grad(first) || ... || wants_grad(t))) return false;
+  if (!first.is_cuda() || first.unsafeGetTensorImpl()->is_python_dispatch()) return true;  // (fake tensors: nothing is launched)
+  const hipStream_t stream = stream_of(first);
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (stream && hipStreamIsCapturing(stream, &status) == hipSuccess && status != hipStreamCaptureStatusNone) {
+    check_captured(first);
+    (check_captured(t), ...);
+  }
+  return true;
 }
 OptT opt(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
 // gradients that cannot be differentiated again: using them so raises
@@ -300,7 +333,7 @@ struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
                                int64_t out_code) {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->set_materialize_grads(false);
-    auto [y, h, scale, inv] = rms_norm(x, r, w, eps, out_code, true);
+    auto [y, h, scale, inv] = PRISM_OP(rms_norm).call(x, r, w, eps, out_code, true);
     ctx->save_for_backward({r ? h : x, w ? *w : Tensor(), inv});
     ctx->saved_data["residual"] = r.has_value();
     ctx->saved_data["dw"] = w && w->requires_grad();
@@ -315,7 +348,7 @@ struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
     const auto [dx, dw] = [&] {
       at::AutoDispatchBelowADInplaceOrView guard;
       const Tensor dy = g[0].defined() ? g[0] : at::zeros_like(dh);  // (only h went on)
-      return rms_norm_bwd(dy, opt(dh), saved[0], opt(saved[1]), saved[2], ctx->saved_data["dw"].toBool());
+      return PRISM_OP(rms_norm_bwd).call(dy, opt(dh), saved[0], opt(saved[1]), saved[2], ctx->saved_data["dw"].toBool());
     }();
     return once({dx, residual ? dx : Tensor(), ctx->saved_data["dw"].toBool() ? dw : Tensor(), Tensor(), Tensor()});
   }
@@ -324,7 +357,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rms_norm_autograd(const Tensor& x, co
                                                              int64_t out_code, bool want_inv) {
   if (!grads_wanted(x, r, w)) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    return rms_norm(x, r, w, eps, out_code, want_inv);
+    return PRISM_OP(rms_norm).call(x, r, w, eps, out_code, want_inv);
   }
   TORCH_CHECK_VALUE(out_code != PRISM_E4M3 && out_code != PRISM_I8, "rms_norm: 8-bit outputs have no gradient");
   const variable_list o = RmsNormGrad::apply(x, r, w, eps, out_code);
@@ -337,7 +370,7 @@ struct RotaryGrad : torch::autograd::Function<RotaryGrad> {
                                bool inverse) {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->set_materialize_grads(false);
-    auto [oq, ok] = rotary(q, k, freqs, pos, axis_pairs, interleaved, amplitude, inverse);
+    auto [oq, ok] = PRISM_OP(rotary).call(q, k, freqs, pos, axis_pairs, interleaved, amplitude, inverse);
     ctx->save_for_backward({freqs, pos});
     ctx->saved_data["axis_pairs"] = axis_pairs;
     ctx->saved_data["interleaved"] = interleaved;
@@ -353,7 +386,7 @@ struct RotaryGrad : torch::autograd::Function<RotaryGrad> {
     const bool both = g[0].defined() && g[1].defined();
     const auto [a, b] = [&] {
       at::AutoDispatchBelowADInplaceOrView guard;
-      return rotary(g[0].defined() ? g[0] : g[1], both ? OptT(g[1]) : OptT(), saved[0], saved[1],
+      return PRISM_OP(rotary).call(g[0].defined() ? g[0] : g[1], both ? OptT(g[1]) : OptT(), saved[0], saved[1],
                     ctx->saved_data["axis_pairs"].toIntVector(), ctx->saved_data["interleaved"].toBool(),
                     ctx->saved_data["amplitude"].toDouble(), !ctx->saved_data["inverse"].toBool());
     }();
@@ -367,7 +400,7 @@ std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const OptT& k, const
                                            bool inverse) {
   if (!grads_wanted(q, k)) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    return rotary(q, k, freqs, pos, axis_pairs, interleaved, amplitude, inverse);
+    return PRISM_OP(rotary).call(q, k, freqs, pos, axis_pairs, interleaved, amplitude, inverse);
   }
   const variable_list o = RotaryGrad::apply(q, k, freqs, pos, axis_pairs.vec(), interleaved, amplitude, inverse);
   return {o[0], o[1]};
@@ -378,7 +411,7 @@ struct WindowGrad : torch::autograd::Function<WindowGrad> {
                                int64_t sinks, bool causal, const OptT& q_lens, const OptT& kv_lens, double sm_scale) {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->set_materialize_grads(false);
-    auto [o, lse] = window_fwd(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, true);
+    auto [o, lse] = PRISM_OP(window_fwd).call(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, true);
     ctx->save_for_backward({q, k, v, o, lse, q_lens ? *q_lens : Tensor(), kv_lens ? *kv_lens : Tensor()});
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
@@ -392,7 +425,7 @@ struct WindowGrad : torch::autograd::Function<WindowGrad> {
     const variable_list s = ctx->get_saved_variables();
     const auto [dq, dk, dv] = [&] {
       at::AutoDispatchBelowADInplaceOrView guard;
-      return window_bwd(g[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["window"].toInt(),
+      return PRISM_OP(window_bwd).call(g[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["window"].toInt(),
                         ctx->saved_data["sinks"].toInt(), ctx->saved_data["causal"].toBool(), opt(s[5]), opt(s[6]),
                         ctx->saved_data["sm_scale"].toDouble());
     }();
@@ -406,7 +439,7 @@ std::tuple<Tensor, Tensor> window_autograd(const Tensor& q, const Tensor& k, con
                                            double sm_scale, bool want_lse) {
   if (!grads_wanted(q, k, v)) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    return window_fwd(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse);
+    return PRISM_OP(window_fwd).call(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse);
   }
   const variable_list o = WindowGrad::apply(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale);
   return {o[0], o[1]};

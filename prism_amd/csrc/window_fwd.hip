@@ -258,7 +258,7 @@ WinCut win_row_cut(int64_t slots, int B, int Hk, int64_t G, int64_t Sq, int64_t 
                    int causal) {
   const int64_t tokens = 128 / G + 1 < Sq ? 128 / G + 1 : Sq;
   const int64_t side = window < Sk ? (causal ? window : 2 * window) : Sk;
-  const int64_t seen = side + tokens + sinks < Sk ? side + tokens + sinks : Sk;
+  const int64_t some = side + tokens + (sinks < Sk ? sinks : Sk), seen = some < Sk ? some : Sk;
   return win_cut((int64_t)B * Hk * ((Sq * G + 127) / 128), slots, (seen + 63) / 64, D);
 }
 

@@ -336,7 +336,7 @@ int prism_window_token_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int64
   const int64_t G = Hq / Hk, tiles = (Sq * G + 31) / 32, items = (int64_t)B * Hk * tiles;
   const int64_t tokens = (32 + G - 1) / G < Sq ? (32 + G - 1) / G : Sq;
   const int64_t side = window < Sk ? (causal ? window : 2 * window) : Sk;
-  const int64_t seen = side + tokens + sinks < Sk ? side + tokens + sinks : Sk;
+  const int64_t some = side + tokens + (sinks < Sk ? sinks : Sk), seen = some < Sk ? some : Sk;
   *floats = 0;
   *splits = 0;
   if (tiles > 1 && items > 64 && (items > 256 || seen > 1024)) return PRISM_OK;  // window_fwd_kernel's

@@ -80,7 +80,8 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor
     [S] or [B, S]; with sections (channels per axis, summing to 2 * pairs, at
     most 4 axes) one entry per axis in a last dimension.  interleaved: pairs of
     channels (2p, 2p + 1), else (p, p + pairs).  amplitude scales the turned
-    channels.  Returns q', with k (q', k').  Differentiable in q and k."""
+    channels.  Returns q', with k (q', k').  Differentiable in q and k (freqs that
+    require gradients are refused)."""
     for t, name in ((q, "q"), (k, "k")):
         if t is not None and t.dim() != 4:
             raise ValueError(f"apply_rotary: {name} must be [B, H, S, D], got {tuple(t.shape)}")
@@ -88,6 +89,8 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor
         raise ValueError(f"apply_rotary: k {tuple(k.shape)} must have q's batch, length and head dim {tuple(q.shape)}")
     if freqs.dtype != torch.float64:
         raise TypeError(f"apply_rotary: freqs must be float64 (far positions lose their place in less), got {freqs.dtype}")
+    if freqs.requires_grad and torch.is_grad_enabled():
+        raise ValueError("apply_rotary has no gradient for freqs: pass them detached")
     if freqs.dim() != 1 or freqs.shape[0] < 1 or 2 * freqs.shape[0] > q.shape[-1]:
         raise ValueError(f"apply_rotary: {tuple(freqs.shape)} frequencies do not fit heads of {q.shape[-1]} channels")
     axis_pairs = []

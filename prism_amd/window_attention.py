@@ -64,6 +64,7 @@ def flash_attn_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window:
         if t is not None and (t.dtype != torch.int32 or t.shape != (B,)):
             raise ValueError(f"{name} must be int32 [{B}], got {t.dtype} {tuple(t.shape)}")
     window = _NO_LIMIT if window is None else min(int(window), _NO_LIMIT)
+    sinks = min(int(sinks), _NO_LIMIT)
     sm_scale = D ** -0.5 if sm_scale is None else float(sm_scale)
     if not 0 < sm_scale < float("inf"):
         raise ValueError(f"sm_scale must be positive and finite, got {sm_scale}")

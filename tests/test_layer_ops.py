@@ -175,3 +175,51 @@ def test_window_plans():
         assert 0 <= floats.value <= 2 * 512 * 128 * 130
         assert lib.prism_window_bwd_plan(B, Hq, Hk, Sq, Sk, 128, W, sinks, 1, ctypes.byref(floats)) == 0
         assert 0 <= floats.value <= 3000 * 256 * 128
+
+
+def test_fake_tensors():
+    """Traced without a GPU: shapes, layouts and which outputs carry gradients."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from prism_amd import _torch_ops
+    _torch_ops.load()
+    bf = torch.bfloat16
+    with FakeTensorMode():
+        for grad in (False, True):
+            def mk(*s):
+                return torch.empty(*s, device="cuda", dtype=bf, requires_grad=grad)  # noqa: B023
+            x, w = mk(3, 5, 64), mk(64)
+            y, h = prism_amd.rms_norm(x, w, residual=x)
+            assert y.shape == h.shape == x.shape and y.dtype == bf and y.requires_grad == h.requires_grad == grad
+            codes, scales = prism_amd.rms_norm_quant(x.detach(), out_dtype=torch.int8)
+            assert codes.dtype == torch.int8 and scales.shape == (3, 5) and scales.dtype == torch.float32
+            q, k = mk(2, 9, 4, 64).transpose(1, 2), mk(2, 9, 2, 64).transpose(1, 2)
+            freqs = torch.empty(32, device="cuda", dtype=torch.float64)
+            a, b = prism_amd.apply_rotary(q, k, freqs, torch.empty(9, device="cuda", dtype=torch.int64))
+            assert a.stride() == q.stride() and b.stride() == k.stride() and a.requires_grad == grad
+            o, lse = prism_amd.flash_attn_window(a, b, b, 5, return_lse=True)
+            assert o.stride() == q.stride() and lse.shape == (2, 4, 9)
+            assert o.requires_grad == grad and not lse.requires_grad
+            odd = mk(2, 4, 9, 65)[..., 1:]
+            assert prism_amd.flash_attn_window(odd, odd, odd, 5).shape == (2, 4, 9, 64)
+
+
+def test_frequencies_take_no_gradient():
+    q, freqs = torch.randn(1, 1, 3, 8), torch.ones(4, dtype=torch.float64, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        prism_amd.apply_rotary(q, None, freqs, torch.arange(3))
+
+
+def test_window_plans_with_every_key_a_sink():
+    """Windows and sinks far beyond any length plan like ones of the length."""
+    lib = _lib.load()
+    far = 1 << 62
+
+    def plans(window, sinks):
+        splits, a, b, c = ctypes.c_int(), ctypes.c_int64(), ctypes.c_int64(), ctypes.c_int64()
+        assert lib.prism_window_token_plan(2, 8, 2, 1, 5000, window, sinks, 1, ctypes.byref(splits), ctypes.byref(a)) == 0
+        assert lib.prism_window_fwd_plan(2, 8, 2, 900, 5000, 64, window, sinks, 1, ctypes.byref(b)) == 0
+        assert lib.prism_window_bwd_plan(2, 8, 2, 900, 5000, 64, window, sinks, 1, ctypes.byref(c)) == 0
+        return splits.value, a.value, b.value, c.value
+
+    assert plans(far, far) == plans(5000, 5000)
+    assert plans(100, far) == plans(100, 5000)
