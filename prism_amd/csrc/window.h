@@ -77,6 +77,7 @@ struct WinArgs {
   // 0) and leaves its sums in part (and m and l in part_ml)
   int whole, splits, items;
   float *part, *part_ml;
+  int ranked;                       // tiles by rank (rank_tile)
 };
 
 // ------------------------------------------------------------ spans
@@ -245,6 +246,49 @@ struct StageCopy {
   }
 };
 
+// Sequences of different lengths (right-padded batches): the tiles of a launch
+// by rank, the first of every sequence and key head, then the second of each,
+// and so on, and behind them the tiles past the sequences' ends.  In a launch of
+// one or two rounds every CU gets a like share of the heavy tiles so, and the empty
+// ones end the launch; in the order by sequences some CUs hold four full tiles and
+// others four empty ones.  Measured (us, by sequences / by rank): 2,598 and 2,306
+// tokens of 4,096, 16 heads over 4, D = 64, window 1,024: forward 46 / 35, dQ 50 /
+// 42, dK/dV 88 / 76; three sequences of 1,500 to 2,700, 12 heads over 4, D = 128,
+// window 2,000: forward 86 / 61, dQ 107 / 77.
+struct RankedTile {
+  int b, hk, rank;
+  bool live;  // else the rank-th of the tiles past the end
+};
+// c: the tiles of sequence `lane` (B <= 64, tiles <= 4,096); all lanes active
+__device__ __forceinline__ RankedTile rank_tile(int c, int B, int Hk, int tiles, int index) {
+  const int lane = (int)threadIdx.x & 63;
+  auto before = [&](int r) {  // tiles of ranks below r
+    int n = 0;
+    for (int b = 0; b < B; ++b) {
+      const int x = __builtin_amdgcn_readlane(c, b);
+      n += x < r ? x : r;
+    }
+    return n * Hk;
+  };
+  RankedTile t;
+  const int live = (int)uniform_u32((uint32_t)before(tiles));
+  t.live = index < live;
+  if (!t.live) {
+    c = tiles - c;
+    index -= live;
+  }
+  // the last rank with no more than `index` tiles before it: by 64, then by one
+  int r = 64 * (__popcll(__builtin_amdgcn_ballot_w64(before(64 * lane) <= index)) - 1);
+  r += __popcll(__builtin_amdgcn_ballot_w64(before(r + lane) <= index)) - 1;
+  t.rank = r;
+  const int j = (int)uniform_u32((uint32_t)(index - before(r)));
+  uint64_t who = __builtin_amdgcn_ballot_w64(lane < B && c > r);
+  for (int x = j / Hk; x > 0; --x) who &= who - 1;
+  t.b = who ? (int)__builtin_ctzll(who) : 0;
+  t.hk = j % Hk;
+  return t;
+}
+
 // Work item -> (sequence, key head, row tile), part of its list and workspace
 // slot (-1: whole).  Row tiles of one key head are neighbours (their windows
 // overlap in an XCD's L2), the last ones, whose causal lists are longest, first.
@@ -253,12 +297,23 @@ struct WinItem {
 };
 __device__ __forceinline__ WinItem win_tile(const WinArgs& a, int index, int split, int slot) {
   WinItem it;
+  it.split = split;
+  it.slot = slot;
+  if (a.ranked) {
+    const int lane = (int)threadIdx.x & 63;
+    int c = 0;
+    if (lane < a.B) c = (seq_span(a, lane).n * a.G + 127) >> 7;
+    const RankedTile t = rank_tile(c, a.B, a.Hk, a.tiles, index);
+    c = __builtin_amdgcn_readlane(c, t.b);
+    it.b = t.b;
+    it.hk = t.hk;
+    it.tile = t.live ? c - 1 - t.rank : c + t.rank;
+    return it;
+  }
   const int bh = index / a.tiles;
   it.tile = a.tiles - 1 - (index - bh * a.tiles);
   it.b = bh / a.Hk;
   it.hk = bh - it.b * a.Hk;
-  it.split = split;
-  it.slot = slot;
   return it;
 }
 __device__ __forceinline__ WinItem win_item(const WinArgs& a, int id) {
@@ -271,8 +326,9 @@ __device__ __forceinline__ WinItem win_item(const WinArgs& a, int id) {
 // times a NaN or an infinity is a NaN.  The kernels therefore look at their sums
 // once, at the end: where one of a wave's 32 rows is not finite, the wave computes
 // its rows again key by key, adding only what each row sees.  (Rows that do see
-// such a value keep it; the others get what they would have without it.)  Slow,
-// about 4 ms for 4,000 keys, and free otherwise.
+// such a value keep it; the others get what they would have without it.)  Slow, 0.5
+// to 1.5 us for each key of the list (4,000 queries of 8 heads over 4,000 keys, one NaN:
+// 80 us become 6.2 ms at D = 128, 52 become 2.2 at 64), and free otherwise.
 template <int NDT>
 __device__ __forceinline__ bool win_not_finite(const f32x16* acc, float l, bool live) {
   float t = 0.0f * l;
@@ -364,6 +420,14 @@ inline WinCut win_cut(int64_t total, int64_t slots, int64_t units, int D) {
   }
   if (c.splits == 1) c.whole = total;
   return c;
+}
+// Whether a launch of `total` tiles goes by rank (rank_tile): sequences of their
+// own lengths, several workgroups a CU (dK/dV at D = 128 has one: 150 us by
+// sequences, 152 by rank), more tiles than CUs, and no more than two rounds (beyond
+// them the order by sequences is better: neighbours share keys in an XCD's L2, and a
+// CU that ends early takes the next tile).
+inline int win_ranked(const int32_t* lens, int B, int64_t tiles, int64_t total, int64_t slots) {
+  return lens && B > 1 && B <= 64 && tiles <= 4096 && slots > 256 && total > 256 && total <= 2 * slots;
 }
 // the cut of a launch over row tiles of 128 (forward, dQ)
 WinCut win_row_cut(int64_t slots, int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks,

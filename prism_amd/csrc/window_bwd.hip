@@ -33,6 +33,7 @@ struct WinBwdArgs {
   // other tiles, rest_whole whole and the others in rest_splits pieces; pieces of
   // a cut tile leave their sums in acc
   int sink_tiles, key_tiles, sink_splits, sink_items, rest_whole, rest_splits, items;
+  int ranked;                // the other tiles by rank (rank_tile)
   float4* acc;
 };
 
@@ -240,28 +241,45 @@ __device__ __forceinline__ TokenRange tokens_of(const WinArgs& a, const SeqSpan&
 struct DkdvItem {
   int b, hk, tile, split, splits, slot;  // slot: workspace piece, -1: the whole list
 };
-__device__ __forceinline__ DkdvItem dkdv_item(const WinBwdArgs& a, int id) {
+// tile t of the rest: (sequence, key head, key tile), for tiles of `keys` keys
+struct KeyTile {
+  int b, hk, tile;
+};
+__device__ __forceinline__ KeyTile rest_tile(const WinBwdArgs& a, int t, int keys) {
   const int nrest = a.key_tiles - a.sink_tiles;
+  if (a.ranked) {
+    const int lane = (int)threadIdx.x & 63;
+    int c = 0;
+    if (lane < a.w.B) {
+      c = (seq_span(a.w, lane).L + keys - 1) / keys - a.sink_tiles;
+      c = c > 0 ? c : 0;
+    }
+    const RankedTile r = rank_tile(c, a.w.B, a.w.Hk, nrest, t);
+    return {r.b, r.hk, a.sink_tiles + r.rank + (r.live ? 0 : __builtin_amdgcn_readlane(c, r.b))};
+  }
+  const int bh = t / nrest, b = bh / a.w.Hk;
+  return {b, bh - b * a.w.Hk, a.sink_tiles + t - bh * nrest};
+}
+__device__ __forceinline__ DkdvItem dkdv_item(const WinBwdArgs& a, int id, int keys) {
   DkdvItem d;
-  int bh;
   if (id < a.sink_items) {
-    const int t = id / a.sink_splits;
-    bh = t / a.sink_tiles;
+    const int t = id / a.sink_splits, bh = t / a.sink_tiles;
     d.tile = t - bh * a.sink_tiles;
+    d.b = bh / a.w.Hk;
+    d.hk = bh - d.b * a.w.Hk;
     d.splits = a.sink_splits;
     d.split = id - t * a.sink_splits;
     d.slot = a.sink_splits > 1 ? id : -1;
   } else {
     const int y = id - a.sink_items, z = y - a.rest_whole;
-    const int t = z < 0 ? y : a.rest_whole + z / a.rest_splits;  // tile of the rest, all heads in a row
-    bh = t / nrest;
-    d.tile = a.sink_tiles + t - bh * nrest;
+    const KeyTile k = rest_tile(a, z < 0 ? y : a.rest_whole + z / a.rest_splits, keys);
+    d.b = k.b;
+    d.hk = k.hk;
+    d.tile = k.tile;
     d.splits = z < 0 ? 1 : a.rest_splits;
     d.split = z < 0 ? 0 : z % a.rest_splits;
     d.slot = z < 0 || a.rest_splits == 1 ? -1 : (a.sink_splits > 1 ? a.sink_items : 0) + z;
   }
-  d.b = bh / a.w.Hk;
-  d.hk = bh - d.b * a.w.Hk;
   return d;
 }
 
@@ -293,7 +311,7 @@ __global__ __launch_bounds__(DkdvTiles<D>::THREADS, D == 64 ? 3 : 1) void window
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
   const int w = (int)uniform_u32(threadIdx.x >> 6);
   const int kh = w & 1, qh = (w >> 1) & 1, tk = w >> 2;
-  const DkdvItem it = dkdv_item(ba, xcd_group_remap<8>((int)blockIdx.x, ba.items));
+  const DkdvItem it = dkdv_item(ba, xcd_group_remap<8>((int)blockIdx.x, ba.items), KEYS);
   const SeqSpan sq = seq_span(a, it.b);
   const int j0 = it.tile * KEYS;
 
@@ -631,11 +649,16 @@ __global__ __launch_bounds__(128 * key_tiles_of(D)) void window_merge_kernel(Win
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, w = threadIdx.x >> 6, blk = (int)blockIdx.y;
   const int x = (int)blockIdx.x, z = x - cut_sinks;
   const bool sink = z < 0;
-  const int S = sink ? a.sink_splits : a.rest_splits, nrest = a.key_tiles - a.sink_tiles;
+  const int S = sink ? a.sink_splits : a.rest_splits;
   const int64_t first = sink ? (int64_t)x * S : (int64_t)cut_sinks * a.sink_splits + (int64_t)z * S;
-  const int bh = sink ? x / a.sink_tiles : (a.rest_whole + z) / nrest;
-  const int tile = sink ? x - bh * a.sink_tiles : a.sink_tiles + a.rest_whole + z - bh * nrest;
-  const int b = bh / a.w.Hk, hk = bh - b * a.w.Hk, key = tile * 32 * KW + 32 * w + l32;
+  KeyTile kt;
+  if (sink) {
+    const int bh = x / a.sink_tiles;
+    kt = {bh / a.w.Hk, bh % a.w.Hk, x - bh * a.sink_tiles};
+  } else {
+    kt = rest_tile(a, a.rest_whole + z, 32 * KW);
+  }
+  const int b = kt.b, hk = kt.hk, key = kt.tile * 32 * KW + 32 * w + l32;
   if (key >= a.w.Sk) return;
   const float4* pa = a.acc + ((first * KW + w) * NB + blk) * 256 + lane;
   float4 acc[4];
@@ -667,6 +690,8 @@ __global__ __launch_bounds__(128 * key_tiles_of(D)) void window_merge_kernel(Win
 // workgroups of window_dq_kernel that the chip holds: two a CU at D = 128, three
 // at 64 (registers)
 int64_t dq_slots(int D) { return D == 128 ? 512 : 768; }
+// of window_dkdv_kernel: one a CU, three at D = 64
+int64_t key_slots(int D) { return D == 128 ? 256 : 768; }
 
 // How the dK/dV lists are cut, for one workgroup a CU (three at D = 64): the sinks' lists into
 // pieces no longer than the others, then the last round of tiles (win_cut).
@@ -689,7 +714,7 @@ DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int6
   p.rest_tiles = BH * (p.key_tiles - p.sink_tiles);
   p.sink_splits = p.sink_tiles ? (whole + n - 1) / n : 1;
   int64_t head = BH * p.sink_tiles * p.sink_splits;  // pieces before the rest's tiles
-  const int64_t slots = D == 64 ? 768 : 256, total = head + p.rest_tiles;
+  const int64_t slots = key_slots(D), total = head + p.rest_tiles;
   const WinCut c = win_cut(total, slots, rest, D);
   p.rest_splits = c.splits;
   p.rest_whole = c.whole > head ? c.whole - head : 0;
@@ -754,6 +779,8 @@ int prism_window_bwd(const void* do_, const void* q, const void* k, const void* 
   PRISM_REQUIRE(p.pieces + cut == 0 || acc, "prism_window_bwd: null workspace");
   a.w.total = (int)total;
   a.w.whole = (int)c.whole; a.w.splits = (int)c.splits; a.w.items = (int)items;
+  a.w.ranked = win_ranked(q_lens, B, a.w.tiles, total, dq_slots(D));
+  a.ranked = win_ranked(kv_lens, B, p.key_tiles, p.rest_tiles, key_slots(D));
   a.w.part = acc + p.pieces * 128 * key_tiles_of(D) * D;
   a.sink_tiles = (int)p.sink_tiles; a.key_tiles = (int)p.key_tiles;
   a.sink_splits = (int)p.sink_splits; a.sink_items = (int)p.sink_items;

@@ -337,6 +337,7 @@ int prism_window_fwd(const void* q, const void* k, const void* v, int dtype, int
   PRISM_REQUIRE(cut == 0 || part, "prism_window_fwd: null workspace");
   a.total = (int)total;
   a.whole = (int)c.whole; a.splits = (int)c.splits; a.items = (int)items;
+  a.ranked = win_ranked(q_lens, B, a.tiles, total, fwd_slots(D));
   a.part = part;
   a.part_ml = part + cut * c.splits * 128 * D;
   auto run = [&](auto kernel, auto join) {

@@ -17,6 +17,7 @@ import torch
 
 import prism_amd
 from tests.test_gpu_window import DT, make, seen_mask
+from tests.test_gpu_window import check as check_forward
 
 pytestmark = pytest.mark.gpu
 
@@ -148,6 +149,30 @@ def test_layouts_broadcasts_and_partial_leaves():
     o = prism_amd.flash_attn_window(q.detach(), x, v.detach(), 20)
     (g1,) = torch.autograd.grad(o.sum(), x)
     assert torch.equal(g1, check(q.detach(), k.detach(), v.detach(), torch.ones_like(o), 20)[1])
+
+
+RAGGED = [  # B, S, Hq, Hk, D, window, sinks, causal: a round or two of tiles, sequences of their own lengths
+    (5, 1000, 8, 4, 64, 200, 70, True), (5, 1000, 7, 7, 128, 300, 4, False), (3, 1000, 16, 2, 128, 300, 0, True),
+    (64, 100, 8, 8, 64, 30, 4, True), (65, 100, 8, 8, 64, 30, 4, True), (33, 130, 9, 9, 128, None, 0, True),
+    (2, 2500, 8, 8, 64, 400, 140, False),
+]
+
+
+@pytest.mark.parametrize("case", RAGGED, ids=lambda c: "-".join(str(x) for x in c))
+def test_ragged_batches(case):
+    """Tiles taken by rank over sequences of different lengths (zero, one, all)."""
+    B, S, Hq, Hk, D, window, sinks, causal = case
+    q, k, v = make(B, S, S, Hq, Hk, D, torch.bfloat16, seed=S + B, projected=True)
+    do = torch.randn_like(q)
+    lens = torch.tensor([S, 0, S // 2 + 37, 64, S - 1, 1] * (B // 6 + 1), dtype=torch.int32, device="cuda")[:B]
+    other = lens.flip(0).contiguous()
+    for ql, kv in ((lens, lens), (other, lens), (lens, None), (None, lens)):
+        mask = seen_mask(B, S, S, window, sinks, causal, ql, kv)
+        rows, keys = ~mask.any(2)[:, None, :, None], ~mask.any(1)[:, None, :, None]
+        kw = dict(sinks=sinks, causal=causal, q_lens=ql, kv_lens=kv)
+        args = (q.masked_fill(rows, math.nan), k.masked_fill(keys, math.nan), v.masked_fill(keys, math.inf))
+        check_forward(*args, window, **kw)
+        check(*args, do.masked_fill(rows, math.nan), window, **kw)
 
 
 def test_captured():
