@@ -4,9 +4,14 @@
 //   dv = P^T do,  dk = scale dS^T q,  dq = scale dS k
 //
 // window_dq_kernel, by 128 rows, over the key list of the forward: S^T and dP^T
-// keep one query per lane column, dQ^T += K^T dS^T.  It also forms delta from
-// the rows of o and do that it holds, and leaves (m2, delta) = (lse log2 e, delta) of
-// every row for the second kernel.
+// keep one query per lane column, dQ^T += K^T dS^T.  It also forms delta and
+// leaves (m2, delta) = (lse log2 e, delta) of every row for the second kernel: from the
+// rows of o and do that it holds, or, where rows see 64 keys at most, as sum_j P_j
+// dP_j in a pass over the tiles before.  o is stored rounded, and the fewer keys the
+// larger delta's error so is beside dS: dq off by 3.0e-3 (norm-wise, bf16, rows that
+// see 1 to 5 keys), 2.6e-3 (8), 2.4e-3 (64), with the pass 2.3e-3, 2.3e-3, 2.4e-3.
+// The pass costs no more than reading o: 14,040 tokens, 40 heads over 8, window 64,
+// D = 128: 200 us with it, 240 without; 2 x 4,001 tokens, window 60 and 4 sinks 52 / 51.
 // window_dkdv_kernel, by 128 keys (64 at D = 64), over the tokens that see them,
 // one query head of the group after the other: the two halves of each 64-row
 // query tile on different waves (partial sums added through LDS in a fixed
@@ -34,6 +39,7 @@ struct WinBwdArgs {
   // a cut tile leave their sums in acc
   int sink_tiles, key_tiles, sink_splits, sink_items, rest_whole, rest_splits, items;
   int ranked;                // the other tiles by rank (rank_tile)
+  int exact;                 // delta from P and dP instead of o (window_dq_kernel)
   float4* acc;
 };
 
@@ -96,17 +102,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_dq_kernel(WinBwdA
     for (int s = 0; s < NS; ++s) {
       qf[s] = ld_bf16x8(qp + 16 * s);
       df[s] = ld_bf16x8(dp + 16 * s);
-      dlt = dot8<E>(ld_bf16x8(op + 16 * s), df[s], dlt);
+      if (!ba.exact) dlt = dot8<E>(ld_bf16x8(op + 16 * s), df[s], dlt);
     }
   }
-  dlt = xor32_add(dlt);
   const float lse = a.lse[lrow];
   // rows that see nothing: P = 2^(s - inf) = 0
   const float mq = lse == -__builtin_inff() ? __builtin_inff() : lse * 1.4426950408889634f;
-  if (r < rows && g == 0 && it.split == 0) {
-    ba.m2[lrow] = mq;
-    ba.delta[lrow] = dlt;
-  }
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     consume_regs(qf[s]);
@@ -121,6 +122,39 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_dq_kernel(WinBwdA
   const bool whole = (wr0 + 31) / a.G <= last;
   WaveSpan ws;
   ws.init(a, kl, wi0 + sq.off, wi1 + sq.off);
+
+  if (ba.exact) {  // (never cut: t0 .. t1 is the whole list)
+    for (int t = t0; t < t1; ++t) {
+      dma_wait_all();
+      __syncthreads();
+      if (w < 2 && t + 1 < t1) copy.issue(kl, 64 * (t + 1), lds0 + (uint32_t)(((t + 1) & 1) * T::STAGE));
+      const uint8_t* sK = smem + (t & 1) * T::STAGE;
+      f32x16 sacc[2] = {f32x16_zero(), f32x16_zero()}, pacc[2] = {f32x16_zero(), f32x16_zero()};
+#pragma unroll
+      for (int x = 0; x < NS; ++x)
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh) {
+          sacc[kh] = E::mfma(rop.load(sK + RT::rows(32 * kh), x), qf[x], sacc[kh]);
+          pacc[kh] = E::mfma(rop.load(sK + RT::BYTES + RT::rows(32 * kh), x), df[x], pacc[kh]);
+        }
+      const uint64_t mm = span_bits(span, 64 * t) >> (4 * g);
+      const uint32_t bits[2] = {(uint32_t)mm, (uint32_t)(mm >> 32)};
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const float p = fast_exp2(__builtin_fmaf(sacc[kh][x], a.scale_log2, -mq));
+          dlt += keep_or_zero(p * pacc[kh][x], bits[kh], 8 * (x >> 2) + (x & 3));
+        }
+    }
+    __syncthreads();
+    if (w < 2 && t1 > t0 + 1) copy.issue(kl, 64 * t0, lds0 + (uint32_t)((t0 & 1) * T::STAGE));
+  }
+  dlt = xor32_add(dlt);
+  if (r < rows && g == 0 && it.split == 0) {
+    ba.m2[lrow] = mq;
+    ba.delta[lrow] = dlt;
+  }
 
   // the dP^T chains start from -delta (at D = 64 from 0, and delta is subtracted
   // after them: 168 registers let three workgroups share a CU)
@@ -781,6 +815,8 @@ int prism_window_bwd(const void* do_, const void* q, const void* k, const void* 
   a.w.whole = (int)c.whole; a.w.splits = (int)c.splits; a.w.items = (int)items;
   a.w.ranked = win_ranked(q_lens, B, a.w.tiles, total, dq_slots(D));
   a.ranked = win_ranked(kv_lens, B, p.key_tiles, p.rest_tiles, key_slots(D));
+  const int64_t near = window < Sk ? window : Sk, keys = (causal ? near : 2 * near - 1) + (sinks < Sk ? sinks : Sk);
+  a.exact = cut == 0 && (keys < Sk ? keys : Sk) <= 64;
   a.w.part = acc + p.pieces * 128 * key_tiles_of(D) * D;
   a.sink_tiles = (int)p.sink_tiles; a.key_tiles = (int)p.key_tiles;
   a.sink_splits = (int)p.sink_splits; a.sink_items = (int)p.sink_items;

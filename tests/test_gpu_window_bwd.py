@@ -9,6 +9,8 @@ Tolerance (u = eps / 2 of the type): with exact P, dP, delta,
   of that bound with |k| and |q|, dv by (u + r) P^T |do|, each by its own
   rounding u |.| and fp32 sums of N terms (N 2^-24 of the terms).  float16
   adds its subnormal steps: 2^-25 for each P and dS, times |do|, |k|, |q|.
+Where rows see 64 keys at most (few), delta is the sum of P dP: r sum P |dP| in
+the place of u D1.
 """
 import math
 
@@ -22,7 +24,7 @@ from tests.test_gpu_window import check as check_forward
 pytestmark = pytest.mark.gpu
 
 
-def check(q, k, v, do, window, *, sinks=0, causal=True, q_lens=None, kv_lens=None, sm_scale=None):
+def check(q, k, v, do, window, *, sinks=0, causal=True, q_lens=None, kv_lens=None, sm_scale=None, few=False):
     B, Hq, Sq, D = q.shape
     Hk, Sk, G = k.shape[1], k.shape[2], Hq // k.shape[1]
     leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
@@ -52,7 +54,8 @@ def check(q, k, v, do, window, *, sinks=0, causal=True, q_lens=None, kv_lens=Non
     d1 = (do64 * o64).abs().sum(-1, keepdim=True)
     d2 = (do64.abs() @ v64.abs().transpose(-1, -2)).masked_fill(~m, 0).amax(-1, keepdim=True)
     sub = 2.0 ** -25 * m * (q.dtype == torch.float16)
-    ds = P * (u * d1 + (r + 1.01 * u) * (dP - delta).abs() + 2.0 ** -24 * (D + n) * d2) + sub
+    d0 = r * (P * dP.abs()).sum(-1, keepdim=True) if few else u * d1
+    ds = P * (d0 + (r + 1.01 * u) * (dP - delta).abs() + 2.0 ** -24 * (D + n) * d2) + sub
     dp = P * (u * 1.01 + r) + sub
     N = n * 2.0 ** -24
     tols = [scale * (ds @ k64.abs() + N * (dS.abs() @ k64.abs())), scale * (tr(ds, q64.abs()) + N * tr(dS.abs(), q64.abs())),
@@ -149,6 +152,23 @@ def test_layouts_broadcasts_and_partial_leaves():
     o = prism_amd.flash_attn_window(q.detach(), x, v.detach(), 20)
     (g1,) = torch.autograd.grad(o.sum(), x)
     assert torch.equal(g1, check(q.detach(), k.detach(), v.detach(), torch.ones_like(o), 20)[1])
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("case", [(3, 5, 5, 8, 2, 64, None, 0, True), (2, 64, 64, 4, 2, 128, None, 0, False),
+                                  (2, 300, 300, 4, 2, 64, 3, 0, True), (1, 200, 333, 6, 2, 128, 40, 24, True),
+                                  (2, 150, 150, 5, 5, 64, 30, 5, False), (1, 300, 300, 40, 1, 128, 60, 4, True),
+                                  (2, 700, 40, 7, 1, 64, 9, 0, True), (1, 2000, 2000, 33, 33, 64, 12, 2, True)],
+                         ids=lambda c: "-".join(str(x) for x in c))
+def test_few_keys_with_a_common_part(case, dt):
+    """Values that share a large part (64, times do of one sign): the rounding of o
+    in delta would be far larger than dS, which does not depend on that part."""
+    B, Sq, Sk, Hq, Hk, D, window, sinks, causal = case
+    q, k, v = make(B, Sq, Sk, Hq, Hk, D, DT[dt], seed=Sq + Sk)
+    do = torch.randn_like(q).abs()
+    lens = torch.tensor([Sk, Sk // 2, 1], dtype=torch.int32, device="cuda")[:B]
+    for n in (None, lens):
+        check(q, k, v + 64, do, window, sinks=sinks, causal=causal, kv_lens=n, q_lens=n if Sq == Sk else None, few=True)
 
 
 RAGGED = [  # B, S, Hq, Hk, D, window, sinks, causal: a round or two of tiles, sequences of their own lengths
