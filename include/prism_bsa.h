@@ -183,10 +183,11 @@ int prism_window_token(const void* q, const void* k, const void* v, int dtype, i
 /* Gradients of prism_window_fwd from do [B, Hq, Sq, D], its o and lse: dq, dk,
  * dv (rows that nothing reaches are 0).  strides (host): batch, head, token of
  * q, k, v, o, do, dq, dk, dv, as above.  rows: workspace of 2 * B * Hq * Sq
- * floats; acc: of as many floats as prism_window_bwd_plan says (NULL for 0).
+ * floats; acc: of as many floats as prism_window_bwd_plan says (NULL for 0;
+ * its kv_lens: whether the call passes them).
  * Deterministic (no atomics). */
 int prism_window_bwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal,
-                          int64_t* floats);
+                          int kv_lens, int64_t* floats);
 int prism_window_bwd(const void* do_, const void* q, const void* k, const void* v, const void* o, const float* lse,
                      int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, const int64_t* strides,
                      int64_t window, int64_t sinks, int causal, const int32_t* q_lens, const int32_t* kv_lens,

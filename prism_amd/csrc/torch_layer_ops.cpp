@@ -267,7 +267,7 @@ std::tuple<Tensor, Tensor, Tensor> window_bwd(const Tensor& do_, const Tensor& q
   const Tensor* all[8] = {&q, &k, &v, &o, &d, &dq, &dk, &dv};
   for (int i = 0; i < 8; ++i) win_strides(*all[i], st + 3 * i);
   const int B = small(s.B, "B"), Hq = small(s.Hq, "heads"), Hk = small(s.Hk, "heads"), D = small(s.D, "D");
-  check_rc(prism_window_bwd_plan(B, Hq, Hk, s.Sq, s.Sk, D, window, sinks, causal, &floats));
+  check_rc(prism_window_bwd_plan(B, Hq, Hk, s.Sq, s.Sk, D, window, sinks, causal, kv_lens.has_value(), &floats));
   Tensor rows = at::empty({2 * s.B * s.Hq * s.Sq}, opts(q, at::kFloat));
   Tensor acc = floats ? at::empty({floats}, opts(q, at::kFloat)) : none_like(q);
   PRISM_TORCH_CALL(prism_window_bwd, d.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),

@@ -23,6 +23,11 @@
 //
 // Numbers: P and dS are rounded to the inputs' type for the products (float16: a
 // dS beyond 65,504 becomes infinite, which a loss scaler sees), the rest is fp32.
+//
+// Bound: the matrix cores at D = 128.  Measured: 14,040 tokens, 5 heads, D = 128, 4,680
+// to both sides, 1,560 sinks: dQ 405 + 6 us, dK/dV 575 + 12 (matrix cores busy 72% and 67%
+// of the cycles); 2 x 4,096 padded tokens (half to all of them), 16 heads over 4, D =
+// 64, window 1,024: dQ 50-58 us, dK/dV 55-93 + 12.
 #include <type_traits>
 
 #include "window.h"
@@ -272,6 +277,15 @@ __device__ __forceinline__ TokenRange tokens_of(const WinArgs& a, const SeqSpan&
   return {i0 > 0 ? i0 : 0, sink || i1 > end ? end : i1};
 }
 
+// tokens that see some key of [j0, j0 + keys) (the first and the last key's, and the
+// sinks' where it has some)
+__device__ __forceinline__ TokenRange tile_tokens(const WinArgs& a, const SeqSpan& s, int j0, int keys) {
+  if (j0 >= s.L || s.n == 0) return {0, -1};
+  const int jl = j0 + keys - 1 < s.L - 1 ? j0 + keys - 1 : s.L - 1;
+  const TokenRange f = tokens_of(a, s, j0), l = tokens_of(a, s, jl);
+  return {f.i0 < l.i0 ? f.i0 : l.i0, f.i1 > l.i1 ? f.i1 : l.i1};
+}
+
 struct DkdvItem {
   int b, hk, tile, split, splits, slot;  // slot: workspace piece, -1: the whole list
 };
@@ -349,16 +363,10 @@ __global__ __launch_bounds__(DkdvTiles<D>::THREADS, D == 64 ? 3 : 1) void window
   const SeqSpan sq = seq_span(a, it.b);
   const int j0 = it.tile * KEYS;
 
-  // tokens that see some key of the tile (the first and the last key's, and the
-  // sinks' when it has some), as 64-token tiles of each head from lo on
-  int lo, hi;
-  {
-    const int jl = j0 + KEYS - 1 < sq.L - 1 ? j0 + KEYS - 1 : sq.L - 1;
-    const TokenRange f = tokens_of(a, sq, j0), l = tokens_of(a, sq, jl < j0 ? j0 : jl);
-    lo = f.i0 < l.i0 ? f.i0 : l.i0;
-    hi = f.i1 > l.i1 ? f.i1 : l.i1;
-    if (j0 >= sq.L || sq.n == 0) { lo = 0; hi = -1; }
-  }
+  // the tile's tokens, as 64-token tiles of each head from lo on
+  const TokenRange tokens = tile_tokens(a, sq, j0, KEYS);
+  const int lo = tokens.i0, hi = tokens.i1;
+  if (hi < lo && it.slot >= 0) return;  // (window_merge_kernel knows)
   const int nti = hi >= lo ? (hi - lo + 64) >> 6 : 0, all = nti * a.G;
   const int e0 = (int)((int64_t)all * it.split / it.splits), e1 = (int)((int64_t)all * (it.split + 1) / it.splits);
   const int n = e1 - e0;
@@ -695,11 +703,13 @@ __global__ __launch_bounds__(128 * key_tiles_of(D)) void window_merge_kernel(Win
   const int b = kt.b, hk = kt.hk, key = kt.tile * 32 * KW + 32 * w + l32;
   if (key >= a.w.Sk) return;
   const float4* pa = a.acc + ((first * KW + w) * NB + blk) * 256 + lane;
+  const TokenRange tokens = tile_tokens(a.w, seq_span(a.w, b), kt.tile * 32 * KW, 32 * KW);
+  const bool seen = tokens.i1 >= tokens.i0;  // else: no piece was left
   float4 acc[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) acc[j] = pa[j * 64];
+  for (int j = 0; j < 4; ++j) acc[j] = seen ? pa[j * 64] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-  for (int s = 1; s < S; ++s)
+  for (int s = 1; s < (seen ? S : 1); ++s)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float4 v = pa[(int64_t)s * KW * NB * 256 + j * 64];
@@ -732,7 +742,7 @@ int64_t key_slots(int D) { return D == 128 ? 256 : 768; }
 struct DkdvPlan {
   int64_t sink_tiles, key_tiles, sink_splits, sink_items, rest_whole, rest_splits, rest_tiles, items, pieces;
 };
-DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal) {
+DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal, int lens) {
   DkdvPlan p{};
   const int64_t keys = 64 * key_tiles_of(D);
   const int64_t BH = (int64_t)B * Hk, whole = G * ((Sq + 63) / 64);
@@ -749,7 +759,13 @@ DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int6
   p.sink_splits = p.sink_tiles ? (whole + n - 1) / n : 1;
   int64_t head = BH * p.sink_tiles * p.sink_splits;  // pieces before the rest's tiles
   const int64_t slots = key_slots(D), total = head + p.rest_tiles;
-  const WinCut c = win_cut(total, slots, rest, D);
+  // Lengths (lens: the call passes them) stand on the device: at D = 64, where three
+  // workgroups share a CU, a batch that has them is cut as if three quarters of its
+  // tiles held anything (the others end at once, and last: rank_tile).  Measured with the
+  // merge (us, as for full sequences / so), 2 x 4,096 tokens, 16 heads over 4, window
+  // 1,024: 2,598 and 2,306 of them 82 / 66; 3,000 and 3,400 93 / 85; 3,900 and 4,096 98 /
+  // 106.  At D = 128 (and for the rows of the forward and dQ) it loses.
+  const WinCut c = win_cut(lens && D == 64 ? (3 * total + 3) / 4 : total, slots, rest, D);
   p.rest_splits = c.splits;
   p.rest_whole = c.whole > head ? c.whole - head : 0;
   if (p.rest_whole > p.rest_tiles) p.rest_whole = p.rest_tiles;
@@ -774,12 +790,12 @@ int64_t bwd_floats(const DkdvPlan& p, const WinCut& c, int64_t row_tiles, int64_
 extern "C" {
 
 int prism_window_bwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal,
-                          int64_t* floats) {
+                          int kv_lens, int64_t* floats) {
   PRISM_REQUIRE(B >= 0 && Hk >= 1 && Hq >= Hk && Hq % Hk == 0 && Sq >= 0 && Sk >= 0 && D >= 1 && window >= 1 &&
                     sinks >= 0 && floats,
                 "prism_window_bwd_plan: bad argument");
   const int64_t G = Hq / Hk;
-  *floats = bwd_floats(dkdv_plan(B, Hk, G, Sq, Sk, D, window, sinks, causal),
+  *floats = bwd_floats(dkdv_plan(B, Hk, G, Sq, Sk, D, window, sinks, causal, kv_lens),
                        win_row_cut(dq_slots(D), B, Hk, G, Sq, Sk, D, window, sinks, causal), (int64_t)B * Hk * ((Sq * G + 127) / 128), D);
   return PRISM_OK;
 }
@@ -807,7 +823,7 @@ int prism_window_bwd(const void* do_, const void* q, const void* k, const void* 
   a.w.tiles = (int)((Sq * a.w.G + 127) / 128);
   const int64_t total = (int64_t)B * Hk * a.w.tiles;
   const WinCut c = win_row_cut(dq_slots(D), B, Hk, a.w.G, Sq, Sk, D, window, sinks, causal);
-  const DkdvPlan p = dkdv_plan(B, Hk, a.w.G, Sq, Sk, D, window, sinks, causal);
+  const DkdvPlan p = dkdv_plan(B, Hk, a.w.G, Sq, Sk, D, window, sinks, causal, kv_lens != nullptr);
   const int64_t cut = total - c.whole, items = c.whole + cut * c.splits;
   PRISM_REQUIRE(items < (1ll << 31) && p.items < (1ll << 31), "prism_window_bwd: too many tiles");
   PRISM_REQUIRE(p.pieces + cut == 0 || acc, "prism_window_bwd: null workspace");

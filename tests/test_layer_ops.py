@@ -173,8 +173,9 @@ def test_window_plans():
                                         (4, 32, 8, 16384, 16384, 1 << 29, 0)):
         assert lib.prism_window_fwd_plan(B, Hq, Hk, Sq, Sk, 128, W, sinks, 1, ctypes.byref(floats)) == 0
         assert 0 <= floats.value <= 2 * 512 * 128 * 130
-        assert lib.prism_window_bwd_plan(B, Hq, Hk, Sq, Sk, 128, W, sinks, 1, ctypes.byref(floats)) == 0
-        assert 0 <= floats.value <= 3000 * 256 * 128
+        for D, lens in ((128, 0), (128, 1), (64, 0), (64, 1)):
+            assert lib.prism_window_bwd_plan(B, Hq, Hk, Sq, Sk, D, W, sinks, 1, lens, ctypes.byref(floats)) == 0
+            assert 0 <= floats.value <= 3000 * 256 * 128
 
 
 def test_fake_tensors():
@@ -218,7 +219,7 @@ def test_window_plans_with_every_key_a_sink():
         splits, a, b, c = ctypes.c_int(), ctypes.c_int64(), ctypes.c_int64(), ctypes.c_int64()
         assert lib.prism_window_token_plan(2, 8, 2, 1, 5000, window, sinks, 1, ctypes.byref(splits), ctypes.byref(a)) == 0
         assert lib.prism_window_fwd_plan(2, 8, 2, 900, 5000, 64, window, sinks, 1, ctypes.byref(b)) == 0
-        assert lib.prism_window_bwd_plan(2, 8, 2, 900, 5000, 64, window, sinks, 1, ctypes.byref(c)) == 0
+        assert lib.prism_window_bwd_plan(2, 8, 2, 900, 5000, 64, window, sinks, 1, 1, ctypes.byref(c)) == 0
         return splits.value, a.value, b.value, c.value
 
     assert plans(far, far) == plans(5000, 5000)
