@@ -157,16 +157,19 @@ int prism_rotary(const void* q, const void* k, int dtype, int B, int64_t S, int 
  * sinks and j <= p (causal), else where |p - j| < window or j < sinks.  o: 0
  * for queries that see nothing and rows i >= n; lse: [B, Hq, Sq] fp32 natural
  * log-sum-exp of the scaled scores (-inf there), or NULL.  Rows of k and v that
- * no query sees are not read.  part: workspace of as many floats as prism_window_fwd_plan says
+ * no query sees are not read.  rest: NULL, or of o's size and strides, takes what
+ * o's rounding left off; prism_window_rest: whether prism_window_bwd has a use for it
+ * (its delta is the more exact).  part: workspace of as many floats as prism_window_fwd_plan says
  * (NULL for 0): row tiles of the launch's last round may be cut over several
  * workgroups, whose sums a second kernel joins in order.  No counterpart in the
  * reference. */
+int prism_window_rest(int64_t Sk, int64_t window, int64_t sinks, int causal);
 int prism_window_fwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal,
                           int64_t* floats);
 int prism_window_fwd(const void* q, const void* k, const void* v, int dtype, int B, int Hq, int Hk, int64_t Sq,
                      int64_t Sk, int D, const int64_t* strides, int64_t window, int64_t sinks, int causal,
-                     const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, float* lse, float* part,
-                     hipStream_t stream);
+                     const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, void* rest, float* lse,
+                     float* part, hipStream_t stream);
 
 /* prism_window_fwd for few query rows over many keys (single tokens over a
  * cache): the keys are cut over `splits` workgroups per 32 rows, whose partial
@@ -177,19 +180,19 @@ int prism_window_token_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int64
                             int* splits, int64_t* floats);
 int prism_window_token(const void* q, const void* k, const void* v, int dtype, int B, int Hq, int Hk, int64_t Sq,
                        int64_t Sk, int D, const int64_t* strides, int64_t window, int64_t sinks, int causal,
-                       const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, float* lse, int splits,
-                       float* part_o, float* part_ml, hipStream_t stream);
+                       const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, void* rest, float* lse,
+                       int splits, float* part_o, float* part_ml, hipStream_t stream);
 
 /* Gradients of prism_window_fwd from do [B, Hq, Sq, D], its o and lse: dq, dk,
- * dv (rows that nothing reaches are 0).  strides (host): batch, head, token of
+ * dv (rows that nothing reaches are 0).  rest: the forward's, or NULL.  strides (host): batch, head, token of
  * q, k, v, o, do, dq, dk, dv, as above.  rows: workspace of 2 * B * Hq * Sq
  * floats; acc: of as many floats as prism_window_bwd_plan says (NULL for 0;
  * its kv_lens: whether the call passes them).
  * Deterministic (no atomics). */
 int prism_window_bwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal,
                           int kv_lens, int64_t* floats);
-int prism_window_bwd(const void* do_, const void* q, const void* k, const void* v, const void* o, const float* lse,
-                     int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, const int64_t* strides,
+int prism_window_bwd(const void* do_, const void* q, const void* k, const void* v, const void* o, const void* rest,
+                     const float* lse, int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, const int64_t* strides,
                      int64_t window, int64_t sinks, int causal, const int32_t* q_lens, const int32_t* kv_lens,
                      float sm_scale, void* dq, void* dk, void* dv, float* rows, float* acc, hipStream_t stream);
 

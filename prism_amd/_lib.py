@@ -32,11 +32,12 @@ SIGNATURES = {
     "prism_rms_norm_bwd": [P, I64, P, I64, P, I64, P, I32, I32, I64, I32, P, P, P, I32, P, P],
     "prism_rotary": [P, P, I32, I32, I64, I32, I32, I32, I32, P, P, P, I32, P, I32, P, I32, F32, I32, P, P, P],
     "prism_window_fwd_plan": [I32, I32, I32, I64, I64, I32, I64, I64, I32, P],
-    "prism_window_fwd": [P, P, P, I32, I32, I32, I32, I64, I64, I32, P, I64, I64, I32, P, P, F32, P, P, P, P],
+    "prism_window_rest": [I64, I64, I64, I32],
+    "prism_window_fwd": [P, P, P, I32, I32, I32, I32, I64, I64, I32, P, I64, I64, I32, P, P, F32, P, P, P, P, P],
     "prism_window_token_plan": [I32, I32, I32, I64, I64, I64, I64, I32, P, P],
-    "prism_window_token": [P, P, P, I32, I32, I32, I32, I64, I64, I32, P, I64, I64, I32, P, P, F32, P, P, I32, P, P, P],
+    "prism_window_token": [P, P, P, I32, I32, I32, I32, I64, I64, I32, P, I64, I64, I32, P, P, F32, P, P, P, I32, P, P, P],
     "prism_window_bwd_plan": [I32, I32, I32, I64, I64, I32, I64, I64, I32, I32, P],
-    "prism_window_bwd": [P, P, P, P, P, P, I32, I32, I32, I32, I64, I64, I32, P, I64, I64, I32, P, P, F32, P, P, P, P, P, P],
+    "prism_window_bwd": [P, P, P, P, P, P, P, I32, I32, I32, I32, I64, I64, I32, P, I64, I64, I32, P, P, F32, P, P, P, P, P, P],
     "prism_zone_layout": [P, I32, P, P, P, P],
     "prism_rearrange_index": [P, I32, I32, I32, P, P, P],
     "prism_gather_pool": [P, I32, I32, I32, I64, I32, P, P, P, I32, I32, I32, I32, I32, I32, I64, P, P, P, P, P, P, P, P],

@@ -112,11 +112,13 @@ def _register_fakes():
         return like(q), like(k) if k is not None else _none(q)
 
     @reg("prism::window_fwd")
-    def _(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse):
-        return like(q, 1 << 24), _empty(q, q.shape[:3], f32) if want_lse else _none(q)
+    def _(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse, want_rest):
+        o = like(q, 1 << 24)
+        return (o, _empty(q, q.shape[:3], f32) if want_lse else _none(q),
+                torch.empty_like(o) if want_rest else _empty(q, (0,), q.dtype))
 
     @reg("prism::window_bwd")
-    def _(do, q, k, v, o, lse, window, sinks, causal, q_lens, kv_lens, sm_scale):
+    def _(do, q, k, v, o, rest, lse, window, sinks, causal, q_lens, kv_lens, sm_scale):
         return like(q, 1 << 24), like(k, 1 << 24), like(v, 1 << 24)
 
     @reg("prism::zone_layout")

@@ -210,15 +210,17 @@ WinShape check_window(const Tensor& q, const Tensor& k, const Tensor& v, const O
   return s;
 }
 
-std::tuple<Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window,
-                                      int64_t sinks, bool causal, const OptT& q_lens_, const OptT& kv_lens_,
-                                      double sm_scale, bool want_lse) {
+std::tuple<Tensor, Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window,
+                                              int64_t sinks, bool causal, const OptT& q_lens_, const OptT& kv_lens_,
+                                              double sm_scale, bool want_lse, bool want_rest) {
   const WinShape s = check_window(q_, k_, v_, q_lens_, kv_lens_);
   const c10::DeviceGuard guard(q_.device());
   const Tensor q = win_rows(q_), k = win_rows(k_), v = win_rows(v_);
   const OptT q_lens = cont(q_lens_), kv_lens = cont(kv_lens_);
   Tensor o = win_like(q_);
   Tensor lse = want_lse ? at::empty({s.B, s.Hq, s.Sq}, opts(q, at::kFloat)) : none_like(q);
+  Tensor rest = want_rest ? at::empty_like(o) : at::empty({0}, o.options());
+  void* rp = want_rest ? rest.data_ptr() : nullptr;
   int64_t st[12];
   win_strides(q, st);
   win_strides(k, st + 3);
@@ -234,19 +236,19 @@ std::tuple<Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_, const 
     float* po = splits > 1 ? part.data_ptr<float>() : nullptr;
     PRISM_TORCH_CALL(prism_window_token, q.data_ptr(), k.data_ptr(), v.data_ptr(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st,
                      window, sinks, causal, (const int32_t*)p(q_lens), (const int32_t*)p(kv_lens), (float)sm_scale,
-                     o.data_ptr(), lp, splits, po, po ? po + floats * s.D : nullptr, stream_of(q));
-    return {o, lse};
+                     o.data_ptr(), rp, lp, splits, po, po ? po + floats * s.D : nullptr, stream_of(q));
+    return {o, lse, rest};
   }
   check_rc(prism_window_fwd_plan(B, Hq, Hk, s.Sq, s.Sk, D, window, sinks, causal, &floats));
   Tensor part = floats ? at::empty({floats}, opts(q, at::kFloat)) : none_like(q);
   PRISM_TORCH_CALL(prism_window_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st,
                    window, sinks, causal, (const int32_t*)p(q_lens), (const int32_t*)p(kv_lens), (float)sm_scale,
-                   o.data_ptr(), lp, floats ? part.data_ptr<float>() : nullptr, stream_of(q));
-  return {o, lse};
+                   o.data_ptr(), rp, lp, floats ? part.data_ptr<float>() : nullptr, stream_of(q));
+  return {o, lse, rest};
 }
 
 std::tuple<Tensor, Tensor, Tensor> window_bwd(const Tensor& do_, const Tensor& q_, const Tensor& k_, const Tensor& v_,
-                                              const Tensor& o_, const Tensor& lse_, int64_t window, int64_t sinks,
+                                              const Tensor& o_, const OptT& rest_, const Tensor& lse_, int64_t window, int64_t sinks,
                                               bool causal, const OptT& q_lens_, const OptT& kv_lens_,
                                               double sm_scale) {
   const WinShape s = check_window(q_, k_, v_, q_lens_, kv_lens_);
@@ -255,11 +257,20 @@ std::tuple<Tensor, Tensor, Tensor> window_bwd(const Tensor& do_, const Tensor& q
     check_dtype(*t.first, q_.scalar_type(), t.second);
     TORCH_CHECK_VALUE(t.first->sizes() == q_.sizes(), "window_bwd: ", t.second, " must have q's shape");
   }
+  same_device(q_, rest_, "rest");
+  check_dtype(rest_, q_.scalar_type(), "rest");
+  if (rest_)
+    TORCH_CHECK_VALUE(rest_->sizes() == o_.sizes() && rest_->strides() == o_.strides(),
+                      "window_bwd: rest must have o's shape and strides");
   same_device(q_, lse_, "lse");
   check_dtype(lse_, at::kFloat, "lse");
   TORCH_CHECK_VALUE(lse_.numel() == s.B * s.Hq * s.Sq, "window_bwd: lse must be [B, Hq, Sq]");
   const c10::DeviceGuard guard(q_.device());
   const Tensor q = win_rows(q_), k = win_rows(k_), v = win_rows(v_), o = win_rows(o_), d = win_rows(do_);
+  const OptT rest = rest_ ? OptT(win_rows(*rest_)) : OptT();
+  if (rest)
+    for (int x = 0; x < 4; ++x)
+      TORCH_CHECK(rest->stride(x) == o.stride(x), "window_bwd: rest must be laid out like o");
   const Tensor lse = lse_.contiguous();
   const OptT q_lens = cont(q_lens_), kv_lens = cont(kv_lens_);
   Tensor dq = win_like(q_), dk = win_like(k_), dv = win_like(v_);
@@ -271,7 +282,7 @@ std::tuple<Tensor, Tensor, Tensor> window_bwd(const Tensor& do_, const Tensor& q
   Tensor rows = at::empty({2 * s.B * s.Hq * s.Sq}, opts(q, at::kFloat));
   Tensor acc = floats ? at::empty({floats}, opts(q, at::kFloat)) : none_like(q);
   PRISM_TORCH_CALL(prism_window_bwd, d.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                   lse.data_ptr<float>(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st, window, sinks, causal,
+                   p(rest), lse.data_ptr<float>(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st, window, sinks, causal,
                    (const int32_t*)p(q_lens), (const int32_t*)p(kv_lens), (float)sm_scale, dq.data_ptr(), dk.data_ptr(),
                    dv.data_ptr(), rows.data_ptr<float>(), floats ? acc.data_ptr<float>() : nullptr, stream_of(q));
   return {dq, dk, dv};
@@ -408,41 +419,44 @@ std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const OptT& k, const
 
 struct WindowGrad : torch::autograd::Function<WindowGrad> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, int64_t window,
-                               int64_t sinks, bool causal, const OptT& q_lens, const OptT& kv_lens, double sm_scale) {
+                               int64_t sinks, bool causal, const OptT& q_lens, const OptT& kv_lens, double sm_scale,
+                               bool want_rest) {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->set_materialize_grads(false);
-    auto [o, lse] = PRISM_OP(window_fwd).call(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, true);
-    ctx->save_for_backward({q, k, v, o, lse, q_lens ? *q_lens : Tensor(), kv_lens ? *kv_lens : Tensor()});
+    const bool use = prism_window_rest(k.size(2), window, sinks, causal), keep = use || want_rest;
+    auto [o, lse, rest] = PRISM_OP(window_fwd).call(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, true, keep);
+    ctx->save_for_backward({q, k, v, o, lse, q_lens ? *q_lens : Tensor(), kv_lens ? *kv_lens : Tensor(),
+                            use ? rest : Tensor()});
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["sm_scale"] = sm_scale;
-    ctx->mark_non_differentiable({lse});
-    return {o, lse};
+    ctx->mark_non_differentiable({lse, rest});
+    return {o, lse, rest};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    if (!g[0].defined()) return variable_list(9);
+    if (!g[0].defined()) return variable_list(10);
     const variable_list s = ctx->get_saved_variables();
     const auto [dq, dk, dv] = [&] {
       at::AutoDispatchBelowADInplaceOrView guard;
-      return PRISM_OP(window_bwd).call(g[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["window"].toInt(),
+      return PRISM_OP(window_bwd).call(g[0], s[0], s[1], s[2], s[3], opt(s[7]), s[4], ctx->saved_data["window"].toInt(),
                         ctx->saved_data["sinks"].toInt(), ctx->saved_data["causal"].toBool(), opt(s[5]), opt(s[6]),
                         ctx->saved_data["sm_scale"].toDouble());
     }();
-    variable_list out(9);
+    variable_list out(10);
     out[0] = dq; out[1] = dk; out[2] = dv;
     return once(std::move(out));
   }
 };
-std::tuple<Tensor, Tensor> window_autograd(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window,
+std::tuple<Tensor, Tensor, Tensor> window_autograd(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window,
                                            int64_t sinks, bool causal, const OptT& q_lens, const OptT& kv_lens,
-                                           double sm_scale, bool want_lse) {
+                                           double sm_scale, bool want_lse, bool want_rest) {
   if (!grads_wanted(q, k, v)) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    return PRISM_OP(window_fwd).call(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse);
+    return PRISM_OP(window_fwd).call(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse, want_rest);
   }
-  const variable_list o = WindowGrad::apply(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale);
-  return {o[0], o[1]};
+  const variable_list o = WindowGrad::apply(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_rest);
+  return {o[0], o[1], o[2]};
 }
 
 }  // namespace
@@ -454,8 +468,8 @@ TORCH_LIBRARY_FRAGMENT(prism, m) {
   m.def("rotary(Tensor q, Tensor? k, Tensor freqs, Tensor positions, int[] axis_pairs, bool interleaved, "
         "float amplitude, bool inverse) -> (Tensor, Tensor)");
   m.def("window_fwd(Tensor q, Tensor k, Tensor v, int window, int sinks, bool causal, Tensor? q_lens, "
-        "Tensor? kv_lens, float sm_scale, bool want_lse) -> (Tensor, Tensor)");
-  m.def("window_bwd(Tensor do, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, int window, int sinks, bool causal, "
+        "Tensor? kv_lens, float sm_scale, bool want_lse, bool want_rest) -> (Tensor, Tensor, Tensor)");
+  m.def("window_bwd(Tensor do, Tensor q, Tensor k, Tensor v, Tensor o, Tensor? rest, Tensor lse, int window, int sinks, bool causal, "
         "Tensor? q_lens, Tensor? kv_lens, float sm_scale) -> (Tensor, Tensor, Tensor)");
 }
 

@@ -69,6 +69,7 @@ struct WinArgs {
   int B, Hk, G, Sq, Sk;
   int window, sinks, causal;
   float scale, scale_log2;
+  uint16_t* rest;                   // what o's rounding left off, at o's strides (win_store_o); or null
   float* lse;                       // [B, Hk G, Sq] natural log, -inf for rows that see nothing; or null
   int tiles;                        // row tiles of a (sequence, key head)
   int total;                        // row tiles of the launch
@@ -382,7 +383,49 @@ __device__ __forceinline__ void win_careful(const WinArgs& a, const KeyList& kl,
   }
 }
 
+// ------------------------------------------------------------ output
+// Lanes l and l + 32 hold channels 8 j + 0 .. 3 and 8 j + 4 .. 7 of the same row (u for
+// block j, v for j + 1, packed): all of block j for the lower half, of j + 1 for the
+// upper, so that a lane stores 16 bytes (2 x 4,096 tokens, 16 heads over 4, D = 64,
+// window 1,024: forward 55 -> 52 us, against stores of 8).
+__device__ __forceinline__ uint4 win_join_halves(uint2 u, uint2 v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(u.x, v.x, false, false);
+  const auto y = __builtin_amdgcn_permlane32_swap(u.y, v.y, false, false);
+  return make_uint4(x[0], y[0], x[1], y[1]);
+}
+template <class E>
+__device__ __forceinline__ uint2 win_pack4(float4 x) {
+  return make_uint2(E::pack(x.x, x.y), E::pack(x.z, x.w));
+}
+// blocks j (x) and j + 1 (y) of a row whose block j begins at p; both halves of the wave
+template <class E>
+__device__ __forceinline__ void win_store(uint16_t* p, int g, float4 x, float4 y) {
+  *reinterpret_cast<uint4*>(p + 8 * g) = win_join_halves(win_pack4<E>(x), win_pack4<E>(y));
+}
+// what rounding to u leaves off x
+template <class E>
+__device__ __forceinline__ float4 win_left(float4 x, uint2 u) {
+  return make_float4(x.x - E::lo(u.x), x.y - E::hi(u.x), x.z - E::lo(u.y), x.w - E::hi(u.y));
+}
+// the same for o at element `at`, and its rest where the call asks for it
+template <class E>
+__device__ __forceinline__ void win_store_o(const WinArgs& a, int64_t at, int g, float4 x, float4 y) {
+  const uint2 u = win_pack4<E>(x), v = win_pack4<E>(y);
+  *reinterpret_cast<uint4*>(a.o.p + at + 8 * g) = win_join_halves(u, v);
+  if (a.rest) win_store<E>(a.rest + at, g, win_left<E>(x, u), win_left<E>(y, v));
+}
+__device__ __forceinline__ float4 win_scaled(f32x16 v, int j, float f) {
+  return make_float4(v[4 * j] * f, v[4 * j + 1] * f, v[4 * j + 2] * f, v[4 * j + 3] * f);
+}
+__device__ __forceinline__ float4 win_scaled(float4 v, float f) { return make_float4(v.x * f, v.y * f, v.z * f, v.w * f); }
+
 // ------------------------------------------------------------ host side (window_fwd.hip)
+// Whether rows see so few keys that the backward forms delta from P and dP
+// (window_dq_kernel): it needs neither o nor its rest then
+inline bool win_few(int64_t Sk, int64_t window, int64_t sinks, int causal) {
+  const int64_t near = window < Sk ? window : Sk, keys = (causal ? near : 2 * near - 1) + (sinks < Sk ? sinks : Sk);
+  return (keys < Sk ? keys : Sk) <= 64;
+}
 // PRISM_OK if the sizes, strides (3 per tensor) and pointers are what the kernels assume
 int win_check(const char* name, int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window,
               int64_t sinks, float sm_scale, const int64_t* strides, int tensors,

@@ -6,10 +6,11 @@
 // window_dq_kernel, by 128 rows, over the key list of the forward: S^T and dP^T
 // keep one query per lane column, dQ^T += K^T dS^T.  It also forms delta and
 // leaves (m2, delta) = (lse log2 e, delta) of every row for the second kernel: from the
-// rows of o and do that it holds, or, where rows see 64 keys at most, as sum_j P_j
-// dP_j in a pass over the tiles before.  o is stored rounded, and the fewer keys the
-// larger delta's error so is beside dS: dq off by 3.0e-3 (norm-wise, bf16, rows that
-// see 1 to 5 keys), 2.6e-3 (8), 2.4e-3 (64), with the pass 2.3e-3, 2.3e-3, 2.4e-3.
+// rows of do, o and o's rest (what its rounding left off, kept by the forward: with
+// the rounded o alone dq is 2.6e-3 off, norm-wise, bf16, with its rest 2.4e-3; of 235
+// us of a step of 2 x 4,096 tokens at D = 64 writing and reading it take 7), or, where rows see 64 keys at most, as sum_j P_j dP_j in a pass over
+// the tiles before (the fewer keys the larger delta's error beside dS: 3.0e-3 from the
+// rounded o for rows that see 1 to 5 keys, 2.3e-3 with the pass).
 // The pass costs no more than reading o: 14,040 tokens, 40 heads over 8, window 64,
 // D = 128: 200 us with it, 240 without; 2 x 4,001 tokens, window 60 and 4 sinks 52 / 51.
 // window_dkdv_kernel, by 128 keys (64 at D = 64), over the tokens that see them,
@@ -102,12 +103,24 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_dq_kernel(WinBwdA
   {
     const uint16_t* qp = a.q.p + b * a.q.b + head * a.q.h + i * a.q.s + 8 * g;
     const uint16_t* dp = ba.do_.p + b * ba.do_.b + head * ba.do_.h + i * ba.do_.s + 8 * g;
-    const uint16_t* op = a.o.p + b * a.o.b + head * a.o.h + i * a.o.s + 8 * g;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       qf[s] = ld_bf16x8(qp + 16 * s);
       df[s] = ld_bf16x8(dp + 16 * s);
-      if (!ba.exact) dlt = dot8<E>(ld_bf16x8(op + 16 * s), df[s], dlt);
+    }
+    if (!ba.exact) {  // (all loads of a branch before the first sum that waits for one)
+      const int64_t at = b * a.o.b + head * a.o.h + i * a.o.s + 8 * g;
+      bf16x8 of[NS], rf[NS];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) of[s] = ld_bf16x8(a.o.p + at + 16 * s);
+      if (a.rest) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) rf[s] = ld_bf16x8(a.rest + at + 16 * s);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) dlt = dot8<E>(rf[s], df[s], dlt);
+      }
+#pragma unroll
+      for (int s = 0; s < NS; ++s) dlt = dot8<E>(of[s], df[s], dlt);
     }
   }
   const float lse = a.lse[lrow];
@@ -256,12 +269,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_dq_kernel(WinBwdA
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-    for (int jj = 0; jj < 4; ++jj) {
-      uint2 o;
-      o.x = E::pack(dq[dt][4 * jj + 0] * a.scale, dq[dt][4 * jj + 1] * a.scale);
-      o.y = E::pack(dq[dt][4 * jj + 2] * a.scale, dq[dt][4 * jj + 3] * a.scale);
-      *reinterpret_cast<uint2*>(dqr + 32 * dt + 8 * jj + 4 * g) = o;
-    }
+    for (int jj = 0; jj < 4; jj += 2)
+      win_store<E>(dqr + 32 * dt + 8 * jj, g, win_scaled(dq[dt], jj, a.scale), win_scaled(dq[dt], jj + 1, a.scale));
 }
 
 // ------------------------------------------------------------ dK / dV
@@ -635,14 +644,9 @@ __global__ __launch_bounds__(DkdvTiles<D>::THREADS, D == 64 ? 3 : 1) void window
     }
     if (key >= a.Sk) continue;
 #pragma unroll
-    for (int jj = 0; jj < 4; ++jj) {
-      uint2 o;
-      o.x = E::pack(dk[dt][4 * jj + 0] * a.scale, dk[dt][4 * jj + 1] * a.scale);
-      o.y = E::pack(dk[dt][4 * jj + 2] * a.scale, dk[dt][4 * jj + 3] * a.scale);
-      *reinterpret_cast<uint2*>(dkr + 32 * dt + 8 * jj + 4 * g) = o;
-      o.x = E::pack(dv[dt][4 * jj + 0], dv[dt][4 * jj + 1]);
-      o.y = E::pack(dv[dt][4 * jj + 2], dv[dt][4 * jj + 3]);
-      *reinterpret_cast<uint2*>(dvr + 32 * dt + 8 * jj + 4 * g) = o;
+    for (int jj = 0; jj < 4; jj += 2) {
+      win_store<E>(dkr + 32 * dt + 8 * jj, g, win_scaled(dk[dt], jj, a.scale), win_scaled(dk[dt], jj + 1, a.scale));
+      win_store<E>(dvr + 32 * dt + 8 * jj, g, win_scaled(dv[dt], jj, 1.0f), win_scaled(dv[dt], jj + 1, 1.0f));
     }
   }
 }
@@ -672,14 +676,9 @@ __global__ __launch_bounds__(256) void window_dq_merge_kernel(WinBwdArgs ba) {
       acc[j].w += v.w;
     }
   const int i = r / a.G, head = it.hk * a.G + (r - i * a.G);
-  uint16_t* out = ba.dq.p + it.b * ba.dq.b + head * ba.dq.h + i * ba.dq.s + 32 * dt + 4 * g;
+  uint16_t* out = ba.dq.p + it.b * ba.dq.b + head * ba.dq.h + i * ba.dq.s + 32 * dt;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint2 u;
-    u.x = E::pack(acc[j].x * a.scale, acc[j].y * a.scale);
-    u.y = E::pack(acc[j].z * a.scale, acc[j].w * a.scale);
-    *reinterpret_cast<uint2*>(out + 8 * j) = u;
-  }
+  for (int j = 0; j < 4; j += 2) win_store<E>(out + 8 * j, g, win_scaled(acc[j], a.scale), win_scaled(acc[j + 1], a.scale));
 }
 
 // the pieces' sums of the cut key tiles (cut_sinks sink tiles, then the rest's),
@@ -721,14 +720,9 @@ __global__ __launch_bounds__(128 * key_tiles_of(D)) void window_merge_kernel(Win
   const bool isk = blk < NDT;
   const WinTensor& t = isk ? a.dk : a.dv;
   const float f = isk ? a.w.scale : 1.0f;
-  uint16_t* out = t.p + b * t.b + hk * t.h + key * t.s + 32 * (isk ? blk : blk - NDT) + 4 * g;
+  uint16_t* out = t.p + b * t.b + hk * t.h + key * t.s + 32 * (isk ? blk : blk - NDT);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint2 u;
-    u.x = E::pack(acc[j].x * f, acc[j].y * f);
-    u.y = E::pack(acc[j].z * f, acc[j].w * f);
-    *reinterpret_cast<uint2*>(out + 8 * j) = u;
-  }
+  for (int j = 0; j < 4; j += 2) win_store<E>(out + 8 * j, g, win_scaled(acc[j], f), win_scaled(acc[j + 1], f));
 }
 
 // workgroups of window_dq_kernel that the chip holds: two a CU at D = 128, three
@@ -800,12 +794,12 @@ int prism_window_bwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, 
   return PRISM_OK;
 }
 
-int prism_window_bwd(const void* do_, const void* q, const void* k, const void* v, const void* o, const float* lse,
-                     int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, const int64_t* strides,
+int prism_window_bwd(const void* do_, const void* q, const void* k, const void* v, const void* o, const void* rest,
+                     const float* lse, int dtype, int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, const int64_t* strides,
                      int64_t window, int64_t sinks, int causal, const int32_t* q_lens, const int32_t* kv_lens,
                      float sm_scale, void* dq, void* dk, void* dv, float* rows, float* acc, hipStream_t stream) {
   if (const int rc = win_check("prism_window_bwd", dtype, B, Hq, Hk, Sq, Sk, D, window, sinks, sm_scale, strides, 8,
-                               {q, k, v, o, do_, dq, dk, dv, acc}))
+                               {q, k, v, o, rest, do_, dq, dk, dv, acc}))
     return rc;
   if (B == 0) return PRISM_OK;
   PRISM_REQUIRE(Sq == 0 || (q && o && do_ && lse && dq && rows), "prism_window_bwd: null pointer");
@@ -813,6 +807,7 @@ int prism_window_bwd(const void* do_, const void* q, const void* k, const void* 
   WinBwdArgs a{};
   a.w = win_args(q, k, v, (void*)o, B, Hq, Hk, Sq, Sk, strides, window, sinks, causal, q_lens, kv_lens, sm_scale);
   a.w.lse = (float*)lse;
+  a.w.rest = (uint16_t*)rest;
   const int64_t* s = strides + 12;
   a.do_ = {(uint16_t*)do_, s[0], s[1], s[2]};
   a.dq = {(uint16_t*)dq, s[3], s[4], s[5]};
@@ -831,8 +826,7 @@ int prism_window_bwd(const void* do_, const void* q, const void* k, const void* 
   a.w.whole = (int)c.whole; a.w.splits = (int)c.splits; a.w.items = (int)items;
   a.w.ranked = win_ranked(q_lens, B, a.w.tiles, total, dq_slots(D));
   a.ranked = win_ranked(kv_lens, B, p.key_tiles, p.rest_tiles, key_slots(D));
-  const int64_t near = window < Sk ? window : Sk, keys = (causal ? near : 2 * near - 1) + (sinks < Sk ? sinks : Sk);
-  a.exact = cut == 0 && (keys < Sk ? keys : Sk) <= 64;
+  a.exact = cut == 0 && win_few(Sk, window, sinks, causal);
   a.w.part = acc + p.pieces * 128 * key_tiles_of(D) * D;
   a.sink_tiles = (int)p.sink_tiles; a.key_tiles = (int)p.key_tiles;
   a.sink_splits = (int)p.sink_splits; a.sink_items = (int)p.sink_items;

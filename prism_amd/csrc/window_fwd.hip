@@ -195,16 +195,12 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void window_fwd_kernel(WinArg
   }
   if (r >= rows) return;
   const float inv = 1.0f / l;
-  uint16_t* op = a.o.p + b * a.o.b + head * a.o.h + i * a.o.s;
+  const int64_t at = b * a.o.b + head * a.o.h + i * a.o.s;
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint2 u;
-      u.x = E::pack(acc_o[dt][4 * j + 0] * inv, acc_o[dt][4 * j + 1] * inv);
-      u.y = E::pack(acc_o[dt][4 * j + 2] * inv, acc_o[dt][4 * j + 3] * inv);
-      *reinterpret_cast<uint2*>(op + 32 * dt + 8 * j + 4 * g) = u;
-    }
+    for (int j = 0; j < 4; j += 2)
+      win_store_o<E>(a, at + 32 * dt + 8 * j, g, win_scaled(acc_o[dt], j, inv), win_scaled(acc_o[dt], j + 1, inv));
   if (a.lse && g == 0)
     a.lse[((int64_t)b * a.Hk * a.G + head) * a.Sq + i] = (m + __log2f(l)) * 0.6931471805599453f;
 }
@@ -246,14 +242,9 @@ __global__ __launch_bounds__(256) void window_fwd_join_kernel(WinArgs a) {
   const bool none = top == NINF && l == 0.0f;
   const float inv = none ? 0.0f : 1.0f / l;
   const int i = r / a.G, head = it.hk * a.G + (r - i * a.G);
-  uint16_t* op = a.o.p + it.b * a.o.b + head * a.o.h + i * a.o.s + 32 * dt + 4 * g;
+  const int64_t at = it.b * a.o.b + head * a.o.h + i * a.o.s + 32 * dt;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint2 u;
-    u.x = E::pack(o[j].x * inv, o[j].y * inv);
-    u.y = E::pack(o[j].z * inv, o[j].w * inv);
-    *reinterpret_cast<uint2*>(op + 8 * j) = u;
-  }
+  for (int j = 0; j < 4; j += 2) win_store_o<E>(a, at + 8 * j, g, win_scaled(o[j], inv), win_scaled(o[j + 1], inv));
   if (a.lse && g == 0 && dt == 0)
     a.lse[((int64_t)it.b * a.Hk * a.G + head) * a.Sq + i] = none ? NINF : (top + __log2f(l)) * 0.6931471805599453f;
 }
@@ -324,17 +315,20 @@ int prism_window_fwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, 
   return PRISM_OK;
 }
 
+int prism_window_rest(int64_t Sk, int64_t window, int64_t sinks, int causal) { return !win_few(Sk, window, sinks, causal); }
+
 int prism_window_fwd(const void* q, const void* k, const void* v, int dtype, int B, int Hq, int Hk, int64_t Sq,
                      int64_t Sk, int D, const int64_t* strides, int64_t window, int64_t sinks, int causal,
-                     const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, float* lse, float* part,
-                     hipStream_t stream) {
+                     const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, void* rest, float* lse,
+                     float* part, hipStream_t stream) {
   if (const int rc = win_check("prism_window_fwd", dtype, B, Hq, Hk, Sq, Sk, D, window, sinks, sm_scale, strides, 4,
-                               {q, k, v, o, part}))
+                               {q, k, v, o, rest, part}))
     return rc;
   if (B == 0 || Sq == 0) return PRISM_OK;
   PRISM_REQUIRE(q && o && (Sk == 0 || (k && v)), "prism_window_fwd: null pointer");
   WinArgs a = win_args(q, k, v, o, B, Hq, Hk, Sq, Sk, strides, window, sinks, causal, q_lens, kv_lens, sm_scale);
   a.lse = lse;
+  a.rest = (uint16_t*)rest;
   a.tiles = (int)((Sq * a.G + 127) / 128);
   const int64_t total = (int64_t)B * Hk * a.tiles;
   const WinCut c = win_row_cut(fwd_slots(D), B, Hk, a.G, Sq, Sk, D, window, sinks, causal);

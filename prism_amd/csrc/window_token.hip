@@ -246,17 +246,16 @@ __global__ __launch_bounds__(256, 1) void window_token_kernel(WinArgs a) {
   }
   if (r >= rows) return;
 #pragma unroll
-  for (int x = 0; x < QR; x += 4) {
-    const int reg = w * QR + x, d = 32 * (reg >> 4) + 8 * ((reg & 15) >> 2) + 4 * g;
+  for (int x = 0; x < QR; x += 8) {
+    const int reg = w * QR + x, d = 32 * (reg >> 4) + 8 * ((reg & 15) >> 2);
+    const float4 u = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]), v = make_float4(o[x + 4], o[x + 5], o[x + 6], o[x + 7]);
     if (a.splits == 1) {
       const float inv = lt > 0.0f || lt != lt ? 1.0f / lt : 0.0f;
-      uint2 u;
-      u.x = E::pack(o[x] * inv, o[x + 1] * inv);
-      u.y = E::pack(o[x + 2] * inv, o[x + 3] * inv);
-      *reinterpret_cast<uint2*>(a.o.p + b * a.o.b + head * a.o.h + i * a.o.s + d) = u;
+      win_store_o<E>(a, b * a.o.b + head * a.o.h + i * a.o.s + d, g, win_scaled(u, inv), win_scaled(v, inv));
     } else {
-      const int64_t at = ((int64_t)split * a.total + id) * 32 + l32;
-      *reinterpret_cast<float4*>(a.part + at * D + d) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+      float* at = a.part + (((int64_t)split * a.total + id) * 32 + l32) * D + d + 4 * g;
+      *reinterpret_cast<float4*>(at) = u;
+      *reinterpret_cast<float4*>(at + 8) = v;
     }
   }
   if (w == 0 && g == 0) {
@@ -301,10 +300,14 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinArgs a) {
     }
   }
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  uint16_t* op = a.o.p + b * a.o.b + head * a.o.h + i * a.o.s + C * lane;
+  const int64_t at = b * a.o.b + head * a.o.h + i * a.o.s + C * lane;
+  auto put = [&](uint16_t* to, uint32_t u) {
+    if constexpr (C > 1) *reinterpret_cast<uint32_t*>(to + at) = u;
+    else to[at] = (uint16_t)u;
+  };
   const uint32_t u = E::pack(o[0] * inv, o[1] * inv);
-  if constexpr (C > 1) *reinterpret_cast<uint32_t*>(op) = u;
-  else *op = (uint16_t)u;
+  put(a.o.p, u);
+  if (a.rest) put(a.rest, E::pack(o[0] * inv - E::lo(u), o[1] * inv - E::hi(u)));
   if (a.lse && lane == 0)
     a.lse[((int64_t)b * a.Hk * a.G + head) * a.Sq + i] =
         l > 0.0f || l != l ? (top + __log2f(l)) * 0.6931471805599453f : NINF;
@@ -355,15 +358,18 @@ int prism_window_token_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int64
 
 int prism_window_token(const void* q, const void* k, const void* v, int dtype, int B, int Hq, int Hk, int64_t Sq,
                        int64_t Sk, int D, const int64_t* strides, int64_t window, int64_t sinks, int causal,
-                       const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, float* lse, int splits,
-                       float* part_o, float* part_ml, hipStream_t stream) {
-  if (const int rc = win_check("prism_window_token", dtype, B, Hq, Hk, Sq, Sk, D, window, sinks, sm_scale, strides, 4, {q, k, v, o})) return rc;
+                       const int32_t* q_lens, const int32_t* kv_lens, float sm_scale, void* o, void* rest, float* lse,
+                       int splits, float* part_o, float* part_ml, hipStream_t stream) {
+  if (const int rc = win_check("prism_window_token", dtype, B, Hq, Hk, Sq, Sk, D, window, sinks, sm_scale, strides, 4,
+                               {q, k, v, o, rest}))
+    return rc;
   if (B == 0 || Sq == 0) return PRISM_OK;
   PRISM_REQUIRE(q && o && (Sk == 0 || (k && v)), "prism_window_token: null pointer");
   PRISM_REQUIRE(splits >= 1 && splits <= kMaxSplits && (splits == 1 || (part_o && part_ml)),
                 "prism_window_token: bad splits or workspace");
   WinArgs a = win_args(q, k, v, o, B, Hq, Hk, Sq, Sk, strides, window, sinks, causal, q_lens, kv_lens, sm_scale);
   a.lse = lse;
+  a.rest = (uint16_t*)rest;
   a.tiles = (int)((Sq * a.G + 31) / 32);
   const int64_t items = (int64_t)B * Hk * a.tiles;
   PRISM_REQUIRE(items * splits < (1ll << 31) && items < (1ll << 28), "prism_window_token: too many row tiles");

@@ -211,20 +211,21 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, posi
 
 
 def window_fwd(q, k, v, window: int, sinks: int, causal: bool, q_lens: Optional[torch.Tensor],
-               kv_lens: Optional[torch.Tensor], sm_scale: float, want_lse: bool):
+               kv_lens: Optional[torch.Tensor], sm_scale: float, want_lse: bool, want_rest: bool = False):
     """(o [B,Hq,Sq,D], lse [B,Hq,Sq] fp32 or None) of attention over a window and
-    sinks.  Differentiable (o in q, k, v)."""
+    sinks, with want_rest also what o's rounding left off (o's shape, dtype and
+    layout).  Differentiable (o in q, k, v)."""
     _cuda(q, k, v, q_lens, kv_lens)
-    o, lse = _op("window_fwd", q, k, v, int(window), int(sinks), bool(causal), q_lens, kv_lens, float(sm_scale),
-                 bool(want_lse))
-    return o, (lse if want_lse else None)
+    o, lse, rest = _op("window_fwd", q, k, v, int(window), int(sinks), bool(causal), q_lens, kv_lens, float(sm_scale),
+                       bool(want_lse), bool(want_rest))
+    return (o, (lse if want_lse else None), rest) if want_rest else (o, (lse if want_lse else None))
 
 
-def window_bwd(do, q, k, v, o, lse, window: int, sinks: int, causal: bool, q_lens: Optional[torch.Tensor],
-               kv_lens: Optional[torch.Tensor], sm_scale: float):
-    """(dq, dk, dv) of window_fwd."""
-    _cuda(do, q, k, v, o, lse, q_lens, kv_lens)
-    return _op("window_bwd", do, q, k, v, o, lse, int(window), int(sinks), bool(causal), q_lens, kv_lens,
+def window_bwd(do, q, k, v, o, rest: Optional[torch.Tensor], lse, window: int, sinks: int, causal: bool,
+               q_lens: Optional[torch.Tensor], kv_lens: Optional[torch.Tensor], sm_scale: float):
+    """(dq, dk, dv) of window_fwd; rest: its rest, or None (delta then from the rounded o)."""
+    _cuda(do, q, k, v, o, rest, lse, q_lens, kv_lens)
+    return _op("window_bwd", do, q, k, v, o, rest, lse, int(window), int(sinks), bool(causal), q_lens, kv_lens,
                float(sm_scale))
 
 

@@ -171,6 +171,34 @@ def test_few_keys_with_a_common_part(case, dt):
         check(q, k, v + 64, do, window, sinks=sinks, causal=causal, kv_lens=n, q_lens=n if Sq == Sk else None, few=True)
 
 
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("case", [(2, 300, 300, 4, 2, 64, 100, 0, True), (1, 130, 900, 2, 2, 128, None, 0, True),
+                                  (1, 3, 2000, 8, 2, 64, 500, 9, True), (2, 1, 70, 4, 1, 128, None, 0, True),
+                                  (1, 300, 300, 40, 1, 128, 66, 4, False), (1, 1300, 1300, 2, 1, 128, 700, 150, False)],
+                         ids=lambda c: "-".join(str(x) for x in c))
+def test_rest_of_the_rounding(case, dt):
+    """o + rest is o unrounded: off by the products' roundings only where P is exact
+    (equal scores of a power of two of keys), and what o stands for elsewhere."""
+    B, Sq, Sk, Hq, Hk, D, window, sinks, causal = case
+    q, k, v = make(B, Sq, Sk, Hq, Hk, D, DT[dt], seed=Sq + Sk)
+    w = 1 << 29 if window is None else window
+    o, lse, rest = prism_amd.ops.window_fwd(q, k, v, w, sinks, causal, None, None, D ** -0.5, True, True)
+    o2, lse2 = prism_amd.ops.window_fwd(q, k, v, w, sinks, causal, None, None, D ** -0.5, True)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2) and rest.stride() == o.stride() and rest.dtype == o.dtype
+    u = torch.finfo(o.dtype).eps / 2
+    assert (rest.float().abs() <= u * o.float().abs() * (1 + u) + 2.0 ** -25).all()
+    # equal scores: o is the mean of the seen values, P = 1 exactly
+    flat = torch.zeros_like(q)
+    o, _, rest = prism_amd.ops.window_fwd(flat, k, v, w, sinks, causal, None, None, D ** -0.5, False, True)
+    m = seen_mask(B, Sq, Sk, window, sinks, causal, None, None)[:, None].double()
+    n = m.sum(-1, keepdim=True)
+    mean = (m @ v.double().repeat_interleave(Hq // Hk, 1)) / n.clamp(min=1)
+    size = (m @ v.double().abs().repeat_interleave(Hq // Hk, 1)) / n.clamp(min=1)
+    # fp32 sums of n terms, the division, rest's own rounding (fp16: its subnormal step)
+    tol = (n + 4) * 2.0 ** -24 * size + u * u * mean.abs() * 1.01 + 2.0 ** -25 * (dt == "fp16")
+    assert ((o.double() + rest.double() - mean).abs() <= tol).all()
+
+
 RAGGED = [  # B, S, Hq, Hk, D, window, sinks, causal: a round or two of tiles, sequences of their own lengths
     (5, 1000, 8, 4, 64, 200, 70, True), (5, 1000, 7, 7, 128, 300, 4, False), (3, 1000, 16, 2, 128, 300, 0, True),
     (64, 100, 8, 8, 64, 30, 4, True), (65, 100, 8, 8, 64, 30, 4, True), (33, 130, 9, 9, 128, None, 0, True),
@@ -234,8 +262,10 @@ def test_empty():
 def test_opcheck():
     q, k, v = make(1, 70, 70, 2, 1, 64, torch.bfloat16)
     n = torch.tensor([50], dtype=torch.int32, device="cuda")
-    torch.library.opcheck(torch.ops.prism.window_fwd.default, (q, k, v, 9, 2, True, n, n, 0.1, True),
+    torch.library.opcheck(torch.ops.prism.window_fwd.default, (q, k, v, 9, 2, True, n, n, 0.1, True, True),
                           test_utils=("test_schema", "test_faketensor"))
-    o, lse = torch.ops.prism.window_fwd(q, k, v, 9, 2, True, n, n, 0.1, True)
-    torch.library.opcheck(torch.ops.prism.window_bwd.default, (q, q, k, v, o, lse, 9, 2, True, n, None, 0.1),
+    torch.library.opcheck(torch.ops.prism.window_fwd.default, (q, k, v, 9, 2, True, n, n, 0.1, False, False),
+                          test_utils=("test_schema", "test_faketensor"))
+    o, lse, rest = torch.ops.prism.window_fwd(q, k, v, 9, 2, True, n, n, 0.1, True, True)
+    torch.library.opcheck(torch.ops.prism.window_bwd.default, (q, q, k, v, o, rest, lse, 9, 2, True, n, None, 0.1),
                           test_utils=("test_schema", "test_faketensor"))

@@ -140,7 +140,7 @@ def test_window_capi_refusals():
     def fwd(dtype=1, B=1, Hq=4, Hk=2, Sq=5, Sk=9, D=64, window=3, sinks=0, scale=0.1, stride=64, p=one):
         st = (ctypes.c_int64 * 12)(*[stride] * 12)
         return lib.prism_window_fwd(p, one, one, dtype, B, Hq, Hk, Sq, Sk, D, st, window, sinks, 1, None, None, scale, one,
-                                    None, one, None)
+                                    None, None, one, None)
 
     for bad in (dict(dtype=0), dict(Hk=3), dict(Hk=0), dict(D=32), dict(window=0), dict(sinks=-1), dict(scale=0.0),
                 dict(stride=65), dict(stride=1 << 24), dict(stride=-64), dict(p=None), dict(p=ctypes.c_void_p(8)),
@@ -149,10 +149,10 @@ def test_window_capi_refusals():
     assert fwd(B=0) == 0
     st = (ctypes.c_int64 * 24)(*[64] * 24)
     token = lambda splits, ws: lib.prism_window_token(  # noqa: E731
-        one, one, one, 1, 1, 4, 2, 1, 9, 64, st, 3, 0, 1, None, None, 0.1, one, None, splits, ws, ws, None)
+        one, one, one, 1, 1, 4, 2, 1, 9, 64, st, 3, 0, 1, None, None, 0.1, one, None, None, splits, ws, ws, None)
     assert [token(0, one), token(257, one), token(2, None)] == [1, 1, 1]
     bwd = lambda lse, rows: lib.prism_window_bwd(  # noqa: E731
-        one, one, one, one, one, lse, 1, 1, 4, 2, 5, 9, 64, st, 3, 0, 1, None, None, 0.1, one, one, one, rows, None, None)
+        one, one, one, one, one, None, lse, 1, 1, 4, 2, 5, 9, 64, st, 3, 0, 1, None, None, 0.1, one, one, one, rows, None, None)
     assert [bwd(None, one), bwd(one, None)] == [1, 1]
 
 
@@ -222,5 +222,10 @@ def test_window_plans_with_every_key_a_sink():
         assert lib.prism_window_bwd_plan(2, 8, 2, 900, 5000, 64, window, sinks, 1, 1, ctypes.byref(c)) == 0
         return splits.value, a.value, b.value, c.value
 
+    # few keys: the backward needs nothing of o's rounding
+    assert [lib.prism_window_rest(*a) for a in ((5000, 64, 0, 1), (5000, 60, 4, 1), (64, far, far, 0), (5000, 32, 1, 0),
+                                                (0, 5, 0, 1))] == [0] * 5
+    assert [lib.prism_window_rest(*a) for a in ((5000, 65, 0, 1), (5000, 60, 5, 1), (65, far, 0, 1), (5000, 33, 0, 0),
+                                                (5000, 1, far, 1))] == [1] * 5
     assert plans(far, far) == plans(5000, 5000)
     assert plans(100, far) == plans(100, 5000)
