@@ -314,7 +314,8 @@ void check_captured(const OptT& t) {
   const auto s = node->stream();
   TORCH_CHECK(!s || s->id() != 0,
               "prism: an input that requires gradients is still held by a graph of eager calls on the default stream; "
-              "free that graph (its outputs and losses), or pass a new leaf, before capturing");
+              "free that graph (its outputs and losses) or pass a new leaf before capturing, or capture under "
+              "torch.no_grad()");
 }
 template <class... T>
 bool grads_wanted(const Tensor& first, const T&... t) {
