@@ -98,24 +98,24 @@ def _register_fakes():
 
     @reg("prism::rms_norm")
     def _(x, residual, weight, eps, out_code, want_inv):
-        return (_empty(x, x.shape, {3: f8, 4: i8}.get(out_code, x.dtype)),
-                _empty(x, x.shape, x.dtype) if residual is not None else _none(x),
-                _empty(x, x.shape[:-1], f32) if out_code >= 3 else _none(x),
-                _empty(x, (x.numel() // x.shape[-1],), f32) if want_inv else _none(x))
+        return ([_empty(x, x.shape, {3: f8, 4: i8}.get(out_code, x.dtype))]
+                + ([_empty(x, x.shape, x.dtype)] if residual is not None else [])
+                + ([_empty(x, x.shape[:-1], f32)] if out_code >= 3 else [])
+                + ([_empty(x, (x.numel() // x.shape[-1],), f32)] if want_inv else []))
 
     @reg("prism::rms_norm_bwd")
     def _(dy, dh, h, weight, inv, want_dw):
-        return _empty(h, h.shape, h.dtype), _empty(h, weight.shape, weight.dtype) if want_dw else _none(h)
+        return [_empty(h, h.shape, h.dtype)] + ([_empty(h, weight.shape, weight.dtype)] if want_dw else [])
 
     @reg("prism::rotary")
     def _(q, k, freqs, positions, axis_pairs, interleaved, amplitude, inverse):
-        return like(q), like(k) if k is not None else _none(q)
+        return [like(t) for t in (q, k) if t is not None]
 
     @reg("prism::window_fwd")
     def _(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse, want_rest):
         o = like(q, 1 << 24)
-        return (o, _empty(q, q.shape[:3], f32) if want_lse else _none(q),
-                torch.empty_like(o) if want_rest else _empty(q, (0,), q.dtype))
+        return ([o] + ([_empty(q, q.shape[:3], f32)] if want_lse else [])
+                + ([torch.empty_like(o)] if want_rest else []))
 
     @reg("prism::window_bwd")
     def _(do, q, k, v, o, rest, lse, window, sinks, causal, q_lens, kv_lens, sm_scale):

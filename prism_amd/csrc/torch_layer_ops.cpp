@@ -18,6 +18,10 @@
 
 namespace {
 
+// An operator's outputs: those that the call has, and no placeholders (an empty
+// tensor costs the host 1 us of the 7 that a small call takes)
+typedef std::vector<Tensor> Outputs;
+
 int type_code(const Tensor& t, const char* name) {
   if (t.scalar_type() == at::kFloat) return PRISM_F32;
   if (t.scalar_type() == at::kBFloat16) return PRISM_BF16;
@@ -42,7 +46,7 @@ Tensor rows_of(const Tensor& t) {  // [M, N] with adjacent columns
   return unit_rows(r);
 }
 // x [.., N]: y, h (with a residual), scale (8-bit outputs), 1 / rms (on request)
-std::tuple<Tensor, Tensor, Tensor, Tensor> rms_norm(const Tensor& x_, const OptT& r_, const OptT& w_, double eps,
+Outputs rms_norm(const Tensor& x_, const OptT& r_, const OptT& w_, double eps,
                                                     int64_t out_code, bool want_inv) {
   on_gpu(x_, "x");
   same_device(x_, r_, "residual");
@@ -59,19 +63,21 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rms_norm(const Tensor& x_, const OptT
   const OptT r = r_ ? OptT(rows_of(*r_)) : OptT(), w = cont(w_);
   const at::ScalarType ot = out_code == PRISM_E4M3 ? at::kFloat8_e4m3fn : out_code == PRISM_I8 ? at::kChar : x.scalar_type();
   const bool quant = out_code == PRISM_E4M3 || out_code == PRISM_I8;
-  Tensor y = at::empty(x_.sizes(), opts(x, ot));
-  Tensor h = r ? at::empty(x_.sizes(), x.options()) : none_like(x);
-  Tensor scale = quant ? at::empty(x_.sizes().slice(0, x_.dim() - 1), opts(x, at::kFloat)) : none_like(x);
-  Tensor inv = want_inv ? at::empty({M}, opts(x, at::kFloat)) : none_like(x);
+  Outputs out{at::empty(x_.sizes(), opts(x, ot))};
+  Tensor h, scale, inv;
+  if (r) out.push_back(h = at::empty(x_.sizes(), x.options()));
+  if (quant) out.push_back(scale = at::empty(x_.sizes().slice(0, x_.dim() - 1), opts(x, at::kFloat)));
+  if (want_inv) out.push_back(inv = at::empty({M}, opts(x, at::kFloat)));
   PRISM_TORCH_CALL(prism_rms_norm, x.data_ptr(), x.stride(0), p(r), r ? r->stride(0) : 0, p(w), wdt, dt, M,
-                   small(N, "N"), (float)eps, r ? h.data_ptr() : nullptr, y.data_ptr(),
+                   small(N, "N"), (float)eps, r ? h.data_ptr() : nullptr, out[0].data_ptr(),
                    (int)(quant ? out_code : dt), quant ? scale.data_ptr<float>() : nullptr,
                    want_inv ? inv.data_ptr<float>() : nullptr, stream_of(x));
-  return {y, h, scale, inv};
+  return out;
 }
 
-std::tuple<Tensor, Tensor> rms_norm_bwd(const Tensor& dy_, const OptT& dh_, const Tensor& h_, const OptT& w_,
-                                        const Tensor& inv_, bool want_dw) {
+// dx, and dw on request
+Outputs rms_norm_bwd(const Tensor& dy_, const OptT& dh_, const Tensor& h_, const OptT& w_, const Tensor& inv_,
+                     bool want_dw) {
   on_gpu(h_, "h");
   same_device(h_, dy_, "dy");
   same_device(h_, dh_, "dh");
@@ -93,16 +99,18 @@ std::tuple<Tensor, Tensor> rms_norm_bwd(const Tensor& dy_, const OptT& dh_, cons
   const Tensor h = rows_of(h_), dy = rows_of(dy_), inv = inv_.contiguous();
   const OptT dh = dh_ ? OptT(rows_of(*dh_)) : OptT(), w = cont(w_);
   Tensor dx = at::empty(h_.sizes(), h.options());
-  if (M == 0) return {dx, want_dw ? at::zeros({N}, w->options()) : none_like(h)};
-  Tensor dw = want_dw ? at::empty({N}, w->options()) : none_like(h);
+  Outputs out{dx};
+  Tensor dw, partial;
+  if (want_dw) out.push_back(dw = M == 0 ? at::zeros({N}, w->options()) : at::empty({N}, w->options()));
+  if (M == 0) return out;
   int parts = 0;
   check_rc(prism_rms_norm_parts(M, small(N, "N"), &parts));
-  Tensor partial = want_dw ? at::empty({parts, N}, opts(h, at::kFloat)) : none_like(h);
+  if (want_dw) partial = at::empty({parts, N}, opts(h, at::kFloat));
   PRISM_TORCH_CALL(prism_rms_norm_bwd, dy.data_ptr(), dy.stride(0), p(dh), dh ? dh->stride(0) : 0, h.data_ptr(),
                    h.stride(0), p(w), wdt, dt, M, small(N, "N"), inv.data_ptr<float>(), dx.data_ptr(),
                    want_dw ? partial.data_ptr<float>() : nullptr, parts, want_dw ? dw.data_ptr() : nullptr,
                    stream_of(h));
-  return {dx, dw};
+  return out;
 }
 
 // ------------------------------------------------------------------ rotary positions
@@ -112,8 +120,9 @@ Tensor like_layout(const Tensor& x) {
   return o.numel() == 0 || o.stride(3) == 1 ? o : at::empty(x.sizes(), x.options());
 }
 
-std::tuple<Tensor, Tensor> rotary(const Tensor& q_, const OptT& k_, const Tensor& freqs_, const Tensor& pos_,
-                                  c10::IntArrayRef axis_pairs, bool interleaved, double amplitude, bool inverse) {
+// q', and k' where there is a k
+Outputs rotary(const Tensor& q_, const OptT& k_, const Tensor& freqs_, const Tensor& pos_, c10::IntArrayRef axis_pairs,
+               bool interleaved, double amplitude, bool inverse) {
   on_gpu(q_, "q");
   same_device(q_, k_, "k");
   same_device(q_, freqs_, "freqs");
@@ -141,7 +150,8 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& q_, const OptT& k_, const Tensor
   const c10::DeviceGuard guard(q_.device());
   const Tensor q = unit_rows(q_), freqs = freqs_.contiguous();
   const OptT k = k_ ? OptT(unit_rows(*k_)) : OptT();
-  Tensor oq = like_layout(q_), ok = k_ ? like_layout(*k_) : none_like(q);
+  Tensor oq = like_layout(q_), ok;
+  if (k_) ok = like_layout(*k_);
   int64_t strides[12] = {q.stride(0), q.stride(1), q.stride(2), oq.stride(0), oq.stride(1), oq.stride(2)};
   if (k) {
     const int64_t s[6] = {k->stride(0), k->stride(1), k->stride(2), ok.stride(0), ok.stride(1), ok.stride(2)};
@@ -161,7 +171,7 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& q_, const OptT& k_, const Tensor
                    freqs.data_ptr<double>(), pos_.data_ptr(), pos_.scalar_type() == at::kLong, pos_strides, (int)A,
                    axis_end, interleaved, (float)amplitude, inverse, oq.data_ptr(), k ? ok.data_ptr() : nullptr,
                    stream_of(q));
-  return {oq, ok};
+  return k ? Outputs{oq, ok} : Outputs{oq};
 }
 
 // ------------------------------------------------------------------ window attention
@@ -210,16 +220,18 @@ WinShape check_window(const Tensor& q, const Tensor& k, const Tensor& v, const O
   return s;
 }
 
-std::tuple<Tensor, Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window,
-                                              int64_t sinks, bool causal, const OptT& q_lens_, const OptT& kv_lens_,
-                                              double sm_scale, bool want_lse, bool want_rest) {
+// o, lse and what o's rounding left off on request
+Outputs window_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window, int64_t sinks, bool causal,
+                   const OptT& q_lens_, const OptT& kv_lens_, double sm_scale, bool want_lse, bool want_rest) {
   const WinShape s = check_window(q_, k_, v_, q_lens_, kv_lens_);
   const c10::DeviceGuard guard(q_.device());
   const Tensor q = win_rows(q_), k = win_rows(k_), v = win_rows(v_);
   const OptT q_lens = cont(q_lens_), kv_lens = cont(kv_lens_);
   Tensor o = win_like(q_);
-  Tensor lse = want_lse ? at::empty({s.B, s.Hq, s.Sq}, opts(q, at::kFloat)) : none_like(q);
-  Tensor rest = want_rest ? at::empty_like(o) : at::empty({0}, o.options());
+  Tensor lse, rest;
+  Outputs out{o};
+  if (want_lse) out.push_back(lse = at::empty({s.B, s.Hq, s.Sq}, opts(q, at::kFloat)));
+  if (want_rest) out.push_back(rest = at::empty_like(o));
   void* rp = want_rest ? rest.data_ptr() : nullptr;
   int64_t st[12];
   win_strides(q, st);
@@ -232,19 +244,21 @@ std::tuple<Tensor, Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_
   int64_t floats = 0;
   check_rc(prism_window_token_plan(B, Hq, Hk, s.Sq, s.Sk, window, sinks, causal, &splits, &floats));
   if (splits) {
-    Tensor part = splits > 1 ? at::empty({floats * (s.D + 2)}, opts(q, at::kFloat)) : none_like(q);
+    Tensor part;
+    if (splits > 1) part = at::empty({floats * (s.D + 2)}, opts(q, at::kFloat));
     float* po = splits > 1 ? part.data_ptr<float>() : nullptr;
     PRISM_TORCH_CALL(prism_window_token, q.data_ptr(), k.data_ptr(), v.data_ptr(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st,
                      window, sinks, causal, (const int32_t*)p(q_lens), (const int32_t*)p(kv_lens), (float)sm_scale,
                      o.data_ptr(), rp, lp, splits, po, po ? po + floats * s.D : nullptr, stream_of(q));
-    return {o, lse, rest};
+    return out;
   }
   check_rc(prism_window_fwd_plan(B, Hq, Hk, s.Sq, s.Sk, D, window, sinks, causal, &floats));
-  Tensor part = floats ? at::empty({floats}, opts(q, at::kFloat)) : none_like(q);
+  Tensor part;
+  if (floats) part = at::empty({floats}, opts(q, at::kFloat));
   PRISM_TORCH_CALL(prism_window_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st,
                    window, sinks, causal, (const int32_t*)p(q_lens), (const int32_t*)p(kv_lens), (float)sm_scale,
                    o.data_ptr(), rp, lp, floats ? part.data_ptr<float>() : nullptr, stream_of(q));
-  return {o, lse, rest};
+  return out;
 }
 
 std::tuple<Tensor, Tensor, Tensor> window_bwd(const Tensor& do_, const Tensor& q_, const Tensor& k_, const Tensor& v_,
@@ -280,7 +294,8 @@ std::tuple<Tensor, Tensor, Tensor> window_bwd(const Tensor& do_, const Tensor& q
   const int B = small(s.B, "B"), Hq = small(s.Hq, "heads"), Hk = small(s.Hk, "heads"), D = small(s.D, "D");
   check_rc(prism_window_bwd_plan(B, Hq, Hk, s.Sq, s.Sk, D, window, sinks, causal, kv_lens.has_value(), &floats));
   Tensor rows = at::empty({2 * s.B * s.Hq * s.Sq}, opts(q, at::kFloat));
-  Tensor acc = floats ? at::empty({floats}, opts(q, at::kFloat)) : none_like(q);
+  Tensor acc;
+  if (floats) acc = at::empty({floats}, opts(q, at::kFloat));
   PRISM_TORCH_CALL(prism_window_bwd, d.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                    p(rest), lse.data_ptr<float>(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st, window, sinks, causal,
                    (const int32_t*)p(q_lens), (const int32_t*)p(kv_lens), (float)sm_scale, dq.data_ptr(), dk.data_ptr(),
@@ -345,35 +360,35 @@ struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
                                int64_t out_code) {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->set_materialize_grads(false);
-    auto [y, h, scale, inv] = PRISM_OP(rms_norm).call(x, r, w, eps, out_code, true);
-    ctx->save_for_backward({r ? h : x, w ? *w : Tensor(), inv});
+    const variable_list o = PRISM_OP(rms_norm).call(x, r, w, eps, out_code, true);  // y, h with a residual, inv
+    ctx->save_for_backward({r ? o[1] : x, w ? *w : Tensor(), o.back()});
     ctx->saved_data["residual"] = r.has_value();
     ctx->saved_data["dw"] = w && w->requires_grad();
-    ctx->mark_non_differentiable(r ? variable_list{scale, inv} : variable_list{h, scale, inv});
-    return {y, h, scale, inv};
+    ctx->mark_non_differentiable({o.back()});
+    return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const variable_list saved = ctx->get_saved_variables();
     const bool residual = ctx->saved_data["residual"].toBool();
     const Tensor dh = residual ? g[1] : Tensor();
     if (!g[0].defined() && !dh.defined()) return variable_list(5);
-    const auto [dx, dw] = [&] {
+    const Outputs d = [&] {
       at::AutoDispatchBelowADInplaceOrView guard;
       const Tensor dy = g[0].defined() ? g[0] : at::zeros_like(dh);  // (only h went on)
       return PRISM_OP(rms_norm_bwd).call(dy, opt(dh), saved[0], opt(saved[1]), saved[2], ctx->saved_data["dw"].toBool());
     }();
-    return once({dx, residual ? dx : Tensor(), ctx->saved_data["dw"].toBool() ? dw : Tensor(), Tensor(), Tensor()});
+    return once({d[0], residual ? d[0] : Tensor(), d.size() > 1 ? d[1] : Tensor(), Tensor(), Tensor()});
   }
 };
-std::tuple<Tensor, Tensor, Tensor, Tensor> rms_norm_autograd(const Tensor& x, const OptT& r, const OptT& w, double eps,
-                                                             int64_t out_code, bool want_inv) {
+Outputs rms_norm_autograd(const Tensor& x, const OptT& r, const OptT& w, double eps, int64_t out_code, bool want_inv) {
   if (!grads_wanted(x, r, w)) {
     at::AutoDispatchBelowADInplaceOrView guard;
     return PRISM_OP(rms_norm).call(x, r, w, eps, out_code, want_inv);
   }
   TORCH_CHECK_VALUE(out_code != PRISM_E4M3 && out_code != PRISM_I8, "rms_norm: 8-bit outputs have no gradient");
-  const variable_list o = RmsNormGrad::apply(x, r, w, eps, out_code);
-  return {o[0], o[1], o[2], o[3]};
+  variable_list o = RmsNormGrad::apply(x, r, w, eps, out_code);
+  if (!want_inv) o.pop_back();
+  return o;
 }
 
 struct RotaryGrad : torch::autograd::Function<RotaryGrad> {
@@ -382,40 +397,38 @@ struct RotaryGrad : torch::autograd::Function<RotaryGrad> {
                                bool inverse) {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->set_materialize_grads(false);
-    auto [oq, ok] = PRISM_OP(rotary).call(q, k, freqs, pos, axis_pairs, interleaved, amplitude, inverse);
+    const variable_list o = PRISM_OP(rotary).call(q, k, freqs, pos, axis_pairs, interleaved, amplitude, inverse);
     ctx->save_for_backward({freqs, pos});
     ctx->saved_data["axis_pairs"] = axis_pairs;
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["amplitude"] = amplitude;
     ctx->saved_data["inverse"] = inverse;
-    if (!k) ctx->mark_non_differentiable({ok});
-    return {oq, ok};
+    return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     variable_list out(8);
-    if (!g[0].defined() && !g[1].defined()) return out;
+    const Tensor dq = g[0], dk = g.size() > 1 ? g[1] : Tensor();
+    if (!dq.defined() && !dk.defined()) return out;
     const variable_list saved = ctx->get_saved_variables();
-    const bool both = g[0].defined() && g[1].defined();
-    const auto [a, b] = [&] {
+    const bool both = dq.defined() && dk.defined();
+    const Outputs d = [&] {
       at::AutoDispatchBelowADInplaceOrView guard;
-      return PRISM_OP(rotary).call(g[0].defined() ? g[0] : g[1], both ? OptT(g[1]) : OptT(), saved[0], saved[1],
+      return PRISM_OP(rotary).call(dq.defined() ? dq : dk, both ? OptT(dk) : OptT(), saved[0], saved[1],
                     ctx->saved_data["axis_pairs"].toIntVector(), ctx->saved_data["interleaved"].toBool(),
                     ctx->saved_data["amplitude"].toDouble(), !ctx->saved_data["inverse"].toBool());
     }();
-    if (g[0].defined()) out[0] = a;
-    if (g[1].defined()) out[1] = both ? b : a;
+    if (dq.defined()) out[0] = d[0];
+    if (dk.defined()) out[1] = d[both ? 1 : 0];
     return once(std::move(out));
   }
 };
-std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const OptT& k, const Tensor& freqs, const Tensor& pos,
-                                           c10::IntArrayRef axis_pairs, bool interleaved, double amplitude,
-                                           bool inverse) {
+Outputs rotary_autograd(const Tensor& q, const OptT& k, const Tensor& freqs, const Tensor& pos,
+                        c10::IntArrayRef axis_pairs, bool interleaved, double amplitude, bool inverse) {
   if (!grads_wanted(q, k)) {
     at::AutoDispatchBelowADInplaceOrView guard;
     return PRISM_OP(rotary).call(q, k, freqs, pos, axis_pairs, interleaved, amplitude, inverse);
   }
-  const variable_list o = RotaryGrad::apply(q, k, freqs, pos, axis_pairs.vec(), interleaved, amplitude, inverse);
-  return {o[0], o[1]};
+  return RotaryGrad::apply(q, k, freqs, pos, axis_pairs.vec(), interleaved, amplitude, inverse);
 }
 
 struct WindowGrad : torch::autograd::Function<WindowGrad> {
@@ -425,15 +438,15 @@ struct WindowGrad : torch::autograd::Function<WindowGrad> {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->set_materialize_grads(false);
     const bool use = prism_window_rest(k.size(2), window, sinks, causal), keep = use || want_rest;
-    auto [o, lse, rest] = PRISM_OP(window_fwd).call(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, true, keep);
-    ctx->save_for_backward({q, k, v, o, lse, q_lens ? *q_lens : Tensor(), kv_lens ? *kv_lens : Tensor(),
-                            use ? rest : Tensor()});
+    const variable_list o = PRISM_OP(window_fwd).call(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, true, keep);
+    ctx->save_for_backward({q, k, v, o[0], o[1], q_lens ? *q_lens : Tensor(), kv_lens ? *kv_lens : Tensor(),
+                            use ? o[2] : Tensor()});
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["sm_scale"] = sm_scale;
-    ctx->mark_non_differentiable({lse, rest});
-    return {o, lse, rest};
+    ctx->mark_non_differentiable(variable_list(o.begin() + 1, o.end()));
+    return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     if (!g[0].defined()) return variable_list(10);
@@ -449,27 +462,29 @@ struct WindowGrad : torch::autograd::Function<WindowGrad> {
     return once(std::move(out));
   }
 };
-std::tuple<Tensor, Tensor, Tensor> window_autograd(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window,
-                                           int64_t sinks, bool causal, const OptT& q_lens, const OptT& kv_lens,
-                                           double sm_scale, bool want_lse, bool want_rest) {
+Outputs window_autograd(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, bool causal,
+                        const OptT& q_lens, const OptT& kv_lens, double sm_scale, bool want_lse, bool want_rest) {
   if (!grads_wanted(q, k, v)) {
     at::AutoDispatchBelowADInplaceOrView guard;
     return PRISM_OP(window_fwd).call(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse, want_rest);
   }
   const variable_list o = WindowGrad::apply(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_rest);
-  return {o[0], o[1], o[2]};
+  Outputs out{o[0]};
+  if (want_lse) out.push_back(o[1]);
+  if (want_rest) out.push_back(o[2]);
+  return out;
 }
 
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(prism, m) {
   m.def("rms_norm(Tensor x, Tensor? residual, Tensor? weight, float eps, int out_code, bool want_inv) "
-        "-> (Tensor, Tensor, Tensor, Tensor)");
-  m.def("rms_norm_bwd(Tensor dy, Tensor? dh, Tensor h, Tensor? weight, Tensor inv, bool want_dw) -> (Tensor, Tensor)");
+        "-> Tensor[]");
+  m.def("rms_norm_bwd(Tensor dy, Tensor? dh, Tensor h, Tensor? weight, Tensor inv, bool want_dw) -> Tensor[]");
   m.def("rotary(Tensor q, Tensor? k, Tensor freqs, Tensor positions, int[] axis_pairs, bool interleaved, "
-        "float amplitude, bool inverse) -> (Tensor, Tensor)");
+        "float amplitude, bool inverse) -> Tensor[]");
   m.def("window_fwd(Tensor q, Tensor k, Tensor v, int window, int sinks, bool causal, Tensor? q_lens, "
-        "Tensor? kv_lens, float sm_scale, bool want_lse, bool want_rest) -> (Tensor, Tensor, Tensor)");
+        "Tensor? kv_lens, float sm_scale, bool want_lse, bool want_rest) -> Tensor[]");
   m.def("window_bwd(Tensor do, Tensor q, Tensor k, Tensor v, Tensor o, Tensor? rest, Tensor lse, int window, int sinks, bool causal, "
         "Tensor? q_lens, Tensor? kv_lens, float sm_scale) -> (Tensor, Tensor, Tensor)");
 }

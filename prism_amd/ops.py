@@ -186,17 +186,17 @@ def rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional
     code = _layer_code(x, "rms_norm") if out_dtype is None else _QUANT_CODES.get(out_dtype)
     if code is None:
         raise TypeError(f"prism_amd: rms_norm: unsupported output dtype {out_dtype} (float8_e4m3fn or int8)")
-    y, h, scale, inv = _op("rms_norm", x, residual, weight, float(eps), code, bool(want_inv))
-    return y, (h if residual is not None else None), (scale if out_dtype is not None else None), \
-        (inv if want_inv else None)
+    out = _op("rms_norm", x, residual, weight, float(eps), code, bool(want_inv))
+    return (out[0], out[1] if residual is not None else None,
+            out[1 if residual is None else 2] if out_dtype is not None else None, out[-1] if want_inv else None)
 
 
 def rms_norm_bwd(dy: torch.Tensor, dh: Optional[torch.Tensor], h: torch.Tensor, weight: Optional[torch.Tensor],
                  inv: torch.Tensor, want_dw: bool):
     """(dx, dw) of rms_norm; dx is also the residual's gradient."""
     _cuda(dy, dh, h, weight, inv)
-    dx, dw = _op("rms_norm_bwd", dy, dh, h, weight, inv, bool(want_dw))
-    return dx, (dw if want_dw else None)
+    out = _op("rms_norm_bwd", dy, dh, h, weight, inv, bool(want_dw))
+    return out[0], (out[1] if want_dw else None)
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, positions: torch.Tensor, axis_pairs,
@@ -205,9 +205,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, posi
     axis_pairs: pairs per axis ([]: one position per token).  Returns (q', k').
     Differentiable (q, k)."""
     _cuda(q, k, freqs, positions)
-    oq, ok = _op("rotary", q, k, freqs, positions, list(axis_pairs), bool(interleaved), float(amplitude),
-                 bool(inverse))
-    return oq, (ok if k is not None else None)
+    out = _op("rotary", q, k, freqs, positions, axis_pairs, bool(interleaved), float(amplitude), bool(inverse))
+    return out[0], (out[1] if k is not None else None)
 
 
 def window_fwd(q, k, v, window: int, sinks: int, causal: bool, q_lens: Optional[torch.Tensor],
@@ -216,9 +215,10 @@ def window_fwd(q, k, v, window: int, sinks: int, causal: bool, q_lens: Optional[
     sinks, with want_rest also what o's rounding left off (o's shape, dtype and
     layout).  Differentiable (o in q, k, v)."""
     _cuda(q, k, v, q_lens, kv_lens)
-    o, lse, rest = _op("window_fwd", q, k, v, int(window), int(sinks), bool(causal), q_lens, kv_lens, float(sm_scale),
-                       bool(want_lse), bool(want_rest))
-    return (o, (lse if want_lse else None), rest) if want_rest else (o, (lse if want_lse else None))
+    out = _op("window_fwd", q, k, v, int(window), int(sinks), bool(causal), q_lens, kv_lens, float(sm_scale),
+              bool(want_lse), bool(want_rest))
+    lse = out[1] if want_lse else None
+    return (out[0], lse, out[-1]) if want_rest else (out[0], lse)
 
 
 def window_bwd(do, q, k, v, o, rest: Optional[torch.Tensor], lse, window: int, sinks: int, causal: bool,

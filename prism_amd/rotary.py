@@ -82,21 +82,22 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor
     channels (2p, 2p + 1), else (p, p + pairs).  amplitude scales the turned
     channels.  Returns q', with k (q', k').  Differentiable in q and k (freqs that
     require gradients are refused)."""
-    for t, name in ((q, "q"), (k, "k")):
-        if t is not None and t.dim() != 4:
-            raise ValueError(f"apply_rotary: {name} must be [B, H, S, D], got {tuple(t.shape)}")
-    if k is not None and (k.shape[0], k.shape[2], k.shape[3]) != (q.shape[0], q.shape[2], q.shape[3]):
-        raise ValueError(f"apply_rotary: k {tuple(k.shape)} must have q's batch, length and head dim {tuple(q.shape)}")
-    if freqs.dtype != torch.float64:
+    qs, ks, pairs = q.shape, None if k is None else k.shape, freqs.shape
+    for s, name in ((qs, "q"), (ks, "k")):
+        if s is not None and len(s) != 4:
+            raise ValueError(f"apply_rotary: {name} must be [B, H, S, D], got {tuple(s)}")
+    if ks is not None and (ks[0] != qs[0] or ks[2:] != qs[2:]):
+        raise ValueError(f"apply_rotary: k {tuple(ks)} must have q's batch, length and head dim {tuple(qs)}")
+    if freqs.dtype is not torch.float64:
         raise TypeError(f"apply_rotary: freqs must be float64 (far positions lose their place in less), got {freqs.dtype}")
     if freqs.requires_grad and torch.is_grad_enabled():
         raise ValueError("apply_rotary has no gradient for freqs: pass them detached")
-    if freqs.dim() != 1 or freqs.shape[0] < 1 or 2 * freqs.shape[0] > q.shape[-1]:
-        raise ValueError(f"apply_rotary: {tuple(freqs.shape)} frequencies do not fit heads of {q.shape[-1]} channels")
+    if len(pairs) != 1 or pairs[0] < 1 or 2 * pairs[0] > qs[3]:
+        raise ValueError(f"apply_rotary: {tuple(pairs)} frequencies do not fit heads of {qs[3]} channels")
     axis_pairs = []
     if sections is not None:
-        if any(int(n) < 2 or int(n) % 2 for n in sections) or sum(int(n) for n in sections) != 2 * freqs.shape[0]:
-            raise ValueError(f"apply_rotary: sections {list(sections)} must be even and sum to {2 * freqs.shape[0]}")
+        if any(int(n) < 2 or int(n) % 2 for n in sections) or sum(int(n) for n in sections) != 2 * pairs[0]:
+            raise ValueError(f"apply_rotary: sections {list(sections)} must be even and sum to {2 * pairs[0]}")
         axis_pairs = [int(n) // 2 for n in sections]
     oq, ok = ops.rotary(q, k, freqs, positions, axis_pairs, interleaved, amplitude)
     return oq if k is None else (oq, ok)

@@ -45,23 +45,25 @@ def flash_attn_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window:
     lse): lse [B, Hq, Sq] float32, the natural log of the sum of exponentials
     of the scaled scores, -inf where nothing is seen (no gradient through it).
     Differentiable in q, k, v; sums over shared heads are fp32."""
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+    qs, ks, vs, dt = q.shape, k.shape, v.shape, q.dtype
+    if len(qs) != 4 or len(ks) != 4 or len(vs) != 4:
         raise ValueError("q, k, v must be [B, H, S, D]")
-    B, Hq, _, D = q.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
-        raise ValueError(f"shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    B, Hq, _, D = qs
+    Hk = ks[1]
+    if ks != vs or ks[0] != B or ks[3] != D:
+        raise ValueError(f"shape mismatch: q {tuple(qs)}, k {tuple(ks)}, v {tuple(vs)}")
     if D not in (64, 128):
         raise ValueError(f"head_dim {D} unsupported by the MI355X kernels (64, 128)")
-    if k.shape[1] < 1 or Hq < k.shape[1] or Hq % k.shape[1]:
-        raise ValueError(f"{Hq} query heads do not share {k.shape[1]} key heads evenly")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"q, k, v must be all bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if Hk < 1 or Hq < Hk or Hq % Hk:
+        raise ValueError(f"{Hq} query heads do not share {Hk} key heads evenly")
+    if (dt is not torch.bfloat16 and dt is not torch.float16) or k.dtype is not dt or v.dtype is not dt:
+        raise TypeError(f"q, k, v must be all bfloat16 or all float16, got {dt}, {k.dtype}, {v.dtype}")
     if window is not None and int(window) < 1:
         raise ValueError(f"window must be at least 1 (or None), got {window}")
     if int(sinks) < 0:
         raise ValueError(f"sinks must not be negative, got {sinks}")
     for t, name in ((q_lens, "q_lens"), (kv_lens, "kv_lens")):
-        if t is not None and (t.dtype != torch.int32 or t.shape != (B,)):
+        if t is not None and (t.dtype is not torch.int32 or t.shape != (B,)):
             raise ValueError(f"{name} must be int32 [{B}], got {t.dtype} {tuple(t.shape)}")
     window = _NO_LIMIT if window is None else min(int(window), _NO_LIMIT)
     sinks = min(int(sinks), _NO_LIMIT)
