@@ -357,27 +357,29 @@ variable_list once(variable_list grads) {
 
 struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptT& r, const OptT& w, double eps,
-                               int64_t out_code) {
+                               int64_t out_code, bool want_inv) {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->set_materialize_grads(false);
-    const variable_list o = PRISM_OP(rms_norm).call(x, r, w, eps, out_code, true);  // y, h with a residual, inv
+    variable_list o = PRISM_OP(rms_norm).call(x, r, w, eps, out_code, true);  // y, h with a residual, inv
     ctx->save_for_backward({r ? o[1] : x, w ? *w : Tensor(), o.back()});
     ctx->saved_data["residual"] = r.has_value();
     ctx->saved_data["dw"] = w && w->requires_grad();
-    ctx->mark_non_differentiable({o.back()});
+    // (what is only kept is no output of the node: each costs the host 2 us)
+    if (want_inv) ctx->mark_non_differentiable({o.back()});
+    else o.pop_back();
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const variable_list saved = ctx->get_saved_variables();
     const bool residual = ctx->saved_data["residual"].toBool();
     const Tensor dh = residual ? g[1] : Tensor();
-    if (!g[0].defined() && !dh.defined()) return variable_list(5);
+    if (!g[0].defined() && !dh.defined()) return variable_list(6);
     const Outputs d = [&] {
       at::AutoDispatchBelowADInplaceOrView guard;
       const Tensor dy = g[0].defined() ? g[0] : at::zeros_like(dh);  // (only h went on)
       return PRISM_OP(rms_norm_bwd).call(dy, opt(dh), saved[0], opt(saved[1]), saved[2], ctx->saved_data["dw"].toBool());
     }();
-    return once({d[0], residual ? d[0] : Tensor(), d.size() > 1 ? d[1] : Tensor(), Tensor(), Tensor()});
+    return once({d[0], residual ? d[0] : Tensor(), d.size() > 1 ? d[1] : Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 Outputs rms_norm_autograd(const Tensor& x, const OptT& r, const OptT& w, double eps, int64_t out_code, bool want_inv) {
@@ -386,9 +388,7 @@ Outputs rms_norm_autograd(const Tensor& x, const OptT& r, const OptT& w, double 
     return PRISM_OP(rms_norm).call(x, r, w, eps, out_code, want_inv);
   }
   TORCH_CHECK_VALUE(out_code != PRISM_E4M3 && out_code != PRISM_I8, "rms_norm: 8-bit outputs have no gradient");
-  variable_list o = RmsNormGrad::apply(x, r, w, eps, out_code);
-  if (!want_inv) o.pop_back();
-  return o;
+  return RmsNormGrad::apply(x, r, w, eps, out_code, want_inv);
 }
 
 struct RotaryGrad : torch::autograd::Function<RotaryGrad> {
@@ -434,7 +434,7 @@ Outputs rotary_autograd(const Tensor& q, const OptT& k, const Tensor& freqs, con
 struct WindowGrad : torch::autograd::Function<WindowGrad> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, int64_t window,
                                int64_t sinks, bool causal, const OptT& q_lens, const OptT& kv_lens, double sm_scale,
-                               bool want_rest) {
+                               bool want_lse, bool want_rest) {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->set_materialize_grads(false);
     const bool use = prism_window_rest(k.size(2), window, sinks, causal), keep = use || want_rest;
@@ -445,11 +445,14 @@ struct WindowGrad : torch::autograd::Function<WindowGrad> {
     ctx->saved_data["sinks"] = sinks;
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["sm_scale"] = sm_scale;
-    ctx->mark_non_differentiable(variable_list(o.begin() + 1, o.end()));
-    return o;
+    variable_list out{o[0]};
+    if (want_lse) out.push_back(o[1]);
+    if (want_rest) out.push_back(o[2]);
+    ctx->mark_non_differentiable(variable_list(out.begin() + 1, out.end()));
+    return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    if (!g[0].defined()) return variable_list(10);
+    if (!g[0].defined()) return variable_list(11);
     const variable_list s = ctx->get_saved_variables();
     const auto [dq, dk, dv] = [&] {
       at::AutoDispatchBelowADInplaceOrView guard;
@@ -457,7 +460,7 @@ struct WindowGrad : torch::autograd::Function<WindowGrad> {
                         ctx->saved_data["sinks"].toInt(), ctx->saved_data["causal"].toBool(), opt(s[5]), opt(s[6]),
                         ctx->saved_data["sm_scale"].toDouble());
     }();
-    variable_list out(10);
+    variable_list out(11);
     out[0] = dq; out[1] = dk; out[2] = dv;
     return once(std::move(out));
   }
@@ -468,11 +471,7 @@ Outputs window_autograd(const Tensor& q, const Tensor& k, const Tensor& v, int64
     at::AutoDispatchBelowADInplaceOrView guard;
     return PRISM_OP(window_fwd).call(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse, want_rest);
   }
-  const variable_list o = WindowGrad::apply(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_rest);
-  Outputs out{o[0]};
-  if (want_lse) out.push_back(o[1]);
-  if (want_rest) out.push_back(o[2]);
-  return out;
+  return WindowGrad::apply(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse, want_rest);
 }
 
 }  // namespace
