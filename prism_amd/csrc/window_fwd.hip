@@ -193,16 +193,19 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void window_fwd_kernel(WinArg
     if (g == 0) reinterpret_cast<float2*>(a.part_ml)[((int64_t)it.slot * 4 + w) * 32 + l32] = make_float2(m, l);
     return;
   }
-  if (r >= rows) return;
+  // (the row again from the lane: nothing of it stays in a register over the loop)
+  const int re = wr0 + (opaque_thread_id() & 31);
+  if (re >= rows) return;
+  const int ie = re / a.G, he = hk * a.G + (re - ie * a.G);
   const float inv = 1.0f / l;
-  const int64_t at = b * a.o.b + head * a.o.h + i * a.o.s;
+  const int64_t at = b * a.o.b + he * a.o.h + ie * a.o.s;
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
     for (int j = 0; j < 4; j += 2)
       win_store_o<E>(a, at + 32 * dt + 8 * j, g, win_scaled(acc_o[dt], j, inv), win_scaled(acc_o[dt], j + 1, inv));
   if (a.lse && g == 0)
-    a.lse[((int64_t)b * a.Hk * a.G + head) * a.Sq + i] = (m + __log2f(l)) * 0.6931471805599453f;
+    a.lse[((int64_t)b * a.Hk * a.G + he) * a.Sq + ie] = (m + __log2f(l)) * 0.6931471805599453f;
 }
 
 // the parts of a cut row tile, in order: one workgroup per tile and 32 channels,
