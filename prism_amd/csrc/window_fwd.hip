@@ -228,18 +228,29 @@ __global__ __launch_bounds__(256) void window_fwd_join_kernel(WinArgs a) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float l = 0.0f;
-#pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 x = ml[(int64_t)s * 128];
-    const float f = x.x == NINF ? 0.0f : fast_exp2(x.x - top);  // (a part that sees nothing has sums of 0)
-    l = __builtin_fmaf(x.y, f, l);
+#pragma unroll 1
+  for (int s = 0; s < a.splits; s += 4) {  // (four parts in flight, past the end the last one again: 11.4 -> 8.5 us)
+    float2 x[4];
+    float4 v[4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float4 v = pa[(int64_t)s * 4 * NDT * 256 + j * 64];
-      o[j].x = __builtin_fmaf(v.x, f, o[j].x);
-      o[j].y = __builtin_fmaf(v.y, f, o[j].y);
-      o[j].z = __builtin_fmaf(v.z, f, o[j].z);
-      o[j].w = __builtin_fmaf(v.w, f, o[j].w);
+    for (int k = 0; k < 4; ++k) {
+      const int64_t t = s + k < a.splits ? s + k : a.splits - 1;
+      x[k] = ml[t * 128];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[k][j] = pa[t * 4 * NDT * 256 + j * 64];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool in = s + k < a.splits;
+      const float f = x[k].x == NINF ? 0.0f : fast_exp2(x[k].x - top);  // (a part that sees nothing has sums of 0)
+      l = in ? __builtin_fmaf(x[k].y, f, l) : l;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        o[j].x = in ? __builtin_fmaf(v[k][j].x, f, o[j].x) : o[j].x;
+        o[j].y = in ? __builtin_fmaf(v[k][j].y, f, o[j].y) : o[j].y;
+        o[j].z = in ? __builtin_fmaf(v[k][j].z, f, o[j].z) : o[j].z;
+        o[j].w = in ? __builtin_fmaf(v[k][j].w, f, o[j].w) : o[j].w;
+      }
     }
   }
   const bool none = top == NINF && l == 0.0f;
