@@ -293,13 +293,12 @@ std::tuple<Tensor, Tensor, Tensor> window_bwd(const Tensor& do_, const Tensor& q
   for (int i = 0; i < 8; ++i) win_strides(*all[i], st + 3 * i);
   const int B = small(s.B, "B"), Hq = small(s.Hq, "heads"), Hk = small(s.Hk, "heads"), D = small(s.D, "D");
   check_rc(prism_window_bwd_plan(B, Hq, Hk, s.Sq, s.Sk, D, window, sinks, causal, kv_lens.has_value(), &floats));
-  Tensor rows = at::empty({2 * s.B * s.Hq * s.Sq}, opts(q, at::kFloat));
-  Tensor acc;
-  if (floats) acc = at::empty({floats}, opts(q, at::kFloat));
+  Tensor work = at::empty({floats + 2 * s.B * s.Hq * s.Sq}, opts(q, at::kFloat));  // acc, then rows
+  float* acc = work.data_ptr<float>();
   PRISM_TORCH_CALL(prism_window_bwd, d.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                    p(rest), lse.data_ptr<float>(), s.dt, B, Hq, Hk, s.Sq, s.Sk, D, st, window, sinks, causal,
                    (const int32_t*)p(q_lens), (const int32_t*)p(kv_lens), (float)sm_scale, dq.data_ptr(), dk.data_ptr(),
-                   dv.data_ptr(), rows.data_ptr<float>(), floats ? acc.data_ptr<float>() : nullptr, stream_of(q));
+                   dv.data_ptr(), acc + floats, floats ? acc : nullptr, stream_of(q));
   return {dq, dk, dv};
 }
 

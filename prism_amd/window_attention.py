@@ -39,12 +39,16 @@ def flash_attn_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window:
     and others that no query of the call sees, are not read and may hold
     anything.  Queries that see no key, and rows i >= n, give 0 (and take no
     gradient).  sm_scale (positive)
-    defaults to D^-1/2.
+    defaults to D^-1/2.  A NaN or an infinity in a key or value reaches the
+    queries that see it and no others (at about 1 us a key); in a backward pass
+    it may reach the gradients of rows in the same tile of 64.
 
     Returns o, of q's shape (and layout, where q is dense), with return_lse (o,
     lse): lse [B, Hq, Sq] float32, the natural log of the sum of exponentials
     of the scaled scores, -inf where nothing is seen (no gradient through it).
-    Differentiable in q, k, v; sums over shared heads are fp32."""
+    Differentiable in q, k, v; sums over shared heads are fp32.  The backward
+    keeps q, k, v, o, lse and (where queries see more than 64 keys) what o's
+    rounding left off, of o's size."""
     qs, ks, vs, dt = q.shape, k.shape, v.shape, q.dtype
     if len(qs) != 4 or len(ks) != 4 or len(vs) != 4:
         raise ValueError("q, k, v must be [B, H, S, D]")
