@@ -56,7 +56,7 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, sections: Opti
             def turns_at(n):
                 return d * math.log(original_length / (n * 2 * math.pi)) / (2 * math.log(b))
             low = max(math.floor(turns_at(beta_fast)), 0)
-            high = min(math.ceil(turns_at(beta_slow)), d // 2 - 1)
+            high = min(math.ceil(turns_at(beta_slow)), d - 1)  # (past the last pair where that turns more often)
             ramp = ((torch.arange(d // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
             f = f * (1 - ramp) + f / factor * ramp
             amplitude = 0.1 * math.log(factor) + 1.0
