@@ -27,3 +27,12 @@ def test_yarn_ramp_past_the_last_pair(dim, factor, length):
             assert share == 0.0
         if turns > slow * base ** (2 / dim):  # (more than one whole pair away from the ramp's end)
             assert share < 1.0 and float(f[i]) > plain / factor
+
+
+@pytest.mark.parametrize("betas", [(1.0, 32.0), (4.0, 4.0), (32.0, 0.0), (32.0, -1.0), (math.nan, 1.0), (32.0, math.nan),
+                                   (math.inf, 1.0)])
+def test_yarn_refuses_ends_out_of_order(betas):
+    fast, slow = betas
+    with pytest.raises(ValueError, match="beta_fast"):
+        prism_amd.rotary_frequencies(64, scaling="yarn", factor=4.0, original_length=8192, beta_fast=fast, beta_slow=slow,
+                                     device="cpu")
