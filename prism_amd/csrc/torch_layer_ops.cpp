@@ -317,6 +317,15 @@ auto prism_op(const char* name, F*) {
 
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const OptT& t) { return t && t->defined() && t->requires_grad(); }
+// The operators have no forward-mode derivatives.  A dual tensor need not require
+// gradients, and below autograd its tangent would be lost without a word: refused.
+bool has_tangent(const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const OptT& t) { return t && t->defined() && has_tangent(*t); }
+template <class... T>
+void check_no_tangents(const char* op, const T&... t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(t) || ...), "prism: ", op,
+                              " has no forward-mode derivatives (an input has a tangent)");
+}
 // A leaf's gradient is added on the stream on which a graph first took the leaf,
 // as long as that graph lives.  If that was the default stream, a backward pass
 // captured into a graph would call on a stream that may not take part in a
@@ -382,6 +391,7 @@ struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
   }
 };
 Outputs rms_norm_autograd(const Tensor& x, const OptT& r, const OptT& w, double eps, int64_t out_code, bool want_inv) {
+  check_no_tangents("rms_norm", x, r, w);
   if (!grads_wanted(x, r, w)) {
     at::AutoDispatchBelowADInplaceOrView guard;
     return PRISM_OP(rms_norm).call(x, r, w, eps, out_code, want_inv);
@@ -423,6 +433,7 @@ struct RotaryGrad : torch::autograd::Function<RotaryGrad> {
 };
 Outputs rotary_autograd(const Tensor& q, const OptT& k, const Tensor& freqs, const Tensor& pos,
                         c10::IntArrayRef axis_pairs, bool interleaved, double amplitude, bool inverse) {
+  check_no_tangents("rotary", q, k, freqs);
   if (!grads_wanted(q, k)) {
     at::AutoDispatchBelowADInplaceOrView guard;
     return PRISM_OP(rotary).call(q, k, freqs, pos, axis_pairs, interleaved, amplitude, inverse);
@@ -466,6 +477,7 @@ struct WindowGrad : torch::autograd::Function<WindowGrad> {
 };
 Outputs window_autograd(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, bool causal,
                         const OptT& q_lens, const OptT& kv_lens, double sm_scale, bool want_lse, bool want_rest) {
+  check_no_tangents("window_fwd", q, k, v);
   if (!grads_wanted(q, k, v)) {
     at::AutoDispatchBelowADInplaceOrView guard;
     return PRISM_OP(window_fwd).call(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse, want_rest);

@@ -36,3 +36,41 @@ def test_yarn_refuses_ends_out_of_order(betas):
     with pytest.raises(ValueError, match="beta_fast"):
         prism_amd.rotary_frequencies(64, scaling="yarn", factor=4.0, original_length=8192, beta_fast=fast, beta_slow=slow,
                                      device="cpu")
+
+
+def fake_calls():
+    """(name, call of one fake tensor, its shape): every input that could carry a derivative."""
+    bf = torch.bfloat16
+    mk = lambda *s, dt=bf: torch.empty(*s, device="cuda", dtype=dt)  # noqa: E731
+    x, w = mk(3, 64), mk(64)
+    q, freqs, at = mk(1, 2, 9, 64), mk(32, dt=torch.float64), mk(9, dt=torch.int64)
+    att = prism_amd.flash_attn_window
+    return [("norm x", lambda t: prism_amd.rms_norm(t, w), x), ("norm weight", lambda t: prism_amd.rms_norm(x, t), w),
+            ("norm residual", lambda t: prism_amd.rms_norm(x, w, residual=t)[1], x),
+            ("norm codes", lambda t: prism_amd.rms_norm_quant(t)[1], x),
+            ("rotary q", lambda t: prism_amd.apply_rotary(t, None, freqs, at), q),
+            ("rotary k", lambda t: prism_amd.apply_rotary(q, t, freqs, at)[1], q),
+            ("rotary freqs", lambda t: prism_amd.apply_rotary(q, None, t, at), freqs),
+            ("window q", lambda t: att(t, q, q, 3), q), ("window k", lambda t: att(q, t, q, 3), q),
+            ("window v", lambda t: att(q, q, t, 3, return_lse=True)[1], q)]
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_tangents_are_refused(requires_grad):
+    import torch.autograd.forward_ad as forward_ad
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        for name, call, t in fake_calls():
+            if requires_grad and name in ("norm codes", "rotary freqs"):
+                continue  # (refused as such)
+            t = t.requires_grad_(requires_grad)
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(t, torch.ones_like(t))
+                for mode in (torch.enable_grad, torch.no_grad):
+                    with mode(), pytest.raises(NotImplementedError, match="forward-mode"):
+                        call(dual)
+            if not requires_grad:
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    torch.func.jvp(call, (t,), (torch.ones_like(t),))
+            t.requires_grad_(False)
+            assert not call(t).requires_grad  # without a tangent: as ever
