@@ -2,7 +2,8 @@
 include/prism_bsa.h as PyTorch operators, torch.ops.prism.*) and registers
 the fake (meta) implementation of every operator, so that shape propagation,
 torch.compile tracing and torch.library.opcheck see the outputs' shapes and
-dtypes without running a kernel.
+dtypes without running a kernel; and the vmap rules of the operators that
+return lists, which torch's own loop over the mapped dimension does not take.
 
 The operator library is the only compute path of prism_amd.ops: if it is
 missing the import fails loudly (there is no CPU or eager fallback).
@@ -32,6 +33,7 @@ def load():
                                   "prism_amd has no fallback path")
             torch.ops.load_library(LIB_PATH)
             _register_fakes()
+            _register_vmaps()
             _loaded = True
     return torch.ops.prism
 
@@ -46,6 +48,24 @@ def _none(like):
 
 def _zones(grid):
     return (grid[0] // 8) * (grid[1] // 8) * (grid[2] // 8)
+
+
+def _register_vmaps():
+    def one(t, d, i):
+        return t if d is None or not isinstance(t, torch.Tensor) else t.select(d, i)
+
+    for name in ("rms_norm", "rms_norm_bwd", "rotary", "window_fwd"):
+        if not hasattr(torch.ops.prism, name):  # (a library built before, as for the fakes)
+            continue
+
+        def rule(info, in_dims, *args, op=getattr(torch.ops.prism, name)):
+            if info.batch_size == 0:
+                raise ValueError("prism: vmap over no elements (nothing says what the outputs' shapes are)")
+            outs = [op(*[one(t, d, i) for t, d in zip(args, in_dims)]) for i in range(info.batch_size)]
+            out = [torch.stack(ts) for ts in zip(*outs)]
+            return out, [0] * len(out)
+
+        torch.library.register_vmap("prism::" + name, rule)
 
 
 def _register_fakes():

@@ -74,3 +74,30 @@ def test_tangents_are_refused(requires_grad):
                     torch.func.jvp(call, (t,), (torch.ones_like(t),))
             t.requires_grad_(False)
             assert not call(t).requires_grad  # without a tangent: as ever
+
+
+def test_vmap_shapes():
+    """Every operator under vmap, over any dimension, with inputs that are not
+    mapped (fake tensors: shapes and which outputs carry gradients)."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    bf = torch.bfloat16
+    with FakeTensorMode():
+        mk = lambda *s, dt=bf: torch.empty(*s, device="cuda", dtype=dt, requires_grad=dt == bf)  # noqa: E731
+        x, w, xs = mk(4, 5, 64), mk(64), mk(5, 4, 64)
+        y, h = torch.vmap(lambda a, r, w: prism_amd.rms_norm(a, w, residual=r), in_dims=(0, 1, None))(x, xs, w)
+        assert y.shape == h.shape == (4, 5, 64) and y.requires_grad and h.requires_grad
+        codes, scales = torch.vmap(prism_amd.rms_norm_quant)(x.detach())
+        assert codes.shape == x.shape and codes.dtype == torch.float8_e4m3fn and scales.shape == (4, 5)
+        bwd = lambda dy, inv: prism_amd.ops.rms_norm_bwd(dy, None, x.detach()[0], w.detach(), inv, True)  # noqa: E731
+        dx, dw = torch.vmap(bwd, in_dims=(1, None))(xs.detach(), mk(5, dt=torch.float32))
+        assert dx.shape == x.shape and dw.shape == (4, 64)
+        q, k, freqs, at = mk(3, 1, 4, 9, 64), mk(1, 2, 9, 64, 3), mk(32, dt=torch.float64), mk(3, 9, dt=torch.int64)
+        a, b = torch.vmap(lambda q, k, at: prism_amd.apply_rotary(q, k, freqs, at), in_dims=(0, 4, 0))(q, k, at)
+        assert a.shape == q.shape and b.shape == (3, 1, 2, 9, 64) and b.requires_grad
+        at2 = mk(9, 2, dt=torch.int32)
+        c = torch.vmap(lambda q: prism_amd.apply_rotary(q, None, freqs, at2, sections=(32, 32)))(q)
+        assert c.shape == q.shape
+        o, lse = torch.vmap(lambda q, k: prism_amd.flash_attn_window(q, k, k, 5, return_lse=True))(a, b)
+        assert o.shape == q.shape and lse.shape == (3, 1, 4, 9) and o.requires_grad and not lse.requires_grad
+        with pytest.raises(ValueError, match="vmap"):
+            torch.vmap(prism_amd.rms_norm)(x[:0])
