@@ -441,13 +441,21 @@ Outputs rotary_autograd(const Tensor& q, const OptT& k, const Tensor& freqs, con
   return RotaryGrad::apply(q, k, freqs, pos, axis_pairs.vec(), interleaved, amplitude, inverse);
 }
 
+// prism_window_rest without fixing a length that is symbolic (a traced program): a
+// window and sinks that reach 64 keys at most at any length, or a length of 64 at
+// most, which as a bound serves all lengths on its side of it.
+bool window_rest(const Tensor& k, int64_t window, int64_t sinks, bool causal) {
+  return prism_window_rest(int64_t{1} << 40, window, sinks, causal) &&
+         k.sym_size(2).sym_gt(64).guard_bool(__FILE__, __LINE__);
+}
+
 struct WindowGrad : torch::autograd::Function<WindowGrad> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, int64_t window,
                                int64_t sinks, bool causal, const OptT& q_lens, const OptT& kv_lens, double sm_scale,
                                bool want_lse, bool want_rest) {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->set_materialize_grads(false);
-    const bool use = prism_window_rest(k.size(2), window, sinks, causal), keep = use || want_rest;
+    const bool use = window_rest(k, window, sinks, causal), keep = use || want_rest;
     const variable_list o = PRISM_OP(window_fwd).call(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, true, keep);
     ctx->save_for_backward({q, k, v, o[0], o[1], q_lens ? *q_lens : Tensor(), kv_lens ? *kv_lens : Tensor(),
                             use ? o[2] : Tensor()});

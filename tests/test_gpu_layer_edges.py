@@ -56,3 +56,25 @@ def test_tangents_are_refused():
         prism_amd.rms_norm(forward_ad.make_dual(x, x))
     with pytest.raises(RuntimeError, match="functorch"):  # (torch's own refusal of C++ nodes)
         torch.func.grad(lambda t: prism_amd.rms_norm(t).float().sum())(x)
+
+
+def test_compiled_training_step_serves_every_length():
+    """Compiled once with dynamic lengths: one program, the eager bits, forward and
+    backward, at lengths on one side of the bound that decides what is kept."""
+    torch._dynamo.reset()
+    freqs = prism_amd.rotary_frequencies(64)[0]
+
+    def step(q, kv, w, at):
+        q, k = prism_amd.apply_rotary(q, kv, freqs, at)
+        return prism_amd.rms_norm(prism_amd.flash_attn_window(q, k, kv, 100, sinks=4), w)
+
+    fast = torch.compile(step, backend="aot_eager", dynamic=True, fullgraph=True)
+    for n in (70, 71, 333, 128):
+        args = [randn(1, 4, n, 64, seed=n), randn(1, 2, n, 64, seed=n + 1), randn(64, seed=2)]
+        runs = []
+        for f in (step, fast):
+            leaves = [t.clone().requires_grad_(True) for t in args]
+            with torch.compiler.set_stance("default" if n == 70 else "fail_on_recompile"):
+                o = f(*leaves, torch.arange(n, device="cuda"))
+            runs.append([o.detach(), *torch.autograd.grad(o, leaves, randn(*o.shape, seed=5))])
+        assert all(torch.equal(a, b) for a, b in zip(*runs)), n

@@ -101,3 +101,41 @@ def test_vmap_shapes():
         assert o.shape == q.shape and lse.shape == (3, 1, 4, 9) and o.requires_grad and not lse.requires_grad
         with pytest.raises(ValueError, match="vmap"):
             torch.vmap(prism_amd.rms_norm)(x[:0])
+
+
+@pytest.mark.parametrize("window,sinks,causal,bound", [(5, 0, True, False), (100, 4, True, True), (None, 0, True, True),
+                                                       (32, 0, False, False), (33, 0, False, True), (30, 40, True, True),
+                                                       (60, 4, True, False), (1 << 62, 1 << 62, False, True)])
+@pytest.mark.parametrize("length", [2, 64, 65, 70, 5000])
+def test_traced_training_step_keeps_symbolic_lengths(window, sinks, causal, bound, length):
+    """One traced program serves every length: a training step's outputs keep the
+    symbol as inference's do, and the one choice that depends on the length (what
+    the backward keeps) is a bound, not a value."""
+    from torch._dynamo.source import ConstantSource
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.symbolic_shapes import DimDynamic, ShapeEnv
+    for grad in (False, True):
+        env = ShapeEnv()
+        with FakeTensorMode(shape_env=env):
+            symbol = env.create_symbol(length, ConstantSource("S"), dynamic_dim=DimDynamic.DYNAMIC)
+            S = env.create_symintnode(symbol, hint=length)
+            mk = lambda *s, dt=torch.bfloat16: torch.empty(*s, device="cuda", dtype=dt,  # noqa: E731
+                                                           requires_grad=grad and dt == torch.bfloat16)  # noqa: B023
+            q, x, f, at = mk(2, 4, S, 64), mk(S, 64), mk(32, dt=torch.float64), mk(S, dt=torch.int64)
+            o, lse = prism_amd.flash_attn_window(q, q, q, window, sinks=sinks, causal=causal, return_lse=True)
+            sizes = [o.shape[2], lse.shape[2], prism_amd.rms_norm(x).shape[0], prism_amd.apply_rotary(q, q, f, at)[1].shape[2]]
+        assert all(isinstance(s, torch.SymInt) and s.node.expr == symbol for s in sizes), sizes
+        guards = {str(g.expr).replace(str(symbol), "S") for g in env.guards}
+        assert guards <= ({"S <= 64" if length <= 64 else "S > 64"} if grad and bound else set()), guards
+
+
+def test_what_the_backward_keeps_goes_by_one_bound():
+    """The rule in use (few keys at any length, or a length of 64 at most) is the
+    C function's at every length."""
+    lib = prism_amd._lib.load()
+    for causal in (0, 1):
+        for window in (1, 2, 31, 32, 33, 60, 63, 64, 65, 100, 1 << 29):
+            for sinks in (0, 1, 4, 5, 30, 63, 64, 65, 1 << 29):
+                any_length = lib.prism_window_rest(1 << 40, window, sinks, causal)
+                for Sk in (0, 1, 2, 31, 32, 33, 62, 63, 64, 65, 66, 99, 100, 129, 5000):
+                    assert lib.prism_window_rest(Sk, window, sinks, causal) == (any_length and Sk > 64)
