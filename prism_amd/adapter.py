@@ -102,13 +102,12 @@ class DynamicBlockSparseAttention:
         if rotary_freqs is not None and (rotary_sections is None or len(rotary_sections) != 3):
             raise ValueError("rotary_freqs needs rotary_sections, the channels per axis (t, h, w)")
         self.rotary_freqs, self.rotary_sections = rotary_freqs, rotary_sections
-        self._positions = None  # ((grid, device), [S, 3]) of the last grid
 
     def _rotate(self, q, k, grid):
-        key = (tuple(int(n) for n in grid), q.device)
-        if self._positions is None or self._positions[0] != key:
-            self._positions = (key, grid_positions(grid, q.device))
-        return apply_rotary(q, k, self.rotary_freqs, self._positions[1], sections=self.rotary_sections)
+        # (positions are formed by each call on its own stream: kept ones would be
+        # read on other streams, in training after inference mode, or from a graph's
+        # memory before its first replay)
+        return apply_rotary(q, k, self.rotary_freqs, grid_positions(grid, q.device), sections=self.rotary_sections)
 
     def advance_pass(self) -> int:
         """Call once per real outer forward (advance_dynamic_block_pass_id)."""

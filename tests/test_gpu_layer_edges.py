@@ -78,3 +78,46 @@ def test_compiled_training_step_serves_every_length():
                 o = f(*leaves, torch.arange(n, device="cuda"))
             runs.append([o.detach(), *torch.autograd.grad(o, leaves, randn(*o.shape, seed=5))])
         assert all(torch.equal(a, b) for a, b in zip(*runs)), n
+
+
+def test_adapter_positions_on_two_streams():
+    """A call behind a long queue of work on one stream does not hold up, or feed,
+    one of the same grid on another."""
+    sections = (24, 20, 20)
+    freqs, _ = prism_amd.rotary_frequencies(64, sections=sections)
+    m = prism_amd.DynamicBlockSparseAttention(rotary_freqs=freqs, rotary_sections=sections)
+    grids = [(3, 10, 12), (5, 6, 12)]
+    q, k = randn(1, 2, 360, 64, seed=1), randn(1, 2, 360, 64, seed=2)
+    want = [prism_amd.apply_rotary(q, k, freqs, prism_amd.grid_positions(g), sections=sections) for g in grids]
+    busy, work = torch.cuda.Stream(), randn(4096, 4096)
+    torch.cuda.synchronize()
+    got = []
+    for i in range(6):
+        with torch.cuda.stream(busy):
+            for _ in range(20):
+                work = (work @ work).clamp(-1, 1)
+            first = m._rotate(q, k, grids[i % 2])
+        got.append((i % 2, m._rotate(q, k, grids[i % 2])))
+        got.append((i % 2, first))
+    torch.cuda.synchronize()
+    for g, (a, b) in got:
+        assert torch.equal(a, want[g][0]) and torch.equal(b, want[g][1])
+
+
+def test_adapter_positions_in_a_graph():
+    """The first call on a grid is captured, the next ones run eagerly before the
+    graph's first replay."""
+    sections = (24, 20, 20)
+    freqs, _ = prism_amd.rotary_frequencies(64, sections=sections)
+    m = prism_amd.DynamicBlockSparseAttention(rotary_freqs=freqs, rotary_sections=sections)
+    q, k = randn(1, 2, 360, 64, seed=1), randn(1, 2, 360, 64, seed=2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = m._rotate(q, k, (3, 10, 12))
+    want = prism_amd.apply_rotary(q, k, freqs, prism_amd.grid_positions((3, 10, 12)), sections=sections)
+    assert all(torch.equal(a, b) for a, b in zip(m._rotate(q, k, (3, 10, 12)), want))
+    for i in range(3):
+        q.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(m._rotate(q, k, (3, 10, 12)), got))

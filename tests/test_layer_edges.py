@@ -139,3 +139,18 @@ def test_what_the_backward_keeps_goes_by_one_bound():
                 any_length = lib.prism_window_rest(1 << 40, window, sinks, causal)
                 for Sk in (0, 1, 2, 31, 32, 33, 62, 63, 64, 65, 66, 99, 100, 129, 5000):
                     assert lib.prism_window_rest(Sk, window, sinks, causal) == (any_length and Sk > 64)
+
+
+def test_adapter_keeps_no_positions():
+    """Inference mode, then training on the same grid; and nothing of a call stays."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    freqs, _ = prism_amd.rotary_frequencies(64, sections=(24, 20, 20), device="cpu")
+    with FakeTensorMode() as mode:
+        m = prism_amd.DynamicBlockSparseAttention(rotary_freqs=mode.from_tensor(freqs).to("cuda"), rotary_sections=(24, 20, 20))
+        before = dict(vars(m))
+        q = torch.empty(1, 2, 24, 64, device="cuda", dtype=torch.bfloat16)
+        with torch.inference_mode():
+            m._rotate(q, q, (2, 3, 4))
+        a, b = m._rotate(q.clone().requires_grad_(True), q, (2, 3, 4))
+        assert a.requires_grad and b.requires_grad
+        assert vars(m) == before
