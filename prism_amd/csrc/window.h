@@ -25,7 +25,18 @@
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
+// Softmax reference.  P = 2^(score - m) is rounded to the type for its product with
+// V.  m is SHIFT below the largest score when it was last moved, and moves when a
+// score is more than MARGIN above that one, so P <= 2^(SHIFT + MARGIN); o = acc / l and
+// lse = m + log2 l do not depend on it.  bfloat16 has float's range: any reference
+// will do, and one that moves rarely costs least.  float16 loses bits below 2^-14 and
+// everything below 2^-25, while l sums P unrounded: a long tail far below one large
+// score would not weigh what it does (one list of 65,000 keys 17.0 nats below a sink:
+// o 0.0039 for 0.0027 with m at the largest score).  P up to 2^15 keeps all of a key's bits down to 2^-26
+// of the largest weight (18 nats) and some down to 2^-37; a margin of 3 moves the
+// reference no more than a few times in a list.
 struct WinBf16 {
+  static constexpr float SHIFT = 0.0f, MARGIN = 8.0f;
   static __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -35,6 +46,7 @@ struct WinBf16 {
 };
 // (operands travel as bf16x8: eight 16-bit values whatever their type)
 struct WinF16 {
+  static constexpr float SHIFT = 12.0f, MARGIN = 3.0f;
   static __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }

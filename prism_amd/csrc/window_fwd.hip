@@ -14,7 +14,8 @@
 // made from three bounds; a wave skips tiles that none of its tokens sees.
 //
 // Numbers: scores, maximum, sum and output are fp32; P is rounded to the inputs'
-// type for the product with V (its error averages out over the keys), o once.
+// type for the product with V (half a step of each key's weight, in any direction;
+// float16 at a reference that keeps small weights in its range, window.h), o once.
 //
 // Bound: the matrix cores and the exponentials' VALU beside each other, at D = 64
 // the VALU (each score costs the same there for half the products).  Measured: 16,001
@@ -132,10 +133,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void window_fwd_kernel(WinArg
 #pragma unroll
     for (int x = 1; x < 16; ++x) mx = fmax_nn(fmax_nn(mx, sacc[0][x]), sacc[1][x]);
     mx = xor32_max(mx) * a.scale_log2;
-    // the running reference moves only when the tile's maximum is more than 8
-    // above it (p <= 2^8): o = acc / l and lse = m + log2 l do not depend on it
-    const bool move = mx > m + 8.0f || (m == NINF && mx != NINF);
-    const float m_new = move ? mx : m;
+    // the running reference moves only when the tile's maximum is far above it (window.h)
+    const bool move = mx > m + (E::SHIFT + E::MARGIN) || (m == NINF && mx != NINF);
+    const float m_new = move ? mx - E::SHIFT : m;
     const float alpha = move ? fast_exp2(m - m_new) : 1.0f;
     const float mb = m_new == NINF ? 0.0f : m_new;
     if (__builtin_amdgcn_ballot_w64(move)) {

@@ -159,8 +159,8 @@ __global__ __launch_bounds__(256, 1) void window_token_kernel(WinArgs a) {
 #pragma unroll
     for (int x = 1; x < 16; ++x) mx = fmax_nn(mx, sacc[x]);
     mx = xor32_max(mx) * a.scale_log2;
-    const bool move = mx > m + 8.0f || (m == NINF && mx != NINF);
-    const float m_new = move ? mx : m;
+    const bool move = mx > m + (E::SHIFT + E::MARGIN) || (m == NINF && mx != NINF);
+    const float m_new = move ? mx - E::SHIFT : m;
     const float alpha = move ? fast_exp2(m - m_new) : 1.0f;
     const float mb = m_new == NINF ? 0.0f : m_new;
     if (__builtin_amdgcn_ballot_w64(move)) {

@@ -121,3 +121,50 @@ def test_adapter_positions_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(m._rotate(q, k, (3, 10, 12)), got))
+
+
+# ------------------------------------------------------------------ float16's range
+def sink_and_tail(Sq, Sk, D, gap, dt, Hq=1):
+    """One key whose score is `gap` (about) above all the others', which are equal;
+    its value is 0, theirs 1 (and 0.5 in every other channel)."""
+    q, k = torch.zeros(1, Hq, Sq, D, device="cuda", dtype=dt), torch.zeros(1, 1, Sk, D, device="cuda", dtype=dt)
+    v = torch.ones(1, 1, Sk, D, device="cuda", dtype=dt)
+    v[..., ::2] = 0.5
+    q[..., 0], k[0, 0, 0, 0], v[0, 0, 0] = 4.0, gap / 4, 0
+    return q, k, v
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("Sq,Sk,D,gap,Hq", [(1, 131073, 64, 17.2, 1), (1, 131073, 128, 17.2, 32), (1, 65001, 64, 17.0, 4),
+                                            (200, 65001, 64, 17.0, 4), (300, 30001, 128, 16.0, 2), (1, 400, 64, 11.0, 1),
+                                            (130, 400, 64, 11.0, 1), (1, 1000, 128, 17.5, 2), (200, 1000, 64, 17.5, 2)])
+def test_long_tails_below_one_large_score(Sq, Sk, D, gap, Hq, dt):
+    """A weight far below the largest still counts with its own precision: each P off
+    by u of itself (no steps of float16's subnormals: 2^-26 of the largest is 18.0
+    nats), all in one direction here; fp32 scores and exponentials (E = (D + 2) 2^-24
+    of a score of `gap`, and 2^-22), sums of n terms, o's rounding u (its values
+    are at most 1)."""
+    q, k, v = sink_and_tail(Sq, Sk, D, gap, dt, Hq)
+    o, lse = prism_amd.flash_attn_window(q, k, v, None, causal=False, sm_scale=1.0, return_lse=True)
+    score = float(q[0, 0, 0, 0]) * float(k[0, 0, 0, 0])
+    tail = torch.tensor(-score, dtype=torch.float64).exp() * (Sk - 1)
+    want = (tail / (1 + tail)) * v[:, :, -1:].double()
+    u = torch.finfo(dt).eps / 2
+    rel = u * 1.01 + 2 * ((D + 2) * 2.0 ** -24 * score + 2.0 ** -22) + Sk * 2.0 ** -24
+    tol = (rel + u) * want + torch.finfo(dt).smallest_normal * u
+    assert ((o.double() - want).abs() <= tol).all(), (float(o.double().amax()), float(want.amax()))
+    assert (lse.double() - (score + float(torch.log1p(tail)))).abs().max() <= 2 * (D + 2) * 2.0 ** -24 * score + 2.0 ** -20
+
+
+def test_scores_that_rise_by_less_than_the_margin():
+    """Each tile's largest score a little above the last one's: float16's P goes to
+    2^15 and no further, with values up to the type's largest."""
+    D, Sk = 64, 64 * 40
+    for step in (0.5, 1.5, 2.07, 2.09, 4.0):  # nats per tile, around the margin of 3 bits
+        q, k = torch.zeros(1, 1, 130, D, device="cuda").half(), torch.zeros(1, 1, Sk, D, device="cuda").half()
+        q[..., 0] = 1
+        k[0, 0, :, 0] = (torch.arange(Sk, device="cuda") // 64) * step
+        v = torch.full((1, 1, Sk, D), 60000.0, device="cuda").half()
+        for n in (1, 130):
+            o = prism_amd.flash_attn_window(q[:, :, :n], k, v, None, causal=False, sm_scale=1.0)
+            assert ((o.float() / v[0, 0, 0, 0].float() - 1).abs() <= 2.0 ** -9).all(), step
