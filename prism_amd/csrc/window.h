@@ -35,8 +35,15 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 // o 0.0039 for 0.0027 with m at the largest score).  P up to 2^15 keeps all of a key's bits down to 2^-26
 // of the largest weight (18 nats) and some down to 2^-37; a margin of 3 moves the
 // reference no more than a few times in a list.
+//
+// Gradients.  The backward takes P, and with it dS = P (dP - delta), times 2^GRAD, and
+// the products' fp32 sums back by BACK: a float16 dS of 4,096 seen keys and do of 1e-3
+// is subnormal (dq and dk 5e-3 off norm-wise, 5e-2 at 1e-4).  With 2^6 what is lost
+// there stays below half of what dq's and dk's own rounding to float16 loses (2e-4 and
+// 8e-4; at 32,768 keys 7e-4 and 7e-3, beside 2e-3 and 2e-2), and dS may be up to 1,023
+// before it becomes infinite; 2^8 would bring little and leave 255.
 struct WinBf16 {
-  static constexpr float SHIFT = 0.0f, MARGIN = 8.0f;
+  static constexpr float SHIFT = 0.0f, MARGIN = 8.0f, GRAD = 0.0f, BACK = 1.0f;
   static __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -46,7 +53,7 @@ struct WinBf16 {
 };
 // (operands travel as bf16x8: eight 16-bit values whatever their type)
 struct WinF16 {
-  static constexpr float SHIFT = 12.0f, MARGIN = 3.0f;
+  static constexpr float SHIFT = 12.0f, MARGIN = 3.0f, GRAD = 6.0f, BACK = 0x1p-6f;
   static __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }

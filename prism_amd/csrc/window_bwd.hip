@@ -5,7 +5,7 @@
 //
 // window_dq_kernel, by 128 rows, over the key list of the forward: S^T and dP^T
 // keep one query per lane column, dQ^T += K^T dS^T.  It also forms delta and
-// leaves (m2, delta) = (lse log2 e, delta) of every row for the second kernel: from the
+// leaves (m2, delta) = (lse log2 e - GRAD, delta) of every row for the second kernel: from the
 // rows of do, o and o's rest (what its rounding left off, kept by the forward: with
 // the rounded o alone dq is 2.6e-3 off, norm-wise, bf16, with its rest 2.4e-3; of 235
 // us of a step of 2 x 4,096 tokens at D = 64 writing and reading it take 7), or, where rows see 64 keys at most, as sum_j P_j dP_j in a pass over
@@ -22,8 +22,9 @@
 // workgroups, whose fp32 sums window_merge_kernel adds in order.  No atomics: the
 // same bits every time; sums over the heads that share a key head are fp32.
 //
-// Numbers: P and dS are rounded to the inputs' type for the products (float16: a
-// dS beyond 65,504 becomes infinite, which a loss scaler sees), the rest is fp32.
+// Numbers: P and dS are rounded to the inputs' type for the products (float16: times
+// 2^GRAD, window.h; a dS beyond 1,023 becomes infinite, which a loss scaler sees), the
+// rest is fp32.
 //
 // Bound: the matrix cores at D = 128.  Measured: 14,040 tokens, 5 heads, D = 128, 4,680
 // to both sides, 1,560 sinks: dQ 405 + 6 us, dK/dV 575 + 12 (matrix cores busy 72% and 67%
@@ -38,7 +39,7 @@ namespace {
 struct WinBwdArgs {
   WinArgs w;                 // (w.o: the forward's output; w.lse: its lse)
   WinTensor do_, dq, dk, dv;
-  float* m2;                 // [B Hq, Sq]
+  float* m2;                 // [B Hq, Sq] lse log2 e - GRAD
   float* delta;              // [B Hq, Sq]
   // dK/dV items: the sink tiles of all heads, sink_splits pieces each, then the
   // other tiles, rest_whole whole and the others in rest_splits pieces; pieces of
@@ -169,8 +170,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_dq_kernel(WinBwdA
     if (w < 2 && t1 > t0 + 1) copy.issue(kl, 64 * t0, lds0 + (uint32_t)((t0 & 1) * T::STAGE));
   }
   dlt = xor32_add(dlt);
+  const float mg = mq - E::GRAD;  // P and dS from here on times 2^GRAD (window.h)
   if (r < rows && g == 0 && it.split == 0) {
-    ba.m2[lrow] = mq;
+    ba.m2[lrow] = mg;
     ba.delta[lrow] = dlt;
   }
 
@@ -224,7 +226,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_dq_kernel(WinBwdA
     for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
-        const float p = fast_exp2(__builtin_fmaf(sacc[kh][x], a.scale_log2, -mq));
+        const float p = fast_exp2(__builtin_fmaf(sacc[kh][x], a.scale_log2, -mg));
         pacc[kh][x] = FROM ? p * pacc[kh][x] : p * (pacc[kh][x] - dlt);
       }
     if (!whole || !ws.all(u0, u0 + 63)) {
@@ -266,11 +268,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_dq_kernel(WinBwdA
   }
   if (r >= rows) return;
   uint16_t* dqr = ba.dq.p + b * ba.dq.b + head * ba.dq.h + i * ba.dq.s;
+  const float f = a.scale * E::BACK;
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
     for (int jj = 0; jj < 4; jj += 2)
-      win_store<E>(dqr + 32 * dt + 8 * jj, g, win_scaled(dq[dt], jj, a.scale), win_scaled(dq[dt], jj + 1, a.scale));
+      win_store<E>(dqr + 32 * dt + 8 * jj, g, win_scaled(dq[dt], jj, f), win_scaled(dq[dt], jj + 1, f));
 }
 
 // ------------------------------------------------------------ dK / dV
@@ -645,8 +648,9 @@ __global__ __launch_bounds__(DkdvTiles<D>::THREADS, D == 64 ? 3 : 1) void window
     if (key >= a.Sk) continue;
 #pragma unroll
     for (int jj = 0; jj < 4; jj += 2) {
-      win_store<E>(dkr + 32 * dt + 8 * jj, g, win_scaled(dk[dt], jj, a.scale), win_scaled(dk[dt], jj + 1, a.scale));
-      win_store<E>(dvr + 32 * dt + 8 * jj, g, win_scaled(dv[dt], jj, 1.0f), win_scaled(dv[dt], jj + 1, 1.0f));
+      const float f = a.scale * E::BACK;
+      win_store<E>(dkr + 32 * dt + 8 * jj, g, win_scaled(dk[dt], jj, f), win_scaled(dk[dt], jj + 1, f));
+      win_store<E>(dvr + 32 * dt + 8 * jj, g, win_scaled(dv[dt], jj, E::BACK), win_scaled(dv[dt], jj + 1, E::BACK));
     }
   }
 }
@@ -678,7 +682,8 @@ __global__ __launch_bounds__(256) void window_dq_merge_kernel(WinBwdArgs ba) {
   const int i = r / a.G, head = it.hk * a.G + (r - i * a.G);
   uint16_t* out = ba.dq.p + it.b * ba.dq.b + head * ba.dq.h + i * ba.dq.s + 32 * dt;
 #pragma unroll
-  for (int j = 0; j < 4; j += 2) win_store<E>(out + 8 * j, g, win_scaled(acc[j], a.scale), win_scaled(acc[j + 1], a.scale));
+  for (int j = 0; j < 4; j += 2)
+    win_store<E>(out + 8 * j, g, win_scaled(acc[j], a.scale * E::BACK), win_scaled(acc[j + 1], a.scale * E::BACK));
 }
 
 // the pieces' sums of the cut key tiles (cut_sinks sink tiles, then the rest's),
@@ -719,7 +724,7 @@ __global__ __launch_bounds__(128 * key_tiles_of(D)) void window_merge_kernel(Win
     }
   const bool isk = blk < NDT;
   const WinTensor& t = isk ? a.dk : a.dv;
-  const float f = isk ? a.w.scale : 1.0f;
+  const float f = (isk ? a.w.scale : 1.0f) * E::BACK;
   uint16_t* out = t.p + b * t.b + hk * t.h + key * t.s + 32 * (isk ? blk : blk - NDT);
 #pragma unroll
   for (int j = 0; j < 4; j += 2) win_store<E>(out + 8 * j, g, win_scaled(acc[j], f), win_scaled(acc[j + 1], f));

@@ -168,3 +168,45 @@ def test_scores_that_rise_by_less_than_the_margin():
         for n in (1, 130):
             o = prism_amd.flash_attn_window(q[:, :, :n], k, v, None, causal=False, sm_scale=1.0)
             assert ((o.float() / v[0, 0, 0, 0].float() - 1).abs() <= 2.0 ** -9).all(), step
+
+
+def gradients64(q, k, v, do, mask):
+    """(dq, dk, dv) of softmax attention over a [Sq, Sk] mask, float64, one key head per query head."""
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    scale = q.shape[-1] ** -0.5
+    P = torch.softmax((q @ k.transpose(-1, -2).contiguous() * scale).masked_fill(~mask, -torch.inf), -1)
+    dP = do @ v.transpose(-1, -2).contiguous()
+    dS = P * (dP - (P * dP).sum(-1, keepdim=True))
+    return scale * (dS @ k), scale * (dS.transpose(-1, -2).contiguous() @ q), P.transpose(-1, -2).contiguous() @ do
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-4])
+@pytest.mark.parametrize("Sq,Sk,window", [(700, 5000, None), (5000, 5000, 4096), (40, 8000, None)])
+def test_float16_gradients_of_small_outputs(Sq, Sk, window, size, D):
+    """Norm-wise, what float16's range costs is what the results' own rounding
+    costs: independent roundings (P, dS, lse, the rest of o) of at most u each, in
+    quadrature 2 u, and the results' rounding with its subnormal steps (rounding the
+    exact results), a tenth more for the steps of dS far below them."""
+    q, k, v, do = (randn(1, 2, n, D, dt=torch.float16, seed=i) for i, n in enumerate((Sq, Sk, Sk, Sq)))
+    do = (do.float() * size).half()
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(prism_amd.flash_attn_window(*leaves, window), leaves, do)
+    p = torch.arange(Sq, device="cuda")[:, None] + Sk - Sq
+    j = torch.arange(Sk, device="cuda")[None]
+    want = gradients64(*[t.detach() for t in leaves], do, (j <= p) & (j > p - (window or 1 << 30)))
+    u = torch.finfo(torch.float16).eps / 2
+    for name, a, b in zip(("dq", "dk", "dv"), got, want):
+        err, own = float((a.double() - b).norm()), float((b.half().double() - b).norm())
+        assert err <= 2 * u * float(b.norm()) + 1.1 * own, name
+
+
+def test_float16_gradients_of_large_outputs():
+    """dS of several hundred is still finite and right."""
+    q, k, v = (randn(1, 2, 300, 64, dt=torch.float16, seed=i) for i in range(3))
+    do = (randn(1, 2, 300, 64, dt=torch.float16, seed=4).float() * 64).half()
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(prism_amd.flash_attn_window(*leaves, None, causal=False), leaves, do)
+    want = gradients64(*[t.detach() for t in leaves], do, torch.ones(300, 300, device="cuda", dtype=torch.bool))
+    for a, b in zip(got, want):  # (four roundings in quadrature and the results' own)
+        assert (a.double() - b).norm() <= 3 * torch.finfo(torch.float16).eps / 2 * b.norm()
