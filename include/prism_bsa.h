@@ -187,7 +187,7 @@ int prism_window_token(const void* q, const void* k, const void* v, int dtype, i
  * dv (rows that nothing reaches are 0).  rest: the forward's, or NULL.  strides (host): batch, head, token of
  * q, k, v, o, do, dq, dk, dv, as above.  rows: workspace of 2 * B * Hq * Sq
  * floats; acc: of as many floats as prism_window_bwd_plan says (NULL for 0;
- * its kv_lens: whether the call passes them).
+ * its kv_lens: whether the call passes them, which changes nothing).
  * Deterministic (no atomics). */
 int prism_window_bwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal,
                           int kv_lens, int64_t* floats);

@@ -741,7 +741,7 @@ int64_t key_slots(int D) { return D == 128 ? 256 : 768; }
 struct DkdvPlan {
   int64_t sink_tiles, key_tiles, sink_splits, sink_items, rest_whole, rest_splits, rest_tiles, items, pieces;
 };
-DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal, int lens) {
+DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal) {
   DkdvPlan p{};
   const int64_t keys = 64 * key_tiles_of(D);
   const int64_t BH = (int64_t)B * Hk, whole = G * ((Sq + 63) / 64);
@@ -758,13 +758,7 @@ DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int6
   p.sink_splits = p.sink_tiles ? (whole + n - 1) / n : 1;
   int64_t head = BH * p.sink_tiles * p.sink_splits;  // pieces before the rest's tiles
   const int64_t slots = key_slots(D), total = head + p.rest_tiles;
-  // Lengths (lens: the call passes them) stand on the device: at D = 64, where three
-  // workgroups share a CU, a batch that has them is cut as if three quarters of its
-  // tiles held anything (the others end at once, and last: rank_tile).  Measured with the
-  // merge (us, as for full sequences / so), 2 x 4,096 tokens, 16 heads over 4, window
-  // 1,024: 2,598 and 2,306 of them 82 / 66; 3,000 and 3,400 93 / 85; 3,900 and 4,096 98 /
-  // 106.  At D = 128 (and for the rows of the forward and dQ) it loses.
-  const WinCut c = win_cut(lens && D == 64 ? (3 * total + 3) / 4 : total, slots, rest, D);
+  const WinCut c = win_cut(total, slots, rest, D);
   p.rest_splits = c.splits;
   p.rest_whole = c.whole > head ? c.whole - head : 0;
   if (p.rest_whole > p.rest_tiles) p.rest_whole = p.rest_tiles;
@@ -789,12 +783,12 @@ int64_t bwd_floats(const DkdvPlan& p, const WinCut& c, int64_t row_tiles, int64_
 extern "C" {
 
 int prism_window_bwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal,
-                          int kv_lens, int64_t* floats) {
+                          int /*kv_lens*/, int64_t* floats) {
   PRISM_REQUIRE(B >= 0 && Hk >= 1 && Hq >= Hk && Hq % Hk == 0 && Sq >= 0 && Sk >= 0 && D >= 1 && window >= 1 &&
                     sinks >= 0 && floats,
                 "prism_window_bwd_plan: bad argument");
   const int64_t G = Hq / Hk;
-  *floats = bwd_floats(dkdv_plan(B, Hk, G, Sq, Sk, D, window, sinks, causal, kv_lens),
+  *floats = bwd_floats(dkdv_plan(B, Hk, G, Sq, Sk, D, window, sinks, causal),
                        win_row_cut(dq_slots(D), B, Hk, G, Sq, Sk, D, window, sinks, causal), (int64_t)B * Hk * ((Sq * G + 127) / 128), D);
   return PRISM_OK;
 }
@@ -823,7 +817,7 @@ int prism_window_bwd(const void* do_, const void* q, const void* k, const void* 
   a.w.tiles = (int)((Sq * a.w.G + 127) / 128);
   const int64_t total = (int64_t)B * Hk * a.w.tiles;
   const WinCut c = win_row_cut(dq_slots(D), B, Hk, a.w.G, Sq, Sk, D, window, sinks, causal);
-  const DkdvPlan p = dkdv_plan(B, Hk, a.w.G, Sq, Sk, D, window, sinks, causal, kv_lens != nullptr);
+  const DkdvPlan p = dkdv_plan(B, Hk, a.w.G, Sq, Sk, D, window, sinks, causal);
   const int64_t cut = total - c.whole, items = c.whole + cut * c.splits;
   PRISM_REQUIRE(items < (1ll << 31) && p.items < (1ll << 31), "prism_window_bwd: too many tiles");
   PRISM_REQUIRE(p.pieces + cut == 0 || acc, "prism_window_bwd: null workspace");

@@ -1,4 +1,5 @@
 """Corners of the layer's operators, on the CPU (no kernel runs)."""
+import ctypes
 import math
 
 import pytest
@@ -154,3 +155,21 @@ def test_adapter_keeps_no_positions():
         a, b = m._rotate(q.clone().requires_grad_(True), q, (2, 3, 4))
         assert a.requires_grad and b.requires_grad
         assert vars(m) == before
+
+
+def bwd_workspace(B, Hq, Hk, S, D, window, sinks, causal=1, lens=0, Sk=None):
+    """Bytes that the window backward's plan asks for, and those of its eight tensors."""
+    floats = ctypes.c_int64()
+    lib = prism_amd._lib.load()
+    assert lib.prism_window_bwd_plan(B, Hq, Hk, S, Sk or S, D, window, sinks, causal, lens, ctypes.byref(floats)) == 0
+    return 4 * floats.value, 2 * B * D * 4 * (Hq * S + Hk * (Sk or S))
+
+
+@pytest.mark.parametrize("case", [(2, 16, 4, 4096, 64, 1024, 4), (16, 32, 8, 2048, 64, 1024, 4), (24, 16, 16, 4096, 64, 1024, 4),
+                                  (24, 16, 16, 16384, 64, 4096, 4), (48, 40, 5, 32768, 64, 1024, 4),
+                                  (16, 32, 8, 2048, 128, 1024, 4), (3, 9, 9, 5000, 64, 300, 0)])
+def test_lengths_take_no_more_workspace(case):
+    """What the sequences' lengths are stands on the device: a call that passes them
+    is cut as one without, not by a guess of how much of the batch is padding."""
+    full, _ = bwd_workspace(*case)
+    assert bwd_workspace(*case, lens=1)[0] <= 2 * full
