@@ -737,7 +737,8 @@ int64_t dq_slots(int D) { return D == 128 ? 512 : 768; }
 int64_t key_slots(int D) { return D == 128 ? 256 : 768; }
 
 // How the dK/dV lists are cut, for one workgroup a CU (three at D = 64): the sinks' lists into
-// pieces no longer than the others, then the last round of tiles (win_cut).
+// pieces no longer than the others (or as two rounds of pieces allow), then the last
+// round of tiles (win_cut).
 struct DkdvPlan {
   int64_t sink_tiles, key_tiles, sink_splits, sink_items, rest_whole, rest_splits, rest_tiles, items, pieces;
 };
@@ -755,9 +756,18 @@ DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int6
   }
   const int64_t n = (rest > 8 ? rest : 8);
   p.rest_tiles = BH * (p.key_tiles - p.sink_tiles);
-  p.sink_splits = p.sink_tiles ? (whole + n - 1) / n : 1;
-  int64_t head = BH * p.sink_tiles * p.sink_splits;  // pieces before the rest's tiles
-  const int64_t slots = key_slots(D), total = head + p.rest_tiles;
+  const int64_t slots = key_slots(D), sinks_in = BH * p.sink_tiles;
+  // Two rounds of the sinks' pieces at most: a piece's sums are 131 KB at D = 128 (33 at
+  // 64), and pieces as short as the other lists would be terabytes of them where a
+  // narrow window stands beside many sinks.  Measured, dK/dV and merge, D = 128, with
+  // pieces of the others' length / up to eight rounds / four / two (us): 65,536 tokens,
+  // 32 heads over 8, window 256, 1,024 sinks 3,375 / 2,825 / 2,790 / 2,805; 2 x 16,384,
+  // window 64, 4,096 sinks 5,770 / 3,405 / 3,524 / 3,358; 20,000 tokens, 8 heads, window
+  // 256, 640 sinks 295 / 285 / 248 / 220; 19 heads, 2,000 sinks 1,515 / 940 / 883 / 902.
+  const int64_t most = sinks_in ? (2 * slots / sinks_in > 1 ? 2 * slots / sinks_in : 1) : 1;
+  p.sink_splits = p.sink_tiles ? (whole + n - 1) / n < most ? (whole + n - 1) / n : most : 1;
+  int64_t head = sinks_in * p.sink_splits;  // pieces before the rest's tiles
+  const int64_t total = head + p.rest_tiles;
   const WinCut c = win_cut(total, slots, rest, D);
   p.rest_splits = c.splits;
   p.rest_whole = c.whole > head ? c.whole - head : 0;
@@ -765,8 +775,8 @@ DkdvPlan dkdv_plan(int B, int Hk, int64_t G, int64_t Sq, int64_t Sk, int D, int6
   if (c.splits == 1) p.rest_whole = p.rest_tiles;
   if (c.whole == 0 && c.splits > 1 && p.sink_tiles) {  // less than a round: the sinks' pieces as short as the others
     const int64_t m = rest / c.splits > 8 ? rest / c.splits : 8;
-    p.sink_splits = (whole + m - 1) / m < 256 ? (whole + m - 1) / m : 256;
-    head = BH * p.sink_tiles * p.sink_splits;
+    p.sink_splits = (whole + m - 1) / m < most ? (whole + m - 1) / m : most;
+    head = sinks_in * p.sink_splits;
   }
   p.sink_items = head;
   p.items = head + p.rest_whole + (p.rest_tiles - p.rest_whole) * p.rest_splits;

@@ -210,3 +210,15 @@ def test_float16_gradients_of_large_outputs():
     want = gradients64(*[t.detach() for t in leaves], do, torch.ones(300, 300, device="cuda", dtype=torch.bool))
     for a, b in zip(got, want):  # (four roundings in quadrature and the results' own)
         assert (a.double() - b).norm() <= 3 * torch.finfo(torch.float16).eps / 2 * b.norm()
+
+
+@pytest.mark.parametrize("case", [(1, 2, 1, 3000, 128, 50, 700, True), (1, 4, 4, 2500, 64, 40, 1500, True),
+                                  (2, 20, 20, 1500, 128, 30, 900, True), (1, 3, 3, 2000, 128, 64, 640, False),
+                                  (1, 60, 60, 700, 64, 20, 500, True), (1, 300, 300, 400, 128, 20, 200, True)],
+                         ids=lambda c: "-".join(str(x) for x in c))
+def test_gradients_of_many_sinks_beside_a_narrow_window(case):
+    """The sinks' lists in many pieces, in few, and whole."""
+    from tests.test_gpu_window_bwd import check
+    B, Hq, Hk, S, D, window, sinks, causal = case
+    q, k, v, do = (randn(B, H, S, D, seed=i) for i, H in enumerate((Hq, Hk, Hk, Hq)))
+    check(q, k, v, do, window, sinks=sinks, causal=causal)

@@ -173,3 +173,18 @@ def test_lengths_take_no_more_workspace(case):
     is cut as one without, not by a guess of how much of the batch is padding."""
     full, _ = bwd_workspace(*case)
     assert bwd_workspace(*case, lens=1)[0] <= 2 * full
+
+
+def test_many_sinks_beside_a_narrow_window_take_a_bounded_workspace():
+    """Two rounds of pieces for the sinks' lists (67 MB at D = 128, 50 at 64) and the
+    cut of the last round, whatever the lengths: within the tensors and 128 MiB,
+    and within 256 MiB."""
+    for B in (1, 2, 8, 48):
+        for Hq, Hk in ((1, 1), (8, 1), (8, 8), (40, 5), (32, 8), (40, 40)):
+            for S in (1000, 4096, 16384, 75600, 131072, 300000):
+                for D in (64, 128):
+                    for window in (1, 64, 256, 1024):
+                        for sinks in (128, 640, 1000, 3600, 20000):
+                            for causal in (0, 1):
+                                work, tensors = bwd_workspace(B, Hq, Hk, S, D, window, sinks, causal)
+                                assert work <= min(tensors + (1 << 27), 1 << 28), (B, Hq, Hk, S, D, window, sinks, causal, work)
