@@ -349,12 +349,16 @@ void launch_norm(const NormArgs& a, hipStream_t stream) {
     rms_norm_kernel<E, VEC, I, W><<<grid, W == 16 ? 1024 : 256, 0, stream>>>(a);
   });
 }
+// up to `parts` workgroups, none without a row; returns how many
 template <class E, int VEC>
-void launch_norm_bwd(const NormBwdArgs& a, int parts, hipStream_t stream) {
+int launch_norm_bwd(const NormBwdArgs& a, int parts, hipStream_t stream) {
   for_shape<E, VEC>(a.N, [&](auto w, auto i) {
     constexpr int W = decltype(w)::value, I = decltype(i)::value;
+    const int64_t groups = W == 1 ? (a.M + 3) / 4 : a.M;
+    parts = groups < parts ? (int)groups : parts;
     rms_norm_bwd_kernel<E, VEC, I, W><<<(unsigned)parts, W == 16 ? 1024 : 256, 0, stream>>>(a);
   });
+  return parts;
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -387,9 +391,10 @@ int prism_rms_norm(const void* x, int64_t x_stride, const void* r, int64_t r_str
   return PRISM_OK;
 }
 
-// Workgroups of the backward, each of which walks rows and leaves a partial sum
-// of dw: at most one per row (four rows where a wave takes one); more of them keep
-// the memory busy, fewer leave less to add.  Measured (us, both kernels) with
+// Workgroups of the backward at most, each of which walks rows and leaves a partial
+// sum of dw; more of them keep the memory busy, fewer leave less to add.  Rows of 257 to
+// 2,048 elements go to a wave or to a workgroup by their type and alignment, which the
+// launch knows: it starts no workgroup without a row (launch_norm_bwd).  Measured (us, both kernels) with
 // 256 / 512 / 1,024: 1,024 rows of 1,536 bf16 8.1 / 8.9 / 11.2; 4,096 of 4,096 36 / 26 /
 // 25; 16,384 of 512 23 / 17 / 15, of 5,120 187 / 134 / 112; 1,024 rows of 16,384 (sixteen
 // waves a row) 28 / 33 / 45.
@@ -414,9 +419,9 @@ int prism_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh, int64_
   const int vec = 16 / elem_size(dtype);
   const bool wide = N % vec == 0 && dy_stride % vec == 0 && (!dh || dh_stride % vec == 0) && h_stride % vec == 0 &&
                     aligned16(dy) && aligned16(dh) && aligned16(h) && aligned16(w) && aligned16(dx);
-  if (dtype == PRISM_F32) wide ? launch_norm_bwd<ElemF32, 4>(a, parts, stream) : launch_norm_bwd<ElemF32, 1>(a, parts, stream);
-  else if (dtype == PRISM_BF16) wide ? launch_norm_bwd<ElemBf16, 8>(a, parts, stream) : launch_norm_bwd<ElemBf16, 1>(a, parts, stream);
-  else wide ? launch_norm_bwd<ElemF16, 8>(a, parts, stream) : launch_norm_bwd<ElemF16, 1>(a, parts, stream);
+  if (dtype == PRISM_F32) parts = wide ? launch_norm_bwd<ElemF32, 4>(a, parts, stream) : launch_norm_bwd<ElemF32, 1>(a, parts, stream);
+  else if (dtype == PRISM_BF16) parts = wide ? launch_norm_bwd<ElemBf16, 8>(a, parts, stream) : launch_norm_bwd<ElemBf16, 1>(a, parts, stream);
+  else parts = wide ? launch_norm_bwd<ElemF16, 8>(a, parts, stream) : launch_norm_bwd<ElemF16, 1>(a, parts, stream);
   if (dw) rms_norm_dw_kernel<<<(unsigned)((N + 31) / 32), 1024, 0, stream>>>(partial, parts, N, w_dtype, dw);
   PRISM_LAUNCH_CHECK("prism_rms_norm_bwd");
   return PRISM_OK;

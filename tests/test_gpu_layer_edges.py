@@ -222,3 +222,30 @@ def test_gradients_of_many_sinks_beside_a_narrow_window(case):
     B, Hq, Hk, S, D, window, sinks, causal = case
     q, k, v, do = (randn(B, H, S, D, seed=i) for i, H in enumerate((Hq, Hk, Hk, Hq)))
     check(q, k, v, do, window, sinks=sinks, causal=causal)
+
+
+# ------------------------------------------------------------------ sizes of launches
+@pytest.mark.parametrize("dt,code,M,N,groups", [
+    (torch.bfloat16, 1, 1024, 1536, 256), (torch.bfloat16, 1, 1024, 1535, 512), (torch.float32, 0, 90, 1024, 23),
+    (torch.float32, 0, 90, 1028, 90), (torch.float16, 2, 7, 2048, 2), (torch.float16, 2, 7, 2056, 7), (torch.bfloat16, 1, 1, 300, 1),
+    (torch.bfloat16, 1, 3000, 2048, 512), (torch.bfloat16, 1, 9, 256, 3), (torch.bfloat16, 1, 300, 9000, 256)])
+def test_norm_backward_starts_no_workgroup_without_a_row(dt, code, M, N, groups):
+    """A workgroup of the backward leaves its sums in a row of the workspace: the
+    rows past those that have rows of the input to add stay as they were."""
+    import ctypes
+    lib = prism_amd._lib.load()
+    parts = ctypes.c_int()
+    assert lib.prism_rms_norm_parts(M, N, ctypes.byref(parts)) == 0 and parts.value >= groups
+    x, dy, w = randn(M, N, dt=dt, seed=1), randn(M, N, dt=dt, seed=2), randn(N, dt=dt, seed=3)
+    inv = torch.rsqrt((x.float() ** 2).mean(-1) + 1e-6)
+    partial = torch.full((parts.value, N), 7.0, device="cuda")
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    rc = lib.prism_rms_norm_bwd(dy.data_ptr(), N, None, 0, x.data_ptr(), N, w.data_ptr(), code, code, M, N, inv.data_ptr(),
+                                dx.data_ptr(), partial.data_ptr(), parts.value, dw.data_ptr(),
+                                torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert (partial[groups:] == 7.0).all() and not (partial[:groups] == 7.0).all(1).any()
+    # each product and sum in fp32: (M + 4) 2^-24 of the terms' magnitudes, and dw's own rounding
+    want = (dy.double() * x.double() * inv.double()[:, None]).sum(0)
+    size = (dy.double() * x.double() * inv.double()[:, None]).abs().sum(0)
+    assert ((dw.double() - want).abs() <= (M + 4) * 2.0 ** -24 * size + torch.finfo(dt).eps / 2 * want.abs() + 2.0 ** -25).all()
