@@ -25,6 +25,9 @@ void prism_set_error(const char* fmt, ...);
     }                                            \
   } while (0)
 
+// A launch holds fewer than 2^32 threads per grid dimension.
+#define PRISM_MAX_THREADS (1ll << 32)
+
 #define PRISM_LAUNCH_CHECK(what)                                               \
   do {                                                                         \
     hipError_t _e = hipGetLastError();                                         \

@@ -31,7 +31,7 @@ struct RotaryArgs {
   void* o[2];
   int64_t xb[2], xh[2], xs[2], ob[2], oh[2], os[2];  // strides in elements
   int H[2];
-  int64_t tokens;                    // B * S
+  int64_t first, tokens;             // of this launch, of B * S
   int S, R, rot_units, units, tpb;   // units of a head: rot_units rotating, then copied; tokens per workgroup
   int heads_per;                     // heads (of q, then k) per blockIdx.y
   const double* freqs;               // [R/2] radians per position
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   constexpr int NP = VEC == 1 ? 1 : INTER ? VEC / 2 : VEC;  // pairs of a rotating unit
   constexpr int HEADS = 4;
   const int slot = (int)threadIdx.x / a.units, u = (int)threadIdx.x - slot * a.units;
-  const int64_t token = (int64_t)blockIdx.x * a.tpb + slot;
+  const int64_t token = a.first + (int64_t)blockIdx.x * a.tpb + slot;
   if (slot >= a.tpb || token >= a.tokens) return;
   const int b = (int)(token / a.S), n = (int)(token - (int64_t)b * a.S);
   const bool rot = u < a.rot_units;
@@ -159,9 +159,14 @@ void launch_rotary(RotaryArgs a, int D, bool inter, hipStream_t stream) {
   const int all = a.H[0] + a.H[1];
   const int64_t slices = gx >= 2048 ? 1 : (2048 + gx - 1) / gx;
   a.heads_per = slices >= all ? 1 : (int)((all + slices - 1) / slices);
-  const dim3 grid((unsigned)gx, (unsigned)((all + a.heads_per - 1) / a.heads_per));
-  if (inter) rotary_kernel<E, VEC, true><<<grid, kThreads, 0, stream>>>(a);
-  else rotary_kernel<E, VEC, false><<<grid, kThreads, 0, stream>>>(a);
+  const unsigned grid_y = (unsigned)((all + a.heads_per - 1) / a.heads_per);
+  const int64_t most = PRISM_MAX_THREADS / 2 / kThreads;  // workgroups at a time
+  for (int64_t at = 0; at < gx; at += most) {
+    const dim3 part((unsigned)(gx - at < most ? gx - at : most), grid_y);
+    a.first = at * a.tpb;
+    if (inter) rotary_kernel<E, VEC, true><<<part, kThreads, 0, stream>>>(a);
+    else rotary_kernel<E, VEC, false><<<part, kThreads, 0, stream>>>(a);
+  }
 }
 
 template <class E>

@@ -829,7 +829,8 @@ int prism_window_bwd(const void* do_, const void* q, const void* k, const void* 
   const WinCut c = win_row_cut(dq_slots(D), B, Hk, a.w.G, Sq, Sk, D, window, sinks, causal);
   const DkdvPlan p = dkdv_plan(B, Hk, a.w.G, Sq, Sk, D, window, sinks, causal);
   const int64_t cut = total - c.whole, items = c.whole + cut * c.splits;
-  PRISM_REQUIRE(items < (1ll << 31) && p.items < (1ll << 31), "prism_window_bwd: too many tiles");
+  PRISM_REQUIRE(items < PRISM_MAX_THREADS / 256 && p.items < PRISM_MAX_THREADS / (256 * key_tiles_of(D)),
+                "prism_window_bwd: too many tiles");
   PRISM_REQUIRE(p.pieces + cut == 0 || acc, "prism_window_bwd: null workspace");
   a.w.total = (int)total;
   a.w.whole = (int)c.whole; a.w.splits = (int)c.splits; a.w.items = (int)items;

@@ -347,7 +347,7 @@ int prism_window_fwd(const void* q, const void* k, const void* v, int dtype, int
   const int64_t total = (int64_t)B * Hk * a.tiles;
   const WinCut c = win_row_cut(fwd_slots(D), B, Hk, a.G, Sq, Sk, D, window, sinks, causal);
   const int64_t cut = total - c.whole, items = c.whole + cut * c.splits;
-  PRISM_REQUIRE(items < (1ll << 31), "prism_window_fwd: too many row tiles");
+  PRISM_REQUIRE(items < PRISM_MAX_THREADS / 256, "prism_window_fwd: too many row tiles");
   PRISM_REQUIRE(cut == 0 || part, "prism_window_fwd: null workspace");
   a.total = (int)total;
   a.whole = (int)c.whole; a.splits = (int)c.splits; a.items = (int)items;

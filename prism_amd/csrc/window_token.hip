@@ -372,7 +372,8 @@ int prism_window_token(const void* q, const void* k, const void* v, int dtype, i
   a.rest = (uint16_t*)rest;
   a.tiles = (int)((Sq * a.G + 31) / 32);
   const int64_t items = (int64_t)B * Hk * a.tiles;
-  PRISM_REQUIRE(items * splits < (1ll << 31) && items < (1ll << 28), "prism_window_token: too many row tiles");
+  PRISM_REQUIRE(items < PRISM_MAX_THREADS / 256 && (splits == 1 || items * (splits > 8 ? splits : 8) < PRISM_MAX_THREADS / 256),
+                "prism_window_token: too many row tiles");
   a.total = (int)items;
   a.splits = splits; a.part = part_o; a.part_ml = part_ml;
   const unsigned grid = (unsigned)(items * splits), join = (unsigned)(items * 8);

@@ -249,3 +249,31 @@ def test_norm_backward_starts_no_workgroup_without_a_row(dt, code, M, N, groups)
     want = (dy.double() * x.double() * inv.double()[:, None]).sum(0)
     size = (dy.double() * x.double() * inv.double()[:, None]).abs().sum(0)
     assert ((dw.double() - want).abs() <= (M + 4) * 2.0 ** -24 * size + torch.finfo(dt).eps / 2 * want.abs() + 2.0 ** -25).all()
+
+
+def test_more_rows_than_a_launch_holds():
+    """2^22 rows of a thousand threads each and more, 2^24 workgroups of tokens and
+    more: rows at the borders and the end give what they give alone."""
+    dt, M, N = torch.bfloat16, (1 << 22) + 5, 1025
+    x, r, w = torch.zeros(M, N, device="cuda", dtype=dt), torch.zeros(M, N, device="cuda", dtype=dt), randn(N, seed=1)
+    some = [slice(0, 3), slice((1 << 21) - 2, (1 << 21) + 3), slice((1 << 22) - 2, M)]
+    for i, s in enumerate(some):
+        x[s], r[s] = randn(s.stop - s.start, N, seed=i), randn(s.stop - s.start, N, seed=i + 9)
+    y, h, _, inv = prism_amd.ops.rms_norm(x, r, w, 1e-6, want_inv=True)
+    for s in some:
+        y2, h2, _, inv2 = prism_amd.ops.rms_norm(x[s], r[s], w, 1e-6, want_inv=True)
+        assert torch.equal(y[s], y2) and torch.equal(h[s], h2) and torch.equal(inv[s], inv2)
+    del y, h
+    codes, scales = prism_amd.rms_norm_quant(x, w, out_dtype=torch.int8)
+    for s in some:
+        c2, s2 = prism_amd.rms_norm_quant(x[s], w, out_dtype=torch.int8)
+        assert torch.equal(codes[s], c2) and torch.equal(scales[s], s2)
+    del x, r, codes
+    S, D = (1 << 25) + 3, 129  # (two tokens a workgroup)
+    q, at, freqs = torch.zeros(1, 1, S, D, device="cuda", dtype=dt), torch.arange(S, device="cuda"), prism_amd.rotary_frequencies(2)[0]
+    some = [slice(0, 3), slice((1 << 24) - 3, (1 << 24) + 3), slice(S - 5, S)]
+    for i, s in enumerate(some):
+        q[:, :, s] = randn(1, 1, s.stop - s.start, D, seed=i)
+    o = prism_amd.apply_rotary(q, None, freqs, at)
+    for s in some:
+        assert torch.equal(o[:, :, s], prism_amd.apply_rotary(q[:, :, s], None, freqs, at[s]))

@@ -188,3 +188,20 @@ def test_many_sinks_beside_a_narrow_window_take_a_bounded_workspace():
                             for causal in (0, 1):
                                 work, tensors = bwd_workspace(B, Hq, Hk, S, D, window, sinks, causal)
                                 assert work <= min(tensors + (1 << 27), 1 << 28), (B, Hq, Hk, S, D, window, sinks, causal, work)
+
+
+def test_launches_of_too_many_tiles_are_refused():
+    """A launch holds fewer than 2^32 threads (before any launch: status 1, and no
+    memory is touched)."""
+    lib, one = prism_amd._lib.load(), ctypes.c_void_p(16)
+    st = (ctypes.c_int64 * 24)(*[64] * 24)
+    shape = lambda B, Sq: (1, B, 1, 1, Sq, 9, 64, st, 3, 0, 1, None, None, 0.1)  # noqa: E731
+    for B in (1 << 24, 1 << 30):
+        assert lib.prism_window_token(one, one, one, *shape(B, 1), one, None, None, 1, None, None, None) == 1
+        assert b"too many" in lib.prism_last_error()
+        assert lib.prism_window_fwd(one, one, one, *shape(B, 40), one, None, None, one, None) == 1
+        assert b"too many" in lib.prism_last_error()
+        assert lib.prism_window_bwd(one, one, one, one, one, None, one, *shape(B, 40), one, one, one, one, one, None) == 1
+        assert b"too many" in lib.prism_last_error()
+    assert lib.prism_window_token(one, one, one, *shape(1 << 21, 1), one, None, None, 2, one, one, None) == 1
+    assert b"too many" in lib.prism_last_error()
