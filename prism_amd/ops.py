@@ -34,8 +34,9 @@ _timings: Optional[Dict[str, List[Tuple[torch.cuda.Event, torch.cuda.Event]]]] =
 
 @contextlib.contextmanager
 def kernel_timing():
-    """Record HIP events around every C-ABI launch made inside the block (but
-    the backward launches of the layer operators, whose autograd nodes are C++).
+    """Record HIP events around every C-ABI launch made inside the block (of the
+    layer operators' backward launches, whose autograd nodes are C++, around those
+    whose forward ran inside the block too).
     Yields a dict name -> list of (start, end) events; after a synchronize,
     ``summarize(d)`` gives per-entry-point call counts and average ms."""
     global _timings
@@ -66,7 +67,34 @@ def _op(name: str, *args):
     out = fn(*args)
     en.record()
     _timings.setdefault(key, []).append((st, en))
+    if name in _NODE_LAUNCHES and out[0].grad_fn is not None:
+        _time_node(out[0].grad_fn, _NODE_LAUNCHES[name])
     return out
+
+
+# Operators whose gradients are C++ nodes, and what those launch
+_NODE_LAUNCHES = {"rms_norm": "prism_rms_norm_bwd", "rotary": "prism_rotary", "window_fwd": "prism_window_bwd"}
+
+
+def _time_node(node, key: str):
+    """Bracket a node's launches by events, on the stream that the engine runs it
+    on, in the block that is open then."""
+    begun = []
+
+    def before(grads):
+        if _timings is not None:
+            begun.append(torch.cuda.Event(enable_timing=True))
+            begun[-1].record()
+
+    def after(grads, _):
+        if begun:
+            st, en = begun.pop(), torch.cuda.Event(enable_timing=True)
+            en.record()
+            if _timings is not None:
+                _timings.setdefault(key, []).append((st, en))
+
+    node.register_prehook(before)
+    node.register_hook(after)
 
 
 def _opt(t: torch.Tensor) -> Optional[torch.Tensor]:

@@ -277,3 +277,38 @@ def test_more_rows_than_a_launch_holds():
     o = prism_amd.apply_rotary(q, None, freqs, at)
     for s in some:
         assert torch.equal(o[:, :, s], prism_amd.apply_rotary(q[:, :, s], None, freqs, at[s]))
+
+
+def test_kernel_timing_sees_backward_launches():
+    """Forward and backward launches, by entry point, on the stream they run on;
+    nothing is left of the block outside it."""
+    from prism_amd import ops
+    freqs, at = prism_amd.rotary_frequencies(64)[0], torch.arange(70, device="cuda")
+    x, w, kv = randn(2, 70, 256, seed=1), randn(256, seed=2), randn(2, 2, 70, 64, seed=3)
+
+    def forward(grad):
+        leaves = [t.clone().requires_grad_(grad) for t in (x, w, kv)]
+        q = prism_amd.rms_norm(leaves[0], leaves[1]).view(2, 70, 4, 64).transpose(1, 2)
+        q, k = prism_amd.apply_rotary(q, leaves[2], freqs, at)
+        return leaves, prism_amd.flash_attn_window(q, k, k, 20, sinks=2)
+
+    def step():
+        leaves, o = forward(True)
+        return [o.detach(), *torch.autograd.grad(o, leaves, torch.ones_like(o))]
+
+    want = step()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with ops.kernel_timing() as tm, torch.cuda.stream(stream):
+        got = [step() for _ in range(3)]
+        forward(False)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+    calls = {name: n for name, (n, ms) in ops.summarize(tm).items() if ms > 0}
+    assert calls == {"prism_rms_norm": 4, "prism_rms_norm_bwd": 3, "prism_rotary": 7, "prism_window_fwd": 4, "prism_window_bwd": 3}
+    with ops.kernel_timing() as tm:
+        leaves, o = forward(True)
+    grads = torch.autograd.grad(o, leaves, torch.ones_like(o))
+    assert all(torch.equal(a, b) for a, b in zip(grads, want[1:]))
+    torch.cuda.synchronize()
+    assert {name: n for name, (n, _) in ops.summarize(tm).items()} == {"prism_rms_norm": 1, "prism_rotary": 1, "prism_window_fwd": 1}
