@@ -274,7 +274,9 @@ struct StageCopy {
 // others four empty ones.  Measured (us, by sequences / by rank): 2,598 and 2,306
 // tokens of 4,096, 16 heads over 4, D = 64, window 1,024: forward 46 / 35, dQ 50 /
 // 42, dK/dV 88 / 76; three sequences of 1,500 to 2,700, 12 heads over 4, D = 128,
-// window 2,000: forward 86 / 61, dQ 107 / 77.
+// window 2,000: forward 86 / 61, dQ 107 / 77.  (With as many heads as an XCD group has
+// items, tiles that share tokens stand in different XCDs: dK/dV of the first case
+// reads 309 MB for 42 MB of inputs.)
 struct RankedTile {
   int b, hk, rank;
   bool live;  // else the rank-th of the tiles past the end
@@ -312,6 +314,8 @@ __device__ __forceinline__ RankedTile rank_tile(int c, int B, int Hk, int tiles,
 // Work item -> (sequence, key head, row tile), part of its list and workspace
 // slot (-1: whole).  Row tiles of one key head are neighbours (their windows
 // overlap in an XCD's L2), the last ones, whose causal lists are longest, first.
+// (Without the causal mask the longest lists are in the middle: neither this order nor
+// the choice of the cut tiles goes by length there, and launches end less evenly.)
 struct WinItem {
   int b, hk, tile, split, slot;
 };

@@ -27,9 +27,11 @@
 // rest is fp32.
 //
 // Bound: the matrix cores at D = 128.  Measured: 14,040 tokens, 5 heads, D = 128, 4,680
-// to both sides, 1,560 sinks: dQ 405 + 6 us, dK/dV 575 + 12 (matrix cores busy 72% and 67%
-// of the cycles); 2 x 4,096 padded tokens (half to all of them), 16 heads over 4, D =
-// 64, window 1,024: dQ 50-58 us, dK/dV 55-93 + 12.
+// to both sides, 1,560 sinks: dQ 402-418 + 6 us, dK/dV 559-579 + 11 (matrix cores busy
+// 71% and 68% of the cycles); 2 x 4,096 padded tokens (half to all of them), 16 heads
+// over 4, D = 64, window 1,024: dQ 45-75 us, dK/dV 76-101 + 5.  There nothing is full
+// (matrix cores 28% in dK/dV, 36% in dQ): launches of one round, whose tiles read
+// their tokens and keys past the L2 (dK/dV 309 MB, dQ 173, of 42 MB of inputs).
 #include <type_traits>
 
 #include "window.h"

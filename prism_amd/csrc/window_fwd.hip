@@ -20,8 +20,8 @@
 // Bound: the matrix cores and the exponentials' VALU beside each other, at D = 64
 // the VALU (each score costs the same there for half the products).  Measured: 16,001
 // tokens, 32 heads over 8, D = 128, window 4,096, 16 sinks 905-970 us (0.97-1.04
-// PFLOP/s of seen pairs; matrix cores busy 53% of the cycles, VALU 51%); 14,040
-// tokens, 5 heads, D = 128, 4,680 to both sides, 1,560 sinks 336 + 11 us.
+// PFLOP/s of seen pairs; matrix cores busy 55% of the cycles, VALU 53%); 14,040
+// tokens, 5 heads, D = 128, 4,680 to both sides, 1,560 sinks 339-348 + 9 us.
 #include "window.h"
 
 namespace {

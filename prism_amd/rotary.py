@@ -82,8 +82,8 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor
     [S] or [B, S]; with sections (channels per axis, summing to 2 * pairs, at
     most 4 axes) one entry per axis in a last dimension.  interleaved: pairs of
     channels (2p, 2p + 1), else (p, p + pairs).  amplitude scales the turned
-    channels.  Returns q', with k (q', k').  Differentiable in q and k (freqs that
-    require gradients are refused)."""
+    channels.  Returns q', with k (q', k').  Differentiable in q and k (once; no
+    forward mode; freqs that require gradients are refused)."""
     qs, ks, pairs = q.shape, None if k is None else k.shape, freqs.shape
     for s, name in ((qs, "q"), (ks, "k")):
         if s is not None and len(s) != 4:

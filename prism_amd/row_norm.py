@@ -42,7 +42,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
     residual.  x: [..., N] (N up to 16,384) float32, bfloat16 or float16;
     weight: [N] of x's dtype or float32, or None for ones; residual: x's shape
     and dtype, or None.  Returns y in x's dtype, with a residual (y, h).
-    Differentiable in x, weight, residual, from y and h."""
+    Differentiable in x, weight, residual, from y and h (once; no forward mode)."""
     _check(x, weight, residual, eps, "rms_norm")
     y, h, _, _ = ops.rms_norm(x, residual, weight, eps)
     return y if residual is None else (y, h)

@@ -48,7 +48,9 @@ def flash_attn_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window:
     of the scaled scores, -inf where nothing is seen (no gradient through it).
     Differentiable in q, k, v; sums over shared heads are fp32.  The backward
     keeps q, k, v, o, lse and (where queries see more than 64 keys) what o's
-    rounding left off, of o's size."""
+    rounding left off, of o's size.  float16: P (dP - delta) beyond 1,023 becomes
+    infinite, which a loss scaler sees.  No second and no forward-mode derivatives
+    (refused)."""
     qs, ks, vs, dt = q.shape, k.shape, v.shape, q.dtype
     if len(qs) != 4 or len(ks) != 4 or len(vs) != 4:
         raise ValueError("q, k, v must be [B, H, S, D]")
