@@ -41,8 +41,8 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, sections: Opti
         raise ValueError(f"base must be above 1 and factor at least 1, got {base} and {factor}")
     if scaling == "yarn" and (original_length is None or original_length < 1):
         raise ValueError("yarn scaling needs the original_length that the model was trained on")
-    if scaling == "yarn" and not math.inf > beta_fast > beta_slow > 0:
-        raise ValueError(f"beta_fast must be above beta_slow, and both positive, got {beta_fast} and {beta_slow}")
+    if scaling == "yarn" and not math.inf > beta_fast >= beta_slow > 0:
+        raise ValueError(f"beta_fast must not be below beta_slow, and both positive, got {beta_fast} and {beta_slow}")
     amplitude, out = 1.0, []
     for d in parts:
         b = float(base)

@@ -30,7 +30,7 @@ def test_yarn_ramp_past_the_last_pair(dim, factor, length):
             assert share < 1.0 and float(f[i]) > plain / factor
 
 
-@pytest.mark.parametrize("betas", [(1.0, 32.0), (4.0, 4.0), (32.0, 0.0), (32.0, -1.0), (math.nan, 1.0), (32.0, math.nan),
+@pytest.mark.parametrize("betas", [(1.0, 32.0), (32.0, 0.0), (32.0, -1.0), (math.nan, 1.0), (32.0, math.nan),
                                    (math.inf, 1.0)])
 def test_yarn_refuses_ends_out_of_order(betas):
     fast, slow = betas
