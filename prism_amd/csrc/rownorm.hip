@@ -349,10 +349,11 @@ void launch_norm(NormArgs a, hipStream_t stream) {
     // (64 W threads a row: as many rows at a time as half of what a launch holds)
     constexpr int64_t most = PRISM_MAX_THREADS / 2 / (64 * W), es = sizeof(typename E::type);
     const int64_t oes = a.out < PRISM_E4M3 ? es : 1;
-    for (int64_t left = a.M; left > 0; left -= most) {
+    for (int64_t left = a.M;; left -= most) {
       a.M = left < most ? left : most;
       const unsigned grid = (unsigned)(W == 1 ? (a.M + 3) / 4 : a.M);
       rms_norm_kernel<E, VEC, I, W><<<grid, W == 16 ? 1024 : 256, 0, stream>>>(a);
+      if (left <= most) return;
       a.x = (const char*)a.x + most * a.xs * es;
       if (a.r) a.r = (const char*)a.r + most * a.rs * es;
       if (a.h) a.h = (char*)a.h + most * a.N * es;
