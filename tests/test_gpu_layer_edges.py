@@ -37,6 +37,10 @@ def test_vmap_gives_the_bits_of_a_loop():
         runs.append([*out, *torch.autograd.grad(out, leaves, [randn(*o.shape, seed=9) for o in out])])
     assert all(torch.equal(a, b) for a, b in zip(*runs))
 
+    for out_dtype in (torch.float8_e4m3fn, torch.int8):
+        got = torch.vmap(lambda t: prism_amd.rms_norm_quant(t, w, out_dtype=out_dtype))(x)  # noqa: B023
+        each = [prism_amd.rms_norm_quant(t, w, out_dtype=out_dtype) for t in x]
+        assert all(torch.equal(a.float(), torch.stack([e[i].float() for e in each])) for i, a in enumerate(got))
     leaves = [t.clone().requires_grad_(True) for t in (x[0], w, q[0])]
     y = prism_amd.rms_norm(leaves[0], leaves[1])
     o = prism_amd.flash_attn_window(*[prism_amd.apply_rotary(leaves[2], None, freqs, at[0])] * 3, 5)
