@@ -123,8 +123,8 @@ int prism_rms_norm(const void* x, int64_t x_stride, const void* r, int64_t r_str
 /* Gradients of prism_rms_norm: dx [M, N] (r has the same one) = s (g - xh
  * mean(g xh)) + dh with g = dy w, xh = h s, s = inv, and dw [N] (w_dtype; NULL
  * to skip) = sum over rows of dy xh.  dh: gradient of h, or NULL.  partial:
- * workspace of parts * N floats for dw (prism_rms_norm_parts), added in a fixed
- * order. */
+ * workspace of parts * N floats for dw (prism_rms_norm_parts; rows of it past the
+ * workgroups that have rows of h stay as they are), added in a fixed order. */
 int prism_rms_norm_parts(int64_t M, int N, int* parts);
 int prism_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh, int64_t dh_stride, const void* h,
                        int64_t h_stride, const void* w, int w_dtype, int dtype, int64_t M, int N, const float* inv,
@@ -188,7 +188,8 @@ int prism_window_token(const void* q, const void* k, const void* v, int dtype, i
  * q, k, v, o, do, dq, dk, dv, as above.  rows: workspace of 2 * B * Hq * Sq
  * floats; acc: of as many floats as prism_window_bwd_plan says (NULL for 0;
  * its kv_lens: whether the call passes them, which changes nothing).
- * Deterministic (no atomics). */
+ * float16: P (dP - delta) beyond 1,023 becomes infinite.  Deterministic (no
+ * atomics). */
 int prism_window_bwd_plan(int B, int Hq, int Hk, int64_t Sq, int64_t Sk, int D, int64_t window, int64_t sinks, int causal,
                           int kv_lens, int64_t* floats);
 int prism_window_bwd(const void* do_, const void* q, const void* k, const void* v, const void* o, const void* rest,
