@@ -38,6 +38,9 @@ extern "C" {
 #define PRISM_E4M3 3
 #define PRISM_I8 4
 
+/* partial rows of prism_qk_norm_rotary_bwd, and its largest number of heads */
+#define PRISM_HEAD_PARTS 1024
+
 /* Message of the last failed call on this host thread ("" if none). */
 const char* prism_last_error(void);
 /* ABI version of this library. */
@@ -129,6 +132,30 @@ int prism_rms_norm_parts(int64_t M, int N, int* parts);
 int prism_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh, int64_t dh_stride, const void* h,
                        int64_t h_stride, const void* w, int w_dtype, int dtype, int64_t M, int N, const float* inv,
                        void* dx, float* partial, int parts, void* dw, hipStream_t stream);
+
+/* ------------------------------------------------------------------ norms and positions of heads */
+
+/* Every head of q [B, Hq, S, D] and k [B, Hk, S, D] (Hq or Hk = 0: none) divided by
+ * the root of its mean square plus eps, times wq / wk ([D] of wdtype: dtype or
+ * PRISM_F32; NULL: ones), then turned as prism_rotary does (R, freqs, pos ...
+ * amplitude as there, strides of q, out_q, k, out_k).  D <= 256, at most
+ * PRISM_HEAD_PARTS heads in all.  Outputs must not overlap inputs.  No counterpart
+ * in the reference (its norms are over whole tokens, wan_video_dit.py:699-705). */
+int prism_qk_norm_rotary(const void* q, const void* k, int dtype, int B, int64_t S, int Hq, int Hk, int D, int R,
+                         const int64_t* strides, const void* wq, const void* wk, int wdtype, float eps,
+                         const double* freqs, const void* pos, int pos64, const int64_t* pos_strides, int axes,
+                         const int32_t* axis_end, int interleaved, float amplitude, void* out_q, void* out_k,
+                         hipStream_t stream);
+/* Its gradients: dq, dk from dyq, dyk (strides of dyq, q, dq, dyk, k, dk), and dwq,
+ * dwk [D] (wdtype; NULL to skip), sums over tokens and heads by way of partial, a
+ * workspace of 2 * PRISM_HEAD_PARTS * D floats (NULL where neither is asked for),
+ * added in a fixed order. */
+int prism_qk_norm_rotary_bwd(const void* dyq, const void* dyk, const void* q, const void* k, int dtype, int B, int64_t S,
+                             int Hq, int Hk, int D, int R, const int64_t* strides, const void* wq, const void* wk,
+                             int wdtype, float eps, const double* freqs, const void* pos, int pos64,
+                             const int64_t* pos_strides, int axes, const int32_t* axis_end, int interleaved,
+                             float amplitude, void* dq, void* dk, float* partial, void* dwq, void* dwk,
+                             hipStream_t stream);
 
 /* ------------------------------------------------------------------ rotary positions */
 

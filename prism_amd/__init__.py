@@ -14,6 +14,7 @@ Public surface (reference names):
 and what the layer runs around it (wan_video_dit.py:699-705):
   rms_norm, rms_norm_quant    residual addition + root-mean-square norm, 8-bit output
   rotary_frequencies, apply_rotary, grid_positions  rotary positions on q and k
+  qk_norm_rotary              norm of every head of q and k, and its rotary positions
 All compute runs in libprism_bsa.so, reached through the torch.ops.prism
 operators of libprism_torch.so (build: python prism_amd/build.py).
 """
@@ -25,6 +26,7 @@ from .dynamic_block_shape import (  # noqa: F401
 from .dynamic_block_attention import _TILE, flash_attn_bsa_3d_dynamic, plan_dynamic  # noqa: F401
 from .adapter import DynamicBlockSparseAttention, a2v_bridge_projection, a2v_token_norms, valid_mask_for  # noqa: F401
 from .rotary import apply_rotary, grid_positions, rotary_frequencies  # noqa: F401
+from .head_norm import qk_norm_rotary  # noqa: F401
 from .row_norm import rms_norm, rms_norm_quant  # noqa: F401
 from .uniform_block_attention import flash_attn_bsa, flash_attn_bsa_3d, flash_attn_bsa_cross  # noqa: F401
 from .window_attention import flash_attn_window  # noqa: F401

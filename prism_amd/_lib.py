@@ -31,6 +31,9 @@ SIGNATURES = {
     "prism_rms_norm_parts": [I64, I32, P],
     "prism_rms_norm_bwd": [P, I64, P, I64, P, I64, P, I32, I32, I64, I32, P, P, P, I32, P, P],
     "prism_rotary": [P, P, I32, I32, I64, I32, I32, I32, I32, P, P, P, I32, P, I32, P, I32, F32, I32, P, P, P],
+    "prism_qk_norm_rotary": [P, P, I32, I32, I64, I32, I32, I32, I32, P, P, P, I32, F32, P, P, I32, P, I32, P, I32, F32, P, P, P],
+    "prism_qk_norm_rotary_bwd": [P, P, P, P, I32, I32, I64, I32, I32, I32, I32, P, P, P, I32, F32, P, P, I32, P, I32, P, I32, F32,
+                                 P, P, P, P, P, P],
     "prism_window_fwd_plan": [I32, I32, I32, I64, I64, I32, I64, I64, I32, P],
     "prism_window_rest": [I64, I64, I64, I32],
     "prism_window_fwd": [P, P, P, I32, I32, I32, I32, I64, I64, I32, P, I64, I64, I32, P, P, F32, P, P, P, P, P],

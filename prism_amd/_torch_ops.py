@@ -54,7 +54,7 @@ def _register_vmaps():
     def one(t, d, i):
         return t if d is None or not isinstance(t, torch.Tensor) else t.select(d, i)
 
-    for name in ("rms_norm", "rms_norm_bwd", "rotary", "window_fwd"):
+    for name in ("rms_norm", "rms_norm_bwd", "rotary", "window_fwd", "qk_norm_rotary", "qk_norm_rotary_bwd"):
         if not hasattr(torch.ops.prism, name):  # (a library built before, as for the fakes)
             continue
 
@@ -130,6 +130,15 @@ def _register_fakes():
     @reg("prism::rotary")
     def _(q, k, freqs, positions, axis_pairs, interleaved, amplitude, inverse):
         return [like(t) for t in (q, k) if t is not None]
+
+    @reg("prism::qk_norm_rotary")
+    def _(q, k, q_weight, k_weight, eps, freqs, positions, axis_pairs, interleaved, amplitude):
+        return [like(t) for t in (q, k) if t is not None]
+
+    @reg("prism::qk_norm_rotary_bwd")
+    def _(dyq, dyk, q, k, q_weight, k_weight, eps, freqs, positions, axis_pairs, interleaved, amplitude, want_dwq, want_dwk):
+        return ([like(x) for x, g in ((q, dyq), (k, dyk)) if g is not None]
+                + [_empty(w, w.shape, w.dtype) for w, want in ((q_weight, want_dwq), (k_weight, want_dwk)) if want])
 
     @reg("prism::window_fwd")
     def _(q, k, v, window, sinks, causal, q_lens, kv_lens, sm_scale, want_lse, want_rest):

@@ -10,6 +10,9 @@
 #define PRISM_E4M3 3
 #define PRISM_I8 4
 
+// partial rows of the head norms' weight gradients (prism_qk_norm_rotary_bwd)
+#define PRISM_HEAD_PARTS 1024
+
 #define PRISM_OK 0
 #define PRISM_EINVAL 1
 #define PRISM_EHIP 2

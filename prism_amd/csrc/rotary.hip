@@ -20,12 +20,13 @@
 // TB/s); 8 tokens 4.8 us.
 #include <type_traits>
 
+#include "angles.h"
 #include "common.h"
 #include "elements.h"
 
 namespace {
 
-constexpr int kThreads = 256, kMaxHeadDim = 256, kMaxAxes = 4;
+constexpr int kThreads = 256, kMaxHeadDim = 256;
 
 struct RotaryArgs {
   const void* x[2];                  // q, k: [B, H, S, D], channels adjacent
@@ -42,27 +43,6 @@ struct RotaryArgs {
   float amp;
   double sign;
 };
-
-// sine and cosine of t turns
-__device__ __forceinline__ void sincos_turns(double t, float& s, float& c) {
-  const double q = rint(4.0 * t);
-  const float x = (float)(t - 0.25 * q) * 6.28318530717958647692f;
-  const float z = x * x;
-  float ps = 2.75573192e-6f;                       // 1/9!
-  ps = __builtin_fmaf(ps, z, -1.98412698e-4f);     // 1/7!
-  ps = __builtin_fmaf(ps, z, 8.33333333e-3f);      // 1/5!
-  ps = __builtin_fmaf(ps, z, -1.66666667e-1f);     // 1/3!
-  ps = __builtin_fmaf(ps * z, x, x);
-  float pc = 2.48015873e-5f;                       // 1/8!
-  pc = __builtin_fmaf(pc, z, -1.38888889e-3f);     // 1/6!
-  pc = __builtin_fmaf(pc, z, 4.16666667e-2f);      // 1/4!
-  pc = __builtin_fmaf(pc, z, -0.5f);
-  pc = __builtin_fmaf(pc, z, 1.0f);
-  const int k = (int)(q - 4.0 * floor(0.25 * q));  // quarter turns mod 4
-  const float a = (k & 1) ? pc : ps, b = (k & 1) ? ps : pc;
-  s = (k & 2) ? -a : a;
-  c = (k == 1 || k == 2) ? -b : b;
-}
 
 // VEC channels per unit (VEC = 1: one pair, or one copied channel, per unit)
 template <class E, int VEC, bool INTER>

@@ -1,0 +1,216 @@
+// PyTorch operators of packed batches and paged caches, and of the heads' norms
+// before them (TORCH_LIBRARY_FRAGMENT(prism)); checks, allocation, streams and
+// gradients as in torch_layer_ops.cpp.
+#include "torch_layer.h"
+
+namespace {
+
+// ------------------------------------------------------------------ norms and positions of heads
+// positions [S], [B, S], and with axes [S, A], [B, S, A], as the kernels take them
+struct Places {
+  int64_t strides[3];
+  int32_t axis_end[4] = {};
+  int axes;
+  bool is64;
+};
+Places places_of(const char* op, const Tensor& pos, c10::IntArrayRef axis_pairs, int64_t B, int64_t S, int64_t pairs) {
+  TORCH_CHECK_TYPE(pos.scalar_type() == at::kInt || pos.scalar_type() == at::kLong,
+                   "prism: positions must be int32 or int64, got ", pos.scalar_type());
+  const bool has_axis = !axis_pairs.empty();
+  const int64_t A = has_axis ? (int64_t)axis_pairs.size() : 1, rank = pos.dim() - (has_axis ? 1 : 0);
+  TORCH_CHECK_VALUE((rank == 1 || rank == 2) && pos.size(rank - 1) == S &&
+                        (rank == 1 || pos.size(0) == B || pos.size(0) == 1) && (!has_axis || pos.size(-1) == A),
+                    op, ": positions must be [S] or [B, S]", has_axis ? " with one entry per axis" : "", ", got ", pos.sizes());
+  TORCH_CHECK_VALUE(A <= 4, op, ": at most 4 axes");
+  Places p;
+  p.strides[0] = rank == 2 && pos.size(0) > 1 ? pos.stride(0) : 0;
+  p.strides[1] = pos.stride(rank - 1);
+  p.strides[2] = has_axis ? pos.stride(-1) : 0;
+  int64_t at = 0;
+  for (int64_t a = 0; a < A; ++a) {
+    at += has_axis ? axis_pairs[a] : pairs;
+    TORCH_CHECK_VALUE(!has_axis || axis_pairs[a] >= 0, op, ": negative axis size");
+    p.axis_end[a] = small(at, "pairs");
+  }
+  p.axes = (int)A;
+  p.is64 = pos.scalar_type() == at::kLong;
+  return p;
+}
+
+struct HeadCall {  // the checked arguments of both directions
+  int dt, wdt;
+  int64_t B, S, D, Hq, Hk;
+};
+HeadCall check_heads(const char* op, const Tensor& q, const OptT& k, const OptT& wq, const OptT& wk, const Tensor& freqs,
+                     const Tensor& pos) {
+  on_gpu(q, "q");
+  same_device(q, k, "k");
+  same_device(q, wq, "q_weight");
+  same_device(q, wk, "k_weight");
+  same_device(q, freqs, "freqs");
+  same_device(q, pos, "positions");
+  TORCH_CHECK_VALUE(q.dim() == 4, op, ": q must be [B, H, S, D]");
+  HeadCall c;
+  c.dt = type_code(q, op);
+  check_dtype(k, q.scalar_type(), "k");
+  check_dtype(freqs, at::kDouble, "freqs");
+  TORCH_CHECK_VALUE(freqs.dim() == 1, op, ": freqs must be [pairs]");
+  c.B = q.size(0); c.Hq = q.size(1); c.S = q.size(2); c.D = q.size(3);
+  c.Hk = k ? k->size(1) : 0;
+  if (k)
+    TORCH_CHECK_VALUE(k->dim() == 4 && k->size(0) == c.B && k->size(2) == c.S && k->size(3) == c.D, op,
+                      ": k must be [B, Hk, S, D] with q's B, S and D");
+  TORCH_CHECK_VALUE(k || !wk, op, ": k_weight without k");
+  c.wdt = wq ? type_code(*wq, "q_weight") : wk ? type_code(*wk, "k_weight") : c.dt;
+  for (const OptT* w : {&wq, &wk})
+    if (*w) {
+      TORCH_CHECK_VALUE((*w)->dim() == 1 && (*w)->size(0) == c.D, op, ": weights must be [D]");
+      TORCH_CHECK_TYPE(type_code(**w, "weight") == c.wdt, op, ": q_weight and k_weight must have one dtype");
+    }
+  return c;
+}
+void put_strides(const Tensor& t, int64_t* s) {
+  for (int d = 0; d < 3; ++d) s[d] = t.stride(d);
+}
+
+// q', and k' where there is a k
+Outputs qk_norm_rotary(const Tensor& q_, const OptT& k_, const OptT& wq_, const OptT& wk_, double eps, const Tensor& freqs_,
+                       const Tensor& pos, c10::IntArrayRef axis_pairs, bool interleaved, double amplitude) {
+  const HeadCall c = check_heads("qk_norm_rotary", q_, k_, wq_, wk_, freqs_, pos);
+  const Places at = places_of("qk_norm_rotary", pos, axis_pairs, c.B, c.S, freqs_.numel());
+  const c10::DeviceGuard guard(q_.device());
+  const Tensor q = unit_rows(q_), freqs = freqs_.contiguous();
+  const OptT k = k_ ? OptT(unit_rows(*k_)) : OptT(), wq = cont(wq_), wk = cont(wk_);
+  Outputs out{like_layout(q_)};
+  int64_t st[12] = {};
+  put_strides(q, st);
+  put_strides(out[0], st + 3);
+  if (k) {
+    out.push_back(like_layout(*k_));
+    put_strides(*k, st + 6);
+    put_strides(out[1], st + 9);
+  }
+  PRISM_TORCH_CALL(prism_qk_norm_rotary, q.data_ptr(), p(k), c.dt, small(c.B, "B"), c.S, small(c.Hq, "heads"),
+                   small(c.Hk, "heads"), small(c.D, "D"), small(2 * freqs.numel(), "rotary dim"), st, p(wq), p(wk), c.wdt,
+                   (float)eps, freqs.data_ptr<double>(), pos.data_ptr(), at.is64, at.strides, at.axes, at.axis_end,
+                   interleaved, (float)amplitude, out[0].data_ptr(), k ? out[1].data_ptr() : nullptr, stream_of(q));
+  return out;
+}
+
+// dq where there is a dyq, dk where there is a dyk, dwq and dwk on request
+Outputs qk_norm_rotary_bwd(const OptT& dyq_, const OptT& dyk_, const Tensor& q_, const OptT& k_, const OptT& wq_,
+                           const OptT& wk_, double eps, const Tensor& freqs_, const Tensor& pos,
+                           c10::IntArrayRef axis_pairs, bool interleaved, double amplitude, bool want_dwq, bool want_dwk) {
+  const HeadCall c = check_heads("qk_norm_rotary_bwd", q_, k_, wq_, wk_, freqs_, pos);
+  const Places at = places_of("qk_norm_rotary_bwd", pos, axis_pairs, c.B, c.S, freqs_.numel());
+  for (const auto& [g, x] : {std::make_pair(&dyq_, OptT(q_)), std::make_pair(&dyk_, k_)}) {
+    same_device(q_, *g, "dy");
+    check_dtype(*g, q_.scalar_type(), "dy");
+    if (*g) TORCH_CHECK_VALUE(x && (*g)->sizes() == x->sizes(), "qk_norm_rotary_bwd: gradients must have their inputs' shape");
+  }
+  TORCH_CHECK_VALUE((!want_dwq || (dyq_ && wq_)) && (!want_dwk || (dyk_ && wk_)),
+                    "qk_norm_rotary_bwd: a weight's gradient needs the weight and its heads' gradient");
+  const c10::DeviceGuard guard(q_.device());
+  const Tensor freqs = freqs_.contiguous();
+  const OptT q = dyq_ ? OptT(unit_rows(q_)) : OptT(), k = dyk_ ? OptT(unit_rows(*k_)) : OptT();
+  const OptT dyq = dyq_ ? OptT(unit_rows(*dyq_)) : OptT(), dyk = dyk_ ? OptT(unit_rows(*dyk_)) : OptT();
+  const OptT wq = cont(wq_), wk = cont(wk_);
+  Outputs out;
+  Tensor dq, dk, dwq, dwk, partial;
+  if (dyq) out.push_back(dq = like_layout(q_));
+  if (dyk) out.push_back(dk = like_layout(*k_));
+  const bool none = c.B * c.S == 0 || (dyq ? c.Hq : 0) + (dyk ? c.Hk : 0) == 0;
+  auto weight_grad = [&](const OptT& w, bool heads) {  // (no rows: nothing writes it)
+    out.push_back(none || !heads ? at::zeros_like(*w) : at::empty_like(*w));
+    return out.back();
+  };
+  if (want_dwq) dwq = weight_grad(wq, c.Hq > 0);
+  if (want_dwk) dwk = weight_grad(wk, c.Hk > 0);
+  if (none) return out;
+  int64_t st[18] = {};
+  if (dyq) {
+    put_strides(*dyq, st);
+    put_strides(*q, st + 3);
+    put_strides(dq, st + 6);
+  }
+  if (dyk) {
+    put_strides(*dyk, st + 9);
+    put_strides(*k, st + 12);
+    put_strides(dk, st + 15);
+  }
+  if (want_dwq || want_dwk) partial = at::empty({2, PRISM_HEAD_PARTS, c.D}, opts(q_, at::kFloat));
+  PRISM_TORCH_CALL(prism_qk_norm_rotary_bwd, p(dyq), p(dyk), p(q), p(k), c.dt, small(c.B, "B"), c.S,
+                   dyq ? small(c.Hq, "heads") : 0, dyk ? small(c.Hk, "heads") : 0, small(c.D, "D"),
+                   small(2 * freqs.numel(), "rotary dim"), st, p(wq), p(wk), c.wdt, (float)eps, freqs.data_ptr<double>(),
+                   pos.data_ptr(), at.is64, at.strides, at.axes, at.axis_end, interleaved, (float)amplitude,
+                   dyq ? dq.data_ptr() : nullptr, dyk ? dk.data_ptr() : nullptr,
+                   partial.defined() ? partial.data_ptr<float>() : nullptr, want_dwq ? dwq.data_ptr() : nullptr,
+                   want_dwk ? dwk.data_ptr() : nullptr, stream_of(q_));
+  return out;
+}
+
+struct QkNormGrad : torch::autograd::Function<QkNormGrad> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptT& k, const OptT& wq, const OptT& wk,
+                               double eps, const Tensor& freqs, const Tensor& pos, std::vector<int64_t> axis_pairs,
+                               bool interleaved, double amplitude) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    ctx->set_materialize_grads(false);
+    const variable_list o = PRISM_OP(qk_norm_rotary).call(q, k, wq, wk, eps, freqs, pos, axis_pairs, interleaved, amplitude);
+    ctx->save_for_backward({q, k ? *k : Tensor(), wq ? *wq : Tensor(), wk ? *wk : Tensor(), freqs, pos});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["axis_pairs"] = axis_pairs;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["amplitude"] = amplitude;
+    ctx->saved_data["dwq"] = wants_grad(wq);
+    ctx->saved_data["dwk"] = wants_grad(wk);
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list out(10);
+    const Tensor dyq = g[0], dyk = g.size() > 1 ? g[1] : Tensor();
+    if (!dyq.defined() && !dyk.defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    const bool dwq = dyq.defined() && ctx->saved_data["dwq"].toBool(), dwk = dyk.defined() && ctx->saved_data["dwk"].toBool();
+    const Outputs d = [&] {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      return PRISM_OP(qk_norm_rotary_bwd).call(opt(dyq), opt(dyk), s[0], opt(s[1]), opt(s[2]), opt(s[3]),
+                    ctx->saved_data["eps"].toDouble(), s[4], s[5], ctx->saved_data["axis_pairs"].toIntVector(),
+                    ctx->saved_data["interleaved"].toBool(), ctx->saved_data["amplitude"].toDouble(), dwq, dwk);
+    }();
+    size_t at = 0;
+    if (dyq.defined()) out[0] = d[at++];
+    if (dyk.defined()) out[1] = d[at++];
+    if (dwq) out[2] = d[at++];
+    if (dwk) out[3] = d[at++];
+    return once(std::move(out));
+  }
+};
+Outputs qk_norm_rotary_autograd(const Tensor& q, const OptT& k, const OptT& wq, const OptT& wk, double eps,
+                                const Tensor& freqs, const Tensor& pos, c10::IntArrayRef axis_pairs, bool interleaved,
+                                double amplitude) {
+  check_no_tangents("qk_norm_rotary", q, k, wq, wk, freqs);
+  if (!grads_wanted(q, k, wq, wk)) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return PRISM_OP(qk_norm_rotary).call(q, k, wq, wk, eps, freqs, pos, axis_pairs, interleaved, amplitude);
+  }
+  return QkNormGrad::apply(q, k, wq, wk, eps, freqs, pos, axis_pairs.vec(), interleaved, amplitude);
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(prism, m) {
+  m.def("qk_norm_rotary(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, float eps, Tensor freqs, "
+        "Tensor positions, int[] axis_pairs, bool interleaved, float amplitude) -> Tensor[]");
+  m.def("qk_norm_rotary_bwd(Tensor? dyq, Tensor? dyk, Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, float eps, "
+        "Tensor freqs, Tensor positions, int[] axis_pairs, bool interleaved, float amplitude, bool want_dwq, "
+        "bool want_dwk) -> Tensor[]");
+}
+
+TORCH_LIBRARY_IMPL(prism, CUDA, m) {
+  m.impl("qk_norm_rotary", &qk_norm_rotary);
+  m.impl("qk_norm_rotary_bwd", &qk_norm_rotary_bwd);
+}
+
+TORCH_LIBRARY_IMPL(prism, AutogradCUDA, m) {
+  m.impl("qk_norm_rotary", &qk_norm_rotary_autograd);
+}

@@ -73,7 +73,8 @@ def _op(name: str, *args):
 
 
 # Operators whose gradients are C++ nodes, and what those launch
-_NODE_LAUNCHES = {"rms_norm": "prism_rms_norm_bwd", "rotary": "prism_rotary", "window_fwd": "prism_window_bwd"}
+_NODE_LAUNCHES = {"rms_norm": "prism_rms_norm_bwd", "rotary": "prism_rotary", "window_fwd": "prism_window_bwd",
+                  "qk_norm_rotary": "prism_qk_norm_rotary_bwd"}
 
 
 def _time_node(node, key: str):
@@ -234,6 +235,18 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, posi
     Differentiable (q, k)."""
     _cuda(q, k, freqs, positions)
     out = _op("rotary", q, k, freqs, positions, axis_pairs, bool(interleaved), float(amplitude), bool(inverse))
+    return out[0], (out[1] if k is not None else None)
+
+
+def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[torch.Tensor],
+                   k_weight: Optional[torch.Tensor], eps: float, freqs: torch.Tensor, positions: torch.Tensor, axis_pairs,
+                   interleaved: bool, amplitude: float):
+    """q [B,Hq,S,D] and k [B,Hk,S,D] (or None), each head normed (times its weight
+    [D]) and turned by positions x freqs.  Returns (q', k').  Differentiable (q, k,
+    weights)."""
+    _cuda(q, k, q_weight, k_weight, freqs, positions)
+    out = _op("qk_norm_rotary", q, k, q_weight, k_weight, float(eps), freqs, positions, axis_pairs, bool(interleaved),
+              float(amplitude))
     return out[0], (out[1] if k is not None else None)
 
 
