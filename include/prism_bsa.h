@@ -133,6 +133,31 @@ int prism_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh, int64_
                        int64_t h_stride, const void* w, int w_dtype, int dtype, int64_t M, int N, const float* inv,
                        void* dx, float* partial, int parts, void* dw, hipStream_t stream);
 
+/* ------------------------------------------------------------------ packed attention */
+
+/* Attention within the sequences of packed tensors: q [Tq, Hq, D], k, v [Tk, Hk, D]
+ * (PRISM_BF16 / PRISM_F16, D 64 or 128, Hq a multiple of Hk); sequence b's queries are
+ * rows cu_q[b] .. cu_q[b + 1] - 1 and its keys cu_k[b] .. cu_k[b + 1] - 1 (int32 [B + 1],
+ * device; not decreasing, values outside the tensors are cut to them).  The queries are
+ * the last of their sequence: query i of n over L keys sees key j <= i + L - n (causal) or
+ * all.  o: rows that see no key, and rows of no sequence, give 0 (lse -inf).  rest: NULL,
+ * or what o's rounding left off (o's layout; the backward takes it).  lse: NULL or [Hq,
+ * Tq] fp32, natural log.  strides (host, elements): head and token of q, k, v, o, multiples
+ * of 8, a token's below 2^24; pointers 16-byte aligned.  plan, part: workspaces of `ints`
+ * int32 and `floats` floats (prism_packed_fwd_plan; NULL where 0), 16-byte aligned. */
+int prism_packed_fwd_plan(int B, int Hq, int Hk, int64_t Tq, int64_t Tk, int D, int64_t* ints, int64_t* floats);
+int prism_packed_fwd(const void* q, const void* k, const void* v, int dtype, int B, int Hq, int Hk, int64_t Tq, int64_t Tk,
+                     int D, const int64_t* strides, const int32_t* cu_q, const int32_t* cu_k, int causal, float sm_scale,
+                     void* o, void* rest, float* lse, int32_t* plan, float* part, hipStream_t stream);
+/* Its gradients (0 for rows of no sequence): rest and lse of the forward; strides of q, k,
+ * v, o (and rest), do_, dq, dk, dv; rows: workspace of 2 Hq Tq floats; plan, part as above
+ * (prism_packed_bwd_plan). */
+int prism_packed_bwd_plan(int B, int Hq, int Hk, int64_t Tq, int64_t Tk, int D, int64_t* ints, int64_t* floats);
+int prism_packed_bwd(const void* do_, const void* q, const void* k, const void* v, const void* o, const void* rest,
+                     const float* lse, int dtype, int B, int Hq, int Hk, int64_t Tq, int64_t Tk, int D,
+                     const int64_t* strides, const int32_t* cu_q, const int32_t* cu_k, int causal, float sm_scale, void* dq,
+                     void* dk, void* dv, float* rows, int32_t* plan, float* part, hipStream_t stream);
+
 /* ------------------------------------------------------------------ norms and positions of heads */
 
 /* Every head of q [B, Hq, S, D] and k [B, Hk, S, D] (Hq or Hk = 0: none) divided by

@@ -54,7 +54,8 @@ def _register_vmaps():
     def one(t, d, i):
         return t if d is None or not isinstance(t, torch.Tensor) else t.select(d, i)
 
-    for name in ("rms_norm", "rms_norm_bwd", "rotary", "window_fwd", "qk_norm_rotary", "qk_norm_rotary_bwd"):
+    for name in ("rms_norm", "rms_norm_bwd", "rotary", "window_fwd", "qk_norm_rotary", "qk_norm_rotary_bwd",
+                 "packed_fwd"):
         if not hasattr(torch.ops.prism, name):  # (a library built before, as for the fakes)
             continue
 
@@ -149,6 +150,21 @@ def _register_fakes():
     @reg("prism::window_bwd")
     def _(do, q, k, v, o, rest, lse, window, sinks, causal, q_lens, kv_lens, sm_scale):
         return like(q, 1 << 24), like(k, 1 << 24), like(v, 1 << 24)
+
+    def near(t):  # [T, H, D]: t's layout where that is dense with adjacent channels and near rows, else contiguous
+        o = torch.empty_like(t)
+        ok = o.numel() == 0 or (o.stride(2) == 1 and (o.shape[0] <= 1 or o.stride(0) < 1 << 24))
+        return o if ok else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+    @reg("prism::packed_fwd")
+    def _(q, k, v, cu_q, cu_k, causal, sm_scale, want_lse, want_rest):
+        o = near(q)
+        return ([o] + ([_empty(q, (q.shape[1], q.shape[0]), f32)] if want_lse else [])
+                + ([torch.empty_like(o)] if want_rest else []))
+
+    @reg("prism::packed_bwd")
+    def _(do, q, k, v, o, rest, lse, cu_q, cu_k, causal, sm_scale):
+        return near(q), near(k), near(v)
 
     @reg("prism::zone_layout")
     def _(shape_ids):

@@ -196,9 +196,150 @@ Outputs qk_norm_rotary_autograd(const Tensor& q, const OptT& k, const OptT& wq, 
   return QkNormGrad::apply(q, k, wq, wk, eps, freqs, pos, axis_pairs.vec(), interleaved, amplitude);
 }
 
+// ------------------------------------------------------------------ packed attention
+// [T, H, D] as the kernels take it: adjacent channels, 16-byte aligned rows at strides of
+// whole 16-byte pieces; else a contiguous copy
+Tensor pack_rows(const Tensor& t) {
+  bool ok = t.numel() == 0 || (t.stride(2) == 1 && (uintptr_t)t.data_ptr() % 16 == 0);
+  for (int d = 0; d < 2 && ok; ++d) ok = t.size(d) <= 1 || t.stride(d) % 8 == 0;
+  if (ok && t.size(0) > 1) ok = t.stride(0) < (1 << 24);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+void pack_strides(const Tensor& t, int64_t* s) {  // head, token
+  s[0] = t.size(1) > 1 ? t.stride(1) : 0;
+  s[1] = t.size(0) > 1 ? t.stride(0) : 0;
+}
+// t's layout where that is dense, has adjacent channels and rows as near as the kernels take them
+Tensor pack_like(const Tensor& t) {
+  Tensor o = at::empty_like(t);
+  const bool ok = o.numel() == 0 || (o.stride(2) == 1 && (o.size(0) <= 1 || o.stride(0) < (1 << 24)));
+  return ok ? o : at::empty(t.sizes(), t.options());
+}
+
+struct PackShape {
+  int dt, B, Hq, Hk, D;
+  int64_t Tq, Tk;
+};
+PackShape check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k) {
+  on_gpu(q, "q");
+  same_device(q, k, "k");
+  same_device(q, v, "v");
+  same_device(q, cu_q, "cu_seqlens");
+  same_device(q, cu_k, "cu_seqlens_k");
+  TORCH_CHECK_TYPE(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf,
+                   "prism: packed attention takes bfloat16 or float16, got ", q.scalar_type());
+  check_dtype(k, q.scalar_type(), "k");
+  check_dtype(v, q.scalar_type(), "v");
+  check_dtype(cu_q, at::kInt, "cu_seqlens");
+  check_dtype(cu_k, at::kInt, "cu_seqlens_k");
+  TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() && k.size(2) == q.size(2),
+                    "packed attention: q must be [Tq, Hq, D], k and v [Tk, Hk, D], got ", q.sizes(), ", ", k.sizes(), ", ",
+                    v.sizes());
+  TORCH_CHECK_VALUE(cu_q.dim() == 1 && cu_q.size(0) >= 1 && cu_k.sizes() == cu_q.sizes(),
+                    "packed attention: cu_seqlens must be [B + 1], got ", cu_q.sizes(), " and ", cu_k.sizes());
+  return {q.scalar_type() == at::kBFloat16 ? PRISM_BF16 : PRISM_F16, small(cu_q.size(0) - 1, "B"), small(q.size(1), "heads"),
+          small(k.size(1), "heads"), small(q.size(2), "D"), q.size(0), k.size(0)};
+}
+
+// o, lse and what o's rounding left off on request
+Outputs packed_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu_q_, const Tensor& cu_k_,
+                   bool causal, double sm_scale, bool want_lse, bool want_rest) {
+  const PackShape s = check_packed(q_, k_, v_, cu_q_, cu_k_);
+  const c10::DeviceGuard guard(q_.device());
+  const Tensor q = pack_rows(q_), k = pack_rows(k_), v = pack_rows(v_), cu_q = cu_q_.contiguous(), cu_k = cu_k_.contiguous();
+  Tensor o = pack_like(q_), lse, rest, work;
+  Outputs out{o};
+  if (want_lse) out.push_back(lse = at::empty({s.Hq, s.Tq}, opts(q, at::kFloat)));
+  if (want_rest) out.push_back(rest = at::empty_like(o));
+  int64_t st[8], ints = 0, floats = 0;
+  const Tensor* all[4] = {&q, &k, &v, &o};
+  for (int i = 0; i < 4; ++i) pack_strides(*all[i], st + 2 * i);
+  check_rc(prism_packed_fwd_plan(s.B, s.Hq, s.Hk, s.Tq, s.Tk, s.D, &ints, &floats));
+  if (ints + floats) work = at::empty({ints + floats}, opts(q, at::kFloat));  // (the list, then the parts)
+  float* wp = ints + floats ? work.data_ptr<float>() : nullptr;
+  PRISM_TORCH_CALL(prism_packed_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), s.dt, s.B, s.Hq, s.Hk, s.Tq, s.Tk, s.D, st,
+                   cu_q.data_ptr<int32_t>(), cu_k.data_ptr<int32_t>(), causal, (float)sm_scale, o.data_ptr(),
+                   want_rest ? rest.data_ptr() : nullptr, want_lse ? lse.data_ptr<float>() : nullptr,
+                   ints ? (int32_t*)wp : nullptr, floats ? wp + ints : nullptr, stream_of(q));
+  return out;
+}
+
+std::tuple<Tensor, Tensor, Tensor> packed_bwd(const Tensor& do_, const Tensor& q_, const Tensor& k_, const Tensor& v_,
+                                              const Tensor& o_, const Tensor& rest_, const Tensor& lse_, const Tensor& cu_q_,
+                                              const Tensor& cu_k_, bool causal, double sm_scale) {
+  const PackShape s = check_packed(q_, k_, v_, cu_q_, cu_k_);
+  for (const auto& t : {std::make_pair(&do_, "do"), std::make_pair(&o_, "o"), std::make_pair(&rest_, "rest")}) {
+    same_device(q_, *t.first, t.second);
+    check_dtype(*t.first, q_.scalar_type(), t.second);
+    TORCH_CHECK_VALUE(t.first->sizes() == q_.sizes(), "packed_bwd: ", t.second, " must have q's shape");
+  }
+  TORCH_CHECK_VALUE(rest_.strides() == o_.strides(), "packed_bwd: rest must have o's strides");
+  same_device(q_, lse_, "lse");
+  check_dtype(lse_, at::kFloat, "lse");
+  TORCH_CHECK_VALUE(lse_.dim() == 2 && lse_.size(0) == s.Hq && lse_.size(1) == s.Tq, "packed_bwd: lse must be [Hq, Tq]");
+  const c10::DeviceGuard guard(q_.device());
+  const Tensor q = pack_rows(q_), k = pack_rows(k_), v = pack_rows(v_), o = pack_rows(o_), rest = pack_rows(rest_), d = pack_rows(do_);
+  for (int x = 0; x < 3; ++x) TORCH_CHECK(rest.stride(x) == o.stride(x), "packed_bwd: rest must be laid out like o");
+  const Tensor lse = lse_.contiguous(), cu_q = cu_q_.contiguous(), cu_k = cu_k_.contiguous();
+  Tensor dq = pack_like(q_), dk = pack_like(k_), dv = pack_like(v_);
+  int64_t st[16], ints = 0, floats = 0;
+  const Tensor* all[8] = {&q, &k, &v, &o, &d, &dq, &dk, &dv};
+  for (int i = 0; i < 8; ++i) pack_strides(*all[i], st + 2 * i);
+  check_rc(prism_packed_bwd_plan(s.B, s.Hq, s.Hk, s.Tq, s.Tk, s.D, &ints, &floats));
+  Tensor work = at::empty({ints + floats + 2 * s.Hq * s.Tq}, opts(q, at::kFloat));  // the lists, the parts, then rows
+  float* wp = work.data_ptr<float>();
+  PRISM_TORCH_CALL(prism_packed_bwd, d.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.data_ptr(),
+                   lse.data_ptr<float>(), s.dt, s.B, s.Hq, s.Hk, s.Tq, s.Tk, s.D, st, cu_q.data_ptr<int32_t>(),
+                   cu_k.data_ptr<int32_t>(), causal, (float)sm_scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                   wp + ints + floats, ints ? (int32_t*)wp : nullptr, floats ? wp + ints : nullptr, stream_of(q));
+  return {dq, dk, dv};
+}
+
+struct PackedGrad : torch::autograd::Function<PackedGrad> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q,
+                               const Tensor& cu_k, bool causal, double sm_scale, bool want_lse, bool want_rest) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    ctx->set_materialize_grads(false);
+    const variable_list o = PRISM_OP(packed_fwd).call(q, k, v, cu_q, cu_k, causal, sm_scale, true, true);
+    ctx->save_for_backward({q, k, v, o[0], o[2], o[1], cu_q, cu_k});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["sm_scale"] = sm_scale;
+    variable_list out{o[0]};
+    if (want_lse) out.push_back(o[1]);
+    if (want_rest) out.push_back(o[2]);
+    ctx->mark_non_differentiable(variable_list(out.begin() + 1, out.end()));
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    if (!g[0].defined()) return variable_list(9);
+    const variable_list s = ctx->get_saved_variables();
+    const auto [dq, dk, dv] = [&] {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      return PRISM_OP(packed_bwd).call(g[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], ctx->saved_data["causal"].toBool(),
+                        ctx->saved_data["sm_scale"].toDouble());
+    }();
+    variable_list out(9);
+    out[0] = dq; out[1] = dk; out[2] = dv;
+    return once(std::move(out));
+  }
+};
+Outputs packed_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k,
+                        bool causal, double sm_scale, bool want_lse, bool want_rest) {
+  check_no_tangents("packed_fwd", q, k, v);
+  if (!grads_wanted(q, k, v)) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return PRISM_OP(packed_fwd).call(q, k, v, cu_q, cu_k, causal, sm_scale, want_lse, want_rest);
+  }
+  return PackedGrad::apply(q, k, v, cu_q, cu_k, causal, sm_scale, want_lse, want_rest);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(prism, m) {
+  m.def("packed_fwd(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor cu_k, bool causal, float sm_scale, bool want_lse, "
+        "bool want_rest) -> Tensor[]");
+  m.def("packed_bwd(Tensor do, Tensor q, Tensor k, Tensor v, Tensor o, Tensor rest, Tensor lse, Tensor cu_q, Tensor cu_k, "
+        "bool causal, float sm_scale) -> (Tensor, Tensor, Tensor)");
   m.def("qk_norm_rotary(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, float eps, Tensor freqs, "
         "Tensor positions, int[] axis_pairs, bool interleaved, float amplitude) -> Tensor[]");
   m.def("qk_norm_rotary_bwd(Tensor? dyq, Tensor? dyk, Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, float eps, "
@@ -209,8 +350,11 @@ TORCH_LIBRARY_FRAGMENT(prism, m) {
 TORCH_LIBRARY_IMPL(prism, CUDA, m) {
   m.impl("qk_norm_rotary", &qk_norm_rotary);
   m.impl("qk_norm_rotary_bwd", &qk_norm_rotary_bwd);
+  m.impl("packed_fwd", &packed_fwd);
+  m.impl("packed_bwd", &packed_bwd);
 }
 
 TORCH_LIBRARY_IMPL(prism, AutogradCUDA, m) {
   m.impl("qk_norm_rotary", &qk_norm_rotary_autograd);
+  m.impl("packed_fwd", &packed_autograd);
 }

@@ -74,7 +74,7 @@ def _op(name: str, *args):
 
 # Operators whose gradients are C++ nodes, and what those launch
 _NODE_LAUNCHES = {"rms_norm": "prism_rms_norm_bwd", "rotary": "prism_rotary", "window_fwd": "prism_window_bwd",
-                  "qk_norm_rotary": "prism_qk_norm_rotary_bwd"}
+                  "qk_norm_rotary": "prism_qk_norm_rotary_bwd", "packed_fwd": "prism_packed_bwd"}
 
 
 def _time_node(node, key: str):
@@ -268,6 +268,23 @@ def window_bwd(do, q, k, v, o, rest: Optional[torch.Tensor], lse, window: int, s
     _cuda(do, q, k, v, o, rest, lse, q_lens, kv_lens)
     return _op("window_bwd", do, q, k, v, o, rest, lse, int(window), int(sinks), bool(causal), q_lens, kv_lens,
                float(sm_scale))
+
+
+def packed_fwd(q, k, v, cu_q: torch.Tensor, cu_k: torch.Tensor, causal: bool, sm_scale: float, want_lse: bool,
+               want_rest: bool = False):
+    """(o [Tq,Hq,D], lse [Hq,Tq] fp32 or None) of attention within the sequences that
+    cu_q and cu_k bound, with want_rest also what o's rounding left off.
+    Differentiable (o in q, k, v)."""
+    _cuda(q, k, v, cu_q, cu_k)
+    out = _op("packed_fwd", q, k, v, cu_q, cu_k, bool(causal), float(sm_scale), bool(want_lse), bool(want_rest))
+    lse = out[1] if want_lse else None
+    return (out[0], lse, out[-1]) if want_rest else (out[0], lse)
+
+
+def packed_bwd(do, q, k, v, o, rest, lse, cu_q: torch.Tensor, cu_k: torch.Tensor, causal: bool, sm_scale: float):
+    """(dq, dk, dv) of packed_fwd; rest: its rest."""
+    _cuda(do, q, k, v, o, rest, lse, cu_q, cu_k)
+    return _op("packed_bwd", do, q, k, v, o, rest, lse, cu_q, cu_k, bool(causal), float(sm_scale))
 
 
 # ------------------------------------------------------------------ geometry
