@@ -158,6 +158,44 @@ int prism_packed_bwd(const void* do_, const void* q, const void* k, const void* 
                      const int64_t* strides, const int32_t* cu_q, const int32_t* cu_k, int causal, float sm_scale, void* dq,
                      void* dk, void* dv, float* rows, int32_t* plan, float* part, hipStream_t stream);
 
+/* ------------------------------------------------------------------ paged caches */
+
+/* Caches (no counterpart in the reference): k_cache, v_cache of `bits` 16 ([page][head]
+ * [place] rows of D elements of dtype) or 4 ([page][head], D / 2 bytes of codes for each place,
+ * an even channel in the low half, then D / 32 scale bytes for each place: value = code's
+ * level (0, 0.5, 1, 1.5, 2, 3, 4, 6, sign in bit 3) x 2^(byte - 127); byte 255: NaN).
+ * dtype PRISM_BF16 / PRISM_F16 (of q, k, v), D 64 or 128, page_size 16 to 256, a power of two.
+ * cache_strides (host): page, head, place of k_cache, then of v_cache, in elements (4 bits:
+ * bytes, places not read), whole 16 bytes.  table: int32 [B, width] (device) at rows
+ * table_stride apart; place p of sequence b is place p % page_size of page table[b][p /
+ * page_size]; entries outside [0, pages) are no pages: not written, not seen.  Pointers
+ * 16-byte aligned.
+ *
+ * prism_paged_append: rows k, v [T, Hk, D] (strides, host: token, head of k, of v) of the
+ * sequences' new tokens, T / B each or rows cu[b] .. cu[b + 1] - 1 (int32 [B + 1]), to places
+ * lens[b] - n + i (lens: int32 [B], with the new tokens).  freqs: float64 [R / 2], or NULL
+ * (keys as they are): k turned as by prism_rotary at pos (as there, strides of token and axis
+ * in pos_strides) or, NULL, at its place; R even, not interleaved a multiple of 16. */
+int prism_paged_append(const void* k, const void* v, int dtype, int64_t T, int Hk, int D, const int64_t* strides, void* k_cache,
+                       void* v_cache, int bits, int64_t pages, int page_size, const int64_t* cache_strides,
+                       const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens, int B,
+                       const int32_t* cu, const double* freqs, int R, int interleaved, const void* pos, int pos64,
+                       const int64_t* pos_strides, int axes, const int32_t* axis_end, float amplitude, hipStream_t stream);
+/* Places 0 .. cu[b + 1] - cu[b] - 1 of every sequence as rows cu[b] .. of k, v [T, Hk, D]
+ * (dense, dtype; rows of no sequence and places without a page: 0). */
+int prism_paged_gather(const void* k_cache, const void* v_cache, int dtype, int bits, int64_t pages, int page_size,
+                       const int64_t* cache_strides, const int32_t* table, int64_t table_stride, int64_t width, int B,
+                       const int32_t* cu, int64_t T, int Hk, int D, void* k, void* v, hipStream_t stream);
+/* Attention of q [B n, Hq, D] (strides, host: token, head of q, of o; multiples of 8): the n
+ * last tokens of each sequence of lens[b] places, token i seeing places j <= lens[b] - n + i.
+ * o: 0 (lse -inf) where nothing is seen.  lse: NULL or [Hq, B n] fp32.  part: workspace of
+ * `floats` floats (prism_paged_plan with places = width * page_size; NULL where 0). */
+int prism_paged_plan(int B, int64_t n, int Hq, int Hk, int D, int bits, int64_t places, int64_t* floats);
+int prism_paged_fwd(const void* q, int dtype, int B, int64_t n, int Hq, int Hk, int D, const int64_t* strides,
+                    const void* k_cache, const void* v_cache, int bits, int64_t pages, int page_size,
+                    const int64_t* cache_strides, const int32_t* table, int64_t table_stride, int64_t width,
+                    const int32_t* lens, float sm_scale, void* o, float* lse, float* part, hipStream_t stream);
+
 /* ------------------------------------------------------------------ norms and positions of heads */
 
 /* Every head of q [B, Hq, S, D] and k [B, Hk, S, D] (Hq or Hk = 0: none) divided by

@@ -12,6 +12,7 @@ Public surface (reference names):
   a2v_bridge_projection       interactionv2.py:348 o-projection with the norms fused
   flash_attn_window           attention over a sliding window and the first tokens
   flash_attn_packed           attention of sequences of different lengths in one tensor
+  paged_cache, append_paged, gather_paged, flash_attn_paged  keys and values in pages, of 16 or 4 bits
 and what the layer runs around it (wan_video_dit.py:699-705):
   rms_norm, rms_norm_quant    residual addition + root-mean-square norm, 8-bit output
   rotary_frequencies, apply_rotary, grid_positions  rotary positions on q and k
@@ -29,6 +30,7 @@ from .adapter import DynamicBlockSparseAttention, a2v_bridge_projection, a2v_tok
 from .rotary import apply_rotary, grid_positions, rotary_frequencies  # noqa: F401
 from .head_norm import qk_norm_rotary  # noqa: F401
 from .packed_attention import flash_attn_packed  # noqa: F401
+from .paged_cache import append_paged, flash_attn_paged, gather_paged, paged_cache  # noqa: F401
 from .row_norm import rms_norm, rms_norm_quant  # noqa: F401
 from .uniform_block_attention import flash_attn_bsa, flash_attn_bsa_3d, flash_attn_bsa_cross  # noqa: F401
 from .window_attention import flash_attn_window  # noqa: F401

@@ -45,6 +45,11 @@ SIGNATURES = {
     "prism_packed_fwd": [P, P, P, I32, I32, I32, I32, I64, I64, I32, P, P, P, I32, F32, P, P, P, P, P, P],
     "prism_packed_bwd_plan": [I32, I32, I32, I64, I64, I32, P, P],
     "prism_packed_bwd": [P, P, P, P, P, P, P, I32, I32, I32, I32, I64, I64, I32, P, P, P, I32, F32, P, P, P, P, P, P, P],
+    "prism_paged_append": [P, P, I32, I64, I32, I32, P, P, P, I32, I64, I32, P, P, I64, I64, P, I32, P, P, I32, I32, P, I32, P,
+                           I32, P, F32, P],
+    "prism_paged_gather": [P, P, I32, I32, I64, I32, P, P, I64, I64, I32, P, I64, I32, I32, P, P, P],
+    "prism_paged_plan": [I32, I64, I32, I32, I32, I32, I64, P],
+    "prism_paged_fwd": [P, I32, I32, I64, I32, I32, I32, P, P, P, I32, I64, I32, P, P, I64, I64, P, F32, P, P, P, P],
     "prism_zone_layout": [P, I32, P, P, P, P],
     "prism_rearrange_index": [P, I32, I32, I32, P, P, P],
     "prism_gather_pool": [P, I32, I32, I32, I64, I32, P, P, P, I32, I32, I32, I32, I32, I32, I64, P, P, P, P, P, P, P, P],

@@ -166,6 +166,19 @@ def _register_fakes():
     def _(do, q, k, v, o, rest, lse, cu_q, cu_k, causal, sm_scale):
         return near(q), near(k), near(v)
 
+    @reg("prism::paged_append")
+    def _(k, v, k_cache, v_cache, page_table, kv_lens, cu_seqlens, freqs, positions, axis_pairs, interleaved, amplitude):
+        return None
+
+    @reg("prism::paged_gather")
+    def _(k_cache, v_cache, page_table, cu_seqlens, total, heads, head_dim, half):
+        dtype = (torch.float16 if half else bf16) if k_cache.dtype is u8 else k_cache.dtype
+        return _empty(k_cache, (total, heads, head_dim), dtype), _empty(k_cache, (total, heads, head_dim), dtype)
+
+    @reg("prism::paged_fwd")
+    def _(q, k_cache, v_cache, page_table, kv_lens, heads, sm_scale, want_lse):
+        return [near(q)] + ([_empty(q, (q.shape[1], q.shape[0]), f32)] if want_lse else [])
+
     @reg("prism::zone_layout")
     def _(shape_ids):
         nz = shape_ids.numel()

@@ -32,6 +32,7 @@ TORCH_OPS_PATH = os.path.join(HERE, "libprism_torch.so")
 
 SOURCES = ["errors.hip", "stats.hip", "layout.hip", "select.hip", "lists.hip", "attn_fwd.hip", "attn_bwd.hip",
            "oproj.hip", "rownorm.hip", "rotary.hip", "headnorm.hip", "window_fwd.hip", "window_token.hip", "window_bwd.hip", "packed_fwd.hip", "packed_bwd.hip",
+           "paged.hip", "paged_token.hip",
            "validate.hip", "peak.hip"]
 CANONICAL = {"stats.hip", "layout.hip", "select.hip"}
 

@@ -25,6 +25,33 @@ __device__ __forceinline__ void sincos_turns(double t, float& s, float& c) {
   c = (k == 1 || k == 2) ? -b : b;
 }
 
+// the same in float64 (series to 1/15! and 1/16!: 5e-17 off on [-pi/4, pi/4])
+__device__ __forceinline__ void sincos_turns(double t, double& s, double& c) {
+  const double q = rint(4.0 * t);
+  const double x = (t - 0.25 * q) * 6.28318530717958647692, z = x * x;
+  double ps = -1.0 / 1307674368000.0;
+  ps = __builtin_fma(ps, z, 1.0 / 6227020800.0);
+  ps = __builtin_fma(ps, z, -1.0 / 39916800.0);
+  ps = __builtin_fma(ps, z, 1.0 / 362880.0);
+  ps = __builtin_fma(ps, z, -1.0 / 5040.0);
+  ps = __builtin_fma(ps, z, 1.0 / 120.0);
+  ps = __builtin_fma(ps, z, -1.0 / 6.0);
+  ps = __builtin_fma(ps * z, x, x);
+  double pc = 1.0 / 20922789888000.0;
+  pc = __builtin_fma(pc, z, -1.0 / 87178291200.0);
+  pc = __builtin_fma(pc, z, 1.0 / 479001600.0);
+  pc = __builtin_fma(pc, z, -1.0 / 3628800.0);
+  pc = __builtin_fma(pc, z, 1.0 / 40320.0);
+  pc = __builtin_fma(pc, z, -1.0 / 720.0);
+  pc = __builtin_fma(pc, z, 1.0 / 24.0);
+  pc = __builtin_fma(pc, z, -0.5);
+  pc = __builtin_fma(pc, z, 1.0);
+  const int k = (int)(q - 4.0 * floor(0.25 * q));
+  const double a = (k & 1) ? pc : ps, b = (k & 1) ? ps : pc;
+  s = (k & 2) ? -a : a;
+  c = (k == 1 || k == 2) ? -b : b;
+}
+
 constexpr int kMaxAxes = 4;
 
 struct Angles {
@@ -34,15 +61,20 @@ struct Angles {
   int pos64, axes, axis_end[kMaxAxes];  // pairs below axis_end[a] (and not of an earlier axis) turn with axis a
   float amp;
   double sign;                       // -1: backwards
-  // sine and cosine, times amp, of pair p of token n of sequence b
-  __device__ __forceinline__ void at(int b, int n, int p, float& s, float& c) const {
+  // position of token n of sequence b as pair p takes it
+  __device__ __forceinline__ double place(int b, int n, int p) const {
     int axis = 0;
     for (int x = 0; x + 1 < axes; ++x) axis += p >= axis_end[x];
     const int64_t i = (int64_t)b * pb + (int64_t)n * ps + (int64_t)axis * pa;
-    const double at = pos64 ? (double)((const int64_t*)pos)[i] : (double)((const int32_t*)pos)[i];
+    return pos64 ? (double)((const int64_t*)pos)[i] : (double)((const int32_t*)pos)[i];
+  }
+  // sine and cosine, times amp, of pair p at that position (float or double)
+  template <class F>
+  __device__ __forceinline__ void turned(double at, int p, F& s, F& c) const {
     const double t = at * (freqs[p] * 0.15915494309189533577);  // turns
     sincos_turns(sign * (t - rint(t)), s, c);
     s *= amp;
     c *= amp;
   }
+  __device__ __forceinline__ void at(int b, int n, int p, float& s, float& c) const { turned(place(b, n, p), p, s, c); }
 };

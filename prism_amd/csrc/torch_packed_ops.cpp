@@ -333,9 +333,150 @@ Outputs packed_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const
   return PackedGrad::apply(q, k, v, cu_q, cu_k, causal, sm_scale, want_lse, want_rest);
 }
 
+// ------------------------------------------------------------------ paged caches
+// A cache as the kernels take it (it is written in place: nothing is copied to fit)
+struct PagedCaches {
+  int bits, page_size;
+  int64_t pages, strides[6];
+};
+PagedCaches check_caches(const char* op, const Tensor& like, const Tensor& kc, const Tensor& vc, int64_t Hk, int64_t D) {
+  same_device(like, kc, "k_cache");
+  same_device(like, vc, "v_cache");
+  const bool four = kc.scalar_type() == at::kByte;
+  TORCH_CHECK_TYPE(vc.scalar_type() == kc.scalar_type() &&
+                       (four || kc.scalar_type() == at::kBFloat16 || kc.scalar_type() == at::kHalf),
+                   "prism: ", op, ": caches must be both bfloat16, float16 or uint8 (4 bits), got ", kc.scalar_type(), " and ",
+                   vc.scalar_type());
+  PagedCaches c;
+  c.bits = four ? 4 : 16;
+  const int64_t place = D / 2 + D / 32;
+  TORCH_CHECK_VALUE(kc.sizes() == vc.sizes() && kc.dim() == (four ? 3 : 4) && kc.size(1) == Hk &&
+                        (four ? D % 32 == 0 && kc.size(2) % place == 0 : kc.size(3) == D),
+                    op, ": caches must be [pages, ", Hk, ", ", four ? "page size (D / 2 + D / 32)]" : "page size, D]", ", got ",
+                    kc.sizes(), " and ", vc.sizes());
+  c.pages = kc.size(0);
+  c.page_size = small(four ? kc.size(2) / place : kc.size(2), "page size");
+  TORCH_CHECK_VALUE(kc.stride(-1) == 1 && vc.stride(-1) == 1, op, ": a cache's channels must be adjacent");
+  int x = 0;
+  for (const Tensor* t : {&kc, &vc}) {
+    c.strides[x++] = t->size(0) > 1 ? t->stride(0) : 0;
+    c.strides[x++] = t->size(1) > 1 ? t->stride(1) : 0;
+    c.strides[x++] = four ? 0 : t->stride(2);
+  }
+  return c;
+}
+void check_table(const char* op, const Tensor& like, const Tensor& table, const OptT& lens) {
+  same_device(like, table, "page_table");
+  same_device(like, lens, "kv_lens");
+  check_dtype(table, at::kInt, "page_table");
+  check_dtype(lens, at::kInt, "kv_lens");
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(1) >= 1, op, ": page_table must be [B, pages of a sequence], got ", table.sizes());
+  if (lens) TORCH_CHECK_VALUE(lens->dim() == 1 && lens->size(0) == table.size(0), op, ": kv_lens must be [B]");
+}
+Tensor unit_table(const Tensor& t) { return t.size(1) == 1 || t.stride(1) == 1 ? t : t.contiguous(); }
+
+void paged_append(const Tensor& k_, const Tensor& v_, const Tensor& kc, const Tensor& vc, const Tensor& table_,
+                  const Tensor& lens_, const OptT& cu_, const OptT& freqs_, const OptT& pos, c10::IntArrayRef axis_pairs,
+                  bool interleaved, double amplitude) {
+  on_gpu(k_, "k");
+  same_device(k_, v_, "v");
+  check_table("append_paged", k_, table_, lens_);
+  same_device(k_, cu_, "cu_seqlens");
+  same_device(k_, freqs_, "freqs");
+  same_device(k_, pos, "positions");
+  TORCH_CHECK_TYPE(k_.scalar_type() == at::kBFloat16 || k_.scalar_type() == at::kHalf,
+                   "prism: append_paged takes bfloat16 or float16, got ", k_.scalar_type());
+  check_dtype(v_, k_.scalar_type(), "v");
+  check_dtype(cu_, at::kInt, "cu_seqlens");
+  check_dtype(freqs_, at::kDouble, "freqs");
+  TORCH_CHECK_VALUE(k_.dim() == 3 && k_.sizes() == v_.sizes(), "append_paged: k and v must be [T, Hk, D], got ", k_.sizes(), " and ",
+                    v_.sizes());
+  const int64_t T = k_.size(0), Hk = k_.size(1), D = k_.size(2), B = table_.size(0);
+  const PagedCaches c = check_caches("append_paged", k_, kc, vc, Hk, D);
+  if (c.bits == 16) check_dtype(kc, k_.scalar_type(), "k_cache");
+  TORCH_CHECK_VALUE(!cu_ || (cu_->dim() == 1 && cu_->size(0) == B + 1), "append_paged: cu_seqlens must be [B + 1]");
+  TORCH_CHECK_VALUE(cu_ || (B == 0 ? T == 0 : T % B == 0), "append_paged: ", T, " tokens do not share out over ", B, " sequences");
+  TORCH_CHECK_VALUE(!freqs_ || freqs_->dim() == 1, "append_paged: freqs must be [pairs]");
+  TORCH_CHECK_VALUE(freqs_ || !pos, "append_paged: positions without freqs");
+  const c10::DeviceGuard guard(k_.device());
+  const Tensor k = pack_rows(k_), v = pack_rows(v_), table = unit_table(table_), lens = lens_.contiguous();
+  const OptT cu = cont(cu_), freqs = cont(freqs_);
+  int64_t st[4] = {k.stride(0), k.size(1) > 1 ? k.stride(1) : 0, v.stride(0), v.size(1) > 1 ? v.stride(1) : 0};
+  if (T == 1) st[0] = st[2] = 0;
+  Places at{};
+  if (pos) at = places_of("append_paged", *pos, axis_pairs, 1, T, freqs->numel());
+  PRISM_TORCH_CALL(prism_paged_append, k.data_ptr(), v.data_ptr(), k.scalar_type() == at::kBFloat16 ? PRISM_BF16 : PRISM_F16, T,
+                   small(Hk, "heads"), small(D, "D"), st, kc.data_ptr(), vc.data_ptr(), c.bits, c.pages, c.page_size, c.strides,
+                   table.data_ptr<int32_t>(), table.size(0) > 1 ? table.stride(0) : 0, table.size(1), lens.data_ptr<int32_t>(),
+                   small(B, "B"), (const int32_t*)p(cu), (const double*)p(freqs), freqs ? small(2 * freqs->numel(), "rotary dim") : 0,
+                   interleaved, p(pos), pos ? at.is64 : false, at.strides + 1, at.axes, at.axis_end, (float)amplitude, stream_of(k));
+  // (torch's own record that the caches changed)
+  for (const Tensor* t : {&kc, &vc})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+std::tuple<Tensor, Tensor> paged_gather(const Tensor& kc, const Tensor& vc, const Tensor& table_, const Tensor& cu_,
+                                        int64_t total, int64_t heads, int64_t D, bool half) {
+  on_gpu(kc, "k_cache");
+  const PagedCaches c = check_caches("gather_paged", kc, kc, vc, heads, D);
+  check_table("gather_paged", kc, table_, OptT());
+  same_device(kc, cu_, "cu_seqlens");
+  check_dtype(cu_, at::kInt, "cu_seqlens");
+  TORCH_CHECK_VALUE(cu_.dim() == 1 && cu_.size(0) == table_.size(0) + 1, "gather_paged: cu_seqlens must be [B + 1]");
+  TORCH_CHECK_VALUE(total >= 0, "gather_paged: total must not be negative");
+  const c10::DeviceGuard guard(kc.device());
+  const Tensor table = unit_table(table_), cu = cu_.contiguous();
+  const at::ScalarType t = c.bits == 16 ? kc.scalar_type() : half ? at::kHalf : at::kBFloat16;
+  Tensor k = at::empty({total, heads, D}, opts(kc, t)), v = at::empty({total, heads, D}, opts(kc, t));
+  PRISM_TORCH_CALL(prism_paged_gather, kc.data_ptr(), vc.data_ptr(), t == at::kHalf ? PRISM_F16 : PRISM_BF16, c.bits, c.pages,
+                   c.page_size, c.strides, table.data_ptr<int32_t>(), table.size(0) > 1 ? table.stride(0) : 0, table.size(1),
+                   small(table.size(0), "B"), cu.data_ptr<int32_t>(), total, small(heads, "heads"), small(D, "D"), k.data_ptr(),
+                   v.data_ptr(), stream_of(kc));
+  return {k, v};
+}
+
+// o, and lse on request
+Outputs paged_fwd(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Tensor& table_, const Tensor& lens_, int64_t heads,
+                  double sm_scale, bool want_lse) {
+  on_gpu(q_, "q");
+  TORCH_CHECK_TYPE(q_.scalar_type() == at::kBFloat16 || q_.scalar_type() == at::kHalf,
+                   "prism: paged attention takes bfloat16 or float16, got ", q_.scalar_type());
+  TORCH_CHECK_VALUE(q_.dim() == 3, "paged attention: q must be [T, Hq, D], got ", q_.sizes());
+  const int64_t T = q_.size(0), Hq = q_.size(1), D = q_.size(2);
+  const PagedCaches c = check_caches("flash_attn_paged", q_, kc, vc, heads, D);
+  if (c.bits == 16) check_dtype(kc, q_.scalar_type(), "k_cache");
+  check_table("flash_attn_paged", q_, table_, lens_);
+  const int64_t B = table_.size(0);
+  TORCH_CHECK_VALUE(B == 0 ? T == 0 : T % B == 0, "flash_attn_paged: ", T, " queries do not share out over ", B, " sequences");
+  const int64_t n = B ? T / B : 0;
+  const c10::DeviceGuard guard(q_.device());
+  const Tensor q = pack_rows(q_), table = unit_table(table_), lens = lens_.contiguous();
+  Tensor o = pack_like(q_), lse, part;
+  Outputs out{o};
+  if (want_lse) out.push_back(lse = at::empty({Hq, T}, opts(q, at::kFloat)));
+  int64_t st[4], floats = 0;
+  st[0] = T > 1 ? q.stride(0) : 0; st[1] = Hq > 1 ? q.stride(1) : 0;
+  st[2] = T > 1 ? o.stride(0) : 0; st[3] = Hq > 1 ? o.stride(1) : 0;
+  check_rc(prism_paged_plan(small(B, "B"), n, small(Hq, "heads"), small(heads, "heads"), small(D, "D"), c.bits,
+                            table.size(1) * c.page_size, &floats));
+  if (floats) part = at::empty({floats}, opts(q, at::kFloat));
+  PRISM_TORCH_CALL(prism_paged_fwd, q.data_ptr(), q.scalar_type() == at::kBFloat16 ? PRISM_BF16 : PRISM_F16, (int)B, n, (int)Hq,
+                   (int)heads, (int)D, st, kc.data_ptr(), vc.data_ptr(), c.bits, c.pages, c.page_size, c.strides,
+                   table.data_ptr<int32_t>(), table.size(0) > 1 ? table.stride(0) : 0, table.size(1), lens.data_ptr<int32_t>(),
+                   (float)sm_scale, o.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr,
+                   floats ? part.data_ptr<float>() : nullptr, stream_of(q));
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(prism, m) {
+  m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor page_table, Tensor kv_lens, "
+        "Tensor? cu_seqlens, Tensor? freqs, Tensor? positions, int[] axis_pairs, bool interleaved, float amplitude) -> ()");
+  m.def("paged_gather(Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor cu_seqlens, int total, int heads, "
+        "int head_dim, bool half) -> (Tensor, Tensor)");
+  m.def("paged_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor kv_lens, int heads, float sm_scale, "
+        "bool want_lse) -> Tensor[]");
   m.def("packed_fwd(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor cu_k, bool causal, float sm_scale, bool want_lse, "
         "bool want_rest) -> Tensor[]");
   m.def("packed_bwd(Tensor do, Tensor q, Tensor k, Tensor v, Tensor o, Tensor rest, Tensor lse, Tensor cu_q, Tensor cu_k, "
@@ -352,6 +493,9 @@ TORCH_LIBRARY_IMPL(prism, CUDA, m) {
   m.impl("qk_norm_rotary_bwd", &qk_norm_rotary_bwd);
   m.impl("packed_fwd", &packed_fwd);
   m.impl("packed_bwd", &packed_bwd);
+  m.impl("paged_append", &paged_append);
+  m.impl("paged_gather", &paged_gather);
+  m.impl("paged_fwd", &paged_fwd);
 }
 
 TORCH_LIBRARY_IMPL(prism, AutogradCUDA, m) {

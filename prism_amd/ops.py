@@ -287,6 +287,30 @@ def packed_bwd(do, q, k, v, o, rest, lse, cu_q: torch.Tensor, cu_k: torch.Tensor
     return _op("packed_bwd", do, q, k, v, o, rest, lse, cu_q, cu_k, bool(causal), float(sm_scale))
 
 
+def paged_append(k, v, k_cache, v_cache, page_table, kv_lens, cu_seqlens: Optional[torch.Tensor],
+                 freqs: Optional[torch.Tensor], positions: Optional[torch.Tensor], axis_pairs, interleaved: bool,
+                 amplitude: float) -> None:
+    """k and v [T,Hk,D] into the pages of their sequences' last places, k turned where
+    freqs are given."""
+    _cuda(k, v, k_cache, v_cache, page_table, kv_lens, cu_seqlens, freqs, positions)
+    _op("paged_append", k, v, k_cache, v_cache, page_table, kv_lens, cu_seqlens, freqs, positions, axis_pairs,
+        bool(interleaved), float(amplitude))
+
+
+def paged_gather(k_cache, v_cache, page_table, cu_seqlens, total: int, heads: int, head_dim: int, half: bool):
+    """(k, v) [total,heads,head_dim]: the sequences' first places, one behind the other."""
+    _cuda(k_cache, v_cache, page_table, cu_seqlens)
+    return _op("paged_gather", k_cache, v_cache, page_table, cu_seqlens, int(total), int(heads), int(head_dim), bool(half))
+
+
+def paged_fwd(q, k_cache, v_cache, page_table, kv_lens, heads: int, sm_scale: float, want_lse: bool):
+    """(o [T,Hq,D], lse [Hq,T] fp32 or None) of attention of the sequences' last T / B
+    tokens over a paged cache of `heads` key heads."""
+    _cuda(q, k_cache, v_cache, page_table, kv_lens)
+    out = _op("paged_fwd", q, k_cache, v_cache, page_table, kv_lens, int(heads), float(sm_scale), bool(want_lse))
+    return out[0], (out[1] if want_lse else None)
+
+
 # ------------------------------------------------------------------ geometry
 class ZoneLayout:
     """Per-call block/tile bookkeeping for one set of shape ids.

@@ -120,3 +120,166 @@ def test_packed_capi_refusals():
         assert lib.prism_packed_bwd_plan(B, 32, 8, T, T, 128, ctypes.byref(ints), ctypes.byref(floats)) == 0
         assert 0 <= floats.value * 4 <= 320 << 20
     assert lib.prism_packed_fwd_plan(1, 3, 2, 10, 10, 128, ctypes.byref(ints), ctypes.byref(floats)) == 1
+
+
+def _paged(bits=16, D=64, page=16, pages=4, heads=2):
+    kc, vc = prism_amd.paged_cache(pages, page, heads, D, bits=bits, device="cpu")
+    table = torch.tensor([[0, 1], [2, -1]], dtype=torch.int32)
+    return kc, vc, table, torch.tensor([17, 4], dtype=torch.int32)
+
+
+def test_paged_cache_shapes():
+    kc, vc = prism_amd.paged_cache(3, 32, 5, 128, dtype=torch.float16, device="cpu")
+    assert kc.shape == vc.shape == (3, 5, 32, 128) and kc.dtype is torch.float16 and not kc.any()
+    kc, vc = prism_amd.paged_cache(3, 32, 5, 128, bits=4, device="cpu")
+    assert kc.shape == vc.shape == (3, 5, 32 * 68) and kc.dtype is torch.uint8
+    for bad in (dict(page_size=24), dict(page_size=8), dict(head_dim=96), dict(pages=0), dict(heads=0), dict(bits=8)):
+        with pytest.raises(ValueError):
+            prism_amd.paged_cache(**{**dict(pages=3, page_size=32, heads=5, head_dim=128, device="cpu"), **bad})
+    with pytest.raises(TypeError):
+        prism_amd.paged_cache(3, 32, 5, 128, dtype=torch.float32, device="cpu")
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_append_refusals(bits):
+    kc, vc, table, lens = _paged(bits)
+    k = torch.randn(2, 2, 64).bfloat16()
+    f, _ = prism_amd.rotary_frequencies(64, device="cpu")
+    call = prism_amd.append_paged
+    with pytest.raises(ValueError, match="GPU"):
+        call(k, k, kc, vc, table, lens)
+    with pytest.raises(ValueError, match="T, Hk, D"):
+        call(k, k[:1], kc, vc, table, lens)
+    with pytest.raises(TypeError, match="bfloat16"):
+        call(k.float(), k.float(), kc, vc, table, lens)
+    with pytest.raises(TypeError, match="bfloat16"):
+        call(k, k.half(), kc, vc, table, lens)
+    with pytest.raises(ValueError, match="key heads"):
+        call(k[:, :1], k[:, :1], kc, vc, table, lens)
+    with pytest.raises(ValueError, match="caches must"):
+        call(k, k, kc, vc[:3], table, lens)
+    with pytest.raises(ValueError, match="caches must" if bits == 16 else "page size"):
+        call(torch.cat([k, k], -1), torch.cat([k, k], -1), kc, vc, table, lens)
+    with pytest.raises(ValueError, match="head_dim"):
+        call(k[..., :32], k[..., :32], kc, vc, table, lens)
+    with pytest.raises(TypeError, match="caches must"):
+        call(k, k, kc.float(), vc.float(), table, lens)
+    with pytest.raises(ValueError, match="page size"):
+        call(k, k, kc[:, :, :8 if bits == 16 else 8 * 34], vc[:, :, :8 if bits == 16 else 8 * 34], table, lens)
+    with pytest.raises(ValueError, match="page_table"):
+        call(k, k, kc, vc, table.long(), lens)
+    with pytest.raises(ValueError, match="page_table"):
+        call(k, k, kc, vc, table[:, :0], lens)
+    with pytest.raises(ValueError, match="kv_lens"):
+        call(k, k, kc, vc, table, lens[:1])
+    with pytest.raises(ValueError, match="kv_lens"):
+        call(k, k, kc, vc, table, lens.long())
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        call(k, k, kc, vc, table, lens, cu_seqlens=lens)
+    with pytest.raises(ValueError, match="share out"):
+        call(k[:1], k[:1], kc, vc, table, lens)
+    with pytest.raises(ValueError, match="gradient"):
+        call(k.clone().requires_grad_(True), k, kc, vc, table, lens)
+    with pytest.raises(TypeError, match="float64"):
+        call(k, k, kc, vc, table, lens, freqs=f.float())
+    with pytest.raises(ValueError, match="fit"):
+        call(k, k, kc, vc, table, lens, freqs=torch.cat([f, f]))
+    with pytest.raises(ValueError, match="multiple of 16"):
+        call(k, k, kc, vc, table, lens, freqs=f[:12], interleaved=False)
+    with pytest.raises(ValueError, match="go with freqs"):
+        call(k, k, kc, vc, table, lens, positions=lens)
+    with pytest.raises(ValueError, match="sections need"):
+        call(k, k, kc, vc, table, lens, freqs=f, sections=(32, 32))
+    with pytest.raises(ValueError, match="sections"):
+        call(k, k, kc, vc, table, lens, freqs=f, sections=(32, 30), positions=table)
+    with pytest.raises(ValueError, match="positions must"):
+        call(k, k, kc, vc, table, lens, freqs=f, positions=lens[:1])
+    if bits == 16:
+        with pytest.raises(TypeError, match="k's dtype"):
+            call(k.half(), k.half(), kc, vc, table, lens)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_paged_refusals(bits):
+    kc, vc, table, lens = _paged(bits)
+    q = torch.randn(4, 8, 64).bfloat16()
+    call = prism_amd.flash_attn_paged
+    with pytest.raises(ValueError, match="GPU"):
+        call(q, kc, vc, table, lens)
+    with pytest.raises(ValueError, match="T, Hq, D"):
+        call(q[0], kc, vc, table, lens)
+    with pytest.raises(TypeError, match="bfloat16"):
+        call(q.float(), kc, vc, table, lens)
+    with pytest.raises(ValueError, match="evenly"):
+        call(q[:, :5], kc, vc, table, lens)
+    with pytest.raises(ValueError, match="evenly"):
+        call(q[:, :1], kc, vc, table, lens)
+    with pytest.raises(ValueError, match="share out"):
+        call(q[:3], kc, vc, table, lens)
+    with pytest.raises(ValueError, match="kv_lens"):
+        call(q, kc, vc, table, lens[None])
+    with pytest.raises(ValueError, match="gradient"):
+        call(q.clone().requires_grad_(True), kc, vc, table, lens)
+    with pytest.raises(ValueError, match="sm_scale"):
+        call(q, kc, vc, table, lens, sm_scale=0.0)
+    if bits == 16:
+        with pytest.raises(TypeError, match="q's dtype"):
+            call(q.half(), kc, vc, table, lens)
+    g = prism_amd.gather_paged
+    b = torch.tensor([0, 3, 9], dtype=torch.int32)
+    with pytest.raises(ValueError, match="GPU"):
+        g(kc, vc, table, b, 9, head_dim=64)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        g(kc, vc, table, b[:2], 9, head_dim=64)
+    with pytest.raises(ValueError, match="total"):
+        g(kc, vc, table, b, -1, head_dim=64)
+    with pytest.raises(TypeError, match="dtype"):
+        g(kc, vc, table, b, 9, head_dim=64, dtype=torch.float32)
+    if bits == 4:
+        with pytest.raises(ValueError, match="head_dim"):
+            g(kc, vc, table, b, 9)
+    else:
+        with pytest.raises(TypeError, match="dtype"):
+            g(kc, vc, table, b, 9, dtype=torch.float16)
+
+
+def test_paged_capi_refusals():
+    lib = _lib.load()
+    one, off = ctypes.c_void_p(16), ctypes.c_void_p(8)
+    st = (ctypes.c_int64 * 4)(64, 64, 64, 64)
+    odd = (ctypes.c_int64 * 4)(63, 64, 64, 64)
+    cs = (ctypes.c_int64 * 6)(*[64] * 6)
+    bad = (ctypes.c_int64 * 6)(*[72] * 5, 60)
+    far = (ctypes.c_int64 * 6)(*[64] * 5, 1 << 24)
+    ends = (ctypes.c_int32 * 4)(8)
+    ps = (ctypes.c_int64 * 2)(1, 1)
+
+    def append(dtype=1, T=4, Hk=2, D=64, s=st, kc=one, bits=16, pages=4, page=16, c=cs, table=one, width=2, lens=one, B=2,
+               cu=None, freqs=one, R=64, inter=1, pos=None, axes=1, k=one):
+        return lib.prism_paged_append(k, one, dtype, T, Hk, D, s, kc, one, bits, pages, page, c, table, 2, width, lens, B, cu,
+                                      freqs, R, inter, pos, 0, ps, axes, ends, 1.0, None)
+
+    assert [append(dtype=0), append(T=-1), append(T=3), append(Hk=0), append(D=80), append(s=odd), append(kc=None), append(kc=off),
+            append(bits=8), append(pages=0), append(page=24), append(page=512), append(page=8), append(c=bad), append(c=far),
+            append(table=None), append(width=0), append(width=1 << 28), append(lens=None), append(B=-1), append(R=63), append(R=66),
+            append(R=24, inter=0), append(pos=one, axes=5), append(pos=one), append(k=None), append(k=off),
+            append(bits=4, c=(ctypes.c_int64 * 6)(*[72] * 6))] == [1] * 28
+
+    def gather(dtype=1, bits=4, D=64, T=4, cu=one, k=one, page=16):
+        return lib.prism_paged_gather(one, one, dtype, bits, 4, page, cs, one, 2, 2, 2, cu, T, 2, D, k, one, None)
+
+    assert [gather(dtype=0), gather(bits=2), gather(D=32), gather(T=-1), gather(cu=None), gather(k=None), gather(k=off),
+            gather(page=17)] == [1] * 8
+
+    def fwd(dtype=1, n=1, Hq=4, Hk=2, s=st, scale=0.1, bits=16, width=2, q=one, lens=one, part=one, B=2):
+        return lib.prism_paged_fwd(q, dtype, B, n, Hq, Hk, 64, s, one, one, bits, 4, 16, cs, one, 2, width, lens, scale, one, None,
+                                   part, None)
+
+    assert [fwd(dtype=0), fwd(n=-1), fwd(n=1 << 30), fwd(Hq=3), fwd(Hq=1), fwd(s=odd), fwd(scale=0.0), fwd(scale=float("nan")),
+            fwd(bits=5), fwd(q=None), fwd(q=off), fwd(lens=None), fwd(width=4000, part=None), fwd(bits=4, width=4000, part=None),
+            fwd(part=off)] == [1] * 15
+    floats = ctypes.c_int64(0)
+    for B, n, places, bits in ((1, 1, 100, 16), (16, 1, 8192, 16), (8, 1, 131072, 4), (1, 3, 1 << 20, 4), (500, 1, 1 << 20, 16)):
+        assert lib.prism_paged_plan(B, n, 32, 8, 128, bits, places, ctypes.byref(floats)) == 0
+        assert 0 <= floats.value * 4 <= 64 << 20
+    assert lib.prism_paged_plan(1, 1, 3, 2, 128, 16, 100, ctypes.byref(floats)) == 1
