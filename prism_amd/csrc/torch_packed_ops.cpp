@@ -468,6 +468,33 @@ Outputs paged_fwd(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Te
   return out;
 }
 
+// (no gradients and no tangents: refused here, where they would be lost without a word)
+template <class... T>
+void check_no_grads(const char* op, const T&... t) {
+  check_no_tangents(op, t...);
+  TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(wants_grad(t) || ...), "prism: ", op,
+                    " has no gradient: call it under torch.no_grad() or on detached tensors");
+}
+void paged_append_autograd(const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc, const Tensor& table,
+                           const Tensor& lens, const OptT& cu, const OptT& freqs, const OptT& pos,
+                           c10::IntArrayRef axis_pairs, bool interleaved, double amplitude) {
+  check_no_grads("paged_append", k, v, kc, vc, freqs);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  PRISM_OP(paged_append).call(k, v, kc, vc, table, lens, cu, freqs, pos, axis_pairs, interleaved, amplitude);
+}
+std::tuple<Tensor, Tensor> paged_gather_autograd(const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& cu,
+                                                 int64_t total, int64_t heads, int64_t D, bool half) {
+  check_no_grads("paged_gather", kc, vc);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return PRISM_OP(paged_gather).call(kc, vc, table, cu, total, heads, D, half);
+}
+Outputs paged_fwd_autograd(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& lens,
+                           int64_t heads, double sm_scale, bool want_lse) {
+  check_no_grads("paged_fwd", q, kc, vc);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return PRISM_OP(paged_fwd).call(q, kc, vc, table, lens, heads, sm_scale, want_lse);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(prism, m) {
@@ -501,4 +528,7 @@ TORCH_LIBRARY_IMPL(prism, CUDA, m) {
 TORCH_LIBRARY_IMPL(prism, AutogradCUDA, m) {
   m.impl("qk_norm_rotary", &qk_norm_rotary_autograd);
   m.impl("packed_fwd", &packed_autograd);
+  m.impl("paged_append", &paged_append_autograd);
+  m.impl("paged_gather", &paged_gather_autograd);
+  m.impl("paged_fwd", &paged_fwd_autograd);
 }
