@@ -52,34 +52,41 @@ __device__ __forceinline__ float weight_at(const HeadArgs& a, int t, int c) {
   return a.w32 ? ((const float*)a.w[t])[c] : E::to_float(((const typename E::type*)a.w[t])[c]);
 }
 
+// The sines and cosines of a workgroup's tokens, [token][pair] in LDS, by all its threads:
+// half a rotation apart two lanes need the same ones, and where a part of the head turns
+// the other lanes have none (9,998 tokens of 16 + 4 heads of 64, 32 channels turning:
+// forward 22.7 us with every lane's own, 18.7 with these, the sums below and fewer slices;
+// backward 38.2 and 24.0)
+template <int VEC>
+__device__ __forceinline__ void put_angles(const HeadArgs& a, int64_t first, float2* table) {
+  const int pairs = a.R >> 1;
+  for (int x = (int)threadIdx.x; x < a.tpb * pairs; x += kThreads) {
+    const int slot = x / pairs, p = x - slot * pairs;
+    const int64_t token = first + slot < a.tokens ? first + slot : a.tokens - 1;
+    const int b = (int)(token / a.S);
+    a.at.at(b, (int)(token - (int64_t)b * a.S), p, table[x].x, table[x].y);
+  }
+}
+
 // a lane's channels [c0, c0 + VEC) of a head: cosines and signed sines, and the lane
 // that holds the pairs' other channels
 template <int VEC, bool INTER>
 struct LaneTurn {
   float cs[INTER ? VEC / 2 : VEC], sn[INTER ? VEC / 2 : VEC];
   int other;  // (half a rotation apart)
-  __device__ __forceinline__ void init(const HeadArgs& a, int b, int n, int u) {
+  __device__ __forceinline__ void init(const HeadArgs& a, const float2* table, int slot, int u) {
     const int c0 = u * VEC, half = a.R / 2;
-    const bool rot = c0 < a.R;
+    const bool rot = c0 < a.R, upper = !INTER && c0 >= half;
     other = (int)threadIdx.x & 63;
-    if constexpr (INTER) {
+    if (!INTER && rot) other += upper ? -(half / VEC) : half / VEC;
+    const float2* mine = table + slot * half + (INTER ? c0 / 2 : upper ? c0 - half : c0);
 #pragma unroll
-      for (int i = 0; i < VEC / 2; ++i) {
-        cs[i] = 1.0f;
-        sn[i] = 0.0f;
-        if (rot) a.at.at(b, n, c0 / 2 + i, sn[i], cs[i]);
-      }
-    } else {
-      const bool upper = c0 >= half;
-      if (rot) other += upper ? -(half / VEC) : half / VEC;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        cs[i] = 1.0f;
-        sn[i] = 0.0f;
-        if (rot) {
-          a.at.at(b, n, c0 + i - (upper ? half : 0), sn[i], cs[i]);
-          if (!upper) sn[i] = -sn[i];
-        }
+    for (int i = 0; i < (INTER ? VEC / 2 : VEC); ++i) {
+      cs[i] = 1.0f;
+      sn[i] = 0.0f;
+      if (rot) {
+        sn[i] = INTER || upper ? mine[i].x : -mine[i].x;
+        cs[i] = mine[i].y;
       }
     }
   }
@@ -110,8 +117,35 @@ __device__ __forceinline__ P from_lane(const P& v, int lane) {
   }
   return r;
 }
-__device__ __forceinline__ float head_sum(float v, int lanes) {
-  for (int off = lanes >> 1; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+// the sums of C values over the lanes of a head, in every one of them.  The values go
+// through each step together (a step alone waits for the one before), by data-parallel
+// moves inside a row of 16 lanes (after two steps a quad's lanes agree, so mirrors do)
+template <int C>
+__device__ __forceinline__ void head_sums(float* v, int lanes) {
+  auto add = [&](auto ctrl) {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      v[i] += __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v[i]), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  if (lanes > 1) add(std::integral_constant<int, 0xb1>{});   // quad_perm [1, 0, 3, 2]
+  if (lanes > 2) add(std::integral_constant<int, 0x4e>{});   // quad_perm [2, 3, 0, 1]
+  if (lanes > 4) add(std::integral_constant<int, 0x141>{});  // row_half_mirror
+  if (lanes > 8) add(std::integral_constant<int, 0x140>{});  // row_mirror
+  if (lanes > 16) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+  }
+  if (lanes > 32) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = xor32_add(v[i]);
+  }
+}
+
+__device__ __forceinline__ float head_sum(float v) {
+  head_sums<1>(&v, 64);
   return v;
 }
 
@@ -131,8 +165,11 @@ __global__ __launch_bounds__(kThreads) void head_norm_kernel(HeadArgs a) {
   const bool live = u * VEC < a.D && token < a.tokens;
   token = token < a.tokens ? token : a.tokens - 1;  // (every lane takes part in the shuffles)
   const int b = (int)(token / a.S), n = (int)(token - (int64_t)b * a.S), c0 = u * VEC;
+  __shared__ float2 table[kThreads / 2 * VEC];  // (tokens x pairs: at most lanes x VEC / 2 pairs)
+  put_angles<VEC>(a, a.first + (int64_t)blockIdx.x * a.tpb, table);
+  __syncthreads();
   LaneTurn<VEC, INTER> turn;
-  turn.init(a, b, n, u);
+  turn.init(a, table, slot, u);
   const float per = 1.0f / (float)a.D;
 #pragma unroll 1
   for (int t = 0; t < 2; ++t) {
@@ -156,22 +193,26 @@ __global__ __launch_bounds__(kThreads) void head_norm_kernel(HeadArgs a) {
         for (int x = 0; x < VEC; ++x) v[i].set(x, 0.0f);
         if (live) v[i] = P::load(a.x[t], src + (int64_t)(h + i) * a.xh[t]);
       }
+      float inv[C];
 #pragma unroll
       for (int i = 0; i < C; ++i) {
-        float f[VEC], p[VEC], ss = 0.0f;
+        inv[i] = 0.0f;
 #pragma unroll
-        for (int x = 0; x < VEC; ++x) {
-          f[x] = v[i].get(x);
-          ss = __builtin_fmaf(f[x], f[x], ss);
-        }
-        const float inv = 1.0f / sqrtf(__builtin_fmaf(head_sum(ss, a.lanes), per, a.eps));
+        for (int x = 0; x < VEC; ++x) inv[i] = __builtin_fmaf(v[i].get(x), v[i].get(x), inv[i]);
+      }
+      head_sums<C>(inv, a.lanes);
+#pragma unroll
+      for (int i = 0; i < C; ++i) inv[i] = 1.0f / sqrtf(__builtin_fmaf(inv[i], per, a.eps));
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        float f[VEC], p[VEC];
         if constexpr (!INTER) {
           const P o = from_lane(v[i], turn.other);
 #pragma unroll
-          for (int x = 0; x < VEC; ++x) p[x] = o.get(x) * inv * wp[x];
+          for (int x = 0; x < VEC; ++x) p[x] = o.get(x) * inv[i] * wp[x];
         }
 #pragma unroll
-        for (int x = 0; x < VEC; ++x) f[x] = f[x] * inv * w[x];
+        for (int x = 0; x < VEC; ++x) f[x] = v[i].get(x) * inv[i] * w[x];
         turn.turn(f, p);
         P o;
 #pragma unroll
@@ -180,7 +221,8 @@ __global__ __launch_bounds__(kThreads) void head_norm_kernel(HeadArgs a) {
       }
     };
     for (; h + HEADS <= end; h += HEADS) some(std::integral_constant<int, HEADS>{});
-    for (; h < end; ++h) some(std::integral_constant<int, 1>{});
+    for (; h + 2 <= end; h += 2) some(std::integral_constant<int, 2>{});
+    if (h < end) some(std::integral_constant<int, 1>{});
   }
 }
 
@@ -189,6 +231,7 @@ __global__ __launch_bounds__(kThreads) void head_norm_bwd_kernel(HeadArgs a) {
   typedef Pack<E, VEC> P;
   constexpr int HEADS = 2;
   __shared__ float red[kThreads * VEC];
+  float2* const table = reinterpret_cast<float2*>(red);  // (until the sums at the end)
   const int u = (int)threadIdx.x & (a.lanes - 1), slot = (int)threadIdx.x / a.lanes, c0 = u * VEC;
   const float per = 1.0f / (float)a.D;
   const int64_t blocks = (a.tokens + a.tpb - 1) / a.tpb;
@@ -207,8 +250,11 @@ __global__ __launch_bounds__(kThreads) void head_norm_bwd_kernel(HeadArgs a) {
       const bool live = c0 < a.D && token < a.tokens;
       token = token < a.tokens ? token : a.tokens - 1;
       const int b = (int)(token / a.S), n = (int)(token - (int64_t)b * a.S);
+      __syncthreads();  // (nobody reads the last tokens' angles any more)
+      put_angles<VEC>(a, block * a.tpb, table);
+      __syncthreads();
       LaneTurn<VEC, INTER> turn;
-      turn.init(a, b, n, u);
+      turn.init(a, table, slot, u);
       const int64_t src = (int64_t)b * a.xb[t] + (int64_t)n * a.xs[t] + c0;
       const int64_t grad = (int64_t)b * a.gb[t] + (int64_t)n * a.gs[t] + c0;
       const int64_t dst = (int64_t)b * a.ob[t] + (int64_t)n * a.os[t] + c0;
@@ -228,31 +274,36 @@ __global__ __launch_bounds__(kThreads) void head_norm_bwd_kernel(HeadArgs a) {
             g[i] = P::load(a.g[t], grad + (int64_t)(h + i) * a.gh[t]);
           }
         }
+        float f[C][VEC], sums[2 * C];  // gradients turned back; sums of x^2 and of g w x
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-          float f[VEC], p[VEC], ss = 0.0f, sg = 0.0f;
+          float p[VEC];
           if constexpr (!INTER) {
             const P o = from_lane(g[i], turn.other);
 #pragma unroll
             for (int x = 0; x < VEC; ++x) p[x] = o.get(x);
           }
+          sums[2 * i] = sums[2 * i + 1] = 0.0f;
 #pragma unroll
-          for (int x = 0; x < VEC; ++x) f[x] = g[i].get(x);
-          turn.turn(f, p);  // (angles of the other sign)
+          for (int x = 0; x < VEC; ++x) f[i][x] = g[i].get(x);
+          turn.turn(f[i], p);  // (angles of the other sign)
 #pragma unroll
           for (int x = 0; x < VEC; ++x) {
             const float y = v[i].get(x);
-            ss = __builtin_fmaf(y, y, ss);
-            sg = __builtin_fmaf(f[x] * w[x], y, sg);
+            sums[2 * i] = __builtin_fmaf(y, y, sums[2 * i]);
+            sums[2 * i + 1] = __builtin_fmaf(f[i][x] * w[x], y, sums[2 * i + 1]);
           }
-          const float inv = 1.0f / sqrtf(__builtin_fmaf(head_sum(ss, a.lanes), per, a.eps));
-          const float mean = head_sum(sg, a.lanes) * inv * per;
+        }
+        head_sums<2 * C>(sums, a.lanes);
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          const float inv = 1.0f / sqrtf(__builtin_fmaf(sums[2 * i], per, a.eps)), mean = sums[2 * i + 1] * inv * per;
           P o;
 #pragma unroll
           for (int x = 0; x < VEC; ++x) {
             const float xh = v[i].get(x) * inv;
-            if (live) dw[x] = __builtin_fmaf(f[x], xh, dw[x]);
-            o.set(x, inv * __builtin_fmaf(-xh, mean, f[x] * w[x]));
+            if (live) dw[x] = __builtin_fmaf(f[i][x], xh, dw[x]);
+            o.set(x, inv * __builtin_fmaf(-xh, mean, f[i][x] * w[x]));
           }
           if (live) o.store(a.o[t], dst + (int64_t)(h + i) * a.oh[t]);
         }
@@ -331,8 +382,8 @@ __global__ __launch_bounds__(kThreads) void head_norm_any_kernel(HeadArgs a, int
             sg = __builtin_fmaf(g[j] * w[j], v[j], sg);
           }
         }
-        const float inv = 1.0f / sqrtf(__builtin_fmaf(head_sum(ss, 64), per, a.eps));
-        const float mean = BWD ? head_sum(sg, 64) * inv * per : 0.0f;
+        const float inv = 1.0f / sqrtf(__builtin_fmaf(head_sum(ss), per, a.eps));
+        const float mean = BWD ? head_sum(sg) * inv * per : 0.0f;
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
           const int c = lane + 64 * j;
@@ -381,8 +432,8 @@ __global__ __launch_bounds__(256) void head_norm_dw_kernel(const float* partial,
 }
 
 // How a launch is cut: `vec` elements a lane (0: one wave a row), tokens per
-// workgroup, and heads per slice (blockIdx.y) so that the chip holds eight workgroups
-// a CU (2,048; the backward 1,024, each leaving a partial row)
+// workgroup, and heads per slice (blockIdx.y): as many slices as one round of the chip
+// holds (six workgroups a CU, the backward four, each leaving a partial row)
 struct HeadCut {
   int vec, lanes, tpb, heads_per;
   int64_t gx, gy;
@@ -395,8 +446,7 @@ HeadCut head_cut(int vec, int64_t tokens, int heads, int D, bool bwd) {
     for (c.lanes = 1; c.lanes * vec < D;) c.lanes *= 2;
   c.tpb = kThreads / c.lanes;
   c.gx = (tokens + c.tpb - 1) / c.tpb;
-  const int64_t want = bwd ? kParts : 2048;
-  const int64_t slices = c.gx >= want ? 1 : (want + c.gx - 1) / c.gx;
+  const int64_t want = bwd ? kParts : 1536, slices = c.gx >= want ? 1 : want / c.gx;
   c.heads_per = slices >= heads ? 1 : (int)((heads + slices - 1) / slices);
   c.gy = (heads + c.heads_per - 1) / c.heads_per;
   if (bwd && c.gx * c.gy > kParts) c.gx = kParts / c.gy > 1 ? kParts / c.gy : 1;
