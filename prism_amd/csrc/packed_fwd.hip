@@ -284,8 +284,16 @@ __global__ __launch_bounds__(kPlanThreads) void pack_plan_kernel(PackArgs a, Pac
   int lanes = 64;
   while (lanes > 1 && (kPlanThreads / lanes) < a.B + 2) lanes >>= 1;
   const int group = tid / lanes, sub = tid & (lanes - 1), groups = kPlanThreads / lanes;
+  // (three walks over the blocks; the group's first sequence, and a thread's first block of it,
+  // often its only ones, are looked up once)
+  PackSeq mine{0, 0, 0, 0};
+  if (group < a.B + 2) mine = pack_seq(a, group, l.keys);
+  const int my_tiles = pack_tiles(a, mine);
+  const int my_cost = sub * l.gs < my_tiles ? pack_cost(a, l, mine, sub * l.gs, my_tiles) : 0;
   auto blocks = [&](auto visit) {
-    for (int s = group; s < a.B + 2; s += groups) {
+    if (sub * l.gs < my_tiles) visit(mine, sub * l.gs, my_cost);
+    for (int t = (sub + lanes) * l.gs; t < my_tiles; t += lanes * l.gs) visit(mine, t, pack_cost(a, l, mine, t, my_tiles));
+    for (int s = group + groups; s < a.B + 2; s += groups) {
       const PackSeq q = pack_seq(a, s, l.keys);
       const int tiles = pack_tiles(a, q);
       for (int t = sub * l.gs; t < tiles; t += lanes * l.gs) visit(q, t, pack_cost(a, l, q, t, tiles));
@@ -313,18 +321,19 @@ __global__ __launch_bounds__(kPlanThreads) void pack_plan_kernel(PackArgs a, Pac
     }
   }
   __syncthreads();
-  // a part's length; without cuts, the longest block's
+  // a part's length, about; without cuts, the longest block's
   const int whole = longest;
   int share = whole;
   if (l.want) {
-    const unsigned long long fair = (total + l.want - 1) / l.want;
-    share = fair < (unsigned long long)whole ? (int)fair : whole;
+    const double fair = ceil((double)total / (double)l.want);
+    share = fair < (double)whole ? (int)fair : whole;
     share = share > l.least ? share : l.least;
   }
-  auto parts_of = [&](int c) { return c <= share ? 1 : (c + share - 1) / share; };
+  auto parts_of = [&](int c) { return l.want == 0 || c < share + share / 2 ? 1 : (c + share / 2) / share; };
+  const float per_bin = (float)(kBins - 1) / (float)whole;
   auto bin_of = [&](int c, int parts) {  // longest first
-    const int len = (c + parts - 1) / parts;
-    return kBins - 1 - (int)((int64_t)len * (kBins - 1) / whole);
+    const int bin = kBins - 1 - (int)((float)c * per_bin / (float)parts);
+    return bin < 0 ? 0 : bin < kBins ? bin : kBins - 1;
   };
   blocks([&](const PackSeq&, int, int c) {
     const int p = parts_of(c);
@@ -387,16 +396,30 @@ PackCut pack_cut(int64_t rows, int unit, int64_t B, int64_t Hk, int64_t slots, i
     c.list.items = (int)(tiles * Hk);
     return c;
   }
-  int gs = 8;
+  // Blocks of eight tiles where sequences have many (16,001 tokens of three, 32 heads over 8:
+  // 737 us, of four 755, of two 769, single ones 797); of two tiles of keys, which are longer and
+  // are cut (eight of 12,000: dQ and dK/dV 614 us, of eight 654).
+  int gs = keys ? 2 : 8;
   while (gs > 1 && mean < 2 * gs) gs /= 2;
   const int64_t per = gs * Hk, blocks = rows / (unit * gs) + B + 2;
-  const int64_t want = tiles * Hk > 6 * slots ? 0 : (2 * slots + per - 1) / per;
+  // Parts.  Rows: as many as make one round of the chip with the tiles, none where the tiles
+  // fill it: a part's sums are written and read (66 KB at D = 128).  Measured (us, uncut / one
+  // round / two rounds of parts), forward, D = 128: one sequence of 4,000, 2 heads 77 / 37 / 41;
+  // 2,047, 32 heads over 8 (one round uncut) 58 / 59 / 76; six of 8,191 in all, 16 over 4, (two
+  // rounds) 73 / 75 / 103.  Keys, whose lists differ most and whose workgroups have a CU each: of
+  // nine tenths of a round.  dQ and dK/dV (uncut / three quarters / nine tenths / 1.2 rounds):
+  // the same 125 / 81 / 78 / 85, 231 / 175 / 163 / 179, 257 / 260 / 238 / 235; four of 5,000
+  // without the mask, 10 over 5, 155 / 160 / 162 / 179.
+  const int64_t fill = slots > tiles * Hk ? slots - tiles * Hk : 0;
+  const int64_t want = keys ? (tiles * Hk > 6 * slots ? 0 : (slots * 9 / 10 + per - 1) / per) : fill / per;
   c.list.gs = gs;
   c.list.per = (int)per;
   c.list.want = (int)want;
+  // A block is cut into length / share parts, rounded, from 1.5 shares on, the shares being `want`
+  // at most in all: no more than 2/3 of want are cut, into no more than 4/3 of it
   c.entries = blocks + want;
-  c.cuts = want;
-  c.pieces = 2 * want * per;
+  c.cuts = (2 * want + 2) / 3;
+  c.pieces = want ? (4 * want + 2) / 3 * per : 0;
   c.list.max_entries = (int)c.entries;
   c.list.max_cuts = (int)c.cuts;
   c.list.max_pieces = (int)c.pieces;
