@@ -226,7 +226,7 @@ __global__ __launch_bounds__(256, 1) void paged16_kernel(PagedArgs a) {
         copy_b128(voff[i & 3], vh[2 * i / KB] + (i >> 2) * RS::ROWS4 * vstep, lds + (uint32_t)(KB + i) * 1024u);
       return;
     }
-#pragma unroll 1
+#pragma unroll 4
     for (int i = 0; i < KB; ++i) {
       const int u = u0 + RS::row(i, lane), key = u < nk ? u : nk - 1, at = RS::byte(i, lane), id = page_of(key);
       const int64_t x = id < 0 ? 0 : id;
@@ -726,7 +726,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     a.lse[(int64_t)head * a.B * a.n + token] = has_weight(l) ? (top + __log2f(l)) * 0.6931471805599453f : NINF;
 }
 
-// How a call is cut: rows of a tile, keys of a tile, and over how many workgroups at most
+// How a call is cut: rows of a tile, keys of a tile, and over how many workgroups at most.
+//
+// One round of the chip at most (one workgroup a CU over 16 bits, two over 4), about sqrt(keys)
+// / 2.5 parts (4 bits, tiles twice as long: / 5), one up to 512 keys, and no part of a sequence
+// below two tiles.  Measured (us, 32 heads over 8, D = 128, pages of 16 or 64; lengths from half
+// to all of the stated): 16 bits, 256 / 512 / 1,024 workgroups: 1 x 32,768 26 / 33 / 34; 16 x
+// 8,192 84 / 85 / 91; 64 x 2,048 82 / 82 / 97; 8 x 131,072 561 / 543 / 537.  4 bits: 18 / 21 /
+// 21; 39 / 35 / 38; 33 / 33 / 42; 209 / 183 / 179; 2 x 131,072 46 / 45 / 52.  Parts of 2 / 8 / 16
+// tiles at least: 1 x 1,000 12.1 / 14.0 / 16.2 (4 bits 10.7 / 12.1 / 12.8), 1 x 4,096 14.8 / 14.7
+// / 17.9 (12.1 / 14.0 / 17.3).
 struct PagedCut {
   int rows, keys, least;
   int64_t tiles, total, splits;
@@ -736,12 +745,12 @@ PagedCut paged_cut(int B, int64_t n, int Hk, int64_t G, int64_t places, int bits
   const int64_t rows = n * G;
   c.rows = bits == 16 || rows > 16 ? 32 : 16;
   c.keys = bits == 16 ? 32 : 64;
-  c.least = bits == 16 ? 8 : 8;
+  c.least = 2;
   c.tiles = (rows + c.rows - 1) / c.rows;
   c.total = (int64_t)B * Hk * c.tiles;
-  const int64_t slots = bits == 16 ? 256 : 1024;
+  const int64_t slots = bits == 16 ? 256 : 512;
   const int64_t by_chip = c.total ? slots / c.total : 1;
-  int64_t s = places <= 512 ? 1 : (int64_t)(__builtin_sqrt((double)places) / 2.5);
+  int64_t s = places <= 512 ? 1 : (int64_t)(__builtin_sqrt((double)places) / (bits == 16 ? 2.5 : 5.0));
   s = s < by_chip ? s : by_chip;
   c.splits = s < 1 ? 1 : s < kMaxSplits ? s : kMaxSplits;
   return c;
