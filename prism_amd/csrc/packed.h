@@ -85,6 +85,10 @@ struct PackItem {
   PackSeq s;
   int hk, tile, part, parts, slot;  // slot: workspace piece, -1: the whole list
   bool live;
+  // the first of `all` list tiles that part p takes (all x parts may pass 32 bits)
+  __device__ __forceinline__ int first_of(int all, int p) const {
+    return slot < 0 ? (p ? all : 0) : (int)((int64_t)all * p / parts);
+  }
   // without a list: sequences in order, tile by tile (B <= 62; all lanes active)
   __device__ __forceinline__ void direct(const PackArgs& a, int id) {
     const int lane = (int)threadIdx.x & 63, x = id / a.Hk;

@@ -61,8 +61,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dq_kernel(PackBwd
   auto token = [&](int r) { return (r < rows ? r : rows - 1) / a.G; };
   const int nk = pack_keys(a, it.s, token(r0 + 127));
   const int every = (nk + 63) >> 6;
-  const int t0 = it.slot < 0 ? 0 : every * it.part / it.parts;
-  const int t1 = it.slot < 0 ? every : every * (it.part + 1) / it.parts;
+  const int t0 = it.first_of(every, it.part), t1 = it.first_of(every, it.part + 1);
 
   PackCopy<D> copy;
   copy.init(a, it, w & 1, lane);
@@ -263,7 +262,7 @@ __global__ __launch_bounds__(DkdvTiles<D>::THREADS, D == 64 ? 3 : 1) void packed
   // the tile's tokens, as 64-token tiles of each head from lo on
   const int lo = pack_first(a, it.s, j0), hi = it.s.n - 1;
   const int nti = hi >= lo ? (hi - lo + 64) >> 6 : 0, all = nti * a.G;
-  const int e0 = (int)((int64_t)all * it.part / it.parts), e1 = (int)((int64_t)all * (it.part + 1) / it.parts);
+  const int e0 = it.first_of(all, it.part), e1 = it.first_of(all, it.part + 1);
   const int n = e1 - e0;
 
   // copies: waves 0-3 issue KB-instructions w, w + 4, ... (Q then dO), wave 3

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_fwd_kernel(PackAr
   auto token = [&](int r) { return (r < rows ? r : rows - 1) / a.G; };
   const int nk = pack_keys(a, it.s, token(r0 + 127));
   const int all = (nk + 63) >> 6;
-  const int t0 = it.slot < 0 ? 0 : all * it.part / it.parts, t1 = it.slot < 0 ? all : all * (it.part + 1) / it.parts;
+  const int t0 = it.first_of(all, it.part), t1 = it.first_of(all, it.part + 1);
 
   const float NINF = -__builtin_inff();
   PackCopy<D> copy;
@@ -290,13 +290,16 @@ __global__ __launch_bounds__(kPlanThreads) void pack_plan_kernel(PackArgs a, Pac
   if (group < a.B + 2) mine = pack_seq(a, group, l.keys);
   const int my_tiles = pack_tiles(a, mine);
   const int my_cost = sub * l.gs < my_tiles ? pack_cost(a, l, mine, sub * l.gs, my_tiles) : 0;
+  // (no thread walks more blocks than sequences that do not overlap can have in all)
   auto blocks = [&](auto visit) {
+    int left = l.max_entries;
     if (sub * l.gs < my_tiles) visit(mine, sub * l.gs, my_cost);
-    for (int t = (sub + lanes) * l.gs; t < my_tiles; t += lanes * l.gs) visit(mine, t, pack_cost(a, l, mine, t, my_tiles));
+    for (int t = (sub + lanes) * l.gs; t < my_tiles && left > 0; t += lanes * l.gs, --left)
+      visit(mine, t, pack_cost(a, l, mine, t, my_tiles));
     for (int s = group + groups; s < a.B + 2; s += groups) {
       const PackSeq q = pack_seq(a, s, l.keys);
       const int tiles = pack_tiles(a, q);
-      for (int t = sub * l.gs; t < tiles; t += lanes * l.gs) visit(q, t, pack_cost(a, l, q, t, tiles));
+      for (int t = sub * l.gs; t < tiles && left > 0; t += lanes * l.gs, --left) visit(q, t, pack_cost(a, l, q, t, tiles));
     }
   };
   if (tid == 0) {
@@ -351,7 +354,7 @@ __global__ __launch_bounds__(kPlanThreads) void pack_plan_kernel(PackArgs a, Pac
   if (tid < kBins) {
     for (int x = 0; x < (tid >> 6); ++x) upto += sums[x];
     at[tid] = upto - count;
-    if (tid == kBins - 1) l.counts[0] = upto < l.max_entries ? upto : l.max_entries;
+    if (tid == kBins - 1) l.counts[0] = (uint32_t)upto < (uint32_t)l.max_entries ? upto : l.max_entries;
   }
   __syncthreads();
   blocks([&](const PackSeq& q, int t, int c) {
@@ -361,16 +364,16 @@ __global__ __launch_bounds__(kPlanThreads) void pack_plan_kernel(PackArgs a, Pac
       const int x = atomicAdd(&cuts, 1);
       slot = atomicAdd(&pieces, p * l.per);
       // (bounds that overlap could ask for more than there is room for: such a block is dropped)
-      if (x >= l.max_cuts || slot + p * l.per > l.max_pieces) slot = -2;
+      if ((uint32_t)x >= (uint32_t)l.max_cuts || slot < 0 || slot > l.max_pieces - p * l.per) slot = -2;
       else l.cuts[x] = PackEntry{q.q0, q.n, q.k0, q.L, t, 0, p, slot};
     }
     for (int y = 0; y < p; ++y)
-      if (first + y < l.max_entries)
+      if ((uint32_t)(first + y) < (uint32_t)l.max_entries)
         l.entries[first + y] = slot == -2 ? PackEntry{0, 0, 0, 0, 0, 0, 1, -1} : PackEntry{q.q0, q.n, q.k0, q.L, t, y, p, slot};
   });
   __syncthreads();
   if (tid == 0) {
-    l.counts[1] = cuts < l.max_cuts ? cuts : l.max_cuts;
+    l.counts[1] = (uint32_t)cuts < (uint32_t)l.max_cuts ? cuts : l.max_cuts;
     l.counts[2] = pieces;
   }
 }

@@ -30,8 +30,8 @@ def flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     cu_seqlens[b] to cu_seqlens[b + 1] - 1 of q, its keys the same rows of k and v, or
     those that cu_seqlens_k [B + 1] says (the next part of a prompt over all of its keys).
     Sequences may be empty; values outside the tensors are cut to them (where they
-    decrease, what stands in the results of those rows is not defined).  The queries are
-    the last of their sequence: with L keys and n queries, query i sees keys j <= i + L - n
+    decrease, nothing outside is read or written, but the results are not defined).  The
+    queries are the last of their sequence: with L keys and n queries, query i sees keys j <= i + L - n
     (causal), or all.  Queries that see no key, and rows of no sequence, give 0, and take
     and give no gradient.  sm_scale (positive) defaults to D^-1/2.  A NaN or an infinity in
     a key or value reaches the queries that see it and no others (at about 1 us a key); in

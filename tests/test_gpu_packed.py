@@ -165,6 +165,38 @@ def test_rows_of_no_sequence(many):
     check(q, k, v, b, do=do)
 
 
+def test_more_list_tiles_times_parts_than_32_bits():
+    """2^28 keys (one row, at stride 0) cut into a thousand parts, all seen by a few rows: with
+    k = 0 and small integers in v every sum of a part is exact, so o is v itself."""
+    n, D = 1 << 28, 64
+    q = make(3, 1, D, torch.bfloat16, 1)
+    k = torch.zeros(1, 1, D, dtype=torch.bfloat16, device=DEV)
+    v = torch.randint(-4, 5, (1, 1, D), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).bfloat16()
+    o, lse = prism_amd.flash_attn_packed(q, k.expand(n, 1, D), v.expand(n, 1, D), cu([3]), cu_seqlens_k=cu([n]), causal=False,
+                                         return_lse=True)
+    assert torch.equal(o, v.expand(3, 1, D)) and ((lse - 28 * math.log(2)).abs() <= 28 * 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("B", [5, 61, 700])
+def test_bounds_that_decrease_stay_inside(B):
+    """Bounds in any order: what comes of them is not defined, but the calls before and
+    after, and tensors beside theirs, are as they were."""
+    T, H, D = 1500, 2, 64
+    pool = torch.full((4, T, H, D), 3.0, dtype=torch.bfloat16, device=DEV)
+    pool[1:3] = make(2 * T, H, D, torch.bfloat16, 3).view(2, T, H, D)
+    q, k = (x.detach().requires_grad_(True) for x in pool[1:3])
+    good = cu([700, 300, 500])
+    want, _ = prism_amd.flash_attn_packed(q, k, k, good, return_lse=True)
+    for seed in range(3):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        any_, other = (torch.randint(-99, T + 99, (B + 1,), generator=g, device=DEV, dtype=torch.int32) for _ in "qk")
+        for causal in (True, False):
+            o = prism_amd.flash_attn_packed(q, k, k, any_, cu_seqlens_k=other, causal=causal)
+            torch.autograd.grad(o, (q, k), torch.ones_like(o))
+    assert torch.equal(want, prism_amd.flash_attn_packed(q, k, k, good))
+    assert (pool[0] == 3).all() and (pool[3] == 3).all()
+
+
 def test_no_tokens_and_no_sequences():
     z = torch.zeros(1, dtype=torch.int32, device=DEV)
     q = torch.randn(9, 4, 64, device=DEV).bfloat16().requires_grad_(True)
