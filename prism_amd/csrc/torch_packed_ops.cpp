@@ -398,6 +398,9 @@ void paged_append(const Tensor& k_, const Tensor& v_, const Tensor& kc, const Te
   TORCH_CHECK_VALUE(cu_ || (B == 0 ? T == 0 : T % B == 0), "append_paged: ", T, " tokens do not share out over ", B, " sequences");
   TORCH_CHECK_VALUE(!freqs_ || freqs_->dim() == 1, "append_paged: freqs must be [pairs]");
   TORCH_CHECK_VALUE(freqs_ || !pos, "append_paged: positions without freqs");
+  for (const Tensor* t : {&kc, &vc})
+    TORCH_CHECK_VALUE(at::has_internal_overlap(*t) != at::MemOverlap::Yes,
+                      "append_paged: a cache whose places share memory (expand) cannot be written");
   const c10::DeviceGuard guard(k_.device());
   const Tensor k = pack_rows(k_), v = pack_rows(v_), table = unit_table(table_), lens = lens_.contiguous();
   const OptT cu = cont(cu_), freqs = cont(freqs_);

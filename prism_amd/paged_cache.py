@@ -98,8 +98,8 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     and strides of whole 16 bytes; 16 bits: of k's dtype.  4 bits: 32 channels share the least
     power of two that keeps them within 6 times it (no smaller than 2^-126), and each is
     rounded to the nearest value (halves to the even code); 32 channels of which one is a NaN
-    or an infinity are read as NaN.  Beside float16 queries or reads, values of 61,440 and
-    more may become infinite.
+    or an infinity are read as NaN.  Values whose level is beyond a type's largest are infinite
+    where they are read in it (float16: from 57,344 on, next to 65,536; bfloat16: 2.98e38).
 
     freqs: float64 [pairs] (rotary_frequencies), or None for keys that are turned already:
     turns k as apply_rotary does, at positions (int32 or int64 [T], with sections [T, axes]) or
@@ -184,7 +184,9 @@ def flash_attn_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     is no page (-1, say) are not seen.  Tokens that see nothing give 0.  Made for few tokens (up
     to 32 rows of tokens x Hq / Hk share one read of the cache); for more, gather_paged and
     flash_attn_packed.  sm_scale (positive) defaults to D^-1/2.  A NaN or an infinity in a key
-    or value reaches the tokens that see it and no others.
+    or value reaches the tokens that see it and no others (a value's in 4 bits: where the
+    key's weight is not below 2^-126 of the largest's).  4 bits: values of 2^100 and more may
+    become infinite in the sums.
 
     Returns o, of q's shape (and layout, where q is dense), with return_lse (o, lse): lse [Hq,
     T] float32, the natural log of the sum of exponentials of the scaled scores, -inf where

@@ -205,6 +205,36 @@ def test_four_bits_at_borders():
         assert torch.isnan(want).any() and want[torch.isfinite(want)].abs().max() >= 6
 
 
+def test_four_bits_beyond_the_types_largest():
+    """The largest level of a type's largest values may lie beyond them: read as infinite, and
+    the value below the border is not."""
+    for dtype, border, below in ((torch.float16, 57344.0, 49152.0), (torch.bfloat16, 7 * 2.0 ** 125, 6 * 2.0 ** 125)):
+        x = torch.zeros(2, 1, 64, dtype=dtype, device=DEV)
+        x[0, 0, 3], x[0, 0, 40], x[1, 0, 9] = border, -border, border * (1 - torch.finfo(dtype).eps)
+        kc, vc = prism_amd.paged_cache(1, 16, 1, 64, dtype=dtype, bits=4)
+        prism_amd.append_paged(x, -x, kc, vc, ints([[0]]), ints([2]))
+        gk, gv = prism_amd.gather_paged(kc, vc, ints([[0]]), cu([2]), 2, head_dim=64, dtype=dtype)
+        for got, sign in ((gk, 1.0), (gv, -1.0)):
+            want = torch.zeros_like(x)
+            want[0, 0, 3], want[0, 0, 40], want[1, 0, 9] = sign * math.inf, -sign * math.inf, sign * below
+            assert torch.equal(got, want)
+
+
+def test_caches_that_share_places_are_refused():
+    k = torch.randn(2, 4, 64, device=DEV).bfloat16()
+    kc, vc = prism_amd.paged_cache(3, 16, 4, 64)
+    for kk, vv in ((kc[:, :1].expand_as(kc), vc), (kc, vc[:1].expand_as(vc))):
+        with pytest.raises(ValueError, match="share memory"):
+            prism_amd.append_paged(k, k, kk, vv, ints([[0], [1]]), ints([1, 1]))
+    assert not kc.any() and not vc.any()
+    # (to read, they may)
+    prism_amd.append_paged(k[:, :1], k[:, :1], *prism_amd.paged_cache(3, 16, 1, 64), ints([[0], [1]]), ints([1, 1]))
+    one = [c[:, :1].expand_as(c) for c in (kc, vc)]
+    kc[:, :1].normal_()
+    vc[:, :1].normal_()
+    check(k, *one, ints([[0], [1]]), [9, 16], page=16)
+
+
 def test_places_that_are_none():
     """Tokens before the table or beyond it, pages that are none, rows of no sequence:
     not stored, and nothing else is changed."""
