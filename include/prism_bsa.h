@@ -14,8 +14,8 @@
  * operators (prism_amd/csrc/torch_ops.cpp) or through ctypes.
  *
  * dtype codes: PRISM_F32 = 0, PRISM_BF16 = 1; the layer's operators (row norms,
- * rotary positions, window attention) also take PRISM_F16 = 2, and the norms
- * write PRISM_E4M3 = 3 (OCP float8 e4m3) and PRISM_I8 = 4.
+ * rotary positions, window and packed attention, paged caches) also take PRISM_F16 = 2,
+ * and the norms write PRISM_E4M3 = 3 (OCP float8 e4m3) and PRISM_I8 = 4.
  * Layouts: "THW order" = the reference's flattened (t, h, w) token order of a
  * padded grid T x Hg x Wg (all multiples of 8); "tile order" = the per-zone
  * anisotropic rearrangement of _build_rearrange_index

@@ -9,7 +9,7 @@
 
 Each csrc/*.hip file is compiled by hipcc for gfx950 only and linked into one
 shared library exporting the C-ABI declared in include/prism_bsa.h;
-csrc/torch_ops.cpp and torch_layer_ops.cpp (host C++, no device code) are built
+csrc/torch_ops.cpp, torch_layer_ops.cpp and torch_packed_ops.cpp (host C++, no device code) are built
 on top of it into libprism_torch.so, the TORCH_LIBRARY(prism) operators.  Files
 whose results are bit-exact parity targets are compiled with
 -ffp-contract=off (their fused operations are written out explicitly).

