@@ -36,6 +36,7 @@ struct PackList {
   int unit;             // rows (of tokens x G, or keys) of a tile
   int keys;             // tiles of keys (dK/dV), else of rows
   int want, least;      // parts: as many as this of equal length in all (0: never cut), of so many list tiles at least
+  int from;             // blocks longer than from / 4 of such a length are cut
   int items;            // workgroups of the launch
 };
 struct PackArgs {
@@ -81,6 +82,16 @@ __device__ __forceinline__ int pack_first(const PackArgs& a, const PackSeq& s, i
   return x < 0 ? 0 : x < s.n ? x : s.n;
 }
 
+// The item of workgroup id: as xcd_group_remap<8>, but every second run of 64 goes to the XCDs
+// the other way round: the list is sorted by length, and the first XCD would have the longest of
+// each run (dQ and dK/dV of 16,001 tokens of three sequences, 32 heads over 8: 2,275 us, so 2,235;
+// of 8,191 of six, 16 over 4: 243, 237; others within 1%).
+__device__ __forceinline__ int pack_id(const PackList& l, int id) {
+  if (id >= (l.items & ~63)) return id;
+  const int run = id >> 6, xcd = id & 7, slot = (id >> 3) & 7;
+  return run * 64 + (run & 1 ? 7 - xcd : xcd) * 8 + slot;
+}
+
 struct PackItem {
   PackSeq s;
   int hk, tile, part, parts, slot;  // slot: workspace piece, -1: the whole list
@@ -109,13 +120,13 @@ struct PackItem {
     parts = 1;
     slot = -1;
   }
-  __device__ __forceinline__ void of_entry(const PackArgs& a, const PackEntry* e, int r) {
+  __device__ __forceinline__ void of_entry(const PackArgs& a, const PackEntry& e, int r) {
     auto u = [](int x) { return (int)uniform_u32((uint32_t)x); };
-    s.q0 = u(e->q0); s.n = u(e->n); s.k0 = u(e->k0); s.L = u(e->L);
+    s.q0 = u(e.q0); s.n = u(e.n); s.k0 = u(e.k0); s.L = u(e.L);
     hk = r / a.list.gs;
     const int x = r - hk * a.list.gs;
-    tile = u(e->tile) + x;
-    part = u(e->part); parts = u(e->parts); slot = u(e->slot);
+    tile = u(e.tile) + x;
+    part = u(e.part); parts = u(e.parts); slot = u(e.slot);
     if (slot >= 0) slot += (hk * a.list.gs + x) * parts + part;
     live = tile < pack_tiles(a, s);
   }
@@ -125,14 +136,15 @@ struct PackItem {
       return;
     }
     const int blk = id / a.list.per;
+    const PackEntry e = a.list.entries[blk];  // (beside the count, which says whether it holds something)
     live = blk < (int)uniform_u32((uint32_t)a.list.counts[0]);
-    if (live) of_entry(a, a.list.entries + blk, id - blk * a.list.per);
+    if (live) of_entry(a, e, id - blk * a.list.per);
   }
   // block of the join's workgroup id
   __device__ __forceinline__ void init_cut(const PackArgs& a, int id) {
     const int blk = id / a.list.per;
     live = blk < (int)uniform_u32((uint32_t)a.list.counts[1]);
-    if (live) of_entry(a, a.list.cuts + blk, id - blk * a.list.per);
+    if (live) of_entry(a, a.list.cuts[blk], id - blk * a.list.per);
   }
 };
 

@@ -14,8 +14,8 @@
 //
 // Bound: the matrix unit and its operands' reads from LDS (busy 46% in dQ and 55% in dK/dV of
 // the time that includes the last, uneven round).  Measured (bf16, D = 128, causal, 8,191
-// tokens of six sequences, 16 heads over 4): dQ 100 us (0.74 PFLOP/s), dK/dV 143 to 150 (0.68),
-// the lists 5.6, the merge 5; before the lists' parts were sized to nine tenths of a round 163
+// tokens of six sequences, 16 heads over 4): dQ 100 us (0.74 PFLOP/s), dK/dV 128 (0.77),
+// the lists 5.6, the merge 6; before the keys were cut by a fair share of a round 163
 // + 98.
 //
 // Numbers: P and dS are rounded to the inputs' type for the products (float16: times
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_dq_kernel(PackBwd
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
   const int w = (int)uniform_u32(threadIdx.x >> 6);
   PackItem it;
-  it.init(a, xcd_group_remap<8>((int)blockIdx.x, a.list.items));
+  it.init(a, pack_id(a.list, (int)blockIdx.x));
   if (!it.live) return;
   const int rows = it.s.n * a.G, r0 = it.tile * 128, wr0 = r0 + 32 * w;
   auto token = [&](int r) { return (r < rows ? r : rows - 1) / a.G; };
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(DkdvTiles<D>::THREADS, D == 64 ? 3 : 1) void packed
   {
     PackArgs b = a;  // (the list of the keys)
     b.list = ba.keys;
-    it.init(b, xcd_group_remap<8>((int)blockIdx.x, ba.keys.items));
+    it.init(b, pack_id(ba.keys, (int)blockIdx.x));
   }
   if (!it.live) return;
   const int j0 = it.tile * KEYS, off = it.s.n - it.s.L;

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void packed_fwd_kernel(PackAr
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
   const int w = (int)uniform_u32(threadIdx.x >> 6);
   PackItem it;
-  it.init(a, xcd_group_remap<8>((int)blockIdx.x, a.list.items));
+  it.init(a, pack_id(a.list, (int)blockIdx.x));
   if (!it.live) return;
   const int rows = it.s.n * a.G, r0 = it.tile * 128, wr0 = r0 + 32 * w, off = it.s.L - it.s.n;
   auto token = [&](int r) { return (r < rows ? r : rows - 1) / a.G; };
@@ -338,7 +338,9 @@ __global__ __launch_bounds__(kPlanThreads) void pack_plan_kernel(PackArgs a, Pac
     share = fair < (double)whole ? (int)fair : whole;
     share = share > l.least ? share : l.least;
   }
-  auto parts_of = [&](int c) { return l.want == 0 || c < share + share / 2 ? 1 : (c + share / 2) / share; };
+  auto parts_of = [&](int c) {
+    return l.want == 0 || 4 * c <= l.from * share ? 1 : (4 * c - (l.from - 4) * share + 4 * share - 1) / (4 * share);
+  };
   const float per_bin = (float)(kBins - 1) / (float)whole;
   auto bin_of = [&](int c, int parts) {  // longest first
     const int bin = kBins - 1 - (int)((float)c * per_bin / (float)parts);
@@ -416,19 +418,22 @@ PackCut pack_cut(int64_t rows, int unit, int64_t B, int64_t Hk, int64_t slots, i
   // round / two rounds of parts), forward, D = 128: one sequence of 4,000, 2 heads 77 / 37 / 41;
   // 2,047, 32 heads over 8 (one round uncut) 58 / 59 / 76; six of 8,191 in all, 16 over 4, (two
   // rounds) 73 / 75 / 103.  Keys, whose lists differ most and whose workgroups have a CU each: of
-  // nine tenths of a round.  dQ and dK/dV (uncut / three quarters / nine tenths / 1.2 rounds):
-  // the same 125 / 81 / 78 / 85, 231 / 175 / 163 / 179, 257 / 260 / 238 / 235; four of 5,000
-  // without the mask, 10 over 5, 155 / 160 / 162 / 179.
+  // 17 twentieths of a round, from 1.25 such lengths on.  dQ and dK/dV (uncut / three quarters /
+  // nine tenths / 1.2 rounds, all from 1.5 on): the same 125 / 81 / 78 / 85, 231 / 175 / 163 / 179,
+  // 257 / 260 / 238 / 235; four of 5,000 without the mask, 10 over 5, 155 / 160 / 162 / 179.  (0.9
+  // from 1.5 / 0.9 from 1.25 / 0.85 from 1.25 / 0.8 from 1.125: 79 / 78 / 78 / 78, 163 / 171 / 159 /
+  // 159, 240 / 225 / 228 / 227, 160 / 171 / 161 / 177.)
   const int64_t fill = slots > tiles * Hk ? slots - tiles * Hk : 0;
-  const int64_t want = keys ? (tiles * Hk > 6 * slots ? 0 : (slots * 9 / 10 + per - 1) / per) : fill / per;
+  const int64_t want = keys ? (tiles * Hk > 6 * slots ? 0 : (slots * 17 / 20 + per - 1) / per) : fill / per;
+  c.list.from = keys ? 5 : 6;
   c.list.gs = gs;
   c.list.per = (int)per;
   c.list.want = (int)want;
-  // A block is cut into length / share parts, rounded, from 1.5 shares on, the shares being `want`
-  // at most in all: no more than 2/3 of want are cut, into no more than 4/3 of it
+  // A block is cut from f = from / 4 shares on, into length / share - f + 1 parts, rounded up, the
+  // shares being `want` at most in all: no more than want / f are cut, into no more than 2 want / f
   c.entries = blocks + want;
-  c.cuts = (2 * want + 2) / 3;
-  c.pieces = want ? (4 * want + 2) / 3 * per : 0;
+  c.cuts = (4 * want + c.list.from - 1) / c.list.from;
+  c.pieces = (8 * want + c.list.from - 1) / c.list.from * per;
   c.list.max_entries = (int)c.entries;
   c.list.max_cuts = (int)c.cuts;
   c.list.max_pieces = (int)c.pieces;
