@@ -55,7 +55,7 @@ def _register_vmaps():
         return t if d is None or not isinstance(t, torch.Tensor) else t.select(d, i)
 
     for name in ("rms_norm", "rms_norm_bwd", "rotary", "window_fwd", "qk_norm_rotary", "qk_norm_rotary_bwd",
-                 "packed_fwd", "paged_fwd"):
+                 "packed_fwd", "paged_fwd", "paged_gather"):
         if not hasattr(torch.ops.prism, name):  # (a library built before, as for the fakes)
             continue
 

@@ -264,6 +264,21 @@ def test_vmap_gives_the_bits_of_a_loop():
     assert torch.equal(got, torch.stack([prism_amd.flash_attn_paged(x, kc, vc, table, ints([36])) for x in q[:, :2]]))
 
 
+def test_vmap_of_the_caches():
+    """Reading under vmap is the loop's; writing is refused, and nothing is written."""
+    table, pages = table_for([36, 20], 16)
+    kc, vc = prism_amd.paged_cache(pages, 16, 2, 64, bits=4)
+    x = randn(56, 2, 64, seed=4)
+    prism_amd.append_paged(x, x, kc, vc, table, ints([36, 20]), cu_seqlens=cu([36, 20]))
+    read = lambda row: prism_amd.gather_paged(kc, vc, row[None], cu([20]), 22, head_dim=64)  # noqa: E731
+    for a, b in zip(torch.vmap(read)(table), zip(*(read(row) for row in table))):
+        assert torch.equal(a, torch.stack(b))
+    before = kc.clone()
+    with pytest.raises(RuntimeError, match="paged_append"):
+        torch.vmap(lambda y: prism_amd.append_paged(y, y, kc, vc, table[:1], ints([3])))(randn(2, 3, 2, 64, seed=5))
+    assert torch.equal(kc, before)
+
+
 def test_tangents_and_second_derivatives_are_refused():
     import torch.autograd.forward_ad as forward_ad
     freqs, _ = prism_amd.rotary_frequencies(64)
