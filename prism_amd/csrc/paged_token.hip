@@ -588,7 +588,8 @@ __global__ __launch_bounds__(256, 2) void paged4_kernel(PagedArgs a) {
         m[x] = m_new;
       }
       // O^T += V^T P^T, 32 channels (one scale) at a time.  (A key that a row does not see has
-      // P = 0, and 0 times any scale, 255's too, is 0 here.)
+      // P = 0, and 0 times any scale, 255's too, is 0 here.  A key that it sees and whose scale is
+      // 255 makes its sums infinite or NaN: see behind the loop.)
 #pragma unroll
       for (int blk = 0; blk < NS; ++blk) {
         bf16x8 pb[NR][2], pl[NR][2];
@@ -635,6 +636,39 @@ __global__ __launch_bounds__(256, 2) void paged4_kernel(PagedArgs a) {
         }
       }
     }
+  }
+
+  // V's scale 255 stands for NaN, but enters P as an infinity (exponent bits alone), and so do the
+  // sums where a code beside it is not 0.  Telling it in the loop would take two instructions for each
+  // of a tile's 16 D / 32 scales of a lane; where a sum is infinite the wave looks at its keys' scales
+  // again instead (the sums of values of 2^100 and more, which may be infinite too, stay as they are).
+  bool endless = false;
+#pragma unroll
+  for (int x = 0; x < NR; ++x)
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int z = 0; z < 4; ++z) endless = endless || __builtin_fabsf(acc[x][c][z]) == __builtin_inff();
+  if (__builtin_amdgcn_ballot_w64(endless)) {
+#pragma unroll 1
+    for (int c0 = it.t0; c0 < it.t1; c0 += chunk)
+#pragma unroll 1
+      for (int t = c0 + w; t < it.t1 && t < c0 + chunk; t += 4)
+#pragma unroll 1
+        for (int u = 64 * t; u < 64 * t + 64 && u < nk; ++u) {
+          const int page = a.table.page(it.b, u >> lg);
+          if (page < 0) continue;
+          const uint8_t* const of_u = vb + (int64_t)page * a.v.page + scales + (u & mask) * (D / 32);
+#pragma unroll
+          for (int blk = 0; blk < NS; ++blk) {
+            const bool none = of_u[blk] == 255;
+#pragma unroll
+            for (int x = 0; x < NR; ++x)
+#pragma unroll
+              for (int z = 0; z < 8; ++z)
+                if (none && u <= last[x]) acc[x][2 * blk + (z >> 2)][z & 3] = __builtin_nanf("");
+          }
+        }
   }
 
   // join the four waves, as in paged16_kernel: wave w adds a quarter of the blocks

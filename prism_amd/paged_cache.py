@@ -184,7 +184,7 @@ def flash_attn_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     is no page (-1, say) are not seen.  Tokens that see nothing give 0.  Made for few tokens (up
     to 32 rows of tokens x Hq / Hk share one read of the cache); for more, gather_paged and
     flash_attn_packed.  sm_scale (positive) defaults to D^-1/2.  A NaN or an infinity in a key
-    or value reaches the tokens that see it and no others (a value's in 4 bits: where the
+    or value reaches the tokens that see it and no others (4 bits: as NaN, a value's where the
     key's weight is not below 2^-126 of the largest's).  4 bits: values of 2^100 and more may
     become infinite in the sums.
 

@@ -1,0 +1,48 @@
+"""Corners of packed batches and paged caches: blocks of 4 bits that are not finite."""
+import math
+
+import pytest
+import torch
+
+import prism_amd
+from tests.test_gpu_paged import ints, table_for
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def randn(*shape, dt=torch.bfloat16, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.randn(shape, generator=g, device=DEV).to(dt)
+
+
+# ------------------------------------------------------------------ 4 bits
+@pytest.mark.parametrize("n", [1, 5])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_blocks_that_are_not_finite_are_nan(dt, D, n):
+    """32 channels of which one is not finite are read as NaN, whatever codes stand beside
+    their scale: those channels of every token that sees them are NaN (no infinities, whose
+    sign would mean nothing), all else is as it was, parts of long sequences too."""
+    Hq, Hk, page = 8, 2, 16
+    for L in (40, 1500):
+        lens = [L, 30]
+        table, pages = table_for(lens, page)
+        kc, vc = prism_amd.paged_cache(pages, page, Hk, D, bits=4)
+        k, v, q = (randn(*s, dt=dt, seed=i) for i, s in enumerate(((L + 30, Hk, D), (L + 30, Hk, D), (2 * n, Hq, D))))
+        bounds = ints([0, L, L + 30])
+        want = None
+        for place, channel, bad in ((None, 0, 0.0), (L - 2, 5, math.nan), (3, 40, math.inf), (L // 2, D - 1, -math.inf)):
+            x = v.clone()
+            if place is not None:
+                x[place, 1, channel] = bad
+            prism_amd.append_paged(k, x, kc, vc, table, ints(lens), cu_seqlens=bounds)
+            o = prism_amd.flash_attn_paged(q, kc, vc, table, ints(lens))
+            if place is None:
+                want = o
+                assert torch.isfinite(o).all()
+                continue
+            hit = torch.zeros(2 * n, Hq, D, dtype=torch.bool, device=DEV)
+            hit[max(0, place - (L - n)):n, Hq // Hk:, channel // 32 * 32:channel // 32 * 32 + 32] = True
+            assert torch.equal(torch.isnan(o), hit) and torch.equal(o[~hit], want[~hit])
+
