@@ -175,12 +175,20 @@ int prism_packed_bwd(const void* do_, const void* q, const void* k, const void* 
  * sequences' new tokens, T / B each or rows cu[b] .. cu[b + 1] - 1 (int32 [B + 1]), to places
  * lens[b] - n + i (lens: int32 [B], with the new tokens).  freqs: float64 [R / 2], or NULL
  * (keys as they are): k turned as by prism_rotary at pos (as there, strides of token and axis
- * in pos_strides) or, NULL, at its place; R even, not interleaved a multiple of 16. */
+ * in pos_strides) or, NULL, at its place; R even, not interleaved a multiple of 16.  The rotation
+ * is formed in float64; prism_paged_append_f64 takes its amplitude so too (yarn's, cut to float32,
+ * moves a key by 3e-8 of itself, some of them over a border). */
 int prism_paged_append(const void* k, const void* v, int dtype, int64_t T, int Hk, int D, const int64_t* strides, void* k_cache,
                        void* v_cache, int bits, int64_t pages, int page_size, const int64_t* cache_strides,
                        const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens, int B,
                        const int32_t* cu, const double* freqs, int R, int interleaved, const void* pos, int pos64,
                        const int64_t* pos_strides, int axes, const int32_t* axis_end, float amplitude, hipStream_t stream);
+int prism_paged_append_f64(const void* k, const void* v, int dtype, int64_t T, int Hk, int D, const int64_t* strides,
+                           void* k_cache, void* v_cache, int bits, int64_t pages, int page_size,
+                           const int64_t* cache_strides, const int32_t* table, int64_t table_stride, int64_t width,
+                           const int32_t* lens, int B, const int32_t* cu, const double* freqs, int R, int interleaved,
+                           const void* pos, int pos64, const int64_t* pos_strides, int axes, const int32_t* axis_end,
+                           double amplitude, hipStream_t stream);
 /* Places 0 .. cu[b + 1] - cu[b] - 1 of every sequence as rows cu[b] .. of k, v [T, Hk, D]
  * (dense, dtype; rows of no sequence and places without a page: 0). */
 int prism_paged_gather(const void* k_cache, const void* v_cache, int dtype, int bits, int64_t pages, int page_size,

@@ -16,6 +16,7 @@ P = ctypes.c_void_p
 I32 = ctypes.c_int
 I64 = ctypes.c_int64
 F32 = ctypes.c_float
+F64 = ctypes.c_double
 U64 = ctypes.c_uint64
 
 # name -> argtypes (every function returns int; the last argument is the stream)
@@ -47,6 +48,8 @@ SIGNATURES = {
     "prism_packed_bwd": [P, P, P, P, P, P, P, I32, I32, I32, I32, I64, I64, I32, P, P, P, I32, F32, P, P, P, P, P, P, P],
     "prism_paged_append": [P, P, I32, I64, I32, I32, P, P, P, I32, I64, I32, P, P, I64, I64, P, I32, P, P, I32, I32, P, I32, P,
                            I32, P, F32, P],
+    "prism_paged_append_f64": [P, P, I32, I64, I32, I32, P, P, P, I32, I64, I32, P, P, I64, I64, P, I32, P, P, I32, I32, P, I32, P,
+                               I32, P, F64, P],
     "prism_paged_gather": [P, P, I32, I32, I64, I32, P, P, I64, I64, I32, P, I64, I32, I32, P, P, P],
     "prism_paged_plan": [I32, I64, I32, I32, I32, I32, I64, P],
     "prism_paged_fwd": [P, I32, I32, I64, I32, I32, I32, P, P, P, I32, I64, I32, P, P, I64, I64, P, F32, P, P, P, P],

@@ -59,7 +59,7 @@ struct Angles {
   const void* pos;                   // int32 / int64
   int64_t pb, ps, pa;                // strides of batch, token, axis
   int pos64, axes, axis_end[kMaxAxes];  // pairs below axis_end[a] (and not of an earlier axis) turn with axis a
-  float amp;
+  double amp;
   double sign;                       // -1: backwards
   // position of token n of sequence b as pair p takes it
   __device__ __forceinline__ double place(int b, int n, int p) const {
@@ -73,8 +73,8 @@ struct Angles {
   __device__ __forceinline__ void turned(double at, int p, F& s, F& c) const {
     const double t = at * (freqs[p] * 0.15915494309189533577);  // turns
     sincos_turns(sign * (t - rint(t)), s, c);
-    s *= amp;
-    c *= amp;
+    s *= (F)amp;
+    c *= (F)amp;
   }
   __device__ __forceinline__ void at(int b, int n, int p, float& s, float& c) const { turned(place(b, n, p), p, s, c); }
 };

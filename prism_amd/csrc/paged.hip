@@ -234,44 +234,11 @@ dim3 cut_tokens(A* a) {
   return dim3((unsigned)gx, (unsigned)((a->Hk + a->heads_per - 1) / a->heads_per));
 }
 
-}  // namespace
-
-int paged_check(const char* name, int dtype, int bits, int Hk, int D, int64_t pages, int page_size, const int64_t* strides,
-                const void* k_cache, const void* v_cache, int64_t width, int64_t B) {
-  PRISM_REQUIRE(dtype == PRISM_BF16 || dtype == PRISM_F16, "%s: dtype code %d (bfloat16 or float16)", name, dtype);
-  PRISM_REQUIRE(bits == 16 || bits == 4, "%s: a cache holds 16 or 4 bits, not %d", name, bits);
-  PRISM_REQUIRE(D == 64 || D == 128, "%s: head_dim %d unsupported (64, 128)", name, D);
-  PRISM_REQUIRE(Hk >= 1 && Hk < (1 << 16), "%s: heads out of range", name);
-  PRISM_REQUIRE(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
-                "%s: page size %d must be 16, 32, 64, 128 or 256", name, page_size);
-  PRISM_REQUIRE(pages >= 1 && pages < (1ll << 31) && width >= 1 && width * page_size < (1ll << 30) && B >= 0 && B < (1ll << 24),
-                "%s: sizes out of range", name);
-  PRISM_REQUIRE(strides && k_cache && v_cache, "%s: null pointer", name);
-  PRISM_REQUIRE(((uintptr_t)k_cache & 15) == 0 && ((uintptr_t)v_cache & 15) == 0, "%s: caches must be 16-byte aligned", name);
-  const int unit = bits == 16 ? 8 : 16;
-  for (int i = 0; i < 6; ++i) {
-    if (bits == 4 && i % 3 == 2) continue;
-    PRISM_REQUIRE(strides[i] >= 0 && strides[i] % unit == 0 && (i % 3 != 2 || strides[i] < (1 << 24)),
-                  "%s: a cache's strides must be whole 16 bytes, a place's below 2^24 elements", name);
-  }
-  return PRISM_OK;
-}
-void paged_sides(PagedSide* k, PagedSide* v, int bits, const int64_t* s, const void* k_cache, const void* v_cache) {
-  const int es = bits == 16 ? 2 : 1;
-  *k = {(uint8_t*)k_cache, s[0] * es, s[1] * es, s[2] * es};
-  *v = {(uint8_t*)v_cache, s[3] * es, s[4] * es, s[5] * es};
-}
-PagedTable paged_table(const int32_t* table, int64_t stride, int64_t width, int64_t pages, int page_size) {
-  return {table, stride, (int)width, (int)pages, __builtin_ctz((unsigned)page_size)};
-}
-
-extern "C" {
-
-int prism_paged_append(const void* k, const void* v, int dtype, int64_t T, int Hk, int D, const int64_t* strides, void* k_cache,
-                       void* v_cache, int bits, int64_t pages, int page_size, const int64_t* cache_strides,
-                       const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens, int B,
-                       const int32_t* cu, const double* freqs, int R, int interleaved, const void* pos, int pos64,
-                       const int64_t* pos_strides, int axes, const int32_t* axis_end, float amplitude, hipStream_t stream) {
+int append(const void* k, const void* v, int dtype, int64_t T, int Hk, int D, const int64_t* strides, void* k_cache,
+           void* v_cache, int bits, int64_t pages, int page_size, const int64_t* cache_strides, const int32_t* table,
+           int64_t table_stride, int64_t width, const int32_t* lens, int B, const int32_t* cu, const double* freqs, int R,
+           int interleaved, const void* pos, int pos64, const int64_t* pos_strides, int axes, const int32_t* axis_end,
+           double amplitude, hipStream_t stream) {
   if (const int rc = paged_check("prism_paged_append", dtype, bits, Hk, D, pages, page_size, cache_strides, k_cache, v_cache, width, B))
     return rc;
   PRISM_REQUIRE(T >= 0 && T < (1ll << 30), "prism_paged_append: too many tokens");
@@ -319,6 +286,58 @@ int prism_paged_append(const void* k, const void* v, int dtype, int64_t T, int H
   else run(ElemF16{});
   PRISM_LAUNCH_CHECK("prism_paged_append");
   return PRISM_OK;
+}
+
+}  // namespace
+
+int paged_check(const char* name, int dtype, int bits, int Hk, int D, int64_t pages, int page_size, const int64_t* strides,
+                const void* k_cache, const void* v_cache, int64_t width, int64_t B) {
+  PRISM_REQUIRE(dtype == PRISM_BF16 || dtype == PRISM_F16, "%s: dtype code %d (bfloat16 or float16)", name, dtype);
+  PRISM_REQUIRE(bits == 16 || bits == 4, "%s: a cache holds 16 or 4 bits, not %d", name, bits);
+  PRISM_REQUIRE(D == 64 || D == 128, "%s: head_dim %d unsupported (64, 128)", name, D);
+  PRISM_REQUIRE(Hk >= 1 && Hk < (1 << 16), "%s: heads out of range", name);
+  PRISM_REQUIRE(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
+                "%s: page size %d must be 16, 32, 64, 128 or 256", name, page_size);
+  PRISM_REQUIRE(pages >= 1 && pages < (1ll << 31) && width >= 1 && width * page_size < (1ll << 30) && B >= 0 && B < (1ll << 24),
+                "%s: sizes out of range", name);
+  PRISM_REQUIRE(strides && k_cache && v_cache, "%s: null pointer", name);
+  PRISM_REQUIRE(((uintptr_t)k_cache & 15) == 0 && ((uintptr_t)v_cache & 15) == 0, "%s: caches must be 16-byte aligned", name);
+  const int unit = bits == 16 ? 8 : 16;
+  for (int i = 0; i < 6; ++i) {
+    if (bits == 4 && i % 3 == 2) continue;
+    PRISM_REQUIRE(strides[i] >= 0 && strides[i] % unit == 0 && (i % 3 != 2 || strides[i] < (1 << 24)),
+                  "%s: a cache's strides must be whole 16 bytes, a place's below 2^24 elements", name);
+  }
+  return PRISM_OK;
+}
+void paged_sides(PagedSide* k, PagedSide* v, int bits, const int64_t* s, const void* k_cache, const void* v_cache) {
+  const int es = bits == 16 ? 2 : 1;
+  *k = {(uint8_t*)k_cache, s[0] * es, s[1] * es, s[2] * es};
+  *v = {(uint8_t*)v_cache, s[3] * es, s[4] * es, s[5] * es};
+}
+PagedTable paged_table(const int32_t* table, int64_t stride, int64_t width, int64_t pages, int page_size) {
+  return {table, stride, (int)width, (int)pages, __builtin_ctz((unsigned)page_size)};
+}
+
+extern "C" {
+
+int prism_paged_append(const void* k, const void* v, int dtype, int64_t T, int Hk, int D, const int64_t* strides, void* k_cache,
+                       void* v_cache, int bits, int64_t pages, int page_size, const int64_t* cache_strides,
+                       const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens, int B,
+                       const int32_t* cu, const double* freqs, int R, int interleaved, const void* pos, int pos64,
+                       const int64_t* pos_strides, int axes, const int32_t* axis_end, float amplitude, hipStream_t stream) {
+  return append(k, v, dtype, T, Hk, D, strides, k_cache, v_cache, bits, pages, page_size, cache_strides, table, table_stride, width,
+                lens, B, cu, freqs, R, interleaved, pos, pos64, pos_strides, axes, axis_end, (double)amplitude, stream);
+}
+
+int prism_paged_append_f64(const void* k, const void* v, int dtype, int64_t T, int Hk, int D, const int64_t* strides,
+                           void* k_cache, void* v_cache, int bits, int64_t pages, int page_size,
+                           const int64_t* cache_strides, const int32_t* table, int64_t table_stride, int64_t width,
+                           const int32_t* lens, int B, const int32_t* cu, const double* freqs, int R, int interleaved,
+                           const void* pos, int pos64, const int64_t* pos_strides, int axes, const int32_t* axis_end,
+                           double amplitude, hipStream_t stream) {
+  return append(k, v, dtype, T, Hk, D, strides, k_cache, v_cache, bits, pages, page_size, cache_strides, table, table_stride, width,
+                lens, B, cu, freqs, R, interleaved, pos, pos64, pos_strides, axes, axis_end, amplitude, stream);
 }
 
 int prism_paged_gather(const void* k_cache, const void* v_cache, int dtype, int bits, int64_t pages, int page_size,

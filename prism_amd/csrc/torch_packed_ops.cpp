@@ -408,11 +408,11 @@ void paged_append(const Tensor& k_, const Tensor& v_, const Tensor& kc, const Te
   if (T == 1) st[0] = st[2] = 0;
   Places at{};
   if (pos) at = places_of("append_paged", *pos, axis_pairs, 1, T, freqs->numel());
-  PRISM_TORCH_CALL(prism_paged_append, k.data_ptr(), v.data_ptr(), k.scalar_type() == at::kBFloat16 ? PRISM_BF16 : PRISM_F16, T,
+  PRISM_TORCH_CALL(prism_paged_append_f64, k.data_ptr(), v.data_ptr(), k.scalar_type() == at::kBFloat16 ? PRISM_BF16 : PRISM_F16, T,
                    small(Hk, "heads"), small(D, "D"), st, kc.data_ptr(), vc.data_ptr(), c.bits, c.pages, c.page_size, c.strides,
                    table.data_ptr<int32_t>(), table.size(0) > 1 ? table.stride(0) : 0, table.size(1), lens.data_ptr<int32_t>(),
                    small(B, "B"), (const int32_t*)p(cu), (const double*)p(freqs), freqs ? small(2 * freqs->numel(), "rotary dim") : 0,
-                   interleaved, p(pos), pos ? at.is64 : false, at.strides + 1, at.axes, at.axis_end, (float)amplitude, stream_of(k));
+                   interleaved, p(pos), pos ? at.is64 : false, at.strides + 1, at.axes, at.axis_end, amplitude, stream_of(k));
   // (torch's own record that the caches changed)
   for (const Tensor* t : {&kc, &vc})
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();

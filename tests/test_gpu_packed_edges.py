@@ -1,11 +1,12 @@
-"""Corners of packed batches and paged caches: blocks of 4 bits that are not finite."""
+"""Corners of packed batches and paged caches: blocks of 4 bits that are not finite, amplitudes
+that float32 does not hold."""
 import math
 
 import pytest
 import torch
 
 import prism_amd
-from tests.test_gpu_paged import ints, table_for
+from tests.test_gpu_paged import ints, levels_of, of_cache, places_of, table_for, turned
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -46,3 +47,25 @@ def test_blocks_that_are_not_finite_are_nan(dt, D, n):
             hit[max(0, place - (L - n)):n, Hq // Hk:, channel // 32 * 32:channel // 32 * 32 + 32] = True
             assert torch.equal(torch.isnan(o), hit) and torch.equal(o[~hit], want[~hit])
 
+
+# ------------------------------------------------------------------ appended keys
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_amplitudes_that_float32_does_not_hold(bits, interleaved):
+    """yarn's amplitude at factor 40, 0.1 ln 40 + 1, is 3.2e-8 off in float32: the keys are those
+    of the float64 rotation, in float16 and its 4 bits, bit for bit (600,000 of them: some 27
+    would fall on another side of a border)."""
+    Hk, D, page, dt = 8, 128, 64, torch.float16
+    lens = [400, 200]
+    T = sum(lens)
+    table, pages = table_for(lens, page)
+    k = randn(T, Hk, D, dt=dt, seed=3)
+    freqs, amplitude = prism_amd.rotary_frequencies(D, scaling="yarn", factor=40, original_length=8192)
+    assert abs(amplitude - torch.tensor(amplitude).item()) > 2e-8
+    who, at = places_of(lens, lens)
+    kc, vc = prism_amd.paged_cache(pages, page, Hk, D, dtype=dt, bits=bits)
+    prism_amd.append_paged(k, k, kc, vc, table, ints(lens), cu_seqlens=ints([0, 400, 600]), freqs=freqs, amplitude=amplitude,
+                           interleaved=interleaved)
+    want = turned(k, at, freqs, interleaved, amplitude, dt)
+    got = of_cache(kc, D)[table[who, at // page].long(), :, at % page]
+    assert torch.equal(got, want.double() if bits == 16 else levels_of(want))
