@@ -347,6 +347,7 @@ PagedCaches check_caches(const char* op, const Tensor& like, const Tensor& kc, c
                        (four || kc.scalar_type() == at::kBFloat16 || kc.scalar_type() == at::kHalf),
                    "prism: ", op, ": caches must be both bfloat16, float16 or uint8 (4 bits), got ", kc.scalar_type(), " and ",
                    vc.scalar_type());
+  TORCH_CHECK_VALUE(D == 64 || D == 128, op, ": head_dim ", D, " unsupported (64, 128)");  // (a place's bytes divide below)
   PagedCaches c;
   c.bits = four ? 4 : 16;
   const int64_t place = D / 2 + D / 32;

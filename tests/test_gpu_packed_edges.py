@@ -1,5 +1,5 @@
 """Corners of packed batches and paged caches: blocks of 4 bits that are not finite, amplitudes
-that float32 does not hold."""
+that float32 does not hold, operator calls without channels."""
 import math
 
 import pytest
@@ -69,3 +69,18 @@ def test_amplitudes_that_float32_does_not_hold(bits, interleaved):
     want = turned(k, at, freqs, interleaved, amplitude, dt)
     got = of_cache(kc, D)[table[who, at // page].long(), :, at % page]
     assert torch.equal(got, want.double() if bits == 16 else levels_of(want))
+
+
+def test_operators_without_channels_are_refused():
+    """Heads of no channels, which the functions of prism_amd refuse, as an error of the
+    operators beneath them too."""
+    table, lens = ints([[0]]), ints([1])
+    for dt in (torch.uint8, torch.bfloat16):
+        c = torch.zeros((1, 2, 0) if dt is torch.uint8 else (1, 2, 16, 0), dtype=dt, device=DEV)
+        x = torch.zeros(1, 2, 0, dtype=torch.bfloat16, device=DEV)
+        with pytest.raises(ValueError):
+            torch.ops.prism.paged_append(x, x, c, c.clone(), table, lens, None, None, None, [], True, 1.0)
+        with pytest.raises(ValueError):
+            torch.ops.prism.paged_fwd(x, c, c, table, lens, 2, 0.125, False)
+        with pytest.raises(ValueError):
+            torch.ops.prism.paged_gather(c, c, table, ints([0, 1]), 1, 2, 0, False)
