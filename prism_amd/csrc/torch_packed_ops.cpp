@@ -402,6 +402,8 @@ void paged_append(const Tensor& k_, const Tensor& v_, const Tensor& kc, const Te
   for (const Tensor* t : {&kc, &vc})
     TORCH_CHECK_VALUE(at::has_internal_overlap(*t) != at::MemOverlap::Yes,
                       "append_paged: a cache whose places share memory (expand) cannot be written");
+  TORCH_CHECK_VALUE(kc.numel() == 0 || kc.data_ptr() != vc.data_ptr(),
+                    "append_paged: k_cache and v_cache share memory: each place would hold the key, the value or pieces of both");
   const c10::DeviceGuard guard(k_.device());
   const Tensor k = pack_rows(k_), v = pack_rows(v_), table = unit_table(table_), lens = lens_.contiguous();
   const OptT cu = cont(cu_), freqs = cont(freqs_);

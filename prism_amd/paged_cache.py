@@ -95,7 +95,7 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     tokens go to (else either's row, or pieces of both, are left).
 
     k_cache, v_cache: of paged_cache, or views with adjacent channels (and places, in 4 bits)
-    and strides of whole 16 bytes; 16 bits: of k's dtype.  4 bits: 32 channels share the least
+    and strides of whole 16 bytes, that share no memory; 16 bits: of k's dtype.  4 bits: 32 channels share the least
     power of two that keeps them within 6 times it (no smaller than 2^-126), and each is
     rounded to the nearest value (halves to the even code); 32 channels of which one is a NaN
     or an infinity are read as NaN.  Values whose level is beyond a type's largest are infinite

@@ -1,5 +1,6 @@
 """Corners of packed batches and paged caches: blocks of 4 bits that are not finite, amplitudes
-that float32 does not hold, operator calls without channels."""
+that float32 does not hold, operator calls without channels,
+caches that are one."""
 import math
 
 import pytest
@@ -84,3 +85,20 @@ def test_operators_without_channels_are_refused():
             torch.ops.prism.paged_fwd(x, c, c, table, lens, 2, 0.125, False)
         with pytest.raises(ValueError):
             torch.ops.prism.paged_gather(c, c, table, ints([0, 1]), 1, 2, 0, False)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_one_cache_for_keys_and_values_is_refused(bits):
+    table, lens = ints([[0, 1]]), ints([20])
+    x = randn(20, 2, 64)
+    pool = torch.stack([c for c in prism_amd.paged_cache(2, 16, 2, 64, bits=bits)], 1)  # [pages, 2, ..]
+    kc, _ = prism_amd.paged_cache(2, 16, 2, 64, bits=bits)
+    for a, b in ((kc, kc), (kc, kc.view(kc.shape)), (pool[:, 1], pool[:, 1])):
+        with pytest.raises(ValueError, match="share memory"):
+            prism_amd.append_paged(x, x, a, b, table, lens)
+    assert not kc.any() and not pool.any()
+    prism_amd.append_paged(x, x, pool[:, 0], pool[:, 1], table, lens)
+    assert torch.equal(pool[:, 0], pool[:, 1]) and pool.any()
+    # (to read, one may be both)
+    o = prism_amd.flash_attn_paged(x[:1], pool[:, 0], pool[:, 0], table, lens)
+    assert torch.equal(o, prism_amd.flash_attn_paged(x[:1], pool[:, 0], pool[:, 1], table, lens))
