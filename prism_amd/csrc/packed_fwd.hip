@@ -371,9 +371,12 @@ __global__ __launch_bounds__(kPlanThreads) void pack_plan_kernel(PackArgs a, Pac
     if (p > 1) {
       const int x = atomicAdd(&cuts, 1);
       slot = atomicAdd(&pieces, p * l.per);
-      // (bounds that overlap could ask for more than there is room for: such a block is dropped)
-      if ((uint32_t)x >= (uint32_t)l.max_cuts || slot < 0 || slot > l.max_pieces - p * l.per) slot = -2;
-      else l.cuts[x] = PackEntry{q.q0, q.n, q.k0, q.L, t, 0, p, slot};
+      // (pack_cut's room is enough for any bounds, as the shares come from the same lengths; a block
+      // without room would be dropped, and its place among the cuts, which are counted, hold nothing)
+      const bool room = (uint32_t)x < (uint32_t)l.max_cuts && slot >= 0 && slot <= l.max_pieces - p * l.per;
+      if ((uint32_t)x < (uint32_t)l.max_cuts)
+        l.cuts[x] = room ? PackEntry{q.q0, q.n, q.k0, q.L, t, 0, p, slot} : PackEntry{0, 0, 0, 0, 0, 0, 1, -1};
+      if (!room) slot = -2;
     }
     for (int y = 0; y < p; ++y)
       if ((uint32_t)(first + y) < (uint32_t)l.max_entries)

@@ -1,12 +1,14 @@
 """Corners of packed batches and paged caches: blocks of 4 bits that are not finite, amplitudes
-that float32 does not hold, operator calls without channels,
-caches that are one."""
+that float32 does not hold, operator calls without channels, caches that are one, bounds that overlap
+(nothing beside a call's outputs and workspaces is written)."""
+import ctypes
 import math
 
 import pytest
 import torch
 
 import prism_amd
+from prism_amd import _lib
 from tests.test_gpu_paged import ints, levels_of, of_cache, places_of, table_for, turned
 
 pytestmark = pytest.mark.gpu
@@ -102,3 +104,62 @@ def test_one_cache_for_keys_and_values_is_refused(bits):
     # (to read, one may be both)
     o = prism_amd.flash_attn_paged(x[:1], pool[:, 0], pool[:, 0], table, lens)
     assert torch.equal(o, prism_amd.flash_attn_paged(x[:1], pool[:, 0], pool[:, 1], table, lens))
+
+
+# ------------------------------------------------------------------ bounds that overlap
+class Guarded:
+    """Buffers inside larger ones of a value that nothing else has."""
+
+    def __init__(self):
+        self.all = []
+
+    def __call__(self, shape, dtype):
+        n, pad, mark = math.prod(shape), 4096, 1234567 if dtype is torch.int32 else -19.75
+        t = torch.full((n + 2 * pad,), mark, dtype=dtype, device=DEV)
+        self.all.append((t, n, pad, mark))
+        return t[pad:pad + n].view(shape)
+
+    def intact(self):
+        return all((t[:pad] == m).all() and (t[pad + n:] == m).all() for t, n, pad, m in self.all)
+
+
+@pytest.mark.parametrize("causal", [1, 0])
+@pytest.mark.parametrize("B", [5, 61, 700])
+def test_bounds_that_overlap_write_nothing_else(B, causal):
+    """Outputs and workspaces of exactly the planned sizes: with bounds in any order, and with
+    hundreds of sequences that each take all tokens, nothing beside them is written, and the
+    lists' counts stay within their room."""
+    lib = _lib.load()
+    T, Hq, Hk, D = 1500, 4, 2, 64
+    g = torch.Generator(device=DEV).manual_seed(B)
+    any_ = [torch.randint(-99, T + 99, (B + 1,), generator=g, device=DEV, dtype=torch.int32) for _ in "qk"]
+    whole = ints([0 if i % 2 == 0 else T for i in range(B + 1)])
+    q, k, do = randn(T, Hq, D, seed=1), randn(T, Hk, D, seed=2), randn(T, Hq, D, seed=3)
+    ptr = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    sizes = []
+    for plan in (lib.prism_packed_fwd_plan, lib.prism_packed_bwd_plan):
+        ints_, floats = ctypes.c_int64(0), ctypes.c_int64(0)
+        assert plan(B, Hq, Hk, T, T, D, ctypes.byref(ints_), ctypes.byref(floats)) == 0
+        sizes.append((ints_.value, floats.value))
+    assert all(n > 0 for n, _ in sizes) and (B == 700 or all(n > 0 for _, n in sizes))  # (lists, and blocks that may be cut)
+    st = lambda *ts: (ctypes.c_int64 * (2 * len(ts)))(*[s for t in ts for s in (t.stride(1), t.stride(0))])  # noqa: E731
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for cq, ck in (any_, any_[::-1], (whole, whole), (whole, any_[0])):
+        new, bf, f32, i32 = Guarded(), torch.bfloat16, torch.float32, torch.int32
+        o, rest, lse, dq, dk, dv = (new(s, t) for s, t in (((T, Hq, D), bf), ((T, Hq, D), bf), ((Hq, T), f32), ((T, Hq, D), bf),
+                                                          ((T, Hk, D), bf), ((T, Hk, D), bf)))
+        plans, parts, rows = [new((n,), i32) for n, _ in sizes], [new((n,), f32) for _, n in sizes], new((2 * Hq * T,), f32)
+        rest.zero_()  # (rows that an overlap leaves out are read by the backward)
+        o.zero_()
+        lse.zero_()
+        torch.cuda.synchronize()
+        assert lib.prism_packed_fwd(ptr(q), ptr(k), ptr(k), 1, B, Hq, Hk, T, T, D, st(q, k, k, o), ptr(cq), ptr(ck), causal, 0.125,
+                                    ptr(o), ptr(rest), ptr(lse), ptr(plans[0]), ptr(parts[0]), stream) == 0
+        assert lib.prism_packed_bwd(ptr(do), ptr(q), ptr(k), ptr(k), ptr(o), ptr(rest), ptr(lse), 1, B, Hq, Hk, T, T, D,
+                                    st(q, k, k, o, do, dq, dk, dv), ptr(cq), ptr(ck), causal, 0.125, ptr(dq), ptr(dk), ptr(dv),
+                                    ptr(rows), ptr(plans[1]), ptr(parts[1]), stream) == 0
+        torch.cuda.synchronize()
+        assert new.intact()
+        for plan, (n, _) in zip(plans, sizes):  # (entries and cuts of eight ints behind the first eight)
+            entries, cuts, pieces = plan[:3].tolist()
+            assert 0 <= entries and 0 <= cuts and 8 * (1 + entries) <= n and 8 * (1 + cuts) <= n and pieces >= 0
