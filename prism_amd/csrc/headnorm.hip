@@ -80,10 +80,12 @@ __device__ __forceinline__ void put_angles(const HeadArgs& a, int64_t first, flo
 template <int VEC, bool INTER>
 struct LaneTurn {
   float cs[INTER ? VEC / 2 : VEC], sn[INTER ? VEC / 2 : VEC];
-  int other;  // (half a rotation apart)
+  int other;   // (half a rotation apart)
+  bool turns;  // the lane's channels turn (a rotation ends between lanes)
   __device__ __forceinline__ void init(const HeadArgs& a, const float2* table, int slot, int u) {
     const int c0 = u * VEC, half = a.R / 2;
     const bool rot = c0 < a.R, upper = !INTER && c0 >= half;
+    turns = rot;
     other = (int)threadIdx.x & 63;
     if (!INTER && rot) other += upper ? -(half / VEC) : half / VEC;
     const float2* mine = table + slot * half + (INTER ? c0 / 2 : upper ? c0 - half : c0);
@@ -100,6 +102,7 @@ struct LaneTurn {
   // v turned; p: the other channels' values (half a rotation apart)
   __device__ __forceinline__ void turn(float* v, const float* p) const {
     if constexpr (INTER) {
+      if (!turns) return;  // (0 times an infinity beside it would make a channel NaN)
 #pragma unroll
       for (int i = 0; i < VEC / 2; ++i) {
         const float x = v[2 * i], y = v[2 * i + 1];

@@ -1,6 +1,6 @@
 """Corners of packed batches and paged caches: blocks of 4 bits that are not finite, amplitudes
 that float32 does not hold, operator calls without channels, caches that are one, bounds that overlap
-(nothing beside a call's outputs and workspaces is written)."""
+(nothing beside a call's outputs and workspaces is written), infinities in head norms."""
 import ctypes
 import math
 
@@ -163,3 +163,30 @@ def test_bounds_that_overlap_write_nothing_else(B, causal):
         for plan, (n, _) in zip(plans, sizes):  # (entries and cuts of eight ints behind the first eight)
             entries, cuts, pieces = plan[:3].tolist()
             assert 0 <= entries and 0 <= cuts and 8 * (1 + entries) <= n and 8 * (1 + cuts) <= n and pieces >= 0
+
+
+# ------------------------------------------------------------------ head norms
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,R", [(128, 128), (128, 64), (36, 36), (36, 16)])
+def test_infinities_in_a_head(D, R, dt):
+    """A NaN fills its head; beside an infinity the inverse root is 0, so that its own channel
+    and the one that turns with it (if it turns) are NaN and the head's others 0; squares whose
+    sum passes float32's range give 0 alike."""
+    q = randn(1, 4, 6, D, dt=dt, seed=1)
+    freqs, _ = prism_amd.rotary_frequencies(R)
+    at = torch.arange(1, 7, device=DEV)
+    for inter in (True, False):
+        partner = lambda c: c if c >= R else c ^ 1 if inter else (c + R // 2) % R  # noqa: E731
+        x = q.clone()
+        x[0, 0, 1, 5], x[0, 1, 2, 9], x[0, 2, 3, D - 1] = math.nan, math.inf, -math.inf
+        if dt is not torch.float16:
+            x[0, 3, 4, 2] = 3e19
+        y = prism_amd.qk_norm_rotary(x, None, None, None, freqs, at, interleaved=inter)
+        want = prism_amd.qk_norm_rotary(q, None, None, None, freqs, at, interleaved=inter)
+        want[0, 0, 1] = math.nan
+        for h, s, c in ((1, 2, 9), (2, 3, D - 1)):
+            want[0, h, s] = 0
+            want[0, h, s, [c, partner(c)]] = math.nan
+        if dt is not torch.float16:
+            want[0, 3, 4] = 0
+        assert torch.equal(y.nan_to_num(nan=99.0), want.nan_to_num(nan=99.0))
