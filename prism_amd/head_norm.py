@@ -26,9 +26,12 @@ def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optiona
     k_weight: [D] of q's dtype or float32 (both the same), or None for ones.  freqs,
     positions, interleaved, sections, amplitude: as for apply_rotary.  Returns q',
     with k (q', k').  Sums are fp32; results are rounded once (apply_rotary of a norm
-    in between rounds twice).  A NaN or infinity makes its own head's results NaN and
-    no others.  Differentiable in q, k and the weights (once; no forward mode; freqs
-    that require gradients are refused)."""
+    in between rounds twice).  A NaN makes all its head's results NaN; beside an infinity
+    the root's inverse is 0, so that its own channel and the one that turns with it are
+    NaN and the head's others 0; a sum of squares beyond float32 (values of 1.8e19 and
+    more) makes a head 0.  No other head's results change (the weights' gradients are
+    sums over all heads).  Differentiable in q, k and the weights (once; no forward
+    mode; freqs that require gradients are refused)."""
     qs, ks, pairs = q.shape, None if k is None else k.shape, freqs.shape
     for s, name in ((qs, "q"), (ks, "k")):
         if s is not None and len(s) != 4:
