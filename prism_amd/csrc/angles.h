@@ -1,5 +1,6 @@
-// Angles of rotary positions (rotary.hip, headnorm.hip, paged.hip): pair p of a
-// token at position n turns by n f_p, positions with one entry per axis of a grid.
+// Angles of rotary positions (headnorm.hip, paged.hip; rotary.hip takes the sines and keeps its
+// own places): pair p of a token at position n turns by n f_p, positions with one entry per axis
+// of a grid.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -24,8 +24,9 @@
 // of them runs at 4.8); loading the first heads before the angles: 678 us.  16 tokens, 32 +
 // 8 heads: 6.5 us, the launch and its one trip to memory.  9,998 tokens, 16 + 4 heads of 64,
 // 32 channels turning: forward 18.7 us (2.7 TB/s), backward 24.0 (3.2 TB/s) and 4.6 for the
-// weights: one round of workgroups, the vector unit issuing 55% of the time (float64 angles,
-// conversions), the rest waits for their first loads.
+// weights: the forward's 1,252 workgroups are 1.2 rounds (four a CU, 104 registers), the backward's
+// 939 one; the vector unit issues 55% of the time (float64 angles, formed by every slice of heads
+// anew; conversions), the rest waits for their first loads.
 #include <type_traits>
 
 #include "angles.h"
@@ -442,8 +443,11 @@ __global__ __launch_bounds__(256) void head_norm_dw_kernel(const float* partial,
 }
 
 // How a launch is cut: `vec` elements a lane (0: one wave a row), tokens per
-// workgroup, and heads per slice (blockIdx.y): as many slices as one round of the chip
-// holds (six workgroups a CU, the backward four, each leaving a partial row)
+// workgroup, and heads per slice (blockIdx.y): as many slices as make 1,536 workgroups,
+// six a CU, the backward 1,024, each leaving a partial row.  (A CU holds four of the backward
+// and of the forward half a rotation apart in bfloat16, six in float16, seven
+// interleaved, eight in halves of a piece; the numbers were measured for the clip and the
+// training step above alone.)
 struct HeadCut {
   int vec, lanes, tpb, heads_per;
   int64_t gx, gy;

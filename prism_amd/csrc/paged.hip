@@ -15,8 +15,10 @@
 // in flight; four lanes share a scale's 32 channels.  Single tokens: one head per thread.
 //
 // Measured (bf16, D = 128): append of 16,001 tokens, 8 heads, 16 bits 30.6 us (131 MB, 4.3
-// TB/s); 8,191 tokens, 8 heads to 4 bits 22 to 24 us (43 MB: the float64 angles and products);
-// with the angles in an LDS table 21.9 and, 16 bits, 32: each lane forms its own.  Gather of
+// TB/s); 8,191 tokens, 8 heads to 4 bits, half a rotation apart, 22 to 24 us from HBM (43 MB: the
+// float64 angles and products); with the angles in an LDS table 21.9 and, 16 bits, 32: each lane
+// forms its own.  The same tensors again and again, from the last cache: 16.3 us, interleaved (four
+// angles a lane in place of eight) 13.2, without a rotation 9.8.  Gather of
 // 32,764 places, 4 bits 37 us (170 MB, 4.6 TB/s).  32 single tokens: 6.5 us.
 #include <type_traits>
 
@@ -221,7 +223,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(GatherArgs a) {
 
 // lanes of a head, tokens of a workgroup, and heads per slice so that a launch has four
 // workgroups a CU where it can (single tokens: one head a thread).  8,192 tokens, 8 heads of
-// 128, 4 bits, append / gather, us, at 512 / 1,024 / 2,048 workgroups: 16.4 / 17.0 / 22.9 (each
+// 128, 4 bits, the same tensors again and again (from the last cache), append / gather, us, at 512 / 1,024 / 2,048 workgroups: 16.4 / 17.0 / 22.9 (each
 // slice forms the angles anew), 10.7 / 9.7 / 9.5; 3,000 tokens of 40 heads, 16 bits: 34 / 35 /
 // 33, 25 / 23.5 / 23.3.
 template <class A>

@@ -32,7 +32,9 @@
 // o once, as window_token.hip.  4 bits: K's and V's values are exact in the operands (K
 // beside float16 queries: as float16), P times V's scale is rounded to bfloat16, whose
 // range holds any scale; beside float16 queries to two of them, 16 bits in all (with one,
-// o is 1.6e-3 off, norm-wise, for float16's own 2e-4).
+// o is 1.6e-3 off, norm-wise, for float16's own 2e-4).  Over 32 rows at D = 128 the second takes 16
+// registers more than there are, which are spilled: 16 x 8,192 keys, 5 tokens x 64 heads over 8, 97 us, beside
+// bfloat16 queries 65.
 #include <type_traits>
 
 #include "paged.h"
@@ -420,7 +422,8 @@ struct Paged4F16 {
   static __device__ __forceinline__ uint4 values(uint32_t w, float s) { return f16_of_codes(w, s); }
   using Out = WinF16;
 };
-// a b, and 0 where either is 0 (v_mul_legacy_f32: 0 times an infinity or a NaN is 0)
+// a b, and 0 where either is 0 (v_mul_legacy_f32: 0 times an infinity or a NaN is 0); the
+// compiler has no builtin for the instruction, so its intrinsic is declared by name
 extern "C" __device__ __attribute__((const)) float prism_mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
 // max and sum over the four lanes l16, l16 + 16, .. that share a row
 __device__ __forceinline__ float rows_max(float x) {
@@ -769,14 +772,20 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
 
 // How a call is cut: rows of a tile, keys of a tile, and over how many workgroups at most.
 //
-// One round of the chip at most (one workgroup a CU over 16 bits, two over 4), about sqrt(keys)
-// / 2.5 parts (4 bits, tiles twice as long: / 5), one up to 512 keys, and no part of a sequence
+// One round of the chip at most (one workgroup a CU over 16 bits, two over 4: what fits at D =
+// 128; at 64 twice as many would), about sqrt(keys) / 2.5 parts (4 bits, tiles twice as long: / 5) of
+// the longest sequence that the table could hold, one up to 512 keys, and no part of a sequence
 // below two tiles.  Measured (us, 32 heads over 8, D = 128, pages of 16 or 64; lengths from half
 // to all of the stated): 16 bits, 256 / 512 / 1,024 workgroups: 1 x 32,768 26 / 33 / 34; 16 x
 // 8,192 84 / 85 / 91; 64 x 2,048 82 / 82 / 97; 8 x 131,072 561 / 543 / 537.  4 bits: 18 / 21 /
 // 21; 39 / 35 / 38; 33 / 33 / 42; 209 / 183 / 179; 2 x 131,072 46 / 45 / 52.  Parts of 2 / 8 / 16
 // tiles at least: 1 x 1,000 12.1 / 14.0 / 16.2 (4 bits 10.7 / 12.1 / 12.8), 1 x 4,096 14.8 / 14.7
-// / 17.9 (12.1 / 14.0 / 17.3).
+// / 17.9 (12.1 / 14.0 / 17.3).  The parts are rounded down, so that counts between are not cut and
+// wait for their longest sequence (TB/s): 16 bits, 16 / 17 / 20 / 24 / 31 / 32 / 33 / 48 sequences of up to 8,192
+// 4.8 / 4.5 / 4.8 / 5.1 / 5.4 / 5.2 / 4.7 / 5.3, D = 64, 16 / 24 / 32 / 48 4.5 / 4.7 / 5.1 / 4.8; 4 bits, 32
+// / 33 / 48 / 64 / 70 of up to 16,384 4.1 / 3.2 / 4.0 / 4.8 / 4.2, D = 64, 32 / 48 / 64 3.9 / 3.3 / 3.9, and 64 / 70
+// of 8,192 with 4 key heads 4.4 / 2.9.  Tables sixteen times as wide as the lengths: 4 x 4,096 19.5 us and 19.7
+// (4 bits 16.0 and 13.4).
 struct PagedCut {
   int rows, keys, least;
   int64_t tiles, total, splits;
